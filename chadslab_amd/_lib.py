@@ -72,6 +72,11 @@ SIGNATURES = {
     "chadq_prompt_i4g32_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "chadq_prompt_i4g32": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                                    c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "chadq_quantize_mxfp4": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
+    "chadq_dequant_mxfp4": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
+    "chadq_product_mxfp4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "chadq_product_mxfp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "chadq_product_mxfp4_grouped": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "chadq_sample_topk_f32": (c_int, [c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
 }
 

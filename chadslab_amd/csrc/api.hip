@@ -5,6 +5,7 @@
 #include <cstring>
 
 #include "chadq_common.h"
+#include "mx.h"
 
 namespace chadq {
 
@@ -105,6 +106,10 @@ bool prompt_i4g32_ok(int, int, int, int);
 size_t prompt_i4g32_workspace_bytes(int, int, int, int, int);
 int prompt_i4g32_launch(const chadq_prompt_layer_i4g32 *, int, const int32_t *, const uint8_t *, const uint16_t *, int, const float *, int, int,
                         int, int, int, int, float, float *, void *, hipStream_t);
+int quantize_mxfp4_launch(const void *, int, uint8_t *, uint8_t *, int64_t, int, hipStream_t);
+int dequant_mxfp4_launch(const uint8_t *, const uint8_t *, float *, int64_t, int, hipStream_t);
+int mx_product_launch(const MxProduct &, void *, size_t, hipStream_t);
+size_t mx_product_workspace_bytes(int, int, int, bool);
 int sample_topk_launch(const float *, int, int, float, const float *, float *, int32_t *, int32_t *, int32_t *, int, hipStream_t);
 
 }  // namespace chadq
@@ -620,6 +625,55 @@ int chadq_prompt_i4g32(const chadq_prompt_layer_i4g32 *layers, int n_layers, con
     CHADQ_REQUIRE(workspace && workspace_bytes >= need, CHADQ_ERR_WORKSPACE, "chadq_prompt_i4g32: workspace of %zu bytes needed, %zu given",
                   need, workspace ? workspace_bytes : (size_t)0);
     return prompt_i4g32_launch(layers, n_layers, tokens, emb, semb, V, rope_table, T, pos, d, hq, dh, ffn, eps, x_last, workspace, st);
+}
+
+int chadq_quantize_mxfp4(const void *x, int dtype, uint8_t *codes, uint8_t *scale, int64_t rows, int K, void *stream) {
+    ENTER();
+    CHADQ_REQUIRE(dtype == CHADQ_F32 || dtype == CHADQ_BF16 || dtype == CHADQ_F16, CHADQ_ERR_SHAPE, "chadq_quantize_mxfp4: unknown type %d", dtype);
+    CHADQ_REQUIRE(rows >= 0 && K >= 0 && K % 32 == 0, CHADQ_ERR_SHAPE, "chadq_quantize_mxfp4: rows=%lld K=%d (K %% 32 != 0?)", (long long)rows, K);
+    CHADQ_REQUIRE(K == 0 || rows <= INT64_MAX / 16 / K, CHADQ_ERR_SHAPE, "chadq_quantize_mxfp4: rows=%lld K=%d are too many values", (long long)rows, K);
+    if (rows == 0 || K == 0) return 0;
+    CHADQ_REQUIRE(x && codes && scale, CHADQ_ERR_NULL, "chadq_quantize_mxfp4: null pointer");
+    CHADQ_REQUIRE(aligned16(x) && (reinterpret_cast<uintptr_t>(codes) & 3) == 0, CHADQ_ERR_ALIGN, "chadq_quantize_mxfp4: x must be 16-byte, codes 4-byte aligned");
+    return quantize_mxfp4_launch(x, dtype, codes, scale, rows, K, st);
+}
+
+int chadq_dequant_mxfp4(const uint8_t *codes, const uint8_t *scale, float *w, int64_t rows, int K, void *stream) {
+    ENTER();
+    CHADQ_REQUIRE(rows >= 0 && K >= 0 && K % 32 == 0, CHADQ_ERR_SHAPE, "chadq_dequant_mxfp4: rows=%lld K=%d (K %% 32 != 0?)", (long long)rows, K);
+    CHADQ_REQUIRE(K == 0 || rows <= INT64_MAX / 16 / K, CHADQ_ERR_SHAPE, "chadq_dequant_mxfp4: rows=%lld K=%d are too many values", (long long)rows, K);
+    if (rows == 0 || K == 0) return 0;
+    CHADQ_REQUIRE(codes && scale && w, CHADQ_ERR_NULL, "chadq_dequant_mxfp4: null pointer");
+    CHADQ_REQUIRE(aligned16(w) && (reinterpret_cast<uintptr_t>(codes) & 3) == 0, CHADQ_ERR_ALIGN, "chadq_dequant_mxfp4: w must be 16-byte, codes 4-byte aligned");
+    return dequant_mxfp4_launch(codes, scale, w, rows, K, st);
+}
+
+size_t chadq_product_mxfp4_workspace_bytes(int M, int N, int K, int x_mxfp4) {
+    return M > 0 && N > 0 && K >= 32 && K % 32 == 0 ? mx_product_workspace_bytes(M, N, K, x_mxfp4 != 0) : 0;
+}
+
+int chadq_product_mxfp4(const void *x, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, void *y, int y_bf16, int M, int N, int K,
+                        void *workspace, size_t workspace_bytes, void *stream) {
+    ENTER();
+    CHADQ_REQUIRE(M >= 0 && N >= 0 && K >= 32 && K % 32 == 0, CHADQ_ERR_SHAPE, "chadq_product_mxfp4: M=%d N=%d K=%d (K must be a positive multiple of 32)", M, N, K);
+    if (M == 0 || N == 0) return 0;
+    CHADQ_REQUIRE(x && w && w_scale && y, CHADQ_ERR_NULL, "chadq_product_mxfp4: null pointer");
+    CHADQ_REQUIRE(aligned16(x) && aligned16(w) && aligned16(workspace), CHADQ_ERR_ALIGN, "chadq_product_mxfp4: x, w and workspace must be 16-byte aligned");
+    const MxProduct p = {x, x_scale, w, w_scale, y, nullptr, M, N, K, 1, y_bf16 != 0, false};
+    return mx_product_launch(p, workspace, workspace ? workspace_bytes : 0, st);
+}
+
+int chadq_product_mxfp4_grouped(const void *x, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const int32_t *offsets,
+                                uint16_t *y_bf16, int M, int E, int N, int K, int clear_rest, void *stream) {
+    ENTER();
+    CHADQ_REQUIRE(M >= 0 && E >= 1 && N >= 0 && K >= 32 && K % 32 == 0, CHADQ_ERR_SHAPE,
+                  "chadq_product_mxfp4_grouped: M=%d E=%d N=%d K=%d (E at least 1, K a positive multiple of 32)", M, E, N, K);
+    if (M == 0 || N == 0) return 0;
+    CHADQ_REQUIRE(x && w && w_scale && offsets && y_bf16, CHADQ_ERR_NULL, "chadq_product_mxfp4_grouped: null pointer");
+    CHADQ_REQUIRE(aligned16(x) && aligned16(w), CHADQ_ERR_ALIGN, "chadq_product_mxfp4_grouped: x and w must be 16-byte aligned");
+    CHADQ_REQUIRE((reinterpret_cast<uintptr_t>(offsets) & 3) == 0, CHADQ_ERR_ALIGN, "chadq_product_mxfp4_grouped: offsets must be 4-byte aligned");
+    const MxProduct p = {x, x_scale, w, w_scale, y_bf16, offsets, M, N, K, E, true, clear_rest != 0};
+    return mx_product_launch(p, nullptr, 0, st);
 }
 
 }  // extern "C"

@@ -1,0 +1,99 @@
+// Microscaled 4-bit floating point (MXFP4): what its kernels share.
+//   codes  e2m1: sign in bit 3, then 0, 0.5, 1, 1.5, 2, 3, 4, 6; two to a byte, even k in the low nibble
+//   scales e8m0: one byte e per 32 codes along K, 2^(e - 127); 255: the block is NaN
+// The conversions of this machine read the exponent field of a scale given as a float: e << 23 serves for every byte (0 reads
+// as 2^-127, 255 as NaN; all 256 bytes x 16 codes checked).
+#pragma once
+#include "chadq_common.h"
+
+namespace chadq {
+
+typedef __attribute__((ext_vector_type(8))) int32_t i32x8;
+
+__device__ __forceinline__ float mx_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// 8 codes (one word) -> 8 bf16 in k order, times the block's scale: exact, one instruction per pair
+__device__ __forceinline__ bf16x8 dequant8_mx(uint32_t w, float s) {
+    const u32x4 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3))};
+    bf16x8 o;
+    __builtin_memcpy(&o, &r, 16);
+    return o;
+}
+
+// 32 codes as the operand of a scaled MFMA (fp4 takes the lower half of its eight registers)
+__device__ __forceinline__ i32x8 mx_operand(u32x4 v) { return i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0}; }
+
+// y[r, n] = sum_k x[r, k] w[g(r), n, k] for the rows r of group g(r) = the g with offsets[g] <= r < offsets[g + 1]
+struct MxProduct {
+    const void *x;            // bf16 [M,K], or codes [M,K/2]
+    const uint8_t *xs;        // scales of the codes [M,K/32]
+    const uint8_t *w, *ws;    // codes [E,N,K/2], scales [E,N,K/32]
+    void *y;                  // fp32 or bf16 [M,N]
+    const int32_t *offsets;   // [E+1] on the device, or null: one group, all rows
+    int M, N, K, E;
+    bool y_bf16, clear_rest;  // clear_rest: rows of no group become 0 (else they are left as they are)
+};
+
+// Row tile t of the groups, TR rows to a tile, a group's last one cut: which group, its first row, how many.  For t past the last
+// tile: group -1, and the rows of no group (in front of offsets[0], behind offsets[E]) that are this tile's to clear.
+// Offsets are taken as clamped into [0, M] and never descending (one that descends counts as the largest before it), so that no
+// contents of theirs lead outside x and y.  Every lane of a wave calls this; the answer is uniform.
+struct MxTile {
+    int group, row0, rows, rest0, rest1;  // rest: rest0 rows from 0 on and the rows from rest1 on
+};
+__device__ __forceinline__ MxTile mx_find_tile(const int32_t *__restrict__ offsets, int E, int M, int TR, int t) {
+    const int lane = threadIdx.x & 63;
+    int before = 0, low = 0, first = 0;  // tiles, largest offset so far
+    for (int c = 0; c < E; c += 64) {
+        const int e = c + lane;
+        auto at = [&](int i) {
+            const int o = offsets[i < E ? i : E];
+            return o < 0 ? 0 : o > M ? M : o;
+        };
+        int lo = at(e);
+        const int next = at(e + 1);
+        lo = lo > low ? lo : low;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(lo, d);
+            if (lane >= d) lo = lo > o ? lo : o;
+        }
+        const int hi = next > lo ? next : lo;
+        int upto = e < E ? (hi - lo + TR - 1) / TR : 0;
+        const int mine = upto;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(upto, d);
+            if (lane >= d) upto += o;
+        }
+        if (c == 0) first = __shfl(lo, 0);
+        const unsigned long long m = __ballot(t < before + upto);
+        if (m) {
+            const int l = __ffsll((long long)m) - 1;
+            const int k = t - before - (__shfl(upto, l) - __shfl(mine, l)), r0 = __shfl(lo, l) + k * TR, end = __shfl(hi, l);
+            return {__builtin_amdgcn_readfirstlane(c + l), __builtin_amdgcn_readfirstlane(r0),
+                    __builtin_amdgcn_readfirstlane(end - r0 < TR ? end - r0 : TR), 0, 0};
+        }
+        before += __shfl(upto, 63);
+        low = __shfl(hi, 63);
+    }
+    const int rest = first + (M - low), r0 = (t - before) * TR;
+    return {-1, __builtin_amdgcn_readfirstlane(r0), __builtin_amdgcn_readfirstlane(rest - r0 < 0 ? 0 : rest - r0 < TR ? rest - r0 : TR),
+            __builtin_amdgcn_readfirstlane(first), __builtin_amdgcn_readfirstlane(low)};
+}
+// Row tiles that suffice for any offsets, those that clear included: full tiles of M rows, one cut per group that can have a row, one of the rest.
+inline int64_t mx_most_tiles(int M, int E, int TR) { return (int64_t)M / TR + (E < M ? E : M) + 2; }
+
+// The columns n0 .. n0 + cols of the tile's rows of no group, set to 0 by the workgroup's threads
+__device__ __forceinline__ void mx_clear(const MxProduct &p, const MxTile &t, int n0, int cols) {
+    const int width = p.N - n0 < cols ? p.N - n0 : cols;
+    for (int i = threadIdx.x; i < t.rows * width; i += blockDim.x) {
+        const int k = t.row0 + i / width, r = k < t.rest0 ? k : t.rest1 + (k - t.rest0);
+        store_sum(reinterpret_cast<float *>(p.y), (size_t)r * p.N + n0 + i % width, 0.f, p.y_bf16);
+    }
+}
+
+}  // namespace chadq

@@ -1,0 +1,106 @@
+// MXFP4: quantisation and its inverse.  Per block of 32 values along K:  e = clamp(floor(log2 max|x|) - 2 + 127, 0, 254),
+// code = the nearest e2m1 to x / 2^(e - 127), ties to the even one, what lies beyond 6 to 6; a block that holds a NaN or an
+// infinity gets e = 255 and codes of 0.  The division by a power of two is exact, so there is nothing to round but the code.
+#include "mx.h"
+
+namespace chadq {
+
+// the bits of 8 consecutive values as fp32
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, float f[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float *p, float f[8]) {
+    const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[i] = a[i];
+        f[4 + i] = b[i];
+    }
+}
+template <>
+__device__ __forceinline__ void load8<__bf16>(const __bf16 *p, float f[8]) {
+    const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(v[i] << 16);
+        f[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
+    }
+}
+template <>
+__device__ __forceinline__ void load8<_Float16>(const _Float16 *p, float f[8]) {
+    const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f16x2 h = as_f16x2(v[i]);
+        f[2 * i] = (float)h.x;
+        f[2 * i + 1] = (float)h.y;
+    }
+}
+
+// Four lanes to a block, 8 values to a lane; rows do not matter, K is a multiple of 32.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const T *__restrict__ x, uint32_t *__restrict__ codes, uint8_t *__restrict__ scale,
+                                                             int64_t n8) {
+    const int64_t stride = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += stride) {  // n8 is a multiple of 4: quads stay whole
+        float f[8];
+        load8<T>(x + i * 8, f);
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t b = __float_as_uint(f[j]) & 0x7FFFFFFFu;  // as integers: a NaN is larger than infinity
+            m = b > m ? b : m;
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const uint32_t o = (uint32_t)(s ? __builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false)    // quad_perm [2,3,0,1]
+                                            : __builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));  // quad_perm [1,0,3,2]
+            m = o > m ? o : m;
+        }
+        const uint32_t e = m >> 23, byte = e == 255 ? 255 : e > 2 ? e - 2 : 0;
+        const float s = mx_scale(byte);
+        uint32_t c = 0;
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[0], f[1], s, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2], f[3], s, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[4], f[5], s, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[6], f[7], s, 3);
+        codes[i] = byte == 255 ? 0u : c;
+        if ((i & 3) == 0) scale[i >> 2] = (uint8_t)byte;
+    }
+}
+
+// w[i] = value(code i) * scale of its block as fp32, exact (beyond fp32's range: infinity); 8 codes to a lane
+__global__ __launch_bounds__(256) void dequant_mxfp4_kernel(const uint32_t *__restrict__ codes, const uint8_t *__restrict__ scale,
+                                                            float *__restrict__ w, int64_t n8) {
+    const int64_t stride = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += stride) {
+        const uint32_t c = codes[i];
+        const float s = mx_scale(scale[i >> 2]);
+        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
+        const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
+        reinterpret_cast<f32x4 *>(w)[2 * i] = f32x4{a.x, a.y, b.x, b.y};
+        reinterpret_cast<f32x4 *>(w)[2 * i + 1] = f32x4{d.x, d.y, e.x, e.y};
+    }
+}
+
+static int grid_for(int64_t items) {
+    const int64_t b = (items + 255) / 256;
+    return b < 1 ? 1 : b > 256 * 32 ? 256 * 32 : (int)b;
+}
+
+int quantize_mxfp4_launch(const void *x, int dtype, uint8_t *codes, uint8_t *scale, int64_t rows, int K, hipStream_t st) {
+    const int64_t n8 = rows * (K / 8);
+    uint32_t *const c = reinterpret_cast<uint32_t *>(codes);
+    if (dtype == CHADQ_F32) hipLaunchKernelGGL(quantize_mxfp4_kernel<float>, dim3(grid_for(n8)), dim3(256), 0, st, reinterpret_cast<const float *>(x), c, scale, n8);
+    else if (dtype == CHADQ_BF16) hipLaunchKernelGGL(quantize_mxfp4_kernel<__bf16>, dim3(grid_for(n8)), dim3(256), 0, st, reinterpret_cast<const __bf16 *>(x), c, scale, n8);
+    else hipLaunchKernelGGL(quantize_mxfp4_kernel<_Float16>, dim3(grid_for(n8)), dim3(256), 0, st, reinterpret_cast<const _Float16 *>(x), c, scale, n8);
+    return hip_check(hipGetLastError(), "quantize_mxfp4 launch");
+}
+
+int dequant_mxfp4_launch(const uint8_t *codes, const uint8_t *scale, float *w, int64_t rows, int K, hipStream_t st) {
+    const int64_t n8 = rows * (K / 8);
+    hipLaunchKernelGGL(dequant_mxfp4_kernel, dim3(grid_for(n8)), dim3(256), 0, st, reinterpret_cast<const uint32_t *>(codes), scale, w, n8);
+    return hip_check(hipGetLastError(), "dequant_mxfp4 launch");
+}
+
+}  // namespace chadq

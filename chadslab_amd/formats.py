@@ -9,6 +9,11 @@ Layouts (this build's choices; the benchmark text fixes only "2 per byte", "grou
                   scale  fp16  [N, K/32]                    value = (u - 8) * scale[n, k // 32]
   QWeightInt4G32Tiles  the same bytes regrouped into contiguous tiles for the mixture-of-experts kernel (a load-time
                   repack on the device; the row-major form stays the interchange format)
+  QWeightMXFP4    packed uint8 [N, K/2]  row-major          byte j of a row = c[2j] | (c[2j+1] << 4), c an e2m1 code: sign << 3 | m,
+                                                            values 0, 0.5, 1, 1.5, 2, 3, 4, 6
+                  scale  uint8 [N, K/32]                    value(c) * 2^(scale[n, k // 32] - 127); 255: the block is NaN
+                  (microscaled 4-bit floating point; the same container holds quantised activations)
+  QExpertsMXFP4   the same for E matrices of one shape: packed [E, N, K/2], scale [E, N, K/32]
 
 The tensors live wherever the caller puts them; the operators in chadslab_amd.ops want them on the GPU.
 Quantising and packing are load-time tools, not the hot path, and are written with torch tensor ops.
@@ -94,6 +99,65 @@ class QWeightInt4G32Tiles:
     @property
     def K(self) -> int:
         return self.packed.size(1) * 2
+
+
+def _check_mxfp4(name: str, packed: torch.Tensor, scale: torch.Tensor, dim: int) -> None:
+    lead = "E,N" if dim == 3 else "N"
+    if packed.dtype != torch.uint8 or packed.dim() != dim:
+        raise ValueError("%s.packed must be uint8 [%s,K/2]" % (name, lead))
+    if packed.shape[-1] * 2 % GROUP:
+        raise ValueError("K must be a multiple of 32")
+    if scale.dtype != torch.uint8 or scale.shape != (*packed.shape[:-1], packed.shape[-1] * 2 // GROUP):
+        raise ValueError("%s.scale must be uint8 [%s,K/32]" % (name, lead))
+
+
+@dataclass
+class QWeightMXFP4:
+    packed: torch.Tensor  # uint8 [N, K/2]
+    scale: torch.Tensor   # uint8 [N, K/32]
+
+    def __post_init__(self):
+        _check_mxfp4("QWeightMXFP4", self.packed, self.scale, 2)
+
+    @property
+    def N(self) -> int:
+        return self.packed.size(0)
+
+    @property
+    def K(self) -> int:
+        return self.packed.size(1) * 2
+
+    def to(self, device) -> "QWeightMXFP4":
+        return QWeightMXFP4(self.packed.to(device).contiguous(), self.scale.to(device).contiguous())
+
+
+@dataclass
+class QExpertsMXFP4:
+    """E matrices of one shape in MXFP4, one behind the other: what ops.qgemm_grouped and ops.moe_ffn take."""
+    packed: torch.Tensor  # uint8 [E, N, K/2]
+    scale: torch.Tensor   # uint8 [E, N, K/32]
+
+    def __post_init__(self):
+        _check_mxfp4("QExpertsMXFP4", self.packed, self.scale, 3)
+
+    @property
+    def E(self) -> int:
+        return self.packed.size(0)
+
+    @property
+    def N(self) -> int:
+        return self.packed.size(1)
+
+    @property
+    def K(self) -> int:
+        return self.packed.size(2) * 2
+
+    def expert(self, e: int) -> QWeightMXFP4:
+        """Matrix e (the same memory)."""
+        return QWeightMXFP4(self.packed[e], self.scale[e])
+
+    def to(self, device) -> "QExpertsMXFP4":
+        return QExpertsMXFP4(self.packed.to(device).contiguous(), self.scale.to(device).contiguous())
 
 
 def pack_int4(q: torch.Tensor) -> torch.Tensor:

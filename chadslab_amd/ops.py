@@ -11,9 +11,9 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .formats import QWeightInt4G32, QWeightInt4G32Tiles, QWeightInt8
+from .formats import GROUP, QExpertsMXFP4, QWeightInt4G32, QWeightInt4G32Tiles, QWeightInt8, QWeightMXFP4
 
-QWeight = Union[QWeightInt4G32, QWeightInt8]
+QWeight = Union[QWeightInt4G32, QWeightInt8, QWeightMXFP4]
 GEMV_MAX_M = 16  # decode batch sizes served by the bandwidth kernel
 
 
@@ -60,9 +60,55 @@ def pack_int4(q: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def dequantize(qw: QWeight) -> torch.Tensor:
-    """fp32 [N,K] dequantised weights (exact)."""
+def _launch(device: torch.device, name: str, *args) -> None:
+    """Library call `name` on the current stream of `device`, whichever device is current."""
+    fn = getattr(_lib.load(), name)
+    if device.index == torch._C._cuda_getDevice():
+        _lib.check(fn(*args, _stream()), name)
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, _stream()), name)
+
+
+def _mxfp4(q: Union[QWeightMXFP4, QExpertsMXFP4], name: str, device: Optional[torch.device] = None):
+    """Codes and scales of a container, checked before their addresses go to the library."""
+    p, s = _dev(q.packed, name + ".packed", torch.uint8), _dev(q.scale, name + ".scale", torch.uint8)
+    for t in (p, s):
+        if t.device != (p.device if device is None else device):
+            raise ValueError("%s must live on %s, got %s" % (name, p.device if device is None else device, t.device))
+    return p, s
+
+
+_MX_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # chadq_dtype
+
+
+def quantize_mxfp4(x: torch.Tensor) -> Union[QWeightMXFP4, QExpertsMXFP4]:
+    """fp32, bf16 or fp16 [R,K] -> QWeightMXFP4, [E,N,K] -> QExpertsMXFP4; K a multiple of 32.
+
+    Per block of 32 values along K the scale is 2^(floor(log2(largest magnitude)) - 2), at least 2^-127; each value goes to the nearest code,
+    ties to the even one, beyond 6 scales to 6.  A block that holds a NaN or an infinity becomes NaN."""
+    if x.dtype not in _MX_TYPES:
+        raise ValueError("x must be float32, bfloat16 or float16, got %s" % x.dtype)
+    if x.dim() not in (2, 3) or x.size(-1) % GROUP:
+        raise ValueError("x must be [R,K] or [E,N,K] with K a multiple of 32, got %s" % (tuple(x.shape),))
+    x = _dev(x, "x", x.dtype)
+    *lead, k = x.shape
+    p = torch.empty(*lead, k // 2, dtype=torch.uint8, device=x.device)
+    s = torch.empty(*lead, k // GROUP, dtype=torch.uint8, device=x.device)
+    if x.numel():
+        _launch(x.device, "chadq_quantize_mxfp4", x.data_ptr(), _MX_TYPES[x.dtype], p.data_ptr(), s.data_ptr(), x.numel() // k, k)
+    return QWeightMXFP4(p, s) if len(lead) == 1 else QExpertsMXFP4(p, s)
+
+
+def dequantize(qw: Union[QWeight, QExpertsMXFP4]) -> torch.Tensor:
+    """fp32 [N,K] dequantised weights (exact); [E,N,K] of QExpertsMXFP4."""
     lib = _lib.load()
+    if isinstance(qw, (QWeightMXFP4, QExpertsMXFP4)):
+        p, s = _mxfp4(qw, "qw")
+        out = torch.empty(*p.shape[:-1], qw.K, dtype=torch.float32, device=p.device)
+        if out.numel():
+            _launch(p.device, "chadq_dequant_mxfp4", p.data_ptr(), s.data_ptr(), out.data_ptr(), out.numel() // qw.K, qw.K)
+        return out
     if isinstance(qw, QWeightInt4G32):
         p, s = _dev(qw.packed, "packed", torch.uint8), _dev(qw.scale, "scale", torch.float16)
         out = torch.empty(qw.N, qw.K, dtype=torch.float32, device=p.device)
@@ -78,8 +124,71 @@ def dequantize(qw: QWeight) -> torch.Tensor:
     raise TypeError("unknown weight container %r" % type(qw))
 
 
-def qgemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor] = None, *, fp32_elements: bool = False) -> torch.Tensor:
-    """Decode product, fp32 out [M,N], M <= 16.  x is bf16 [M,K] for int4 weights, fp32 [M,K] for int8 weights.
+def _product_mxfp4(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeightMXFP4, out: Optional[torch.Tensor], y_dtype: torch.dtype) -> torch.Tensor:
+    """x (bf16 or MXFP4) [M,K] times MXFP4 weights -> fp32 or bf16 [M,N]."""
+    x_mx = isinstance(x, QWeightMXFP4)
+    if (not x_mx and x.dim() != 2) or (x.K if x_mx else x.size(1)) != qw.K:
+        raise ValueError("x must be [M,%d], got %s" % (qw.K, (x.N, x.K) if x_mx else tuple(x.shape)))
+    if x_mx:
+        xt, xs = _mxfp4(x, "x")
+        xs_ptr = xs.data_ptr()
+    else:
+        xt, xs_ptr = _dev(x, "x", torch.bfloat16), None
+    p, s = _mxfp4(qw, "weights", xt.device)
+    m, n, k = xt.size(0), qw.N, qw.K
+    y = _out(out, (m, n), y_dtype, xt.device)
+    if m == 0 or n == 0:
+        return y
+    if k == 0:
+        return y.zero_()
+    need = _lib.load().chadq_product_mxfp4_workspace_bytes(m, n, k, int(x_mx))
+    ws = torch.empty(need, dtype=torch.uint8, device=xt.device) if need else None  # a fresh one per call, as moe_ffn's
+    _launch(xt.device, "chadq_product_mxfp4", xt.data_ptr(), xs_ptr, p.data_ptr(), s.data_ptr(), y.data_ptr(), int(y_dtype == torch.bfloat16), m, n, k,
+            ws.data_ptr() if need else None, need)
+    return y
+
+
+def _no_mxfp4(x, qw) -> None:
+    if isinstance(x, QWeightMXFP4):
+        raise TypeError("MXFP4 activations go with MXFP4 weights, got %r" % type(qw))
+
+
+def qgemm_grouped(x: Union[torch.Tensor, QWeightMXFP4], experts: QExpertsMXFP4, offsets: torch.Tensor,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rows sorted by expert, each group times its own matrix: y[r] = x[r] @ dequant(experts[e]).T for offsets[e] <= r < offsets[e+1].
+
+    x bf16 [R,K] or QWeightMXFP4 of R rows; offsets int32 [E+1] on the GPU, read there (groups of any size, empty ones too, no host round trip); y bf16
+    [R,N], fp32 sums.  Rows in front of offsets[0] and behind offsets[E] are 0 in a fresh result and left as they are in `out`.  Offsets beyond [0, R] count as its ends, one
+    that descends as the largest before it."""
+    x_mx = isinstance(x, QWeightMXFP4)
+    if not isinstance(experts, QExpertsMXFP4):
+        raise TypeError("qgemm_grouped wants QExpertsMXFP4, got %r" % type(experts))
+    e, n, k = experts.E, experts.N, experts.K
+    if (not x_mx and x.dim() != 2) or (x.K if x_mx else x.size(1)) != k:
+        raise ValueError("x must be [R,%d], got %s" % (k, (x.N, x.K) if x_mx else tuple(x.shape)))
+    if x_mx:
+        xt, xs = _mxfp4(x, "x")
+        xs_ptr = xs.data_ptr()
+    else:
+        xt, xs_ptr = _dev(x, "x", torch.bfloat16), None
+    p, s = _mxfp4(experts, "experts", xt.device)
+    offsets = _dev(offsets, "offsets", torch.int32)
+    if e < 1 or tuple(offsets.shape) != (e + 1,) or offsets.device != xt.device:
+        raise ValueError("offsets must be int32 [%d] on %s, one more than there are experts (at least one), got %s on %s"
+                         % (e + 1, xt.device, tuple(offsets.shape), offsets.device))
+    y = _out(out, (xt.size(0), n), torch.bfloat16, xt.device)
+    if y.numel() == 0:
+        return y
+    if k == 0:
+        raise ValueError("K must be at least 32")
+    _launch(xt.device, "chadq_product_mxfp4_grouped", xt.data_ptr(), xs_ptr, p.data_ptr(), s.data_ptr(), offsets.data_ptr(), y.data_ptr(), xt.size(0), e, n, k,
+            int(out is None))
+    return y
+
+
+def qgemv(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, out: Optional[torch.Tensor] = None, *, fp32_elements: bool = False) -> torch.Tensor:
+    """Decode product, fp32 out [M,N], M <= 16.  x is bf16 [M,K] for int4 weights, fp32 [M,K] for int8 weights, bf16 [M,K] or
+    QWeightMXFP4 for MXFP4 weights.
 
     fp32_elements (int8 weights only): fp32 arithmetic on every activation (chadq_gemv_i8row_fp32) instead of the
     matrix-core kernel's per-block fixed point, whose error on a small activation grows with the largest one of its
@@ -91,6 +200,14 @@ def _gemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor], fp32_elemen
     """qgemv with the sums as fp32 or, bf16_out, rounded to bf16 by the kernel that forms them."""
     lib = _lib.load()
     y_dtype = torch.bfloat16 if bf16_out else torch.float32
+    if isinstance(qw, QWeightMXFP4):
+        if fp32_elements:
+            raise ValueError("fp32_elements applies to int8 weights (fp32 activations) only")
+        m = x.N if isinstance(x, QWeightMXFP4) else x.size(0) if x.dim() == 2 else 0
+        if m > GEMV_MAX_M:
+            raise ValueError("qgemv takes at most %d rows, got %d" % (GEMV_MAX_M, m))
+        return _product_mxfp4(x, qw, out, y_dtype)
+    _no_mxfp4(x, qw)
     n, k = qw.N, qw.K
     if x.dim() != 2 or x.size(1) != k:
         raise ValueError("x must be [M,%d], got %s" % (k, tuple(x.shape)))
@@ -126,9 +243,12 @@ def _gemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor], fp32_elemen
     raise TypeError("unknown weight container %r" % type(qw))
 
 
-def qgemm(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Prefill product on the matrix cores: x bf16 [M,K] -> bf16 [M,N], fp32 accumulate."""
+def qgemm(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Prefill product on the matrix cores: x bf16 [M,K], or QWeightMXFP4 for MXFP4 weights, -> bf16 [M,N], fp32 accumulate."""
     lib = _lib.load()
+    if isinstance(qw, QWeightMXFP4):
+        return _product_mxfp4(x, qw, out, torch.bfloat16)
+    _no_mxfp4(x, qw)
     n, k = qw.N, qw.K
     if x.dim() != 2 or x.size(1) != k:
         raise ValueError("x must be [M,%d], got %s" % (k, tuple(x.shape)))
@@ -159,13 +279,16 @@ def qgemm(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor] = None) -> t
     raise TypeError("unknown weight container %r" % type(qw))
 
 
-def qlinear(x: torch.Tensor, qw: QWeight, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+def qlinear(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y = x @ dequant(W).T over the last axis of x.
 
     Up to 16 rows go to the bandwidth-bound GEMV (fp32 result); more rows go to the MFMA GEMM (bf16 result).
     out_dtype picks the result type.  The GEMV writes bf16 itself if that is asked for (the same sums rounded once); any
-    other type than the kernel's native one is a cast.
+    other type than the kernel's native one is a cast.  x may be a QWeightMXFP4 where the weights are.
     """
+    if isinstance(x, QWeightMXFP4):
+        y = _qlinear_2d(x, qw, out_dtype if out_dtype == torch.bfloat16 else None)
+        return y if out_dtype is None or y.dtype == out_dtype else y.to(out_dtype)
     native = _lib.native()
     y = native.linear(x, qw, out_dtype)
     if y is not None:
@@ -184,6 +307,10 @@ def qlinear(x: torch.Tensor, qw: QWeight, *, out_dtype: Optional[torch.dtype] = 
 
 def _qlinear_2d(x2: torch.Tensor, qw: QWeight, written: Optional[torch.dtype]) -> torch.Tensor:
     """What the native call leaves: misplaced or strided weights, other types, everything that raises."""
+    if isinstance(qw, QWeightMXFP4):  # (no rows at all: an empty result, of the type that few rows have)
+        few = (x2.N if isinstance(x2, QWeightMXFP4) else x2.size(0)) <= GEMV_MAX_M
+        return _product_mxfp4(x2, qw, None, torch.float32 if few and written is None else torch.bfloat16)
+    _no_mxfp4(x2, qw)
     m = x2.size(0)
     use_gemv = m <= GEMV_MAX_M and not (isinstance(qw, QWeightInt8) and x2.dtype == torch.bfloat16)
     if isinstance(qw, QWeightInt8) and x2.dtype == torch.float32 and not use_gemv:

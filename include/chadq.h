@@ -26,6 +26,7 @@
  *      int8 per-row : W int8 [N,K] row-major, scale fp32 [N];  w = W[n,k] * scale[n]
  *      int4 group-32: Wp uint8 [N,K/2] row-major, byte j of a row = (u[2j]) | (u[2j+1] << 4),
  *                     u = q + 8 in [0,15]; scale fp16 [N,K/32]; w = (u - 8) * scale[n,k/32]
+ *      MXFP4        : codes uint8 [N,K/2] row-major, e2m1, even k in the low nibble; scale uint8 [N,K/32], 2^(byte - 127)
  *      bf16 / fp16 values travel as uint16_t bit patterns.
  */
 #ifndef CHADQ_H
@@ -403,6 +404,44 @@ size_t chadq_prompt_i4g32_workspace_bytes(int T, int d, int hq, int dh, int ffn)
 int chadq_prompt_i4g32(const chadq_prompt_layer_i4g32 *layers, int n_layers, const int32_t *tokens, const uint8_t *emb,
                        const uint16_t *semb, int V, const float *rope_table, int T, int pos, int d, int hq, int dh, int ffn,
                        int max_ctx, float eps, float *x_last, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- microscaled 4-bit floating point (MXFP4) ------------------------------------------- */
+
+/*
+ * Format: codes uint8 [N,K/2] row-major, two to a byte, the even k in the low nibble; a code
+ * is sign << 3 | m with the values 0, 0.5, 1, 1.5, 2, 3, 4, 6; scale uint8 [N,K/32], byte e: 2^(e - 127), 255: the block is NaN.
+ * K % 32 == 0.  The same arrays hold weights and activations.
+ */
+typedef enum chadq_dtype { CHADQ_F32 = 0, CHADQ_BF16 = 1, CHADQ_F16 = 2 } chadq_dtype;
+
+/*
+ * x [rows,K] of the given type -> codes and scales: e = clamp(floor(log2 max|x|) - 2 + 127, 0, 254) per block, the nearest code of
+ * x / 2^(e - 127), ties to the even one, beyond 6 to 6 (signs kept, of zeros too).  A block with a NaN or an infinity: e = 255, codes 0.
+ * x 16-byte, codes 4-byte aligned.
+ */
+int chadq_quantize_mxfp4(const void *x, int dtype, uint8_t *codes, uint8_t *scale, int64_t rows, int K, void *stream);
+
+/* fp32 [rows,K] of codes and scales, exact (beyond fp32's range: infinity).  w 16-byte, codes 4-byte aligned. */
+int chadq_dequant_mxfp4(const uint8_t *codes, const uint8_t *scale, float *w, int64_t rows, int K, void *stream);
+
+/*
+ * y[m,n] = sum_k x[m,k] w[n,k], fp32 sums, y fp32 or (y_bf16) the same rounded once.  x_scale NULL: x is bf16 [M,K], multiplied as it is;
+ * else x holds the codes [M,K/2] of MXFP4 activations.  Any M, N >= 0; K a positive multiple of 32; x and codes 16-byte aligned.
+ * A NaN block of w makes column n NaN, one of x row m.  workspace: chadq_product_mxfp4_workspace_bytes bytes (16-byte aligned; 0: none needed), for the
+ * sums of parts of K where that is the quicker form; without it (NULL or fewer bytes) the product is one part.
+ */
+size_t chadq_product_mxfp4_workspace_bytes(int M, int N, int K, int x_mxfp4);
+int chadq_product_mxfp4(const void *x, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, void *y, int y_bf16, int M, int N, int K,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The same for rows sorted by group, each group times its own matrix: w [E,N,K/2], w_scale [E,N,K/32], offsets int32 [E+1] on the device;
+ * rows offsets[e] .. offsets[e+1] - 1 of x and y belong to group e.  Groups may be empty.  Rows of no group (in front of offsets[0], behind
+ * offsets[E]) become 0 where clear_rest is set and are left as they are otherwise.  Offsets are taken as clamped into [0, M], one that descends as the
+ * largest before it.  y bf16 [M,N].  E >= 1.
+ */
+int chadq_product_mxfp4_grouped(const void *x, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const int32_t *offsets,
+                                uint16_t *y_bf16, int M, int E, int N, int K, int clear_rest, void *stream);
 
 #ifdef __cplusplus
 }

@@ -271,6 +271,38 @@ def quantize_int8_row(w: np.ndarray):
     return q, s
 
 
+MX_VALUES = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def quantize_mxfp4(x: np.ndarray):
+    """Floats [R,K] -> (codes uint8 [R,K/2], scale bytes uint8 [R,K/32]).  Scale exponent floor(log2(max|x|)) - 2, at least -127; the
+    nearest code, ties to the even one, beyond 6 to 6; a block with a NaN or an infinity: byte 255, codes 0."""
+    x = np.asarray(x, dtype=np.float64)
+    r, k = x.shape
+    g = x.reshape(r, k // 32, 32)
+    bad = ~np.isfinite(g).all(axis=2)
+    g = np.where(bad[:, :, None], 0.0, g)
+    amax = np.abs(g).max(axis=2)
+    e = np.clip(np.frexp(np.where(amax > 0, amax, 2.0 ** -149))[1] - 1 - 2, -127, 127)
+    v = np.ldexp(g, -e[:, :, None])
+    a = np.abs(v)
+    off = np.abs(a[..., None] - MX_VALUES)  # ties: of two codes next to each other one is even
+    best = off.min(axis=-1, keepdims=True)
+    even_first = np.argsort(np.arange(8) % 2, kind="stable")
+    c = even_first[np.argmax((off == best)[..., even_first], axis=-1)].astype(np.uint8)
+    c = np.where(a >= 6, 7, c) | (np.signbit(v).astype(np.uint8) << 3)
+    c = np.where(bad[:, :, None], 0, c).astype(np.uint8).reshape(r, k)
+    return (c[:, 0::2] | (c[:, 1::2] << 4)).astype(np.uint8), np.where(bad, 255, e + 127).astype(np.uint8)
+
+
+def dequant_mxfp4(codes: np.ndarray, scale: np.ndarray) -> np.ndarray:
+    """float64 [..,K] of codes uint8 [..,K/2] and scale bytes [..,K/32]."""
+    c = np.stack((codes & 15, codes >> 4), axis=-1).reshape(*codes.shape[:-1], -1)
+    v = np.where(c & 8, -1.0, 1.0) * MX_VALUES[c & 7]
+    s = np.where(scale == 255, np.nan, np.ldexp(1.0, scale.astype(np.int32) - 127))
+    return v * np.repeat(s, 32, axis=-1)
+
+
 def rel_l2(a: np.ndarray, ref: np.ndarray) -> float:
     a = np.asarray(a, dtype=np.float64)
     ref = np.asarray(ref, dtype=np.float64)
