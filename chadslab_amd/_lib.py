@@ -77,6 +77,8 @@ SIGNATURES = {
     "chadq_product_mxfp4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "chadq_product_mxfp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "chadq_product_mxfp4_grouped": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "chadq_moe_ffn_mxfp4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "chadq_moe_ffn_mxfp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "chadq_sample_topk_f32": (c_int, [c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
 }
 
@@ -84,6 +86,11 @@ SIGNATURES = {
 class MoeExpertI4G32(ctypes.Structure):
     """Mirror of chadq_moe_expert_i4g32: six device pointers."""
     _fields_ = [(n, c_void_p) for n in ("wg", "sg", "wu", "su", "wd", "sd")]
+
+
+class MoeMXFP4(ctypes.Structure):
+    """Mirror of chadq_moe_mxfp4: six device pointers."""
+    _fields_ = [(n, c_void_p) for n in ("gate", "gate_scale", "up", "up_scale", "down", "down_scale")]
 
 
 class PromptLayerI4G32(ctypes.Structure):

@@ -108,8 +108,8 @@ int prompt_i4g32_launch(const chadq_prompt_layer_i4g32 *, int, const int32_t *, 
                         int, int, int, int, float, float *, void *, hipStream_t);
 int quantize_mxfp4_launch(const void *, int, uint8_t *, uint8_t *, int64_t, int, hipStream_t);
 int dequant_mxfp4_launch(const uint8_t *, const uint8_t *, float *, int64_t, int, hipStream_t);
-int mx_product_launch(const MxProduct &, void *, size_t, hipStream_t);
-size_t mx_product_workspace_bytes(int, int, int, bool);
+size_t moe_mxfp4_workspace_bytes(int, int, int, int, int);
+int moe_ffn_mxfp4_launch(const uint16_t *, const float *, const chadq_moe_mxfp4 *, uint16_t *, int, int, int, int, int, int, void *, hipStream_t);
 int sample_topk_launch(const float *, int, int, float, const float *, float *, int32_t *, int32_t *, int32_t *, int, hipStream_t);
 
 }  // namespace chadq
@@ -674,6 +674,31 @@ int chadq_product_mxfp4_grouped(const void *x, const uint8_t *x_scale, const uin
     CHADQ_REQUIRE((reinterpret_cast<uintptr_t>(offsets) & 3) == 0, CHADQ_ERR_ALIGN, "chadq_product_mxfp4_grouped: offsets must be 4-byte aligned");
     const MxProduct p = {x, x_scale, w, w_scale, y_bf16, offsets, M, N, K, E, true, clear_rest != 0};
     return mx_product_launch(p, nullptr, 0, st);
+}
+
+// (the rows of the products, T * top_k, are counted in 32 bits)
+static bool moe_mxfp4_sizes_ok(int T, int H, int F, int E, int top_k) {
+    return moe_sizes_ok(T, H, F, E, top_k) && (int64_t)T * top_k <= INT32_MAX;
+}
+
+size_t chadq_moe_ffn_mxfp4_workspace_bytes(int T, int H, int F, int E, int top_k) {
+    return moe_mxfp4_sizes_ok(T, H, F, E, top_k) ? moe_mxfp4_workspace_bytes(T, H, F, E, top_k) : 0;
+}
+
+int chadq_moe_ffn_mxfp4(const uint16_t *x_bf16, const float *logits, const chadq_moe_mxfp4 *experts, uint16_t *y_bf16, int T, int H, int F, int E, int top_k,
+                        int renorm, void *workspace, size_t workspace_bytes, void *stream) {
+    ENTER();
+    CHADQ_REQUIRE(moe_mxfp4_sizes_ok(T, H, F, E, top_k), CHADQ_ERR_SHAPE,
+                  "chadq_moe_ffn_mxfp4: T=%d H=%d F=%d E=%d top_k=%d (H, F multiples of 32; E <= 16; top_k <= min(E, 8))", T, H, F, E, top_k);
+    CHADQ_REQUIRE(x_bf16 && logits && experts && y_bf16 && experts->gate && experts->gate_scale && experts->up && experts->up_scale && experts->down &&
+                      experts->down_scale,
+                  CHADQ_ERR_NULL, "chadq_moe_ffn_mxfp4: null pointer");
+    const size_t need = moe_mxfp4_workspace_bytes(T, H, F, E, top_k);
+    CHADQ_REQUIRE(workspace && workspace_bytes >= need, CHADQ_ERR_WORKSPACE, "chadq_moe_ffn_mxfp4: workspace of %zu bytes needed, %zu given", need,
+                  workspace ? workspace_bytes : (size_t)0);
+    CHADQ_REQUIRE(aligned16(x_bf16) && aligned16(experts->gate) && aligned16(experts->up) && aligned16(experts->down) && aligned16(workspace) && aligned16(y_bf16),
+                  CHADQ_ERR_ALIGN, "chadq_moe_ffn_mxfp4: x, y, codes and workspace must be 16-byte aligned");
+    return moe_ffn_mxfp4_launch(x_bf16, logits, experts, y_bf16, T, H, F, E, top_k, renorm, workspace, st);
 }
 
 }  // extern "C"

@@ -13,6 +13,7 @@
 // the SiLU gate and the weighted combine.
 #include "chadq_common.h"
 #include "expert_prep.h"
+#include "mx.h"
 
 namespace chadq {
 
@@ -28,7 +29,7 @@ struct MoeWs {  // workspace carved up on the host
     float *w;            // [T,top_k] routing weight of each pair
     int32_t *pos;        // [P] row of the pair in expert-sorted order
     int32_t *tok;        // [P] token of the sorted row
-    int32_t *cnt;        // [E] rows per expert, then [E] offsets
+    int32_t *cnt;        // [E] rows per expert, then [E+1] offsets
     GemmGroup *groups;   // [3*E] gate, up, down
     int32_t *tiles;      // token tiles of the expert GEMMs: expert | tile << 16, -1 past the last one
     uint16_t *xs;        // [P,H] gathered activations (bf16)
@@ -204,7 +205,7 @@ __global__ __launch_bounds__(1024) void moe_route_kernel(const float *__restrict
         s_off[tid] = o;
         ws.cnt[tid] = s_base[tid];
         ws.cnt[E + tid] = o;
-        if (tid == E - 1) s_off[E] = o + s_base[tid];
+        if (tid == E - 1) s_off[E] = ws.cnt[2 * E] = o + s_base[tid];
     }
     __syncthreads();
     for (int p = tid; p < P; p += B) {
@@ -290,6 +291,7 @@ __global__ __launch_bounds__(64) void moe_route_few_kernel(const float *__restri
     if (lane < E) {
         ws.cnt[lane] = m;
         ws.cnt[E + lane] = o;
+        if (lane == E - 1) ws.cnt[2 * E] = o + m;
         ws.tiles[lane] = tile;
         gg.y = ws.g + (size_t)o * F;
         gu.y = ws.u + (size_t)o * F;
@@ -366,7 +368,7 @@ static size_t moe_layout(uint8_t *base, int T, int H, int F, int E, int top_k, M
     w.w = (float *)take(P * 4);
     w.pos = (int32_t *)take(P * 4);
     w.tok = (int32_t *)take(P * 4);
-    w.cnt = (int32_t *)take((size_t)2 * E * 4);
+    w.cnt = (int32_t *)take(((size_t)2 * E + 1) * 4);
     w.groups = (GemmGroup *)take((size_t)3 * E * sizeof(GemmGroup));
     w.tiles = (int32_t *)take(((size_t)E + P / 32 + 1) * 4);
     w.xs = (uint16_t *)take(P * H * 2);
@@ -492,6 +494,58 @@ int moe_ffn_i4g32_launch(const uint16_t *x, const float *logits, const chadq_moe
     hipLaunchKernelGGL(moe_combine_kernel, dim3(quads < 1024 * 256 ? (int)((quads + 255) / 256) : 1024), dim3(256), 0, st, ws.yp, ws.pos, ws.w, y, T, H, top_k, nsplit,
                        (size_t)P * H);
     return hip_check(hipGetLastError(), "moe act/combine launch");
+}
+
+// ---- the same on MXFP4 experts, E matrices of each kind one behind the other: router, gate and up with the SiLU gate in one product by
+// group that reads the activations through the sorted token list, down to fp32, combine.
+static size_t moe_mx_layout(uint8_t *base, int T, int H, int F, int E, int top_k, MoeWs *ws) {
+    const size_t P = (size_t)T * top_k;
+    size_t o = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t *p = base ? base + o : nullptr;
+        o += align_up(bytes);
+        return p;
+    };
+    MoeWs w = {};
+    w.idx = (int32_t *)take(P * 4);
+    w.w = (float *)take(P * 4);
+    w.pos = (int32_t *)take(P * 4);
+    w.tok = (int32_t *)take(P * 4);
+    w.cnt = (int32_t *)take(((size_t)2 * E + 1) * 4);
+    w.groups = (GemmGroup *)take((size_t)3 * E * sizeof(GemmGroup));  // the router's, read by nobody here
+    w.tiles = (int32_t *)take((size_t)E * 4);
+    w.h = (uint16_t *)take(P * F * 2);
+    w.yp = (float *)take(P * H * 4);
+    if (ws) *ws = w;
+    return o;
+}
+
+size_t moe_mxfp4_workspace_bytes(int T, int H, int F, int E, int top_k) { return moe_mx_layout(nullptr, T, H, F, E, top_k, nullptr); }
+
+int moe_ffn_mxfp4_launch(const uint16_t *x, const float *logits, const chadq_moe_mxfp4 *ex, uint16_t *y, int T, int H, int F, int E, int top_k, int renorm,
+                         void *workspace, hipStream_t st) {
+    MoeWs ws;
+    moe_mx_layout(reinterpret_cast<uint8_t *>(workspace), T, H, F, E, top_k, &ws);
+    const int P = T * top_k;
+    const MoeExperts none = {};
+    if (P <= 64) hipLaunchKernelGGL(moe_route_few_kernel, dim3(1), dim3(64), 0, st, logits, T, E, top_k, renorm, ws, none, H, F, x);
+    else hipLaunchKernelGGL(moe_route_kernel, dim3(1), dim3(P <= 256 ? 256 : P <= 512 ? 512 : 1024), 0, st, logits, ws.idx, ws.w, T, E, top_k, renorm, ws, none, H, F, x,
+                            0, 0, nullptr);
+    int rc = hip_check(hipGetLastError(), "moe route launch");
+    if (rc) return rc;
+    MxProduct gu = {x, nullptr, ex->gate, ex->gate_scale, ws.h, ws.cnt + E, P, F, H, E, true, false};
+    gu.rows = ws.tok;
+    gu.w2 = ex->up;
+    gu.w2s = ex->up_scale;
+    rc = mx_product_launch(gu, nullptr, 0, st);
+    if (rc) return rc;
+    const MxProduct down = {ws.h, nullptr, ex->down, ex->down_scale, ws.yp, ws.cnt + E, P, H, F, E, false, false};
+    rc = mx_product_launch(down, nullptr, 0, st);
+    if (rc) return rc;
+    const int64_t quads = (int64_t)T * (H / 4);
+    hipLaunchKernelGGL(moe_combine_kernel, dim3(quads < 1024 * 256 ? (int)((quads + 255) / 256) : 1024), dim3(256), 0, st, ws.yp, ws.pos, ws.w, y, T, H, top_k, 1,
+                       (size_t)P * H);
+    return hip_check(hipGetLastError(), "moe combine launch");
 }
 
 }  // namespace chadq

@@ -35,7 +35,13 @@ struct MxProduct {
     const int32_t *offsets;   // [E+1] on the device, or null: one group, all rows
     int M, N, K, E;
     bool y_bf16, clear_rest;  // clear_rest: rows of no group become 0 (else they are left as they are)
+    // mixture of experts: row r of the groups is row rows[r] of x (null: r); with a second matrix per group, of w's shape, the result
+    // is bf16( silu(x w) (x w2) )
+    const int32_t *rows = nullptr;
+    const uint8_t *w2 = nullptr, *w2s = nullptr;
 };
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
 
 // Row tile t of the groups, TR rows to a tile, a group's last one cut: which group, its first row, how many.  For t past the last
 // tile: group -1, and the rows of no group (in front of offsets[0], behind offsets[E]) that are this tile's to clear.
@@ -95,5 +101,8 @@ __device__ __forceinline__ void mx_clear(const MxProduct &p, const MxTile &t, in
         store_sum(reinterpret_cast<float *>(p.y), (size_t)r * p.N + n0 + i % width, 0.f, p.y_bf16);
     }
 }
+
+int mx_product_launch(const MxProduct &p, void *workspace, size_t workspace_bytes, hipStream_t st);
+size_t mx_product_workspace_bytes(int M, int N, int K, bool x_mxfp4);
 
 }  // namespace chadq

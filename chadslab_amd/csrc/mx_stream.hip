@@ -12,17 +12,19 @@
 namespace chadq {
 
 // RT: weight rows of a block in use (<= 16); KU: units of a chunk of activations, a multiple of W * DEPTH
-template <bool X4, int MT, int NT, int W, int DEPTH>
+// GATED: every second block is of w2, of the same rows as the block of w before it
+template <bool X4, bool GATED, int MT, int NT, int W, int DEPTH>
 __global__ __launch_bounds__(64 * W) void mx_stream_kernel(MxProduct p, int RT, int KU) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, kg = lane >> 4;
-    const int n0 = blockIdx.y * (NT * RT), G = p.K >> 5, U = (G + 3) >> 2;
+    constexpr int NO = GATED ? NT / 2 : NT;  // blocks of results
+    const int n0 = blockIdx.y * (NO * RT), G = p.K >> 5, U = (G + 3) >> 2;
     MxTile t = {0, (int)blockIdx.x * (16 * MT), p.M - (int)blockIdx.x * (16 * MT), 0, 0};
     if (p.offsets) {
         t = mx_find_tile(p.offsets, p.E, p.M, 16 * MT, blockIdx.x);
         if (t.group < 0) {
-            if (p.clear_rest) mx_clear(p, t, n0, NT * RT);
+            if (p.clear_rest) mx_clear(p, t, n0, NO * RT);
             return;
         }
     }
@@ -30,11 +32,11 @@ __global__ __launch_bounds__(64 * W) void mx_stream_kernel(MxProduct p, int RT, 
     const uint8_t *wrow[NT], *srow[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-        int n = n0 + i * RT + (l16 < RT ? l16 : RT - 1);
+        int n = n0 + (GATED ? i / 2 : i) * RT + (l16 < RT ? l16 : RT - 1);
         n = n < p.N ? n : p.N - 1;
         const size_t r = (size_t)t.group * p.N + n;
-        wrow[i] = p.w + r * (size_t)(p.K >> 1);
-        srow[i] = p.ws + r * (size_t)G;
+        wrow[i] = (GATED && i % 2 ? p.w2 : p.w) + r * (size_t)(p.K >> 1);
+        srow[i] = (GATED && i % 2 ? p.w2s : p.ws) + r * (size_t)G;
     }
     u32x4 q[DEPTH][NT];
     uint32_t s[DEPTH][NT];
@@ -60,7 +62,10 @@ __global__ __launch_bounds__(64 * W) void mx_stream_kernel(MxProduct p, int RT, 
         for (int i = tid; i < rows * per; i += 64 * W) {
             const int r = i / per, b = (i % per) * 16, at = u0 * UB + b;
             u32x4 v = {0u, 0u, 0u, 0u};
-            if (at < xrow) v = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint8_t *>(p.x) + (size_t)(t.row0 + r) * xrow + at);
+            if (at < xrow) {
+                const int src = p.rows ? p.rows[t.row0 + r] : t.row0 + r;
+                v = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint8_t *>(p.x) + (size_t)src * xrow + at);
+            }
             *reinterpret_cast<u32x4 *>(lds + r * pitch + b) = v;
         }
         if constexpr (X4)
@@ -130,10 +135,20 @@ __global__ __launch_bounds__(64 * W) void mx_stream_kernel(MxProduct p, int RT, 
 #pragma unroll
         for (int b = 0; b < NT; ++b) part[(wave * MT * NT + a * NT + b) * 64 + lane] = acc[a][b];
     __syncthreads();
-    for (int i = tid; i < MT * NT * 64; i += 64 * W) {
+    auto sum = [&](int i) {
         f32x4 v = part[i];
         for (int w = 1; w < W; ++w) v += part[w * MT * NT * 64 + i];
-        const int m = i / (64 * NT) * 16 + (i & 15), b = i / 64 % NT, r = (i & 63) / 16 * 4;
+        return v;
+    };
+    for (int i = tid; i < MT * NO * 64; i += 64 * W) {
+        const int m = i / (64 * NO) * 16 + (i & 15), b = i / 64 % NO, r = (i & 63) / 16 * 4;
+        const int at = (i / (64 * NO) * NT + (GATED ? 2 * b : b)) * 64 + (i & 63);
+        f32x4 v = sum(at);
+        if constexpr (GATED) {
+            const f32x4 u = sum(at + 64);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = silu_mul(v[j], u[j]);
+        }
         if (m >= rows) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -143,9 +158,9 @@ __global__ __launch_bounds__(64 * W) void mx_stream_kernel(MxProduct p, int RT, 
     }
 }
 
-template <bool X4, int MT>
+template <bool X4, bool GATED, int MT>
 static int launch(const MxProduct &p, hipStream_t st) {
-    constexpr int NT = 2, W = 8, DEPTH = 4 / MT, RT = 16;
+    constexpr int NT = 2, W = 8, DEPTH = 4 / MT, RT = 16, NO = GATED ? NT / 2 : NT;
     const int U = (p.K + 127) / 128, step = W * DEPTH;
     const int rows = p.M < 16 * MT ? p.M : 16 * MT, unit = rows * (X4 ? 68 : 256);
     int ku = (65536 / unit) / step * step;  // units of a chunk: 64 KiB of activations, whole rounds of the waves
@@ -154,23 +169,28 @@ static int launch(const MxProduct &p, hipStream_t st) {
     const size_t part = (size_t)W * MT * NT * 1024, chunk = (size_t)rows * (ku * (X4 ? 64 : 256) + 16 + (X4 ? ku * 4 + 4 : 0));
     const size_t lds = part > chunk ? part : chunk;
     const int64_t tiles = p.offsets ? mx_most_tiles(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
-    const int64_t cols = ((int64_t)p.N + NT * RT - 1) / (NT * RT);
+    const int64_t cols = ((int64_t)p.N + NO * RT - 1) / (NO * RT);
     if (tiles > INT32_MAX || cols > 65535) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
     static std::atomic<bool> set[64];  // more LDS than the default limit: once per device
     int dev = 0;
     CHADQ_HIP(hipGetDevice(&dev));
     if (dev >= 64 || !set[dev].load()) {
-        CHADQ_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&mx_stream_kernel<X4, MT, NT, W, DEPTH>), hipFuncAttributeMaxDynamicSharedMemorySize, 163840));
+        CHADQ_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&mx_stream_kernel<X4, GATED, MT, NT, W, DEPTH>), hipFuncAttributeMaxDynamicSharedMemorySize, 163840));
         if (dev < 64) set[dev].store(true);
     }
-    hipLaunchKernelGGL((mx_stream_kernel<X4, MT, NT, W, DEPTH>), dim3((int)tiles, (int)cols), dim3(64 * W), lds, st, p, RT, ku);
+    hipLaunchKernelGGL((mx_stream_kernel<X4, GATED, MT, NT, W, DEPTH>), dim3((int)tiles, (int)cols), dim3(64 * W), lds, st, p, RT, ku);
     return hip_check(hipGetLastError(), "mxfp4 product launch");
 }
 
-int mx_stream_launch(const MxProduct &p, hipStream_t st) {
+template <bool X4, bool GATED>
+static int launch_rows(const MxProduct &p, hipStream_t st) {
     const int per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;
-    if (p.xs) return per <= 16 ? launch<true, 1>(p, st) : per <= 32 ? launch<true, 2>(p, st) : launch<true, 4>(p, st);
-    return per <= 16 ? launch<false, 1>(p, st) : per <= 32 ? launch<false, 2>(p, st) : launch<false, 4>(p, st);
+    return per <= 16 ? launch<X4, GATED, 1>(p, st) : per <= 32 ? launch<X4, GATED, 2>(p, st) : launch<X4, GATED, 4>(p, st);
+}
+
+int mx_stream_launch(const MxProduct &p, hipStream_t st) {
+    if (p.w2) return launch_rows<false, true>(p, st);
+    return p.xs ? launch_rows<true, false>(p, st) : launch_rows<false, false>(p, st);
 }
 
 size_t mx_product_workspace_bytes(int, int, int, bool) { return 0; }

@@ -6,6 +6,7 @@ CPU: tensors must already be on the GPU, and a missing library raises.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Union
 
 import torch
@@ -360,7 +361,10 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, experts, *, top_k: int = 2, r
     triples with gate/up [F,H] and down [H,F], all QWeightInt4G32 or all QWeightInt4G32Tiles (to_tiles(): faster from
     some 16 tokens on).  Dequantised weights are rounded to bf16 (row order) or fp16 (tile order), so the two orders agree within
     rounding; at most 16 tokens take exact weights in row order and, where the experts hit hold at most 64 MB, in tile order
-    too, with the same bits from both.  Returns bf16 [T,H]."""
+    too, with the same bits from both.  Or experts is one triple of QExpertsMXFP4, gate and up [E,F,H] and down [E,H,F]: weights multiplied as
+    they are.  Returns bf16 [T,H]."""
+    if isinstance(experts, (tuple, list)) and any(isinstance(m, QExpertsMXFP4) for m in experts):
+        return _moe_ffn_mxfp4(x, logits, experts, top_k, renorm)
     y = _lib.native().moe_ffn(x, logits, experts, top_k, renorm)
     if y is not None:
         return y
@@ -398,4 +402,28 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, experts, *, top_k: int = 2, r
     fn = lib.chadq_moe_ffn_i4g32_tiled if tiled else lib.chadq_moe_ffn_i4g32
     _lib.check(fn(x.data_ptr(), z.data_ptr(), arr, y.data_ptr(), t, h, f, e, top_k, int(renorm), ws.data_ptr(), need, _stream()),
                "chadq_moe_ffn_i4g32_tiled" if tiled else "chadq_moe_ffn_i4g32")
+    return y
+
+
+def _moe_ffn_mxfp4(x: torch.Tensor, logits: torch.Tensor, experts, top_k: int, renorm: bool) -> torch.Tensor:
+    if len(experts) != 3 or not all(isinstance(m, QExpertsMXFP4) for m in experts):
+        raise TypeError("MXFP4 experts are one (gate, up, down) triple of QExpertsMXFP4")
+    x, z = _dev(x, "x", torch.bfloat16), _dev(logits, "logits", torch.float32)
+    if x.dim() != 2:
+        raise ValueError("x must be [T,H], got %s" % (tuple(x.shape),))
+    gate, up, down = experts
+    (t, h), e, f = x.shape, gate.E, gate.N
+    if tuple(z.shape) != (t, e) or z.device != x.device:
+        raise ValueError("logits must be [%d,%d] on %s" % (t, e, x.device))
+    if (gate.K, up.E, up.N, up.K) != (h, e, f, h) or (down.E, down.N, down.K) != (e, h, f):
+        raise ValueError("gate and up must be [%d,%d,%d] and down [%d,%d,%d]" % (e, f, h, e, h, f))
+    lib = _lib.load()
+    y = torch.empty(t, h, dtype=torch.bfloat16, device=x.device)
+    need = lib.chadq_moe_ffn_mxfp4_workspace_bytes(t, h, f, e, top_k)
+    if need == 0:
+        raise ValueError("unsupported MoE sizes T=%d H=%d F=%d E=%d top_k=%d" % (t, h, f, e, top_k))
+    ts = [v for name, m in (("gate", gate), ("up", up), ("down", down)) for v in _mxfp4(m, name, x.device)]
+    arr = _lib.MoeMXFP4(*[v.data_ptr() for v in ts])
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)  # as moe_ffn's
+    _launch(x.device, "chadq_moe_ffn_mxfp4", x.data_ptr(), z.data_ptr(), ctypes.byref(arr), y.data_ptr(), t, h, f, e, top_k, int(renorm), ws.data_ptr(), need)
     return y

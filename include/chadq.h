@@ -443,6 +443,17 @@ int chadq_product_mxfp4(const void *x, const uint8_t *x_scale, const uint8_t *w,
 int chadq_product_mxfp4_grouped(const void *x, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const int32_t *offsets,
                                 uint16_t *y_bf16, int M, int E, int N, int K, int clear_rest, void *stream);
 
+/*
+ * chadq_moe_ffn_i4g32's operator on MXFP4 experts: gate, up [E,F,H], down [E,H,F], codes and scales of the E matrices one behind the other.  Weights are
+ * multiplied as they are; h = bf16(silu(gate) * up), fp32 sums, y bf16 [T,H].  Sizes and workspace as there.
+ */
+typedef struct chadq_moe_mxfp4 {
+    const uint8_t *gate, *gate_scale, *up, *up_scale, *down, *down_scale;
+} chadq_moe_mxfp4;
+size_t chadq_moe_ffn_mxfp4_workspace_bytes(int T, int H, int F, int E, int top_k);
+int chadq_moe_ffn_mxfp4(const uint16_t *x_bf16, const float *logits, const chadq_moe_mxfp4 *experts, uint16_t *y_bf16, int T, int H, int F, int E, int top_k,
+                        int renorm, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

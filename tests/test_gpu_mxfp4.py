@@ -398,3 +398,92 @@ def test_weights_and_activations_quantised_and_multiplied(ops):
     xb = dev(x).to(torch.bfloat16)
     check(ops.qlinear(xb, qw), xb.double(), w64)
     check(ops.qlinear(ops.quantize_mxfp4(xb), qw), dev(O.dequant_mxfp4(*O.quantize_mxfp4(xb.double().cpu().numpy()))), w64)
+
+
+# ---- mixture of experts ---------------------------------------------------------------------------------------------------
+def moe_oracle(x64, logits, gate, up, down, top_k, renorm):
+    idx, w = O.moe_route(logits, top_k, renorm)
+    y = np.zeros_like(x64)
+    for t in range(len(x64)):
+        for j in range(top_k):
+            g, u = gate[idx[t, j]] @ x64[t], up[idx[t, j]] @ x64[t]
+            y[t] += float(w[t, j]) * (down[idx[t, j]] @ (g / (1 + np.exp(-g)) * u))
+    return y
+
+
+@pytest.mark.parametrize("tokens,h,f,experts,top_k,renorm", [(1, 32, 64, 4, 2, True), (4, 256, 512, 8, 2, True), (7, 96, 160, 3, 3, False), (33, 288, 352, 16, 4, True),
+                                                             (100, 512, 1056, 8, 2, False), (300, 256, 224, 5, 1, True), (64, 64, 32, 1, 1, True)])
+def test_moe(ops, tokens, h, f, experts, top_k, renorm):
+    """Against 64 bits without rounding in between: what is rounded is h, half a step of bf16 (2^-8), and the result; the errors of h are
+    independent, so the norm of the result's error is at most 2^-8 (h) + 2^-8 (y) of its own and the fp32 sums' and weights' 2^-18."""
+    from chadslab_amd import QExpertsMXFP4
+
+    r = np.random.Generator(np.random.PCG64(tokens + h + f))
+    mats = [weights(r, experts, *shape, spread=0.5) for shape in ((f, h), (f, h), (h, f))]
+    x, x64 = activations(r, tokens, h, False)
+    logits = r.standard_normal((tokens, experts)).astype(np.float32)
+    if experts > 3:
+        logits[:, 1] = -50.0  # nobody's choice, as long as there are enough others
+        logits[0, 2] = logits[0, 0]
+    triple = tuple(QExpertsMXFP4(dev(c), dev(s)) for c, s in mats)
+    y = ops.moe_ffn(x, dev(logits), triple, top_k=top_k, renorm=renorm)
+    want = moe_oracle(x64.cpu().numpy(), logits, *(O.dequant_mxfp4(c, s) for c, s in mats), top_k, renorm)
+    assert y.dtype == torch.bfloat16 and O.rel_l2(y.double().cpu().numpy(), want) <= 2 * 2.0 ** -8 + 2.0 ** -18
+
+
+def test_moe_is_its_parts_and_replays(ops):
+    """The layer against its own operators in a row (route, sort, products by group, gate, down, weighted sum), eager and from a graph."""
+    from chadslab_amd import QExpertsMXFP4
+
+    r = np.random.Generator(np.random.PCG64(77))
+    tokens, h, f, experts, top_k = 90, 256, 320, 8, 2
+    gate, up, down = (QExpertsMXFP4(*(dev(a) for a in weights(r, experts, *shape))) for shape in ((f, h), (f, h), (h, f)))
+    x, _ = activations(r, tokens, h, False)
+    logits = dev(r.standard_normal((tokens, experts)).astype(np.float32))
+
+    def parts():
+        idx, w = ops.moe_route(logits, top_k)
+        order = torch.sort(idx.flatten().long(), stable=True).indices
+        offsets = torch.searchsorted(idx.flatten().long().sort().values, torch.arange(experts + 1, device=DEV)).to(torch.int32)
+        xs = x[order // top_k]
+        g, u = ops.qgemm_grouped(xs, gate, offsets).float(), ops.qgemm_grouped(xs, up, offsets).float()
+        d = ops.qgemm_grouped((g * torch.sigmoid(g) * u).to(torch.bfloat16), down, offsets).float()
+        y = torch.empty_like(d)
+        y[order] = d
+        return (y.view(tokens, top_k, h) * w[..., None]).sum(1)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ops.moe_ffn(x, logits, (gate, up, down), top_k=top_k)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        y = ops.moe_ffn(x, logits, (gate, up, down), top_k=top_k)
+    for turn in range(3):
+        x.copy_(activations(r, tokens, h, False)[0])
+        logits.copy_(torch.randn_like(logits))
+        eager, want = ops.moe_ffn(x, logits, (gate, up, down), top_k=top_k), parts()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager)
+        # gate and up (half a step of bf16 each, silu's slope is at most 1.1), h and the result are rounded here, h and the result there
+        assert float((eager.double() - want.double()).norm() / want.double().norm()) <= (1.1 + 1 + 2 * 2) * 2.0 ** -8
+
+
+def test_moe_refusals(ops):
+    from chadslab_amd import QExpertsMXFP4
+
+    r = np.random.Generator(np.random.PCG64(1))
+    gate, up, down = (QExpertsMXFP4(*(dev(a) for a in weights(r, 4, *shape))) for shape in ((64, 32), (64, 32), (32, 64)))
+    x, z = torch.zeros(3, 32, dtype=torch.bfloat16, device=DEV), torch.zeros(3, 4, device=DEV)
+    assert not ops.moe_ffn(x, z, (gate, up, down)).any()
+    with pytest.raises(TypeError, match="triple"):
+        ops.moe_ffn(x, z, (gate, up))
+    with pytest.raises(ValueError, match="gate and up"):
+        ops.moe_ffn(x, z, (gate, down, up))
+    with pytest.raises(ValueError, match="logits"):
+        ops.moe_ffn(x, z[:, :3], (gate, up, down))
+    for bad in (0, 5):
+        with pytest.raises(ValueError, match="unsupported"):
+            ops.moe_ffn(x, z, (gate, up, down), top_k=bad)
