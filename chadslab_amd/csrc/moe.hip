@@ -535,6 +535,7 @@ int moe_ffn_mxfp4_launch(const uint16_t *x, const float *logits, const chadq_moe
     if (rc) return rc;
     MxProduct gu = {x, nullptr, ex->gate, ex->gate_scale, ws.h, ws.cnt + E, P, F, H, E, true, false};
     gu.rows = ws.tok;
+    gu.x_rows = T;
     gu.w2 = ex->up;
     gu.w2s = ex->up_scale;
     rc = mx_product_launch(gu, nullptr, 0, st);

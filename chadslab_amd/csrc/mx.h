@@ -38,28 +38,30 @@ struct MxProduct {
     // mixture of experts: row r of the groups is row rows[r] of x (null: r); with a second matrix per group, of w's shape, the result
     // is bf16( silu(x w) (x w2) )
     const int32_t *rows = nullptr;
+    int x_rows = 0;           // ... which has so many
     const uint8_t *w2 = nullptr, *w2s = nullptr;
 };
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
 
-// Row tile t of the groups, TR rows to a tile, a group's last one cut: which group, its first row, how many.  For t past the last
-// tile: group -1, and the rows of no group (in front of offsets[0], behind offsets[E]) that are this tile's to clear.
-// Offsets are taken as clamped into [0, M] and never descending (one that descends counts as the largest before it), so that no
-// contents of theirs lead outside x and y.  Every lane of a wave calls this; the answer is uniform.
+// Row tiles of the groups, TR rows to a tile, a group's last one cut; behind them the tiles of the rows of no group (in front of offsets[0] and
+// behind offsets[E]), for those who clear them.  Offsets are taken as clamped into [0, M] and never descending (one that descends counts as
+// the largest before it), so that no contents of theirs lead outside x and y.  Every lane of a wave calls this; the answers are uniform.
 struct MxTile {
-    int group, row0, rows, rest0, rest1;  // rest: rest0 rows from 0 on and the rows from rest1 on
+    int group, row0, rows, rest0, rest1;  // group -1: rows of no group, counted as rest0 rows from 0 on and then the rows from rest1 on
 };
-__device__ __forceinline__ MxTile mx_find_tile(const int32_t *__restrict__ offsets, int E, int M, int TR, int t) {
-    const int lane = threadIdx.x & 63;
-    int before = 0, low = 0, first = 0;  // tiles, largest offset so far
-    for (int c = 0; c < E; c += 64) {
-        const int e = c + lane;
+struct MxTiles {
+    const int32_t *__restrict__ offsets;
+    int E, M, TR;
+
+    // 64 groups from c on: the lane's first row, the one behind its last, and tiles up to and with it; low: largest offset so far
+    __device__ __forceinline__ void scan(int c, int low, int &lo, int &hi, int &upto) const {
+        const int lane = threadIdx.x & 63, e = c + lane;
         auto at = [&](int i) {
             const int o = offsets[i < E ? i : E];
             return o < 0 ? 0 : o > M ? M : o;
         };
-        int lo = at(e);
+        lo = at(e);
         const int next = at(e + 1);
         lo = lo > low ? lo : low;
 #pragma unroll
@@ -67,30 +69,46 @@ __device__ __forceinline__ MxTile mx_find_tile(const int32_t *__restrict__ offse
             const int o = __shfl_up(lo, d);
             if (lane >= d) lo = lo > o ? lo : o;
         }
-        const int hi = next > lo ? next : lo;
-        int upto = e < E ? (hi - lo + TR - 1) / TR : 0;
-        const int mine = upto;
+        hi = next > lo ? next : lo;
+        upto = e < E ? (hi - lo + TR - 1) / TR : 0;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const int o = __shfl_up(upto, d);
             if (lane >= d) upto += o;
         }
-        if (c == 0) first = __shfl(lo, 0);
-        const unsigned long long m = __ballot(t < before + upto);
-        if (m) {
-            const int l = __ffsll((long long)m) - 1;
-            const int k = t - before - (__shfl(upto, l) - __shfl(mine, l)), r0 = __shfl(lo, l) + k * TR, end = __shfl(hi, l);
-            return {__builtin_amdgcn_readfirstlane(c + l), __builtin_amdgcn_readfirstlane(r0),
-                    __builtin_amdgcn_readfirstlane(end - r0 < TR ? end - r0 : TR), 0, 0};
-        }
-        before += __shfl(upto, 63);
-        low = __shfl(hi, 63);
     }
-    const int rest = first + (M - low), r0 = (t - before) * TR;
-    return {-1, __builtin_amdgcn_readfirstlane(r0), __builtin_amdgcn_readfirstlane(rest - r0 < 0 ? 0 : rest - r0 < TR ? rest - r0 : TR),
-            __builtin_amdgcn_readfirstlane(first), __builtin_amdgcn_readfirstlane(low)};
-}
-// Row tiles that suffice for any offsets, those that clear included: full tiles of M rows, one cut per group that can have a row, one of the rest.
+    // tiles of the groups, and (clear) of the rows of none
+    __device__ __forceinline__ int count(bool clear) const {
+        int n = 0, low = 0, first = 0;
+        for (int c = 0; c < E; c += 64) {
+            int lo, hi, upto;
+            scan(c, low, lo, hi, upto);
+            if (c == 0) first = __builtin_amdgcn_readlane(lo, 0);
+            n += __builtin_amdgcn_readlane(upto, 63);
+            low = __builtin_amdgcn_readlane(hi, 63);
+        }
+        return n + (clear ? (first + (M - low) + TR - 1) / TR : 0);
+    }
+    __device__ __forceinline__ MxTile find(int t) const {
+        int before = 0, low = 0, first = 0;
+        for (int c = 0; c < E; c += 64) {
+            int lo, hi, upto;
+            scan(c, low, lo, hi, upto);
+            if (c == 0) first = __builtin_amdgcn_readlane(lo, 0);
+            const unsigned long long m = __ballot(t < before + upto);
+            if (m) {
+                const int l = __ffsll((long long)m) - 1, r0 = __builtin_amdgcn_readlane(lo, l), end = __builtin_amdgcn_readlane(hi, l);
+                const int r = r0 + (t - before - (__builtin_amdgcn_readlane(upto, l) - (end - r0 + TR - 1) / TR)) * TR;
+                return {c + l, r, end - r < TR ? end - r : TR, 0, 0};
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+            low = __builtin_amdgcn_readlane(hi, 63);
+        }
+        const int rest = first + (M - low), r0 = (t - before) * TR;
+        return {-1, r0, rest - r0 < 0 ? 0 : rest - r0 < TR ? rest - r0 : TR, first, low};
+    }
+};
+// Row tiles that suffice for any offsets: full tiles of M rows, one cut per group that can have a row, one of the rest.
 inline int64_t mx_most_tiles(int M, int E, int TR) { return (int64_t)M / TR + (E < M ? E : M) + 2; }
 
 // The columns n0 .. n0 + cols of the tile's rows of no group, set to 0 by the workgroup's threads
@@ -102,6 +120,9 @@ __device__ __forceinline__ void mx_clear(const MxProduct &p, const MxTile &t, in
     }
 }
 
+int mx_stream_launch(const MxProduct &p, hipStream_t st);
+bool mx_tile_ok(const MxProduct &p);
+int mx_tile_launch(const MxProduct &p, hipStream_t st);
 int mx_product_launch(const MxProduct &p, void *workspace, size_t workspace_bytes, hipStream_t st);
 size_t mx_product_workspace_bytes(int M, int N, int K, bool x_mxfp4);
 

@@ -22,7 +22,7 @@ __global__ __launch_bounds__(64 * W) void mx_stream_kernel(MxProduct p, int RT, 
     const int n0 = blockIdx.y * (NO * RT), G = p.K >> 5, U = (G + 3) >> 2;
     MxTile t = {0, (int)blockIdx.x * (16 * MT), p.M - (int)blockIdx.x * (16 * MT), 0, 0};
     if (p.offsets) {
-        t = mx_find_tile(p.offsets, p.E, p.M, 16 * MT, blockIdx.x);
+        t = MxTiles{p.offsets, p.E, p.M, 16 * MT}.find(blockIdx.x);
         if (t.group < 0) {
             if (p.clear_rest) mx_clear(p, t, n0, NO * RT);
             return;
@@ -195,6 +195,9 @@ int mx_stream_launch(const MxProduct &p, hipStream_t st) {
 
 size_t mx_product_workspace_bytes(int, int, int, bool) { return 0; }
 
-int mx_product_launch(const MxProduct &p, void *, size_t, hipStream_t st) { return mx_stream_launch(p, st); }
+int mx_product_launch(const MxProduct &p, void *, size_t, hipStream_t st) {
+    const int per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;
+    return per > 64 && mx_tile_ok(p) ? mx_tile_launch(p, st) : mx_stream_launch(p, st);
+}
 
 }  // namespace chadq
