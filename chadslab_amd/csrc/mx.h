@@ -23,6 +23,15 @@ __device__ __forceinline__ bf16x8 dequant8_mx(uint32_t w, float s) {
     return o;
 }
 
+// The bare barrier behind a wait for the wave's own LDS accesses (__syncthreads() would also wait for every outstanding memory request); the
+// empty asm statements keep the compiler from moving LDS accesses across it.
+__device__ __forceinline__ void wg_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // 32 codes as the operand of a scaled MFMA (fp4 takes the lower half of its eight registers)
 __device__ __forceinline__ i32x8 mx_operand(u32x4 v) { return i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0}; }
 

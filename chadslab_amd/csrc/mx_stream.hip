@@ -1,34 +1,52 @@
-// Products of few rows on MXFP4 weights: y[m,n] = sum_k x[m,k] value(w[n,k]) 2^(e[n,k/32] - 127), x bf16 or MXFP4, one matrix or
-// (groups) one per run of rows.  HBM-bound: every weight is read once per tile of 16 MT rows.
+// Products of at most 16 rows (of a group) on MXFP4 weights: y[m,n] = sum_k x[m,k] value(w[n,k]) 2^(e[n,k/32] - 127), x bf16 or MXFP4, one
+// matrix or one per group of rows.  HBM-bound: every weight is read once per tile of 16 rows.
 //
 // A workgroup's W waves share NT blocks of at most 16 weight rows and split K among them, 128 k (a unit: four scale blocks, one to each
-// 16 lanes) at a time.  Weights go from memory straight into the operand registers, 16 bytes = one scale block per lane; the
-// activations wait in LDS, zeros behind K, where a lane past the end of its weight row reads that row's last block again (what is
-// NaN there makes the row's result NaN in any case).  bf16 activations: the codes become bf16 with their scale, exactly, by one conversion per pair, and
-// v_mfma_f32_16x16x32_bf16 sums in fp32.  MXFP4 activations: both operands go to v_mfma_scale_f32_16x16x128_f8f6f4 as they are.  The weights
-// are the first operand, so that a lane ends up with four consecutive n of one activation row.  The waves' sums meet in LDS, added in their order.
+// 16 lanes) at a time, D units of a wave one behind the other, their weights requested a round (D units of every wave) ahead.  Weights go from memory
+// straight into the operand registers, 16 bytes = one scale block per lane; the activations wait in LDS, requested before the first weights, zeros behind
+// K, where a lane past the end of its weight row reads that row's last block again (what is NaN there makes the row's result NaN in any case).
+// bf16 activations: the codes become bf16 with their scale, exactly, by one conversion per pair, and v_mfma_f32_16x16x32_bf16 sums in fp32.
+// MXFP4 activations: both operands go to v_mfma_scale_f32_16x16x128_f8f6f4 as they are.  The weights are the first operand, so that a lane ends up
+// with four consecutive n of one activation row.  The waves' sums meet in LDS, added in their order.
 #include "mx.h"
 
 namespace chadq {
 
-// RT: weight rows of a block in use (<= 16); KU: units of a chunk of activations, a multiple of W * DEPTH
+// RT: weight rows of a block in use (<= 16); KU: units of a chunk of activations, whole rounds
 // GATED: every second block is of w2, of the same rows as the block of w before it
-template <bool X4, bool GATED, int MT, int NT, int W, int DEPTH>
+template <bool X4, bool GATED, int NT, int W, int D>
 __global__ __launch_bounds__(64 * W) void mx_stream_kernel(MxProduct p, int RT, int KU) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, kg = lane >> 4;
     constexpr int NO = GATED ? NT / 2 : NT;  // blocks of results
-    const int n0 = blockIdx.y * (NO * RT), G = p.K >> 5, U = (G + 3) >> 2;
-    MxTile t = {0, (int)blockIdx.x * (16 * MT), p.M - (int)blockIdx.x * (16 * MT), 0, 0};
+    const int n0 = blockIdx.y * (NO * RT), G = p.K >> 5, U = (G + 3) >> 2, rounds = (U + W * D - 1) / (W * D);
+    MxTile t = {0, (int)blockIdx.x * 16, p.M - (int)blockIdx.x * 16, 0, 0};
     if (p.offsets) {
-        t = MxTiles{p.offsets, p.E, p.M, 16 * MT}.find(blockIdx.x);
+        t = MxTiles{p.offsets, p.E, p.M, 16}.find(blockIdx.x);
         if (t.group < 0) {
             if (p.clear_rest) mx_clear(p, t, n0, NO * RT);
             return;
         }
     }
-    const int rows = t.rows < 16 * MT ? t.rows : 16 * MT;
+    const int rows = t.rows < 16 ? t.rows : 16;
+
+    // ---- activations.  A chunk: rows of KU units, 16 bytes apart beyond that (16 rows then cover the banks)
+    constexpr int UB = X4 ? 64 : 256;  // bytes of a unit
+    const int pitch = KU * UB + 16, per = KU * UB / 1024;
+    const int xrow = X4 ? p.K >> 1 : p.K * 2;  // bytes of a row
+    auto stage = [&](int u0) {  // 1 KiB of a row per request; past a row's end nothing is read and zeros arrive
+        for (int i = wave; i < rows * per; i += W) {
+            const int r = i / per, b = i % per * 1024, at = u0 * UB + b + lane * 16;
+            const int src = __builtin_amdgcn_readfirstlane(p.rows ? p.rows[t.row0 + r] : t.row0 + r);
+            const __amdgpu_buffer_rsrc_t rs =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(reinterpret_cast<const uint8_t *>(p.x)) + (size_t)src * xrow, 0, xrow, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)(lds + r * pitch + b), 16, at < xrow ? (uint32_t)at : 0x80000000u, 0, 0, 0);
+        }
+    };
+    stage(0);
+
+    // ---- weights
     const uint8_t *wrow[NT], *srow[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -38,118 +56,89 @@ __global__ __launch_bounds__(64 * W) void mx_stream_kernel(MxProduct p, int RT, 
         wrow[i] = (GATED && i % 2 ? p.w2 : p.w) + r * (size_t)(p.K >> 1);
         srow[i] = (GATED && i % 2 ? p.w2s : p.ws) + r * (size_t)G;
     }
-    u32x4 q[DEPTH][NT];
-    uint32_t s[DEPTH][NT];
-    auto load = [&](int u, int d) {
-        int b = 4 * u + kg;
+    const int xm = l16 < rows ? l16 : rows - 1;  // the lane's activation row (one of the tile's, where it has fewer)
+    const uint8_t *const xsrow = X4 ? p.xs + (size_t)(t.row0 + xm) * G : nullptr;
+    u32x4 q[D][NT];
+    uint32_t s[D][NT], xs[D];
+    auto load = [&](int round, int d) {
+        int b = ((round * W + wave) * D + d) * 4 + kg;
         b = b < G ? b : G - 1;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            q[d][i] = load_nt_b128(wrow[i] + (size_t)b * 16);
-            s[d][i] = srow[i][b];
-        }
+        for (int i = 0; i < NT; ++i) q[d][i] = load_nt_b128(wrow[i] + (size_t)b * 16);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) s[d][i] = srow[i][b];
+        if constexpr (X4) xs[d] = xsrow[b];
     };
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) load(wave + d * W, d);
+    for (int d = 0; d < D; ++d) load(0, d);
+    __builtin_amdgcn_sched_barrier(0);
 
-    // chunk: rows of KU units, 16 bytes apart beyond that (16 rows then cover the banks); behind them the scales of MXFP4 rows
-    constexpr int UB = X4 ? 64 : 256;  // bytes of a unit
-    const int pitch = KU * UB + 16, spitch = KU * 4 + 4;
-    uint8_t *const xsl = lds + rows * pitch;
-    const int xrow = X4 ? p.K >> 1 : p.K * 2;  // bytes of a row
-    auto stage = [&](int u0) {
-        const int per = KU * UB / 16;
-        for (int i = tid; i < rows * per; i += 64 * W) {
-            const int r = i / per, b = (i % per) * 16, at = u0 * UB + b;
-            u32x4 v = {0u, 0u, 0u, 0u};
-            if (at < xrow) {
-                const int src = p.rows ? p.rows[t.row0 + r] : t.row0 + r;
-                v = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint8_t *>(p.x) + (size_t)src * xrow + at);
-            }
-            *reinterpret_cast<u32x4 *>(lds + r * pitch + b) = v;
-        }
-        if constexpr (X4)
-            for (int i = tid; i < rows * KU * 4; i += 64 * W) {
-                const int r = i / (KU * 4), b = i % (KU * 4), at = u0 * 4 + b;
-                xsl[r * spitch + b] = at < G ? p.xs[(size_t)(t.row0 + r) * G + at] : (uint8_t)0;
-            }
-    };
+    f32x4 acc[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint8_t *const xl = lds + xm * pitch + (X4 ? kg * 16 : kg * 64) + wave * D * UB;
 
-    f32x4 acc[MT][NT];
+    wait_vmcnt<D * (2 * NT + X4)>();  // what has been requested since the activations
+    wg_barrier();
+    int at = 0;  // of the round in its chunk
+    auto turn = [&](int round, bool more) {
+        const uint8_t *const xr = xl + at * (W * D * UB);
 #pragma unroll
-    for (int a = 0; a < MT; ++a)
+        for (int d = 0; d < D; ++d) {
+            if constexpr (X4) {
+                const i32x8 xo = mx_operand(*reinterpret_cast<const u32x4 *>(xr + d * UB));
 #pragma unroll
-        for (int b = 0; b < NT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int xm[MT];  // the lane's activation row in each row block (one of the tile's, where the block has fewer)
+                for (int i = 0; i < NT; ++i)
+                    acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[d][i]), xo, acc[i], 4, 4, 0, (int)s[d][i], 0, (int)xs[d]);
+            } else {
 #pragma unroll
-    for (int a = 0; a < MT; ++a) xm[a] = a * 16 + l16 < rows ? a * 16 + l16 : rows - 1;
-
-    for (int u0 = 0; u0 < U; u0 += KU) {
-        if (u0) __syncthreads();
-        stage(u0);
-        __syncthreads();
-        const int end = U - u0 < KU ? U - u0 : KU;
-        for (int i = wave; i < end; i += W * DEPTH) {
+                for (int j = 0; j < 4; ++j) {
+                    const bf16x8 xo = *reinterpret_cast<const bf16x8 *>(xr + d * UB + j * 16);
 #pragma unroll
-            for (int d = 0; d < DEPTH; ++d) {
-                const int v = i + d * W;
-                if (v < end) {
-                    if constexpr (X4) {
-                        i32x8 xo[MT];
-                        int xsc[MT];
-#pragma unroll
-                        for (int a = 0; a < MT; ++a) {
-                            xo[a] = mx_operand(*reinterpret_cast<const u32x4 *>(lds + xm[a] * pitch + v * 64 + kg * 16));
-                            xsc[a] = xsl[xm[a] * spitch + v * 4 + kg];
-                        }
-#pragma unroll
-                        for (int b = 0; b < NT; ++b)
-#pragma unroll
-                            for (int a = 0; a < MT; ++a)
-                                acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[d][b]), xo[a], acc[a][b], 4, 4, 0, (int)s[d][b], 0, xsc[a]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            bf16x8 xo[MT];
-#pragma unroll
-                            for (int a = 0; a < MT; ++a) xo[a] = *reinterpret_cast<const bf16x8 *>(lds + xm[a] * pitch + v * 256 + kg * 64 + j * 16);
-#pragma unroll
-                            for (int b = 0; b < NT; ++b) {
-                                const bf16x8 wo = dequant8_mx(q[d][b][j], mx_scale(s[d][b]));
-#pragma unroll
-                                for (int a = 0; a < MT; ++a) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wo, xo[a], acc[a][b], 0, 0, 0);
-                            }
-                        }
-                    }
+                    for (int i = 0; i < NT; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dequant8_mx(q[d][i][j], mx_scale(s[d][i])), xo, acc[i], 0, 0, 0);
                 }
-                load(u0 + v + W * DEPTH, d);
             }
+            if (more) load(round + 1, d);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        ++at;
+    };
+    int round = 0;
+    for (; round + 1 < rounds; ++round) {
+        turn(round, true);
+        if (at * (W * D) == KU) {  // the next chunk
+            wg_barrier();
+            stage((round + 1) * (W * D));
+            wait_vmcnt<0>();
+            wg_barrier();
+            at = 0;
         }
     }
+    turn(round, false);
 
     // ---- the waves' sums: [wave][block][lane] of four n each
-    __syncthreads();
+    wg_barrier();
     f32x4 *const part = reinterpret_cast<f32x4 *>(lds);
 #pragma unroll
-    for (int a = 0; a < MT; ++a)
-#pragma unroll
-        for (int b = 0; b < NT; ++b) part[(wave * MT * NT + a * NT + b) * 64 + lane] = acc[a][b];
-    __syncthreads();
+    for (int i = 0; i < NT; ++i) part[(wave * NT + i) * 64 + lane] = acc[i];
+    wg_barrier();
     auto sum = [&](int i) {
         f32x4 v = part[i];
-        for (int w = 1; w < W; ++w) v += part[w * MT * NT * 64 + i];
+#pragma unroll
+        for (int w = 1; w < W; ++w) v += part[w * NT * 64 + i];
         return v;
     };
-    for (int i = tid; i < MT * NO * 64; i += 64 * W) {
-        const int m = i / (64 * NO) * 16 + (i & 15), b = i / 64 % NO, r = (i & 63) / 16 * 4;
-        const int at = (i / (64 * NO) * NT + (GATED ? 2 * b : b)) * 64 + (i & 63);
-        f32x4 v = sum(at);
+    for (int i = tid; i < NO * 64; i += 64 * W) {
+        const int m = i & 15, b = i / 64, r = (i & 63) / 16 * 4, e = (GATED ? 2 * b : b) * 64 + (i & 63);
+        if (m >= rows || r >= RT) continue;
+        f32x4 v = sum(e);
         if constexpr (GATED) {
-            const f32x4 u = sum(at + 64);
+            const f32x4 u = sum(e + 64);
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = silu_mul(v[j], u[j]);
         }
-        if (m >= rows) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int n = n0 + b * RT + r + j;
@@ -158,46 +147,62 @@ __global__ __launch_bounds__(64 * W) void mx_stream_kernel(MxProduct p, int RT, 
     }
 }
 
-template <bool X4, bool GATED, int MT>
-static int launch(const MxProduct &p, hipStream_t st) {
-    constexpr int NT = 2, W = 8, DEPTH = 4 / MT, RT = 16, NO = GATED ? NT / 2 : NT;
-    const int U = (p.K + 127) / 128, step = W * DEPTH;
-    const int rows = p.M < 16 * MT ? p.M : 16 * MT, unit = rows * (X4 ? 68 : 256);
-    int ku = (65536 / unit) / step * step;  // units of a chunk: 64 KiB of activations, whole rounds of the waves
-    const int all = (U + step - 1) / step * step;
-    ku = ku < step ? step : ku > all ? all : ku;
-    const size_t part = (size_t)W * MT * NT * 1024, chunk = (size_t)rows * (ku * (X4 ? 64 : 256) + 16 + (X4 ? ku * 4 + 4 : 0));
-    const size_t lds = part > chunk ? part : chunk;
-    const int64_t tiles = p.offsets ? mx_most_tiles(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
-    const int64_t cols = ((int64_t)p.N + NO * RT - 1) / (NO * RT);
+template <bool X4, bool GATED, int NT, int W, int D>
+static int launch(const MxProduct &p, int RT, hipStream_t st) {
+    constexpr int NO = GATED ? NT / 2 : NT, UB = X4 ? 64 : 256;
+    const int U = (p.K + 127) / 128, round = W * D, rounds = (U + round - 1) / round, rows = p.M < 16 ? p.M : 16;
+    const int most = (W == 8 ? 73728 : 147456) / (rows * round * UB), chunk = most < 1 ? 1 : most > rounds ? rounds : most;  // rounds of a chunk
+    const int ku = chunk * round;
+    static_assert(W * D * UB % 1024 == 0, "a request fills a KiB of a row");
+    const size_t part = (size_t)W * NT * 1024, xb = (size_t)rows * (ku * UB + 16), lds = part > xb ? part : xb;
+    if (lds > 163840) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: %zu bytes of LDS", lds);
+    const int64_t tiles = p.offsets ? mx_most_tiles(p.M, p.E, 16) : (p.M + 15) / 16, cols = ((int64_t)p.N + NO * RT - 1) / (NO * RT);
     if (tiles > INT32_MAX || cols > 65535) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
     static std::atomic<bool> set[64];  // more LDS than the default limit: once per device
     int dev = 0;
     CHADQ_HIP(hipGetDevice(&dev));
     if (dev >= 64 || !set[dev].load()) {
-        CHADQ_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&mx_stream_kernel<X4, GATED, MT, NT, W, DEPTH>), hipFuncAttributeMaxDynamicSharedMemorySize, 163840));
+        CHADQ_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&mx_stream_kernel<X4, GATED, NT, W, D>), hipFuncAttributeMaxDynamicSharedMemorySize, 163840));
         if (dev < 64) set[dev].store(true);
     }
-    hipLaunchKernelGGL((mx_stream_kernel<X4, GATED, MT, NT, W, DEPTH>), dim3((int)tiles, (int)cols), dim3(64 * W), lds, st, p, RT, ku);
+    hipLaunchKernelGGL((mx_stream_kernel<X4, GATED, NT, W, D>), dim3((int)tiles, (int)cols), dim3(64 * W), lds, st, p, RT, ku);
     return hip_check(hipGetLastError(), "mxfp4 product launch");
 }
 
+template <bool X4, bool GATED, int NT>
+static int launch_waves(const MxProduct &p, int RT, hipStream_t st) {
+    const int U = (p.K + 127) / 128;
+    // 16 waves, one workgroup to a compute unit, where two workgroups' activations would not fit beside each other (or are read twice)
+    if ((p.offsets ? 16 : p.M) > 8) return launch<X4, GATED, NT, 16, 2>(p, RT, st);
+    if constexpr (!X4)
+        if (U <= 8) return launch<X4, GATED, NT, 8, 1>(p, RT, st);
+    if constexpr (NT < 4)
+        if (U > 16) return launch<X4, GATED, NT, 8, 4>(p, RT, st);
+    return launch<X4, GATED, NT, 8, 2>(p, RT, st);
+}
+
 template <bool X4, bool GATED>
-static int launch_rows(const MxProduct &p, hipStream_t st) {
-    const int per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;
-    return per <= 16 ? launch<X4, GATED, 1>(p, st) : per <= 32 ? launch<X4, GATED, 2>(p, st) : launch<X4, GATED, 4>(p, st);
+static int launch_blocks(const MxProduct &p, hipStream_t st) {
+    constexpr int PAIR = GATED ? 2 : 1;  // blocks of a result block
+    if (p.offsets) return launch_waves<X4, GATED, 2 * PAIR>(p, 16, st);
+    // As many rows to a workgroup as give every compute unit the same number of them (one, or two of 8 waves)
+    const int most = p.M > 8 && !GATED ? 64 : 32, rounds = (p.N + 256 * most - 1) / (256 * most), rows = (p.N + 256 * rounds - 1) / (256 * rounds);
+    const int blocks = (rows + 15) / 16;
+    if (blocks <= 1) return launch_waves<X4, GATED, 1 * PAIR>(p, rows, st);
+    if (blocks == 2 || PAIR == 2) return launch_waves<X4, GATED, 2 * PAIR>(p, (rows + 1) / 2, st);
+    return launch_waves<X4, GATED, 4>(p, (rows + 3) / 4, st);
 }
 
 int mx_stream_launch(const MxProduct &p, hipStream_t st) {
-    if (p.w2) return launch_rows<false, true>(p, st);
-    return p.xs ? launch_rows<true, false>(p, st) : launch_rows<false, false>(p, st);
+    if (p.w2) return launch_blocks<false, true>(p, st);
+    return p.xs ? launch_blocks<true, false>(p, st) : launch_blocks<false, false>(p, st);
 }
 
 size_t mx_product_workspace_bytes(int, int, int, bool) { return 0; }
 
 int mx_product_launch(const MxProduct &p, void *, size_t, hipStream_t st) {
     const int per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;
-    return per > 64 && mx_tile_ok(p) ? mx_tile_launch(p, st) : mx_stream_launch(p, st);
+    return per > 16 && mx_tile_ok(p) ? mx_tile_launch(p, st) : mx_stream_launch(p, st);
 }
 
 }  // namespace chadq

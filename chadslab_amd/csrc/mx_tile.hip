@@ -30,12 +30,6 @@ struct Cfg {
     static_assert(BPS == 4 || BPS == 8, "scale bytes of a row and step: 4 or 8");
 };
 
-__device__ __forceinline__ void wg_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 // how the 16-byte pieces of row r are permuted: rows of 64 bytes, four of them to the banks, or of 128, two
 template <int ROW>
 __device__ __forceinline__ int key(int r) {
@@ -170,8 +164,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN
     int slot = 0;
     for (int i = 0; i < steps; ++i) {
         wait_vmcnt<(ST - 2) * C::REQ>();     // the wave's part of stage i is there
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): its scales are written
-        wg_barrier();                        // everybody's; and stage i - 1 has been read
+        wg_barrier();                        // everybody's, and the scales; stage i - 1 has been read
         const uint8_t *const cur = lds + slot * C::STAGE, *const sc = lds + C::S_OFF + (i & 1) * C::S_STAGE;
         scales(i + 1);
         request(i + ST - 1, lds + (slot == 0 ? ST - 1 : slot - 1) * C::STAGE);
