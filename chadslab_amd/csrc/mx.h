@@ -33,7 +33,29 @@ __device__ __forceinline__ void wg_barrier() {
 }
 
 // 32 codes as the operand of a scaled MFMA (fp4 takes the lower half of its eight registers)
-__device__ __forceinline__ i32x8 mx_operand(u32x4 v) { return i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0}; }
+__device__ __forceinline__ i32x8 mx_operand(u32x4 v) {
+    const auto w = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+    return __builtin_bit_cast(i32x8, w);
+}
+
+// B scale bytes (4 or 8) from byte `at` of a row of G on, zeros behind its end; any alignment
+template <int B>
+__device__ __forceinline__ uint64_t load_scales(const uint8_t *row, int at, int G) {
+    uint64_t v = 0;
+    if (G >= B) {
+        const int o = at < G - B ? at : G - B, cut = at - o < B - 1 ? at - o : B - 1;
+        if constexpr (B == 8) {
+            __builtin_memcpy(&v, row + o, 8);
+        } else {
+            uint32_t u;
+            __builtin_memcpy(&u, row + o, 4);
+            v = u;
+        }
+        return v >> (8 * cut);
+    }
+    for (int i = 0; i < G; ++i) v |= (uint64_t)row[i] << (8 * i);
+    return v;
+}
 
 // y[r, n] = sum_k x[r, k] w[g(r), n, k] for the rows r of group g(r) = the g with offsets[g] <= r < offsets[g + 1]
 struct MxProduct {
@@ -59,6 +81,20 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + 
 struct MxTile {
     int group, row0, rows, rest0, rest1;  // group -1: rows of no group, counted as rest0 rows from 0 on and then the rows from rest1 on
 };
+// Inclusive scan over the wave's lanes, of values that are not negative: inside the 16-lane rows, then across them
+template <typename OP>
+__device__ __forceinline__ int wave_scan(int v, OP op) {
+#define CHADQ_SCAN_STEP(CTRL, MASK) v = op(v, __builtin_amdgcn_update_dpp(0, v, CTRL, MASK, 0xF, false));
+    CHADQ_SCAN_STEP(0x111, 0xF)  // row_shr 1, 2, 4, 8
+    CHADQ_SCAN_STEP(0x112, 0xF)
+    CHADQ_SCAN_STEP(0x114, 0xF)
+    CHADQ_SCAN_STEP(0x118, 0xF)
+    CHADQ_SCAN_STEP(0x142, 0xA)  // row_bcast15 into rows 1 and 3
+    CHADQ_SCAN_STEP(0x143, 0xC)  // row_bcast31 into rows 2 and 3
+#undef CHADQ_SCAN_STEP
+    return v;
+}
+
 struct MxTiles {
     const int32_t *__restrict__ offsets;
     int E, M, TR;
@@ -72,19 +108,9 @@ struct MxTiles {
         };
         lo = at(e);
         const int next = at(e + 1);
-        lo = lo > low ? lo : low;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(lo, d);
-            if (lane >= d) lo = lo > o ? lo : o;
-        }
+        lo = wave_scan(lo > low ? lo : low, [](int a, int b) { return a > b ? a : b; });
         hi = next > lo ? next : lo;
-        upto = e < E ? (hi - lo + TR - 1) / TR : 0;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(upto, d);
-            if (lane >= d) upto += o;
-        }
+        upto = wave_scan(e < E ? (hi - lo + TR - 1) / TR : 0, [](int a, int b) { return a + b; });
     }
     // tiles of the groups, and (clear) of the rows of none
     __device__ __forceinline__ int count(bool clear) const {
@@ -121,11 +147,11 @@ struct MxTiles {
 inline int64_t mx_most_tiles(int M, int E, int TR) { return (int64_t)M / TR + (E < M ? E : M) + 2; }
 
 // The columns n0 .. n0 + cols of the tile's rows of no group, set to 0 by the workgroup's threads
-__device__ __forceinline__ void mx_clear(const MxProduct &p, const MxTile &t, int n0, int cols) {
-    const int width = p.N - n0 < cols ? p.N - n0 : cols;
+__device__ __forceinline__ void mx_clear(void *y, bool y_bf16, int N, const MxTile &t, int n0, int cols) {
+    const int width = N - n0 < cols ? N - n0 : cols;
     for (int i = threadIdx.x; i < t.rows * width; i += blockDim.x) {
         const int k = t.row0 + i / width, r = k < t.rest0 ? k : t.rest1 + (k - t.rest0);
-        store_sum(reinterpret_cast<float *>(p.y), (size_t)r * p.N + n0 + i % width, 0.f, p.y_bf16);
+        store_sum(reinterpret_cast<float *>(y), (size_t)r * N + n0 + i % width, 0.f, y_bf16);
     }
 }
 

@@ -36,25 +36,6 @@ __device__ __forceinline__ int key(int r) {
     return ROW == 64 ? (r >> 2) & 3 : (r >> 1) & 7;
 }
 
-// B scale bytes from byte `at` of a row of G on, zeros behind its end
-template <int B>
-__device__ __forceinline__ uint64_t load_scales(const uint8_t *row, int at, int G) {
-    uint64_t v = 0;
-    if (G >= B) {
-        const int o = at < G - B ? at : G - B, cut = at - o < B - 1 ? at - o : B - 1;
-        if constexpr (B == 8) {
-            __builtin_memcpy(&v, row + o, 8);
-        } else {
-            uint32_t u;
-            __builtin_memcpy(&u, row + o, 4);
-            v = u;
-        }
-        return v >> (8 * cut);
-    }
-    for (int i = 0; i < G; ++i) v |= (uint64_t)row[i] << (8 * i);
-    return v;
-}
-
 template <bool X4, bool GATED, int WN, int WM, int NB, int MB, int BPS, int ST>
 __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN * WM / 4, WN * WM / 4))) void mx_tile_kernel(MxProduct p) {
     typedef Cfg<X4, WN, WM, NB, MB, BPS, ST> C;
@@ -77,7 +58,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN
     if (p.offsets) {
         t = groups.find(tm);
         if (t.group < 0) {
-            mx_clear(p, t, n0, TO);
+            mx_clear(p.y, p.y_bf16, p.N, t, n0, TO);
             return;
         }
     }
