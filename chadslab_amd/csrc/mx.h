@@ -4,6 +4,8 @@
 // The conversions of this machine read the exponent field of a scale given as a float: e << 23 serves for every byte (0 reads
 // as 2^-127, 255 as NaN; all 256 bytes x 16 codes checked).
 #pragma once
+#include <type_traits>
+
 #include "chadq_common.h"
 
 namespace chadq {
@@ -38,22 +40,18 @@ __device__ __forceinline__ i32x8 mx_operand(u32x4 v) {
     return __builtin_bit_cast(i32x8, w);
 }
 
-// B scale bytes (4 or 8) from byte `at` of a row of G on, zeros behind its end; any alignment
+// B scale bytes (1, 2, 4 or 8) from byte `at` of a row of G on, anything behind its end; any alignment
 template <int B>
 __device__ __forceinline__ uint64_t load_scales(const uint8_t *row, int at, int G) {
     uint64_t v = 0;
-    if (G >= B) {
+    if (G >= 8) {
         const int o = at < G - B ? at : G - B, cut = at - o < B - 1 ? at - o : B - 1;
-        if constexpr (B == 8) {
-            __builtin_memcpy(&v, row + o, 8);
-        } else {
-            uint32_t u;
-            __builtin_memcpy(&u, row + o, 4);
-            v = u;
-        }
-        return v >> (8 * cut);
+        typedef std::conditional_t<B == 8, uint64_t, std::conditional_t<B == 4, uint32_t, std::conditional_t<B == 2, uint16_t, uint8_t>>> bytes_t;
+        bytes_t u;
+        __builtin_memcpy(&u, row + o, B);
+        return (bytes_t)(u >> (8 * cut));
     }
-    for (int i = 0; i < G; ++i) v |= (uint64_t)row[i] << (8 * i);
+    for (int i = 0; i < B; ++i) v |= (uint64_t)row[at + i < G ? at + i : G - 1] << (8 * i);
     return v;
 }
 
