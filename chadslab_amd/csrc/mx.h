@@ -40,20 +40,20 @@ __device__ __forceinline__ i32x8 mx_operand(u32x4 v) {
     return __builtin_bit_cast(i32x8, w);
 }
 
-// B scale bytes (1, 2, 4 or 8) from byte `at` of a row of G on, anything behind its end; any alignment
+// B scale bytes (1, 2, 4 or 8, no more than the row has) from byte `at` of a row of G on, anything behind its end; any alignment.  What is loaded near the
+// end begins before `at`: the shift that puts that right is left to the reader (get), who does not want to wait for it earlier.
 template <int B>
-__device__ __forceinline__ uint64_t load_scales(const uint8_t *row, int at, int G) {
-    uint64_t v = 0;
-    if (G >= 8) {
-        const int o = at < G - B ? at : G - B, cut = at - o < B - 1 ? at - o : B - 1;
-        typedef std::conditional_t<B == 8, uint64_t, std::conditional_t<B == 4, uint32_t, std::conditional_t<B == 2, uint16_t, uint8_t>>> bytes_t;
-        bytes_t u;
-        __builtin_memcpy(&u, row + o, B);
-        return (bytes_t)(u >> (8 * cut));
+struct MxScales {
+    typedef std::conditional_t<B == 8, uint64_t, std::conditional_t<B == 4, uint32_t, std::conditional_t<B == 2, uint16_t, uint8_t>>> bytes_t;
+    bytes_t raw;
+    int cut;
+    __device__ __forceinline__ void load(const uint8_t *row, int at, int G) {
+        const int o = at < G - B ? at : G - B;
+        cut = at - o < B - 1 ? at - o : B - 1;
+        __builtin_memcpy(&raw, row + o, B);
     }
-    for (int i = 0; i < B; ++i) v |= (uint64_t)row[at + i < G ? at + i : G - 1] << (8 * i);
-    return v;
-}
+    __device__ __forceinline__ bytes_t get() const { return (bytes_t)(raw >> (8 * cut)); }
+};
 
 // y[r, n] = sum_k x[r, k] w[g(r), n, k] for the rows r of group g(r) = the g with offsets[g] <= r < offsets[g + 1]
 struct MxProduct {

@@ -18,15 +18,6 @@ namespace chadq {
 
 constexpr int MXS_W = 8;  // waves
 
-// B scale bytes (1, 2, 4 or 8) to LDS
-template <int B>
-__device__ __forceinline__ void store_scales(uint8_t *d, uint64_t v) {
-    if constexpr (B == 8) *reinterpret_cast<uint64_t *>(d) = v;
-    else if constexpr (B == 4) *reinterpret_cast<uint32_t *>(d) = (uint32_t)v;
-    else if constexpr (B == 2) *reinterpret_cast<uint16_t *>(d) = (uint16_t)v;
-    else *d = (uint8_t)v;
-}
-
 // What the first requests need comes first in the arguments, where it arrives in registers with the wave.
 // RT: weight rows of a wave in use (<= 8); wk: log2 WK; chunk: rounds of a chunk of activations; inv: 65536 / KiB of its rows, rounded up
 // GATED: gate rows w and up rows w2, bf16(silu(gate) up)
@@ -36,7 +27,7 @@ __global__ __launch_bounds__(64 * MXS_W) __attribute__((amdgpu_waves_per_eu(4)))
     int y_bf16, const uint8_t *__restrict__ xs, const int32_t *__restrict__ offsets, int E, bool clear_rest, const int32_t *__restrict__ xrows,
     const uint8_t *__restrict__ w2, const uint8_t *__restrict__ w2s) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    constexpr int W = MXS_W, NB = GATED ? 2 : 1, UB = X4 ? 128 : 512, SP = 8 * D + 4;  // bytes of a unit of an activation row; of a row's scales in LDS
+    constexpr int W = MXS_W, NB = GATED ? 2 : 1, UB = X4 ? 128 : 512, SP = 8 * D + 8;  // bytes of a unit of an activation row; of a row's scales in LDS
     constexpr int SCALES = W * (NB + X4 * MT) * 8 * SP;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, kg = lane >> 4;
@@ -81,7 +72,7 @@ __global__ __launch_bounds__(64 * MXS_W) __attribute__((amdgpu_waves_per_eu(4)))
 #pragma unroll
     for (int a = 0; a < MT; ++a) xm[a] = a * 8 + xr < rows ? a * 8 + xr : rows - 1;
     u32x4 q[D][NB];
-    uint64_t s[NB], sx[MT];
+    MxScales<D> s[NB], sx[MT];
     auto first_unit = [&](int round) { return ((round << wk) + kp) * D; };
     auto load_w = [&](int round, int d) {
         int b = (first_unit(round) + d) * 8 + wb;
@@ -92,10 +83,10 @@ __global__ __launch_bounds__(64 * MXS_W) __attribute__((amdgpu_waves_per_eu(4)))
     auto load_s = [&](int round) {
         const int at = first_unit(round) * 8;
 #pragma unroll
-        for (int i = 0; i < NB; ++i) s[i] = load_scales<D>(srow[i], at + wb * D, G);
+        for (int i = 0; i < NB; ++i) s[i].load(srow[i], at + wb * D, G);
         if constexpr (X4)
 #pragma unroll
-            for (int a = 0; a < MT; ++a) sx[a] = load_scales<D>(xs + (size_t)(t.row0 + xm[a]) * G, at + xb * D, G);
+            for (int a = 0; a < MT; ++a) sx[a].load(xs + (size_t)(t.row0 + xm[a]) * G, at + xb * D, G);
     };
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -113,17 +104,17 @@ __global__ __launch_bounds__(64 * MXS_W) __attribute__((amdgpu_waves_per_eu(4)))
 #pragma unroll
     for (int a = 0; a < MT; ++a) xl[a] = xlds + xm[a] * pitch + xb * (UB / 8) + kp * D * UB;
     uint8_t *const sl = lds + wave * ((NB + X4 * MT) * 8 * SP);
-    if (G >= 8) wait_vmcnt<NB + X4 * MT + D * NB>();  // what has been requested since the activations
-    else wait_vmcnt<0>();
+    wait_vmcnt<NB + X4 * MT + D * NB>();  // what has been requested since the activations
     wg_barrier();
     int at = 0;  // of the round in its chunk
+    auto put_scales = [](uint8_t *d, const MxScales<D> &v) { *reinterpret_cast<typename MxScales<D>::bytes_t *>(d) = v.get(); };
     auto turn = [&](int round, bool more) {
         uint32_t sc[NB][D], sxc[MT][D];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) store_scales<D>(sl + (i * 8 + wr) * SP + wb * D, s[i]);
+        for (int i = 0; i < NB; ++i) put_scales(sl + (i * 8 + wr) * SP + wb * D, s[i]);
         if constexpr (X4)
 #pragma unroll
-            for (int a = 0; a < MT; ++a) store_scales<D>(sl + ((NB + a) * 8 + xr) * SP + xb * D, sx[a]);
+            for (int a = 0; a < MT; ++a) put_scales(sl + ((NB + a) * 8 + xr) * SP + xb * D, sx[a]);
         asm volatile("" ::: "memory");  // a wave's LDS accesses keep their order
 #pragma unroll
         for (int d = 0; d < D; ++d) {
@@ -225,7 +216,7 @@ __global__ __launch_bounds__(64 * MXS_W) __attribute__((amdgpu_waves_per_eu(4)))
 
 template <bool X4, bool GATED, bool GROUPED, int MT, int D>
 static int launch(const MxProduct &p, int RT, int wk, hipStream_t st) {
-    constexpr int W = MXS_W, NB = GATED ? 2 : 1, UB = X4 ? 128 : 512, SCALES = W * (NB + X4 * MT) * 8 * (8 * D + 4);
+    constexpr int W = MXS_W, NB = GATED ? 2 : 1, UB = X4 ? 128 : 512, SCALES = W * (NB + X4 * MT) * 8 * (8 * D + 8);
     const int U = (p.K + 255) / 256, round = D << wk, rounds = (U + round - 1) / round, rows = p.M < 8 * MT ? p.M : 8 * MT;
     const int most = 73728 / (rows * round * UB), chunk = most < 1 ? 1 : most > rounds ? rounds : most;  // two workgroups to a compute unit
     const size_t per = ((size_t)chunk * round * UB + 1023) / 1024, xb = rows * (per * 1024 + 16), part = wk ? W * MT * NB * 256 : 0;
@@ -257,8 +248,10 @@ static int launch_rows(const MxProduct &p, hipStream_t st) {
         const int rows = (int)((p.N + 256 * turns - 1) / (256 * turns));
         const int wk = rows > 32 ? 0 : rows > 16 ? 1 : rows > 8 ? 2 : 3, s = MXS_W >> wk, RT = (rows + s - 1) / s, own = (U + (1 << wk) - 1) >> wk;
         const int fit = 131072 / ((p.M < 16 ? p.M : 16) * (X4 ? 128 : 512) << wk), most = own < fit ? own : fit;
-        return most > 4   ? launch<X4, GATED, GROUPED, MT, 8>(p, RT, wk, st)
-               : most > 2 ? launch<X4, GATED, GROUPED, MT, 4>(p, RT, wk, st)
+        // (MXFP4 x: eight registers for an operand that uses four, so eight units ahead would not fit)
+        if constexpr (!X4)
+            if (most > 4) return launch<X4, GATED, GROUPED, MT, 8>(p, RT, wk, st);
+        return most > 2   ? launch<X4, GATED, GROUPED, MT, 4>(p, RT, wk, st)
                : most > 1 ? launch<X4, GATED, GROUPED, MT, 2>(p, RT, wk, st)
                           : launch<X4, GATED, GROUPED, MT, 1>(p, RT, wk, st);
     }

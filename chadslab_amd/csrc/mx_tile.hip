@@ -114,19 +114,25 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN
         const int n = wrow(r) < nrows ? wrow(r) : nrows - 1, m = r - TN < t.rows ? r - TN : t.rows - 1;
         srow[i] = !X4 || r < TN ? (second(r) ? p.w2s : p.ws) + (wfirst + n) * (size_t)G : p.xs + (size_t)(t.row0 + m) * G;
     }
-    uint64_t sv[C::SPT];
+    MxScales<BPS> sv[C::SPT];
     auto scales = [&](int step) {
 #pragma unroll
         for (int i = 0; i < C::SPT; ++i)
-            if (C::SROWS % C::T == 0 || tid + i * C::T < C::SROWS) sv[i] = load_scales<BPS>(srow[i], step * BPS, G);
+            if (C::SROWS % C::T == 0 || tid + i * C::T < C::SROWS) {
+                if (G >= BPS) {
+                    sv[i].load(srow[i], step * BPS, G);
+                } else {  // K < 32 BPS
+                    sv[i].raw = 0;
+                    sv[i].cut = 0;
+                    for (int b = 0; b < G; ++b) sv[i].raw |= (typename MxScales<BPS>::bytes_t)srow[i][b] << (8 * b);
+                }
+            }
     };
     auto keep = [&](int step) {
 #pragma unroll
         for (int i = 0; i < C::SPT; ++i)
             if (C::SROWS % C::T == 0 || tid + i * C::T < C::SROWS) {
-                uint8_t *const d = lds + C::S_OFF + (step & 1) * C::S_STAGE + (tid + i * C::T) * BPS;
-                if constexpr (BPS == 8) *reinterpret_cast<uint64_t *>(d) = sv[i];
-                else *reinterpret_cast<uint32_t *>(d) = (uint32_t)sv[i];
+                *reinterpret_cast<typename MxScales<BPS>::bytes_t *>(lds + C::S_OFF + (step & 1) * C::S_STAGE + (tid + i * C::T) * BPS) = sv[i].get();
             }
     };
 
