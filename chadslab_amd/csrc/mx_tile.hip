@@ -9,26 +9,40 @@
 // edges.  Scales are 4 or 8 bytes of a row and step, at any alignment: one thread loads those of a row a step ahead and puts them into LDS.  16-byte pieces of
 // a row are XOR-swizzled by the row so that the 16 rows that a read takes at a time cover all banks.
 #include <type_traits>
+#include <utility>
 
 #include "mx.h"
 
 namespace chadq {
 namespace mxt {
 
-template <bool X4, int WN, int WM, int NB, int MB, int BPS, int ST>
+template <bool X4, int WN, int WM, int WK, int NB, int MB, int BPS, int ST>
 struct Cfg {
-    static constexpr int NW = WN * WM, T = 64 * NW, TN = 32 * NB * WN, TM = 32 * MB * WM;
+    static constexpr int NW = WN * WM * WK, T = 64 * NW, TN = 32 * NB * WN, TM = 32 * MB * WM;
     static constexpr int WROW = BPS * 16;                                 // bytes of a weight row per step
     static constexpr int XROW = X4 ? WROW : 128, XPARTS = X4 ? 1 : BPS / 2;  // of an activation row, in parts of at most 128
-    static constexpr int W_STAGE = TN * WROW, X_STAGE = TM * XROW * XPARTS, STAGE = W_STAGE + X_STAGE;
-    static constexpr int WI = W_STAGE / (1024 * NW), XI = X_STAGE / (1024 * NW), REQ = WI + XI;  // DMA instructions per wave and step
-    static_assert(WI * 1024 * NW == W_STAGE && XI * 1024 * NW == X_STAGE, "the same number of whole DMA instructions for each wave");
+    static constexpr int W_STAGE = TN * WROW, X_STAGE = TM * XROW * XPARTS;
+    // DMA instructions per wave and step, as many for each (what is too many of them for few rows fills a place nobody reads)
+    static constexpr int WI = W_STAGE / (1024 * NW), XI = (X_STAGE + 1024 * NW - 1) / (1024 * NW), REQ = WI + XI, STAGE = W_STAGE + XI * 1024 * NW;
+    static_assert(WI * 1024 * NW == W_STAGE && X_STAGE % 1024 == 0, "whole DMA instructions");
     static constexpr int SROWS = X4 ? TN + TM : TN, SPT = (SROWS + T - 1) / T;  // rows of scales per step, per thread
     static constexpr int S_STAGE = SROWS * BPS, S_OFF = ST * STAGE;
-    static constexpr int OPER = ST * STAGE + 2 * S_STAGE;
-    static constexpr int lds(int to) { return OPER > TM * (to * 2 + 16) ? OPER : TM * (to * 2 + 16); }  // to: result columns of a tile
+    static constexpr int HB = BPS / 2 / WK;                               // scale blocks of a lane and step
+    static constexpr int SL = X4 ? HB : 4 * HB, AH = SL >= 4 ? 2 : 1;     // slices of a step; how far ahead fragments are read
+    static_assert(HB * WK * 2 == BPS && SL >= AH, "each wave has whole blocks");
+    static constexpr int OPER = ST * STAGE + 2 * S_STAGE, RED = WN * WM * (WK - 1) * NB * MB * 4096;
+    static constexpr int lds(int to) {  // to: result columns of a tile
+        const int ep = TM * (to * 2 + 16), a = OPER > RED ? OPER : RED;
+        return a > ep ? a : ep;
+    }
     static_assert(BPS == 4 || BPS == 8, "scale bytes of a row and step: 4 or 8");
 };
+
+// f(0), f(1), ... with the numbers as types
+template <typename F, int... S>
+__device__ __forceinline__ void each(F &f, std::integer_sequence<int, S...>) {
+    (f(std::integral_constant<int, S>{}), ...);
+}
 
 // how the 16-byte pieces of row r are permuted: rows of 64 bytes, four of them to the banks, or of 128, two
 template <int ROW>
@@ -36,13 +50,13 @@ __device__ __forceinline__ int key(int r) {
     return ROW == 64 ? (r >> 2) & 3 : (r >> 1) & 7;
 }
 
-template <bool X4, bool GATED, int WN, int WM, int NB, int MB, int BPS, int ST>
-__global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN * WM / 4, WN * WM / 4))) void mx_tile_kernel(MxProduct p) {
-    typedef Cfg<X4, WN, WM, NB, MB, BPS, ST> C;
+template <bool X4, bool GATED, int WN, int WM, int WK, int NB, int MB, int BPS, int ST>
+__global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_eu(WN * WM * WK / 4, WN * WM * WK / 4))) void mx_tile_kernel(MxProduct p) {
+    typedef Cfg<X4, WN, WM, WK, NB, MB, BPS, ST> C;
     constexpr int TN = C::TN, TM = C::TM, TO = GATED ? TN / 2 : TN, NW = C::NW;  // TO: result columns
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int l32 = lane & 31, kq = lane >> 5, wn = wave % WN, wm = wave / WN;
+    const int l32 = lane & 31, kq = lane >> 5, wn = wave % WN, wm = wave / WN % WM, wk = wave / (WN * WM);
     const int G = p.K >> 5, steps = (G + BPS - 1) / BPS;
 
     // ---- which tile: workgroup i runs on XCD i % 8; each XCD takes consecutive tiles, which go through 8 row tiles before the next columns, so
@@ -91,10 +105,10 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN
             const int e = ((q - C::WI) * NW + wave) * (64 / PPR) + lane / PPR, r = e % TM;
             place[q] = e / TM * 128 + 16 * ((lane % PPR) ^ key<C::XROW>(r));
             const int src = r < t.rows ? (p.rows ? p.rows[t.row0 + r] : r) : 0;
-            off[q] = r < t.rows ? (uint32_t)src * (uint32_t)xbytes + place[q] : kOut;
+            off[q] = r < t.rows && e < TM * C::XPARTS ? (uint32_t)src * (uint32_t)xbytes + place[q] : kOut;
         }
     }
-    static_assert(!GATED || C::WROW == 64 || C::WROW == 128, "a DMA instruction's rows are of one block");
+    static_assert(!GATED || 1024 / C::WROW <= 32, "a DMA instruction's rows are of one block");
     auto request = [&](int step, uint8_t *stage) {
 #pragma unroll
         for (int q = 0; q < C::REQ; ++q) {
@@ -114,8 +128,8 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN
         const int n = wrow(r) < nrows ? wrow(r) : nrows - 1, m = r - TN < t.rows ? r - TN : t.rows - 1;
         srow[i] = !X4 || r < TN ? (second(r) ? p.w2s : p.ws) + (wfirst + n) * (size_t)G : p.xs + (size_t)(t.row0 + m) * G;
     }
-    MxScales<BPS> sv[C::SPT];
-    auto scales = [&](int step) {
+    MxScales<BPS> s0[C::SPT], sv[C::SPT];
+    auto scales = [&](MxScales<BPS> *sv, int step) {
 #pragma unroll
         for (int i = 0; i < C::SPT; ++i)
             if (C::SROWS % C::T == 0 || tid + i * C::T < C::SROWS) {
@@ -128,7 +142,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN
                 }
             }
     };
-    auto keep = [&](int step) {
+    auto keep = [&](const MxScales<BPS> *sv, int step) {
 #pragma unroll
         for (int i = 0; i < C::SPT; ++i)
             if (C::SROWS % C::T == 0 || tid + i * C::T < C::SROWS) {
@@ -144,79 +158,128 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[a][b][v] = 0.f;
 
-    scales(0);
+    scales(s0, 0);
+    scales(sv, 1);
 #pragma unroll
-    for (int j = 0; j < ST - 1; ++j) request(j, lds + j * C::STAGE);
-    keep(0);
-    int slot = 0;
-    for (int i = 0; i < steps; ++i) {
-        wait_vmcnt<(ST - 2) * C::REQ>();     // the wave's part of stage i is there
-        wg_barrier();                        // everybody's, and the scales; stage i - 1 has been read
-        const uint8_t *const cur = lds + slot * C::STAGE, *const sc = lds + C::S_OFF + (i & 1) * C::S_STAGE;
-        scales(i + 1);
-        request(i + ST - 1, lds + (slot == 0 ? ST - 1 : slot - 1) * C::STAGE);
-        const uint8_t *const wl = cur + (wn * NB * 32 + l32) * C::WROW, *const sl = sc + (wn * NB * 32 + l32) * BPS + kq * (BPS / 2);
-        const int wkey = key<C::WROW>(l32), xkey = key<C::XROW>(l32);
-        const uint8_t *const xl = cur + C::W_STAGE + (wm * MB * 32 + l32) * C::XROW;
-        uint32_t ws[NB];
-#pragma unroll
-        for (int a = 0; a < NB; ++a) ws[a] = BPS == 8 ? *reinterpret_cast<const uint32_t *>(sl + a * 32 * BPS) : *reinterpret_cast<const uint16_t *>(sl + a * 32 * BPS);
+    for (int j = 0; j < ST; ++j) request(j, lds + j * C::STAGE);
+    keep(s0, 0);
+    wait_vmcnt<(ST - 1) * C::REQ>();
+    wg_barrier();
+
+    // ---- fragments.  The lane's block h of a step is kq * BPS / 2 + wk * HB + h; a slice is one of its blocks (MXFP4 x) or 8 k of it (bf16)
+    const int blk0 = kq * (BPS / 2) + wk * C::HB;
+    const uint32_t wkey = key<C::WROW>(l32), xkey = key<C::XROW>(l32);
+    const uint32_t wl = (wn * NB * 32 + l32) * C::WROW, xl = C::W_STAGE + (wm * MB * 32 + l32) * C::XROW;
+    const uint32_t sl = C::S_OFF + (wn * NB * 32 + l32) * BPS + kq * (BPS / 2), xsl = C::S_OFF + (TN + wm * MB * 32 + l32) * BPS + kq * (BPS / 2);
+    constexpr int SL = C::SL, AH = C::AH, HB = C::HB, FB = 2 * AH;  // FB: fragment buffers
+    u32x4 xf[FB][MB], wf[X4 ? FB : 1][X4 ? NB : 1];
+    u32x4 q[2][X4 ? 1 : HB][X4 ? 1 : NB];  // bf16: the packed weights of this step and the next
+    uint32_t ws[2][NB], xs[2][X4 ? MB : 1];
+    bf16x8 wo[2][X4 ? 1 : NB];
+    auto read = [&](int s, int buf, const uint8_t *stage) {
         if constexpr (X4) {
-            uint32_t xs[MB];
-            const uint8_t *const xsl = sc + (TN + wm * MB * 32 + l32) * BPS + kq * (BPS / 2);
 #pragma unroll
-            for (int b = 0; b < MB; ++b) xs[b] = BPS == 8 ? *reinterpret_cast<const uint32_t *>(xsl + b * 32 * BPS) : *reinterpret_cast<const uint16_t *>(xsl + b * 32 * BPS);
-            auto slice = [&](auto jc) {
-                constexpr int j = decltype(jc)::value;
-                i32x8 w[NB], x[MB];
+            for (int a = 0; a < NB; ++a) wf[buf][a] = *reinterpret_cast<const u32x4 *>(stage + wl + a * 32 * C::WROW + 16 * ((blk0 + s) ^ wkey));
 #pragma unroll
-                for (int a = 0; a < NB; ++a) w[a] = mx_operand(*reinterpret_cast<const u32x4 *>(wl + a * 32 * C::WROW + 16 * ((kq * (BPS / 2) + j) ^ wkey)));
+            for (int b = 0; b < MB; ++b) xf[buf][b] = *reinterpret_cast<const u32x4 *>(stage + xl + b * 32 * C::XROW + 16 * ((blk0 + s) ^ xkey));
+        } else {
+            const uint32_t piece = blk0 * 4 + s;  // of 8 bf16
 #pragma unroll
-                for (int b = 0; b < MB; ++b) x[b] = mx_operand(*reinterpret_cast<const u32x4 *>(xl + b * 32 * C::XROW + 16 * ((kq * (BPS / 2) + j) ^ xkey)));
+            for (int b = 0; b < MB; ++b) xf[buf][b] = *reinterpret_cast<const u32x4 *>(stage + xl + piece / 8 * (TM * 128) + b * 4096 + 16 * ((piece % 8) ^ xkey));
+        }
+    };
+    auto read_step = [&](int step, int par, const uint8_t *stage) {  // what is read once per step
+        const uint8_t *const sc = lds + (step & 1) * C::S_STAGE;
+        auto word = [&](uint32_t at) { return BPS == 8 ? *reinterpret_cast<const uint32_t *>(sc + at) : (uint32_t)*reinterpret_cast<const uint16_t *>(sc + at); };
+#pragma unroll
+        for (int a = 0; a < NB; ++a) ws[par][a] = word(sl + a * 32 * BPS);
+        if constexpr (X4) {
+#pragma unroll
+            for (int b = 0; b < MB; ++b) xs[par][b] = word(xsl + b * 32 * BPS);
+        } else {
+#pragma unroll
+            for (int h = 0; h < HB; ++h)
+#pragma unroll
+                for (int a = 0; a < NB; ++a) q[par][h][a] = *reinterpret_cast<const u32x4 *>(stage + wl + a * 32 * C::WROW + 16 * ((blk0 + h) ^ wkey));
+        }
+    };
+    auto dequant = [&](int s, int par, int buf) {
+        if constexpr (!X4)
+#pragma unroll
+            for (int a = 0; a < NB; ++a) wo[buf][a] = dequant8_mx(q[par][s / 4][a][s % 4], mx_scale((ws[par][a] >> (8 * (wk * HB + s / 4))) & 255u));
+    };
+
+    read_step(0, 0, lds);
+#pragma unroll
+    for (int s = 0; s < AH; ++s) read(s, s, lds);
+    dequant(0, 0, 0);
+    int slot = 0;
+    // Step i, the parity of its registers (par).  In front of slice SL - AH, whose fragments and the later ones' are in registers, the wave waits for its part of stage
+    // i + 1; behind the barrier everybody's is there and stage i has been read: step i + ST is requested into its place, and the next
+    // step's first fragments are read beside the last slices' MFMAs.
+    auto step = [&](int i, auto par_c) {
+        constexpr int par = decltype(par_c)::value;
+        uint8_t *const cur = lds + slot * C::STAGE, *const nxt = lds + (slot + 1 == ST ? 0 : slot + 1) * C::STAGE;
+        auto slice = [&](auto sc) {
+            constexpr int s = decltype(sc)::value, at = par * SL + s;  // (fragment buffers in turn over two steps)
+            if constexpr (s == SL - AH) {
+                keep(sv, i + 1);
+                wait_vmcnt<(ST - 2) * C::REQ>();
+                wg_barrier();
+                scales(sv, i + 2);
+                request(i + ST, cur);
+                read_step(i + 1, par ^ 1, nxt);
+            }
+            if constexpr (s + AH < SL) read(s + AH, (at + AH) % FB, cur);
+            else read(s + AH - SL, (at + AH) % FB, nxt);
+            if constexpr (s + 1 < SL) dequant(s + 1, par, (at + 1) & 1);
+            else dequant(0, par ^ 1, (at + 1) & 1);
+#pragma unroll
+            for (int a = 0; a < NB; ++a)
+#pragma unroll
+                for (int b = 0; b < MB; ++b) {
+                    if constexpr (X4)
+                        acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wf[at % FB][a]), mx_operand(xf[at % FB][b]), acc[a][b], 4, 4, s,
+                                                                                    (int)(ws[par][a] >> (8 * wk * HB)), s, (int)(xs[par][b] >> (8 * wk * HB)));
+                    else
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wo[at & 1][a], __builtin_bit_cast(bf16x8, xf[at % FB][b]), acc[a][b], 0, 0, 0);
+                }
+        };
+        each(slice, std::make_integer_sequence<int, SL>{});
+        slot = slot + 1 == ST ? 0 : slot + 1;
+    };
+    static_assert(2 * SL % FB == 0 && 2 * SL % 2 == 0, "the buffers after two steps are those at the beginning");
+    for (int i = 0; i < steps; i += 2) {
+        step(i, std::integral_constant<int, 0>{});
+        if (i + 1 < steps) step(i + 1, std::integral_constant<int, 1>{});
+    }
+    wait_vmcnt<0>();  // (the last requests, of zeros that nobody reads: no memory of this workgroup may be written once it has ended)
+    if constexpr (WK > 1) {  // the sums of the waves along K, in their order
+        __syncthreads();
+        f32x4 *const red = reinterpret_cast<f32x4 *>(lds) + (size_t)(wm * WN + wn) * (WK - 1) * NB * MB * 256 + lane;
+        if (wk > 0)
+#pragma unroll
+            for (int a = 0; a < NB; ++a)
+#pragma unroll
+                for (int b = 0; b < MB; ++b)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        red[(((wk - 1) * NB + a) * MB + b) * 256 + g * 64] = f32x4{acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
+        __syncthreads();
+        if (wk == 0)
+#pragma unroll
+            for (int k = 0; k < WK - 1; ++k)
 #pragma unroll
                 for (int a = 0; a < NB; ++a)
 #pragma unroll
                     for (int b = 0; b < MB; ++b)
-                        acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[a], x[b], acc[a][b], 4, 4, j, (int)ws[a], j, (int)xs[b]);
-            };
-            slice(std::integral_constant<int, 0>{});
-            slice(std::integral_constant<int, 1>{});
-            if constexpr (BPS == 8) {
-                slice(std::integral_constant<int, 2>{});
-                slice(std::integral_constant<int, 3>{});
-            }
-        } else {
 #pragma unroll
-            for (int h = 0; h < BPS / 2; ++h) {  // the lane's blocks: kq * BPS / 2 + h
-                u32x4 q[NB];
-                float s[NB];
-                const int blk = kq * (BPS / 2) + h;
+                        for (int g = 0; g < 4; ++g) {
+                            const f32x4 v = red[((k * NB + a) * MB + b) * 256 + g * 64];
 #pragma unroll
-                for (int a = 0; a < NB; ++a) {
-                    q[a] = *reinterpret_cast<const u32x4 *>(wl + a * 32 * C::WROW + 16 * (blk ^ wkey));
-                    s[a] = mx_scale((ws[a] >> (8 * h)) & 255u);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int piece = blk * 4 + j;  // of 8 bf16
-                    bf16x8 x[MB];
-#pragma unroll
-                    for (int b = 0; b < MB; ++b)
-                        x[b] = *reinterpret_cast<const bf16x8 *>(xl + piece / 8 * (TM * 128) + b * 4096 + 16 * ((piece % 8) ^ xkey));
-#pragma unroll
-                    for (int a = 0; a < NB; ++a) {
-                        const bf16x8 w = dequant8_mx(q[a][j], s[a]);
-#pragma unroll
-                        for (int b = 0; b < MB; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, x[b], acc[a][b], 0, 0, 0);
-                    }
-                }
-            }
-        }
-        keep(i + 1);
-        slot = slot + 1 == ST ? 0 : slot + 1;
+                            for (int e = 0; e < 4; ++e) acc[a][b][4 * g + e] += v[e];
+                        }
     }
-
-    wait_vmcnt<0>();  // (the last requests, of zeros that nobody reads: no memory of this workgroup may be written once it has ended)
     // ---- results.  A lane's values of a block: activation row l32, n = 8 g + 4 kq + 0..3 for g = 0..3
     constexpr int NO = GATED ? NB / 2 : NB;
     static_assert(!GATED || NB % 2 == 0, "gate and up blocks side by side");
@@ -228,6 +291,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN
 #pragma unroll
             for (int v = 0; v < 16; ++v) out[a][b][v / 4][v % 4] = GATED ? silu_mul(acc[2 * a][b][v], acc[2 * a + 1][b][v]) : acc[GATED ? 2 * a : a][b][v];
     if (!p.y_bf16) {
+        if (wk > 0) return;
         float *const y = reinterpret_cast<float *>(p.y);
         const bool quads = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
 #pragma unroll
@@ -250,6 +314,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN
     // through LDS, so that whole rows are stored
     __syncthreads();
     constexpr int PITCH = TO * 2 + 16;
+    if (wk == 0)
 #pragma unroll
     for (int a = 0; a < NO; ++a)
 #pragma unroll
@@ -275,9 +340,9 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(WN
     }
 }
 
-template <bool X4, bool GATED, int WN, int WM, int NB, int MB, int BPS, int ST>
+template <bool X4, bool GATED, int WN, int WM, int WK, int NB, int MB, int BPS, int ST>
 static int launch(const MxProduct &p, hipStream_t st) {
-    typedef Cfg<X4, WN, WM, NB, MB, BPS, ST> C;
+    typedef Cfg<X4, WN, WM, WK, NB, MB, BPS, ST> C;
     constexpr int TO = GATED ? C::TN / 2 : C::TN, LDS = C::lds(TO);
     static_assert(LDS <= 163840, "LDS of a compute unit");
     const int64_t tm = p.offsets ? mx_most_tiles(p.M, p.E, C::TM) : (p.M + C::TM - 1) / C::TM, tiles = tm * ((p.N + TO - 1) / TO);
@@ -286,10 +351,10 @@ static int launch(const MxProduct &p, hipStream_t st) {
     int dev = 0;
     CHADQ_HIP(hipGetDevice(&dev));
     if (dev >= 64 || !set[dev].load()) {
-        CHADQ_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&mx_tile_kernel<X4, GATED, WN, WM, NB, MB, BPS, ST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+        CHADQ_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&mx_tile_kernel<X4, GATED, WN, WM, WK, NB, MB, BPS, ST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
         if (dev < 64) set[dev].store(true);
     }
-    hipLaunchKernelGGL((mx_tile_kernel<X4, GATED, WN, WM, NB, MB, BPS, ST>), dim3((int)((tiles + 7) / 8 * 8)), dim3(C::T), LDS, st, p);
+    hipLaunchKernelGGL((mx_tile_kernel<X4, GATED, WN, WM, WK, NB, MB, BPS, ST>), dim3((int)((tiles + 7) / 8 * 8)), dim3(C::T), LDS, st, p);
     return hip_check(hipGetLastError(), "mxfp4 product launch");
 }
 
@@ -301,11 +366,30 @@ bool mx_tile_ok(const MxProduct &p) {
     return row * 256 < INT32_MAX && (!p.rows || row * p.x_rows < INT32_MAX);
 }
 
+#ifndef MXT_A
+#define MXT_A 0
+#endif
 int mx_tile_launch(const MxProduct &p, hipStream_t st) {
     using namespace mxt;
-    if (p.w2) return launch<false, true, 2, 4, 2, 1, 4, 3>(p, st);  // 128 weight rows (64 results) x 128
-    if (p.xs) return launch<true, false, 2, 4, 4, 2, 4, 4>(p, st);  // 256 x 256
-    return launch<false, false, 4, 2, 1, 2, 4, 3>(p, st);           // 128 x 128
+    //                                    WN WM WK NB MB BPS ST
+    const int per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;
+    if (p.w2) {
+        if (per <= 32) return launch<false, true, 2, 1, 4, 2, 1, 8, 4>(p, st);  // 128 weight rows (64 results) x 32
+        if (per <= 64) return launch<false, true, 2, 1, 4, 2, 2, 8, 3>(p, st);  // x 64
+        return launch<false, true, 2, 2, 2, 2, 2, 4, 3>(p, st);                 // x 128
+    }
+    if (p.xs) {
+        if (per <= 32) return launch<true, false, 2, 1, 4, 1, 1, 8, 6>(p, st);  // 64 x 32
+        if (per <= 64) return launch<true, false, 2, 1, 4, 1, 2, 8, 6>(p, st);  // 64 x 64
+        if (MXT_A == 1 || per <= 1024) return launch<true, false, 2, 2, 2, 2, 2, 8, 4>(p, st);  // 128 x 128
+        if (MXT_A == 2) return launch<true, false, 2, 4, 1, 4, 2, 8, 2>(p, st);  // 256 x 256
+        return launch<true, false, 2, 4, 1, 4, 2, 4, 4>(p, st);  // 256 x 256
+    }
+    if (per <= 32) return launch<false, false, 2, 1, 4, 1, 1, 8, 5>(p, st);  // 64 x 32
+    if (per <= 64) return launch<false, false, 2, 1, 4, 1, 2, 8, 3>(p, st);  // 64 x 64
+    if (MXT_A == 1 && per > 1024) return launch<false, false, 4, 2, 1, 2, 2, 4, 3>(p, st);  // 256 x 128
+    if (MXT_A == 2) return launch<false, false, 4, 2, 1, 1, 2, 4, 3>(p, st);  // 128 x 128
+    return launch<false, false, 2, 2, 2, 2, 2, 4, 3>(p, st);  // 128 x 128
 }
 
 }  // namespace chadq
