@@ -26,7 +26,7 @@ struct Cfg {
     static constexpr int WI = W_STAGE / (1024 * NW), XI = (X_STAGE + 1024 * NW - 1) / (1024 * NW), REQ = WI + XI, STAGE = W_STAGE + XI * 1024 * NW;
     static_assert(WI * 1024 * NW == W_STAGE && X_STAGE % 1024 == 0, "whole DMA instructions");
     static constexpr int SROWS = X4 ? TN + TM : TN, SPT = (SROWS + T - 1) / T;  // rows of scales per step, per thread
-    static constexpr int S_STAGE = SROWS * BPS, S_OFF = ST * STAGE;
+    static constexpr int SG = 16 / BPS, S_STAGE = SROWS * 16, S_OFF = ST * STAGE;  // steps to a load of 16 scales
     static constexpr int HB = BPS / 2 / WK;                               // scale blocks of a lane and step
     static constexpr int SL = X4 ? HB : 4 * HB, AH = SL >= 4 ? 2 : 1;     // slices of a step; how far ahead fragments are read
     static_assert(HB * WK * 2 == BPS && SL >= AH, "each wave has whole blocks");
@@ -128,26 +128,26 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
         const int n = wrow(r) < nrows ? wrow(r) : nrows - 1, m = r - TN < t.rows ? r - TN : t.rows - 1;
         srow[i] = !X4 || r < TN ? (second(r) ? p.w2s : p.ws) + (wfirst + n) * (size_t)G : p.xs + (size_t)(t.row0 + m) * G;
     }
-    MxScales<BPS> s0[C::SPT], sv[C::SPT];
-    auto scales = [&](MxScales<BPS> *sv, int step) {
+    u32x4 sv[C::SPT];
+    auto scales = [&](int group) {  // the 16 of SG steps; behind the end of a row zeros (there the activations are zeros)
 #pragma unroll
         for (int i = 0; i < C::SPT; ++i)
             if (C::SROWS % C::T == 0 || tid + i * C::T < C::SROWS) {
-                if (G >= BPS) {
-                    sv[i].load(srow[i], step * BPS, G);
-                } else {  // K < 32 BPS
-                    sv[i].raw = 0;
-                    sv[i].cut = 0;
-                    for (int b = 0; b < G; ++b) sv[i].raw |= (typename MxScales<BPS>::bytes_t)srow[i][b] << (8 * b);
+                if (group * 16 + 16 <= G) {
+                    __builtin_memcpy(&sv[i], srow[i] + group * 16, 16);
+                } else {
+                    uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int b = 0; b < 16; ++b)
+                        if (group * 16 + b < G) v[b / 4] |= (uint32_t)srow[i][group * 16 + b] << (8 * (b % 4));
+                    sv[i] = u32x4{v[0], v[1], v[2], v[3]};
                 }
             }
     };
-    auto keep = [&](const MxScales<BPS> *sv, int step) {
+    auto keep = [&](int group) {
 #pragma unroll
         for (int i = 0; i < C::SPT; ++i)
-            if (C::SROWS % C::T == 0 || tid + i * C::T < C::SROWS) {
-                *reinterpret_cast<typename MxScales<BPS>::bytes_t *>(lds + C::S_OFF + (step & 1) * C::S_STAGE + (tid + i * C::T) * BPS) = sv[i].get();
-            }
+            if (C::SROWS % C::T == 0 || tid + i * C::T < C::SROWS) *reinterpret_cast<u32x4 *>(lds + C::S_OFF + (group & 1) * C::S_STAGE + (tid + i * C::T) * 16) = sv[i];
     };
 
     f32x16 acc[NB][MB];
@@ -158,11 +158,10 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[a][b][v] = 0.f;
 
-    scales(s0, 0);
-    scales(sv, 1);
+    scales(0);
 #pragma unroll
     for (int j = 0; j < ST; ++j) request(j, lds + j * C::STAGE);
-    keep(s0, 0);
+    keep(0);
     wait_vmcnt<(ST - 1) * C::REQ>();
     wg_barrier();
 
@@ -170,7 +169,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
     const int blk0 = kq * (BPS / 2) + wk * C::HB;
     const uint32_t wkey = key<C::WROW>(l32), xkey = key<C::XROW>(l32);
     const uint32_t wl = (wn * NB * 32 + l32) * C::WROW, xl = C::W_STAGE + (wm * MB * 32 + l32) * C::XROW;
-    const uint32_t sl = C::S_OFF + (wn * NB * 32 + l32) * BPS + kq * (BPS / 2), xsl = C::S_OFF + (TN + wm * MB * 32 + l32) * BPS + kq * (BPS / 2);
+    const uint32_t sl = C::S_OFF + (wn * NB * 32 + l32) * 16 + kq * (BPS / 2), xsl = C::S_OFF + (TN + wm * MB * 32 + l32) * 16 + kq * (BPS / 2);
     constexpr int SL = C::SL, AH = C::AH, HB = C::HB, FB = 2 * AH;  // FB: fragment buffers
     u32x4 xf[FB][MB], wf[X4 ? FB : 1][X4 ? NB : 1];
     u32x4 q[2][X4 ? 1 : HB][X4 ? 1 : NB];  // bf16: the packed weights of this step and the next
@@ -189,13 +188,13 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
         }
     };
     auto read_step = [&](int step, int par, const uint8_t *stage) {  // what is read once per step
-        const uint8_t *const sc = lds + (step & 1) * C::S_STAGE;
+        const uint8_t *const sc = lds + (step / C::SG & 1) * C::S_STAGE + step % C::SG * BPS;
         auto word = [&](uint32_t at) { return BPS == 8 ? *reinterpret_cast<const uint32_t *>(sc + at) : (uint32_t)*reinterpret_cast<const uint16_t *>(sc + at); };
 #pragma unroll
-        for (int a = 0; a < NB; ++a) ws[par][a] = word(sl + a * 32 * BPS);
+        for (int a = 0; a < NB; ++a) ws[par][a] = word(sl + a * 32 * 16);
         if constexpr (X4) {
 #pragma unroll
-            for (int b = 0; b < MB; ++b) xs[par][b] = word(xsl + b * 32 * BPS);
+            for (int b = 0; b < MB; ++b) xs[par][b] = word(xsl + b * 32 * 16);
         } else {
 #pragma unroll
             for (int h = 0; h < HB; ++h)
@@ -223,10 +222,11 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
         auto slice = [&](auto sc) {
             constexpr int s = decltype(sc)::value, at = par * SL + s;  // (fragment buffers in turn over two steps)
             if constexpr (s == SL - AH) {
-                keep(sv, i + 1);
+                // (the first step of a group asks for the next group's scales, its last one puts them into LDS)
+                if ((i + 1) % C::SG == 0) keep((i + 1) / C::SG);
                 wait_vmcnt<(ST - 2) * C::REQ>();
                 wg_barrier();
-                scales(sv, i + 2);
+                if (i % C::SG == 0) scales(i / C::SG + 1);
                 request(i + ST, cur);
                 read_step(i + 1, par ^ 1, nxt);
             }
