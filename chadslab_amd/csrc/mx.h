@@ -34,6 +34,13 @@ __device__ __forceinline__ void wg_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// A value that is the same in every lane, for the compiler: a buffer's descriptor from a pointer that it takes for a lane's own costs a loop per request.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint8_t *uniform(const void *p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<uint8_t *>((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+
 // 32 codes as the operand of a scaled MFMA (fp4 takes the lower half of its eight registers)
 __device__ __forceinline__ i32x8 mx_operand(u32x4 v) {
     const auto w = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);

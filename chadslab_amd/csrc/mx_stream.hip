@@ -40,6 +40,7 @@ __global__ __launch_bounds__(64 * MXS_W) __attribute__((amdgpu_waves_per_eu(4)))
             if (clear_rest) mx_clear(y, y_bf16, N, t, nwg, (W >> wk) * RT);
             return;
         }
+        t = {uniform(t.group), uniform(t.row0), uniform(t.rows), 0, 0};
     }
     const int rows = t.rows < 8 * MT ? t.rows : 8 * MT;
 
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(64 * MXS_W) __attribute__((amdgpu_waves_per_eu(4)))
         for (int i = wave; i < rows * per; i += W) {  // past a row's end nothing is read and zeros arrive
             const int r = (i * inv) >> 16, b = (i - r * per) * 1024, at = round * rbytes + b + lane * 16;
             const int src = GATED ? __builtin_amdgcn_readfirstlane(xrows[t.row0 + r]) : t.row0 + r;
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(x) + (size_t)src * xrow, 0, xrow, 0x00020000);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(uniform(x + (size_t)src * xrow), 0, xrow, 0x00020000);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)(xlds + r * pitch + b), 16, at < xrow ? (uint32_t)at : 0x80000000u, 0, 0, 0);
         }
     };

@@ -76,6 +76,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
             return;
         }
     }
+    t = {uniform(t.group), uniform(t.row0), uniform(t.rows), 0, 0};
 
     // ---- requests
     const int wbytes = p.K >> 1, xbytes = X4 ? wbytes : p.K * 2;  // of a row
@@ -85,11 +86,11 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
     auto wrow = [](int r) { return GATED ? (r >> 6) * 32 + (r & 31) : r; };
     const size_t wfirst = (size_t)t.group * p.N + n0;
     auto weights = [&](const uint8_t *w) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(w) + wfirst * wbytes, 0, nrows * wbytes, 0x00020000);
+        return __builtin_amdgcn_make_buffer_rsrc(uniform(w + wfirst * wbytes), 0, uniform(nrows * wbytes), 0x00020000);
     };
     const __amdgpu_buffer_rsrc_t wrsrc = weights(p.w), w2rsrc = GATED ? weights(p.w2) : wrsrc;
     const __amdgpu_buffer_rsrc_t xrsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t *>(reinterpret_cast<const uint8_t *>(p.x)) + (p.rows ? (size_t)0 : (size_t)t.row0 * xbytes), 0, p.rows ? p.x_rows * xbytes : t.rows * xbytes, 0x00020000);
+        uniform(reinterpret_cast<const uint8_t *>(p.x) + (p.rows ? (size_t)0 : (size_t)t.row0 * xbytes)), 0, uniform((p.rows ? p.x_rows : t.rows) * xbytes), 0x00020000);
     constexpr uint32_t kOut = 0x80000000u;
     uint32_t off[C::REQ];
     int place[C::REQ];  // of the lane's piece in its row and step
@@ -109,16 +110,13 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
         }
     }
     static_assert(!GATED || 1024 / C::WROW <= 32, "a DMA instruction's rows are of one block");
-    auto request = [&](int step, uint8_t *stage) {
-#pragma unroll
-        for (int q = 0; q < C::REQ; ++q) {
-            const bool isw = q < C::WI;
-            const int soff = step * (isw ? C::WROW : C::XROW * C::XPARTS);
-            const uint32_t o = soff + place[q] < (isw ? wbytes : xbytes) ? off[q] : kOut;
-            const bool two = isw && GATED && second((q * NW + wave) * (1024 / C::WROW));
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(isw ? (two ? w2rsrc : wrsrc) : xrsrc, (__attribute__((address_space(3))) void *)(stage + (q * NW + wave) * 1024), 16, o, soff,
-                                                     0, 0);
-        }
+    auto request = [&](int q, int step, uint8_t *stage) {
+        const bool isw = q < C::WI;
+        const int soff = step * (isw ? C::WROW : C::XROW * C::XPARTS);
+        const uint32_t o = soff + place[q] < (isw ? wbytes : xbytes) ? off[q] : kOut;
+        const bool two = isw && GATED && second((q * NW + wave) * (1024 / C::WROW));
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(isw ? (two ? w2rsrc : wrsrc) : xrsrc, (__attribute__((address_space(3))) void *)(stage + (q * NW + wave) * 1024), 16, o, soff, 0,
+                                                 0);
     };
     // scales: the thread's rows
     const uint8_t *srow[C::SPT];
@@ -160,9 +158,11 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
 
     scales(0);
 #pragma unroll
-    for (int j = 0; j < ST; ++j) request(j, lds + j * C::STAGE);
+    for (int j = 0; j < ST - 1; ++j)
+#pragma unroll
+        for (int r = 0; r < C::REQ; ++r) request(r, j, lds + j * C::STAGE);
     keep(0);
-    wait_vmcnt<(ST - 1) * C::REQ>();
+    wait_vmcnt<(ST - 2) * C::REQ>();
     wg_barrier();
 
     // ---- fragments.  The lane's block h of a step is kq * BPS / 2 + wk * HB + h; a slice is one of its blocks (MXFP4 x) or 8 k of it (bf16)
@@ -175,21 +175,28 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
     u32x4 q[2][X4 ? 1 : HB][X4 ? 1 : NB];  // bf16: the packed weights of this step and the next
     uint32_t ws[2][NB], xs[2][X4 ? MB : 1];
     bf16x8 wo[2][X4 ? 1 : NB];
-    auto read = [&](int s, int buf, const uint8_t *stage) {
+    uint32_t xoff[SL], woff[HB];  // of a slice's fragment of the first activation block, of a block's weights
+#pragma unroll
+    for (int s = 0; s < SL; ++s) {
+        const uint32_t piece = X4 ? blk0 + s : blk0 * 4 + s;  // of 16 bytes
+        xoff[s] = xl + (X4 ? 0 : piece / 8 * (TM * 128)) + 16 * ((X4 ? piece : piece % 8) ^ xkey);
+    }
+#pragma unroll
+    for (int h = 0; h < HB; ++h) woff[h] = wl + 16 * ((blk0 + h) ^ wkey);
+    constexpr int NR = X4 ? NB + MB : MB;  // fragments of a slice: of the weights (MXFP4 x), of the activations
+    auto read = [&](int s, int f, int buf, const uint8_t *stage) {
         if constexpr (X4) {
-#pragma unroll
-            for (int a = 0; a < NB; ++a) wf[buf][a] = *reinterpret_cast<const u32x4 *>(stage + wl + a * 32 * C::WROW + 16 * ((blk0 + s) ^ wkey));
-#pragma unroll
-            for (int b = 0; b < MB; ++b) xf[buf][b] = *reinterpret_cast<const u32x4 *>(stage + xl + b * 32 * C::XROW + 16 * ((blk0 + s) ^ xkey));
+            if (f < NB) wf[buf][f] = *reinterpret_cast<const u32x4 *>(stage + woff[s] + f * 32 * C::WROW);
+            else xf[buf][f - NB] = *reinterpret_cast<const u32x4 *>(stage + xoff[s] + (f - NB) * 32 * C::XROW);
         } else {
-            const uint32_t piece = blk0 * 4 + s;  // of 8 bf16
-#pragma unroll
-            for (int b = 0; b < MB; ++b) xf[buf][b] = *reinterpret_cast<const u32x4 *>(stage + xl + piece / 8 * (TM * 128) + b * 4096 + 16 * ((piece % 8) ^ xkey));
+            xf[buf][f] = *reinterpret_cast<const u32x4 *>(stage + xoff[s] + f * 4096);
         }
     };
     auto read_step = [&](int step, int par, const uint8_t *stage) {  // what is read once per step
         const uint8_t *const sc = lds + (step / C::SG & 1) * C::S_STAGE + step % C::SG * BPS;
-        auto word = [&](uint32_t at) { return BPS == 8 ? *reinterpret_cast<const uint32_t *>(sc + at) : (uint32_t)*reinterpret_cast<const uint16_t *>(sc + at); };
+        auto word = [&](uint32_t at) {  // the wave's blocks first
+            return (BPS == 8 ? *reinterpret_cast<const uint32_t *>(sc + at) : (uint32_t)*reinterpret_cast<const uint16_t *>(sc + at)) >> (8 * wk * HB);
+        };
 #pragma unroll
         for (int a = 0; a < NB; ++a) ws[par][a] = word(sl + a * 32 * 16);
         if constexpr (X4) {
@@ -199,26 +206,29 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
 #pragma unroll
             for (int h = 0; h < HB; ++h)
 #pragma unroll
-                for (int a = 0; a < NB; ++a) q[par][h][a] = *reinterpret_cast<const u32x4 *>(stage + wl + a * 32 * C::WROW + 16 * ((blk0 + h) ^ wkey));
+                for (int a = 0; a < NB; ++a) q[par][h][a] = *reinterpret_cast<const u32x4 *>(stage + woff[h] + a * 32 * C::WROW);
         }
     };
-    auto dequant = [&](int s, int par, int buf) {
-        if constexpr (!X4)
-#pragma unroll
-            for (int a = 0; a < NB; ++a) wo[buf][a] = dequant8_mx(q[par][s / 4][a][s % 4], mx_scale((ws[par][a] >> (8 * (wk * HB + s / 4))) & 255u));
+    auto dequant = [&](int s, int a, int par, int buf) {
+        if constexpr (!X4) wo[buf][a] = dequant8_mx(q[par][s / 4][a][s % 4], mx_scale((ws[par][a] >> (8 * (s / 4))) & 255u));
     };
 
     read_step(0, 0, lds);
 #pragma unroll
-    for (int s = 0; s < AH; ++s) read(s, s, lds);
-    dequant(0, 0, 0);
+    for (int s = 0; s < AH; ++s)
+#pragma unroll
+        for (int f = 0; f < NR; ++f) read(s, f, s, lds);
+#pragma unroll
+    for (int a = 0; a < NB; ++a) dequant(0, a, 0, 0);
     int slot = 0;
     // Step i, the parity of its registers (par).  In front of slice SL - AH, whose fragments and the later ones' are in registers, the wave waits for its part of stage
-    // i + 1; behind the barrier everybody's is there and stage i has been read: step i + ST is requested into its place, and the next
-    // step's first fragments are read beside the last slices' MFMAs.
+    // i + 1; behind the barrier everybody's is there and stage i has been read: step i + ST is requested into its place, one request behind an MFMA here and there up
+    // to the next barrier, and the next step's first fragments are read beside the last slices' MFMAs.
+    constexpr int NE = NB * MB, NP = SL * NE, LATE = (SL - AH) * NE;  // MFMAs of a slice, of a step, of a step in front of its barrier
     auto step = [&](int i, auto par_c) {
         constexpr int par = decltype(par_c)::value;
         uint8_t *const cur = lds + slot * C::STAGE, *const nxt = lds + (slot + 1 == ST ? 0 : slot + 1) * C::STAGE;
+        uint8_t *const prv = lds + (slot == 0 ? ST - 1 : slot - 1) * C::STAGE;
         auto slice = [&](auto sc) {
             constexpr int s = decltype(sc)::value, at = par * SL + s;  // (fragment buffers in turn over two steps)
             if constexpr (s == SL - AH) {
@@ -227,27 +237,40 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
                 wait_vmcnt<(ST - 2) * C::REQ>();
                 wg_barrier();
                 if (i % C::SG == 0) scales(i / C::SG + 1);
-                request(i + ST, cur);
                 read_step(i + 1, par ^ 1, nxt);
             }
-            if constexpr (s + AH < SL) read(s + AH, (at + AH) % FB, cur);
-            else read(s + AH - SL, (at + AH) % FB, nxt);
-            if constexpr (s + 1 < SL) dequant(s + 1, par, (at + 1) & 1);
-            else dequant(0, par ^ 1, (at + 1) & 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int a = 0; a < NB; ++a)
+            for (int e = 0; e < NE; ++e) {
+                const int a = e / MB, b = e % MB;
+                if constexpr (X4)
+                    acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wf[at % FB][a]), mx_operand(xf[at % FB][b]), acc[a][b], 4, 4, s, (int)ws[par][a], s,
+                                                                                (int)xs[par][b]);
+                else
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wo[at & 1][a], __builtin_bit_cast(bf16x8, xf[at % FB][b]), acc[a][b], 0, 0, 0);
 #pragma unroll
-                for (int b = 0; b < MB; ++b) {
-                    if constexpr (X4)
-                        acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wf[at % FB][a]), mx_operand(xf[at % FB][b]), acc[a][b], 4, 4, s,
-                                                                                    (int)(ws[par][a] >> (8 * wk * HB)), s, (int)(xs[par][b] >> (8 * wk * HB)));
-                    else
-                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wo[at & 1][a], __builtin_bit_cast(bf16x8, xf[at % FB][b]), acc[a][b], 0, 0, 0);
+                for (int f = e * NR / NE; f < (e + 1) * NR / NE; ++f) {
+                    if constexpr (s + AH < SL) read(s + AH, f, (at + AH) % FB, cur);
+                    else read(s + AH - SL, f, (at + AH) % FB, nxt);
                 }
+#pragma unroll
+                for (int d = e * NB / NE; d < (e + 1) * NB / NE; ++d) {
+                    if constexpr (s + 1 < SL) dequant(s + 1, d, par, (at + 1) & 1);
+                    else dequant(0, d, par ^ 1, (at + 1) & 1);
+                }
+                constexpr bool late = s >= SL - AH;
+                const int pos = s * NE + e + (late ? -LATE : NP - LATE);
+#pragma unroll
+                for (int r = pos * C::REQ / NP; r < (pos + 1) * C::REQ / NP; ++r) request(r, late ? i + ST : i + ST - 1, late ? cur : prv);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
         each(slice, std::make_integer_sequence<int, SL>{});
         slot = slot + 1 == ST ? 0 : slot + 1;
     };
+    // (the requests of step ST - 1 that a step before the first one would have made behind its barrier)
+#pragma unroll
+    for (int r = 0; r < (NP - LATE) * C::REQ / NP; ++r) request(r, ST - 1, lds + (ST - 1) * C::STAGE);
     static_assert(2 * SL % FB == 0 && 2 * SL % 2 == 0, "the buffers after two steps are those at the beginning");
     for (int i = 0; i < steps; i += 2) {
         step(i, std::integral_constant<int, 0>{});
@@ -366,30 +389,49 @@ bool mx_tile_ok(const MxProduct &p) {
     return row * 256 < INT32_MAX && (!p.rows || row * p.x_rows < INT32_MAX);
 }
 
-#ifndef MXT_A
-#define MXT_A 0
+#ifndef MXT_FORCE
+#define MXT_FORCE -1
 #endif
-int mx_tile_launch(const MxProduct &p, hipStream_t st) {
+enum Tile { T64x32, T64x64, T128x64, T256x64, T128x128, T256x128, T256x256, TILES };  // weight rows x activation rows
+
+static int launch_tile(const MxProduct &p, int tile, hipStream_t st) {
     using namespace mxt;
-    //                                    WN WM WK NB MB BPS ST
-    const int per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;
+    if (MXT_FORCE >= 0) tile = MXT_FORCE;
+    //                                                       WN WM WK NB MB BPS ST
     if (p.w2) {
-        if (per <= 32) return launch<false, true, 2, 1, 4, 2, 1, 8, 4>(p, st);  // 128 weight rows (64 results) x 32
-        if (per <= 64) return launch<false, true, 2, 1, 4, 2, 2, 8, 3>(p, st);  // x 64
-        return launch<false, true, 2, 2, 2, 2, 2, 4, 3>(p, st);                 // x 128
+        switch (tile) {
+        case T64x32: case T64x64: return launch<false, true, 2, 1, 4, 2, 1, 8, 4>(p, st);  // (128 x 32)
+        case T128x64: return launch<false, true, 2, 1, 4, 2, 2, 8, 3>(p, st);
+        case T256x64: return launch<false, true, 4, 1, 2, 2, 2, 4, 4>(p, st);
+        case T128x128: return launch<false, true, 2, 2, 2, 2, 2, 4, 3>(p, st);
+        default: return launch<false, true, 4, 2, 1, 2, 2, 4, 3>(p, st);
+        }
     }
     if (p.xs) {
-        if (per <= 32) return launch<true, false, 2, 1, 4, 1, 1, 8, 6>(p, st);  // 64 x 32
-        if (per <= 64) return launch<true, false, 2, 1, 4, 1, 2, 8, 6>(p, st);  // 64 x 64
-        if (MXT_A == 1 || per <= 1024) return launch<true, false, 2, 2, 2, 2, 2, 8, 4>(p, st);  // 128 x 128
-        if (MXT_A == 2) return launch<true, false, 2, 4, 1, 4, 2, 8, 2>(p, st);  // 256 x 256
-        return launch<true, false, 2, 4, 1, 4, 2, 4, 4>(p, st);  // 256 x 256
+        switch (tile) {
+        case T64x32: return launch<true, false, 2, 1, 4, 1, 1, 8, 6>(p, st);
+        case T64x64: return launch<true, false, 2, 1, 4, 1, 2, 8, 6>(p, st);
+        case T128x64: return launch<true, false, 4, 1, 2, 1, 2, 8, 6>(p, st);
+        case T256x64: return launch<true, false, 4, 1, 2, 2, 2, 8, 3>(p, st);
+        case T128x128: return launch<true, false, 2, 2, 2, 2, 2, 8, 4>(p, st);
+        case T256x128: return launch<true, false, 4, 2, 1, 2, 2, 8, 3>(p, st);
+        default: return launch<true, false, 2, 4, 1, 4, 2, 4, 4>(p, st);
+        }
     }
-    if (per <= 32) return launch<false, false, 2, 1, 4, 1, 1, 8, 5>(p, st);  // 64 x 32
-    if (per <= 64) return launch<false, false, 2, 1, 4, 1, 2, 8, 3>(p, st);  // 64 x 64
-    if (MXT_A == 1 && per > 1024) return launch<false, false, 4, 2, 1, 2, 2, 4, 3>(p, st);  // 256 x 128
-    if (MXT_A == 2) return launch<false, false, 4, 2, 1, 1, 2, 4, 3>(p, st);  // 128 x 128
-    return launch<false, false, 2, 2, 2, 2, 2, 4, 3>(p, st);  // 128 x 128
+    switch (tile) {
+    case T64x32: return launch<false, false, 2, 1, 4, 1, 1, 8, 5>(p, st);
+    case T64x64: return launch<false, false, 2, 1, 4, 1, 2, 8, 3>(p, st);
+    case T128x64: return launch<false, false, 4, 1, 2, 1, 2, 4, 5>(p, st);
+    case T256x64: return launch<false, false, 4, 1, 2, 2, 2, 4, 4>(p, st);
+    case T128x128: return launch<false, false, 2, 2, 2, 2, 2, 4, 3>(p, st);
+    default: return launch<false, false, 4, 2, 1, 2, 2, 4, 3>(p, st);
+    }
+}
+
+int mx_tile_launch(const MxProduct &p, hipStream_t st) {
+    const int per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;
+    const int tile = per <= 32 ? T64x32 : per <= 64 ? T64x64 : p.xs && per > 1024 ? T256x256 : T128x128;
+    return launch_tile(p, tile, st);
 }
 
 }  // namespace chadq
