@@ -26,11 +26,11 @@ struct Cfg {
     static constexpr int WI = W_STAGE / (1024 * NW), XI = (X_STAGE + 1024 * NW - 1) / (1024 * NW), REQ = WI + XI, STAGE = W_STAGE + XI * 1024 * NW;
     static_assert(WI * 1024 * NW == W_STAGE && X_STAGE % 1024 == 0, "whole DMA instructions");
     static constexpr int SROWS = X4 ? TN + TM : TN, SPT = (SROWS + T - 1) / T;  // rows of scales per step, per thread
-    static constexpr int SG = 16 / BPS, S_STAGE = SROWS * 16, S_OFF = ST * STAGE;  // steps to a load of 16 scales
+    static constexpr int GB = 2 * BPS, S_STAGE = SROWS * GB, S_OFF = ST * STAGE;  // a row's scales of two steps, loaded together
     static constexpr int HB = BPS / 2 / WK;                               // scale blocks of a lane and step
     static constexpr int SL = X4 ? HB : 4 * HB, AH = SL >= 4 ? 2 : 1;     // slices of a step; how far ahead fragments are read
     static_assert(HB * WK * 2 == BPS && SL >= AH, "each wave has whole blocks");
-    static constexpr int OPER = ST * STAGE + 2 * S_STAGE, RED = WN * WM * (WK - 1) * NB * MB * 4096;
+    static constexpr int DUMP = S_OFF + 2 * S_STAGE, OPER = DUMP + (SROWS % T ? 1024 : 0), RED = WN * WM * (WK - 1) * NB * MB * 4096;
     static constexpr int lds(int to) {  // to: result columns of a tile
         const int ep = TM * (to * 2 + 16), a = OPER > RED ? OPER : RED;
         return a > ep ? a : ep;
@@ -118,34 +118,40 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
         __builtin_amdgcn_raw_ptr_buffer_load_lds(isw ? (two ? w2rsrc : wrsrc) : xrsrc, (__attribute__((address_space(3))) void *)(stage + (q * NW + wave) * 1024), 16, o, soff, 0,
                                                  0);
     };
-    // scales: the thread's rows
+    // scales: the thread's rows, GB bytes = two steps' (a group) at a time.  Those of the last group, if it is no whole one, are loaded byte by byte before the loop
+    // (zeros behind the end of the row, where the activations are zeros too).  No branch: a thread without a row loads another one's and writes where nobody reads, and
+    // so does the loop behind the last whole group.
+    constexpr int GB = C::GB, GW = GB / 4;
+    typedef __attribute__((ext_vector_type(GW))) uint32_t group_t;
+    const int whole = G / GB;
     const uint8_t *srow[C::SPT];
+    group_t sv[C::SPT], tail[C::SPT];
 #pragma unroll
     for (int i = 0; i < C::SPT; ++i) {
-        const int r = tid + i * C::T;
+        const int r = tid + i * C::T < C::SROWS ? tid + i * C::T : 0;
         const int n = wrow(r) < nrows ? wrow(r) : nrows - 1, m = r - TN < t.rows ? r - TN : t.rows - 1;
         srow[i] = !X4 || r < TN ? (second(r) ? p.w2s : p.ws) + (wfirst + n) * (size_t)G : p.xs + (size_t)(t.row0 + m) * G;
+#pragma unroll
+        for (int e = 0; e < GW; ++e) tail[i][e] = 0;
+        if (G % GB)
+#pragma unroll
+            for (int b = 0; b < GB; ++b) tail[i][b / 4] |= (whole * GB + b < G ? (uint32_t)srow[i][whole * GB + b] : 0u) << (8 * (b % 4));
+        if (whole == 0) srow[i] = p.w;  // (readable, for the loop)
     }
-    u32x4 sv[C::SPT];
-    auto scales = [&](int group) {  // the 16 of SG steps; behind the end of a row zeros (there the activations are zeros)
+    auto scales = [&](int group) {
+        const int at = (group < whole ? group : whole > 0 ? whole - 1 : 0) * GB;
 #pragma unroll
-        for (int i = 0; i < C::SPT; ++i)
-            if (C::SROWS % C::T == 0 || tid + i * C::T < C::SROWS) {
-                if (group * 16 + 16 <= G) {
-                    __builtin_memcpy(&sv[i], srow[i] + group * 16, 16);
-                } else {
-                    uint32_t v[4] = {0, 0, 0, 0};
-#pragma unroll
-                    for (int b = 0; b < 16; ++b)
-                        if (group * 16 + b < G) v[b / 4] |= (uint32_t)srow[i][group * 16 + b] << (8 * (b % 4));
-                    sv[i] = u32x4{v[0], v[1], v[2], v[3]};
-                }
-            }
+        for (int i = 0; i < C::SPT; ++i) __builtin_memcpy(&sv[i], srow[i] + at, GB);
     };
     auto keep = [&](int group) {
 #pragma unroll
-        for (int i = 0; i < C::SPT; ++i)
-            if (C::SROWS % C::T == 0 || tid + i * C::T < C::SROWS) *reinterpret_cast<u32x4 *>(lds + C::S_OFF + (group & 1) * C::S_STAGE + (tid + i * C::T) * 16) = sv[i];
+        for (int i = 0; i < C::SPT; ++i) {
+            const int r = tid + i * C::T;
+            group_t v;
+#pragma unroll
+            for (int e = 0; e < GW; ++e) v[e] = group < whole ? sv[i][e] : tail[i][e];
+            *reinterpret_cast<group_t *>(lds + (C::SROWS % C::T == 0 || r < C::SROWS ? C::S_OFF + (group & 1) * C::S_STAGE + r * GB : C::DUMP + lane * GB)) = v;
+        }
     };
 
     f32x16 acc[NB][MB];
@@ -169,7 +175,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
     const int blk0 = kq * (BPS / 2) + wk * C::HB;
     const uint32_t wkey = key<C::WROW>(l32), xkey = key<C::XROW>(l32);
     const uint32_t wl = (wn * NB * 32 + l32) * C::WROW, xl = C::W_STAGE + (wm * MB * 32 + l32) * C::XROW;
-    const uint32_t sl = C::S_OFF + (wn * NB * 32 + l32) * 16 + kq * (BPS / 2), xsl = C::S_OFF + (TN + wm * MB * 32 + l32) * 16 + kq * (BPS / 2);
+    const uint32_t sl = C::S_OFF + (wn * NB * 32 + l32) * GB + kq * (BPS / 2), xsl = C::S_OFF + (TN + wm * MB * 32 + l32) * GB + kq * (BPS / 2);
     constexpr int SL = C::SL, AH = C::AH, HB = C::HB, FB = 2 * AH;  // FB: fragment buffers
     u32x4 xf[FB][MB], wf[X4 ? FB : 1][X4 ? NB : 1];
     u32x4 q[2][X4 ? 1 : HB][X4 ? 1 : NB];  // bf16: the packed weights of this step and the next
@@ -193,15 +199,15 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
         }
     };
     auto read_step = [&](int step, int par, const uint8_t *stage) {  // what is read once per step
-        const uint8_t *const sc = lds + (step / C::SG & 1) * C::S_STAGE + step % C::SG * BPS;
+        const uint8_t *const sc = lds + (step >> 1 & 1) * C::S_STAGE + (step & 1) * BPS;
         auto word = [&](uint32_t at) {  // the wave's blocks first
             return (BPS == 8 ? *reinterpret_cast<const uint32_t *>(sc + at) : (uint32_t)*reinterpret_cast<const uint16_t *>(sc + at)) >> (8 * wk * HB);
         };
 #pragma unroll
-        for (int a = 0; a < NB; ++a) ws[par][a] = word(sl + a * 32 * 16);
+        for (int a = 0; a < NB; ++a) ws[par][a] = word(sl + a * 32 * GB);
         if constexpr (X4) {
 #pragma unroll
-            for (int b = 0; b < MB; ++b) xs[par][b] = word(xsl + b * 32 * 16);
+            for (int b = 0; b < MB; ++b) xs[par][b] = word(xsl + b * 32 * GB);
         } else {
 #pragma unroll
             for (int h = 0; h < HB; ++h)
@@ -233,10 +239,10 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
             constexpr int s = decltype(sc)::value, at = par * SL + s;  // (fragment buffers in turn over two steps)
             if constexpr (s == SL - AH) {
                 // (the first step of a group asks for the next group's scales, its last one puts them into LDS)
-                if ((i + 1) % C::SG == 0) keep((i + 1) / C::SG);
+                if constexpr (par == 1) keep((i + 1) >> 1);
                 wait_vmcnt<(ST - 2) * C::REQ>();
                 wg_barrier();
-                if (i % C::SG == 0) scales(i / C::SG + 1);
+                if constexpr (par == 0) scales((i >> 1) + 1);
                 read_step(i + 1, par ^ 1, nxt);
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -271,10 +277,11 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
     // (the requests of step ST - 1 that a step before the first one would have made behind its barrier)
 #pragma unroll
     for (int r = 0; r < (NP - LATE) * C::REQ / NP; ++r) request(r, ST - 1, lds + (ST - 1) * C::STAGE);
-    static_assert(2 * SL % FB == 0 && 2 * SL % 2 == 0, "the buffers after two steps are those at the beginning");
+    static_assert(2 * SL % FB == 0, "the buffers after two steps are those at the beginning");
+    // (A step behind the last one works on zeros.  No branch inside the loop: the compiler would move MFMAs behind it, past the barrier.)
     for (int i = 0; i < steps; i += 2) {
         step(i, std::integral_constant<int, 0>{});
-        if (i + 1 < steps) step(i + 1, std::integral_constant<int, 1>{});
+        step(i + 1, std::integral_constant<int, 1>{});
     }
     wait_vmcnt<0>();  // (the last requests, of zeros that nobody reads: no memory of this workgroup may be written once it has ended)
     if constexpr (WK > 1) {  // the sums of the waves along K, in their order
