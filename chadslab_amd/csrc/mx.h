@@ -76,6 +76,9 @@ struct MxProduct {
     const int32_t *rows = nullptr;
     int x_rows = 0;           // ... which has so many
     const uint8_t *w2 = nullptr, *w2s = nullptr;
+    // K in parts of part_k (a multiple of 512; 0: one part), the sums of part i as fp32 [M,N] from y + i M N on
+    int part_k = 0;
+    int parts() const { return part_k ? (K + part_k - 1) / part_k : 1; }
 };
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }

@@ -28,7 +28,7 @@ struct Cfg {
     static constexpr int SROWS = X4 ? TN + TM : TN, SPT = (SROWS + T - 1) / T;  // rows of scales per step, per thread
     static constexpr int GB = 2 * BPS, S_STAGE = SROWS * GB, S_OFF = ST * STAGE;  // a row's scales of two steps, loaded together
     static constexpr int HB = BPS / 2 / WK;                               // scale blocks of a lane and step
-    static constexpr int SL = X4 ? HB : 4 * HB, AH = SL >= 4 ? 2 : 1;     // slices of a step; how far ahead fragments are read
+    static constexpr int SL = X4 ? HB : 4 * HB, AH = SL >= 4 && NB * MB < 8 ? 2 : 1;  // slices of a step; how far ahead fragments are read
     static_assert(HB * WK * 2 == BPS && SL >= AH, "each wave has whole blocks");
     static constexpr int DUMP = S_OFF + 2 * S_STAGE, OPER = DUMP + (SROWS % T ? 1024 : 0), RED = WN * WM * (WK - 1) * NB * MB * 4096;
     static constexpr int lds(int to) {  // to: result columns of a tile
@@ -57,7 +57,9 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, kq = lane >> 5, wn = wave % WN, wm = wave / WN % WM, wk = wave / (WN * WM);
-    const int G = p.K >> 5, steps = (G + BPS - 1) / BPS;
+    // K of this workgroup: the scale blocks of its part, from step s0 on
+    const int G = p.K >> 5, s0 = p.part_k ? (int)blockIdx.y * (p.part_k / (32 * BPS)) : 0, gend = p.part_k && (s0 * BPS + p.part_k / 32) < G ? s0 * BPS + p.part_k / 32 : G;
+    const int steps = (gend - s0 * BPS + BPS - 1) / BPS;
 
     // ---- which tile: workgroup i runs on XCD i % 8; each XCD takes consecutive tiles, which go through 8 row tiles before the next columns, so
     // that what runs on it at one time shares rows and columns through its L2
@@ -112,8 +114,8 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
     static_assert(!GATED || 1024 / C::WROW <= 32, "a DMA instruction's rows are of one block");
     auto request = [&](int q, int step, uint8_t *stage) {
         const bool isw = q < C::WI;
-        const int soff = step * (isw ? C::WROW : C::XROW * C::XPARTS);
-        const uint32_t o = soff + place[q] < (isw ? wbytes : xbytes) ? off[q] : kOut;
+        const int soff = (s0 + step) * (isw ? C::WROW : C::XROW * C::XPARTS);
+        const uint32_t o = soff + place[q] < gend * (isw || X4 ? 16 : 64) ? off[q] : kOut;
         const bool two = isw && GATED && second((q * NW + wave) * (1024 / C::WROW));
         __builtin_amdgcn_raw_ptr_buffer_load_lds(isw ? (two ? w2rsrc : wrsrc) : xrsrc, (__attribute__((address_space(3))) void *)(stage + (q * NW + wave) * 1024), 16, o, soff, 0,
                                                  0);
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
         if (whole == 0) srow[i] = p.w;  // (readable, for the loop)
     }
     auto scales = [&](int group) {
-        const int at = (group < whole ? group : whole > 0 ? whole - 1 : 0) * GB;
+        const int g = s0 / 2 + group, at = (g < whole ? g : whole > 0 ? whole - 1 : 0) * GB;
 #pragma unroll
         for (int i = 0; i < C::SPT; ++i) __builtin_memcpy(&sv[i], srow[i] + at, GB);
     };
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
             const int r = tid + i * C::T;
             group_t v;
 #pragma unroll
-            for (int e = 0; e < GW; ++e) v[e] = group < whole ? sv[i][e] : tail[i][e];
+            for (int e = 0; e < GW; ++e) v[e] = s0 / 2 + group < whole ? sv[i][e] : tail[i][e];
             *reinterpret_cast<group_t *>(lds + (C::SROWS % C::T == 0 || r < C::SROWS ? C::S_OFF + (group & 1) * C::S_STAGE + r * GB : C::DUMP + lane * GB)) = v;
         }
     };
@@ -322,7 +324,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
             for (int v = 0; v < 16; ++v) out[a][b][v / 4][v % 4] = GATED ? silu_mul(acc[2 * a][b][v], acc[2 * a + 1][b][v]) : acc[GATED ? 2 * a : a][b][v];
     if (!p.y_bf16) {
         if (wk > 0) return;
-        float *const y = reinterpret_cast<float *>(p.y);
+        float *const y = reinterpret_cast<float *>(p.y) + (size_t)blockIdx.y * p.M * p.N;
         const bool quads = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
 #pragma unroll
         for (int a = 0; a < NO; ++a)
@@ -384,7 +386,7 @@ static int launch(const MxProduct &p, hipStream_t st) {
         CHADQ_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&mx_tile_kernel<X4, GATED, WN, WM, WK, NB, MB, BPS, ST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
         if (dev < 64) set[dev].store(true);
     }
-    hipLaunchKernelGGL((mx_tile_kernel<X4, GATED, WN, WM, WK, NB, MB, BPS, ST>), dim3((int)((tiles + 7) / 8 * 8)), dim3(C::T), LDS, st, p);
+    hipLaunchKernelGGL((mx_tile_kernel<X4, GATED, WN, WM, WK, NB, MB, BPS, ST>), dim3((int)((tiles + 7) / 8 * 8), p.parts()), dim3(C::T), LDS, st, p);
     return hip_check(hipGetLastError(), "mxfp4 product launch");
 }
 
@@ -399,7 +401,7 @@ bool mx_tile_ok(const MxProduct &p) {
 #ifndef MXT_FORCE
 #define MXT_FORCE -1
 #endif
-enum Tile { T64x32, T64x64, T128x64, T256x64, T128x128, T256x128, T256x256, TILES };  // weight rows x activation rows
+enum Tile { T64x32, T64x64, T128x64, T256x64, T128x128, T256x128, T256x256, T256x96, T128x96, T256x32, TILES };  // weight rows x activation rows
 
 static int launch_tile(const MxProduct &p, int tile, hipStream_t st) {
     using namespace mxt;
@@ -410,6 +412,9 @@ static int launch_tile(const MxProduct &p, int tile, hipStream_t st) {
         case T64x32: case T64x64: return launch<false, true, 2, 1, 4, 2, 1, 8, 4>(p, st);  // (128 x 32)
         case T128x64: return launch<false, true, 2, 1, 4, 2, 2, 8, 3>(p, st);
         case T256x64: return launch<false, true, 4, 1, 2, 2, 2, 4, 4>(p, st);
+        case T256x96: return launch<false, true, 4, 1, 2, 2, 3, 4, 3>(p, st);
+        case T128x96: return launch<false, true, 2, 1, 4, 2, 3, 8, 2>(p, st);
+        case T256x32: return launch<false, true, 4, 1, 2, 2, 1, 4, 6>(p, st);
         case T128x128: return launch<false, true, 2, 2, 2, 2, 2, 4, 3>(p, st);
         default: return launch<false, true, 4, 2, 1, 2, 2, 4, 3>(p, st);
         }
@@ -420,9 +425,12 @@ static int launch_tile(const MxProduct &p, int tile, hipStream_t st) {
         case T64x64: return launch<true, false, 2, 1, 4, 1, 2, 8, 6>(p, st);
         case T128x64: return launch<true, false, 4, 1, 2, 1, 2, 8, 6>(p, st);
         case T256x64: return launch<true, false, 4, 1, 2, 2, 2, 8, 3>(p, st);
+        case T256x96: return launch<true, false, 4, 1, 2, 2, 3, 8, 3>(p, st);
+        case T128x96: return launch<true, false, 4, 1, 2, 1, 3, 8, 4>(p, st);
+        case T256x32: return launch<true, false, 4, 1, 2, 2, 1, 8, 3>(p, st);
         case T128x128: return launch<true, false, 2, 2, 2, 2, 2, 8, 4>(p, st);
         case T256x128: return launch<true, false, 4, 2, 1, 2, 2, 8, 3>(p, st);
-        default: return launch<true, false, 2, 4, 1, 4, 2, 4, 4>(p, st);
+        default: return launch<true, false, 2, 4, 1, 4, 2, 8, 2>(p, st);
         }
     }
     switch (tile) {
@@ -430,6 +438,9 @@ static int launch_tile(const MxProduct &p, int tile, hipStream_t st) {
     case T64x64: return launch<false, false, 2, 1, 4, 1, 2, 8, 3>(p, st);
     case T128x64: return launch<false, false, 4, 1, 2, 1, 2, 4, 5>(p, st);
     case T256x64: return launch<false, false, 4, 1, 2, 2, 2, 4, 4>(p, st);
+    case T256x96: return launch<false, false, 4, 1, 2, 2, 3, 4, 3>(p, st);
+    case T128x96: return launch<false, false, 4, 1, 2, 1, 3, 4, 4>(p, st);
+    case T256x32: return launch<false, false, 4, 1, 2, 2, 1, 4, 6>(p, st);
     case T128x128: return launch<false, false, 2, 2, 2, 2, 2, 4, 3>(p, st);
     default: return launch<false, false, 4, 2, 1, 2, 2, 4, 3>(p, st);
     }
