@@ -120,24 +120,26 @@ struct MxTiles {
         hi = next > lo ? next : lo;
         upto = wave_scan(e < E ? (hi - lo + TR - 1) / TR : 0, [](int a, int b) { return a + b; });
     }
-    // tiles of the groups, and (clear) of the rows of none
-    __device__ __forceinline__ int count(bool clear) const {
-        int n = 0, low = 0, first = 0;
+    // Tiles of the groups, and (clear) of the rows of none.  at(tiles): which tile the workgroup takes of so many (or -1: none).  Returns that tile.
+    // One pass over the offsets where they are few, as their round trip to memory is what a workgroup begins with.
+    template <typename F>
+    __device__ __forceinline__ MxTile place(bool clear, F at) const {
+        int before = 0, low = 0, first = 0, lo, hi, upto;
         for (int c = 0; c < E; c += 64) {
-            int lo, hi, upto;
             scan(c, low, lo, hi, upto);
             if (c == 0) first = __builtin_amdgcn_readlane(lo, 0);
-            n += __builtin_amdgcn_readlane(upto, 63);
+            before += __builtin_amdgcn_readlane(upto, 63);
             low = __builtin_amdgcn_readlane(hi, 63);
         }
-        return n + (clear ? (first + (M - low) + TR - 1) / TR : 0);
-    }
-    __device__ __forceinline__ MxTile find(int t) const {
-        int before = 0, low = 0, first = 0;
+        const int rest = first + (M - low), t = at(before + (clear ? (rest + TR - 1) / TR : 0));
+        if (t < 0) return {-1, 0, 0, 0, 0};
+        if (t >= before) {
+            const int r0 = (t - before) * TR;
+            return {-1, r0, rest - r0 < 0 ? 0 : rest - r0 < TR ? rest - r0 : TR, first, low};
+        }
+        before = low = 0;
         for (int c = 0; c < E; c += 64) {
-            int lo, hi, upto;
-            scan(c, low, lo, hi, upto);
-            if (c == 0) first = __builtin_amdgcn_readlane(lo, 0);
+            if (E > 64) scan(c, low, lo, hi, upto);
             const unsigned long long m = __ballot(t < before + upto);
             if (m) {
                 const int l = __ffsll((long long)m) - 1, r0 = __builtin_amdgcn_readlane(lo, l), end = __builtin_amdgcn_readlane(hi, l);
@@ -147,8 +149,10 @@ struct MxTiles {
             before += __builtin_amdgcn_readlane(upto, 63);
             low = __builtin_amdgcn_readlane(hi, 63);
         }
-        const int rest = first + (M - low), r0 = (t - before) * TR;
-        return {-1, r0, rest - r0 < 0 ? 0 : rest - r0 < TR ? rest - r0 : TR, first, low};
+        return {-1, 0, 0, 0, 0};
+    }
+    __device__ __forceinline__ MxTile find(int t) const {
+        return place(false, [t](int) { return t; });
     }
 };
 // Row tiles that suffice for any offsets: full tiles of M rows, one cut per group that can have a row, one of the rest.
@@ -165,7 +169,14 @@ __device__ __forceinline__ void mx_clear(void *y, bool y_bf16, int N, const MxTi
 
 int mx_stream_launch(const MxProduct &p, hipStream_t st);
 bool mx_tile_ok(const MxProduct &p);
-int mx_tile_launch(const MxProduct &p, hipStream_t st);
+struct MxTilePick {
+    int tile, part_k;  // 0: one part
+};
+constexpr int kMxParts = 8;  // parts of K at most
+MxTilePick mx_tile_pick(const MxProduct &p, int most_parts);
+int mx_tile_part_k(int M, int N, int K, int E, bool x_mx, int most_parts);
+int mx_tile_launch(const MxProduct &p, int tile, hipStream_t st);
+int mx_tile_parts_launch(const MxProduct &p, const MxTilePick &pick, float *part, hipStream_t st);
 int mx_product_launch(const MxProduct &p, void *workspace, size_t workspace_bytes, hipStream_t st);
 size_t mx_product_workspace_bytes(int M, int N, int K, bool x_mxfp4);
 

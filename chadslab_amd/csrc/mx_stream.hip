@@ -270,11 +270,20 @@ int mx_stream_launch(const MxProduct &p, hipStream_t st) {
     return p.xs ? launch_kind<true, false, false>(p, st) : launch_kind<false, false, false>(p, st);
 }
 
-size_t mx_product_workspace_bytes(int, int, int, bool) { return 0; }
+// Up to 16 rows (of a group, on average) stream the weights, more go through the tiles
+static bool streams(int M, int E) { return (M + E - 1) / E <= 16; }
 
-int mx_product_launch(const MxProduct &p, void *, size_t, hipStream_t st) {
-    const int per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;
-    return per > 16 && mx_tile_ok(p) ? mx_tile_launch(p, st) : mx_stream_launch(p, st);
+size_t mx_product_workspace_bytes(int M, int N, int K, bool x_mxfp4) {
+    if (streams(M, 1)) return 0;
+    const int part_k = mx_tile_part_k(M, N, K, 1, x_mxfp4, kMxParts);
+    return part_k ? (size_t)((K + part_k - 1) / part_k) * M * N * 4 : 0;
+}
+
+int mx_product_launch(const MxProduct &p, void *workspace, size_t workspace_bytes, hipStream_t st) {
+    if (streams(p.M, p.offsets ? p.E : 1) || !mx_tile_ok(p)) return mx_stream_launch(p, st);
+    const size_t need = p.offsets ? 0 : mx_product_workspace_bytes(p.M, p.N, p.K, p.xs != nullptr);
+    if (need && workspace_bytes >= need) return mx_tile_parts_launch(p, mx_tile_pick(p, kMxParts), reinterpret_cast<float *>(workspace), st);
+    return mx_tile_launch(p, mx_tile_pick(p, 1).tile, st);
 }
 
 }  // namespace chadq

@@ -8,6 +8,7 @@
 // piece past the end of a row or of the matrix is requested beyond the buffer's range and arrives as zeros, so nothing in the loop knows about
 // edges.  Scales are 4 or 8 bytes of a row and step, at any alignment: one thread loads those of a row a step ahead and puts them into LDS.  16-byte pieces of
 // a row are XOR-swizzled by the row so that the 16 rows that a read takes at a time cover all banks.
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -64,19 +65,25 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
     // ---- which tile: workgroup i runs on XCD i % 8; each XCD takes consecutive tiles, which go through 8 row tiles before the next columns, so
     // that what runs on it at one time shares rows and columns through its L2
     const int tiles_n = (p.N + TO - 1) / TO;
-    const MxTiles groups = {p.offsets, p.E, p.M, TM};
-    const int tiles_m = p.offsets ? groups.count(p.clear_rest) : (p.M + TM - 1) / TM;
-    const int64_t total = (int64_t)tiles_m * tiles_n, per_xcd = (total + 7) >> 3, id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per_xcd || id >= total) return;
-    const int band = (int)(id / (8 * tiles_n)), in = (int)(id % (8 * tiles_n)), high = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
-    const int tm = band * 8 + in % high, n0 = in / high * TO;
-    MxTile t = {0, tm * TM, p.M - tm * TM < TM ? p.M - tm * TM : TM, 0, 0};
+    int n0 = 0;
+    auto take = [&](int tiles_m) {
+        const int64_t total = (int64_t)tiles_m * tiles_n, per_xcd = (total + 7) >> 3, id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+        if ((blockIdx.x >> 3) >= per_xcd || id >= total) return -1;
+        const int band = (int)(id / (8 * tiles_n)), in = (int)(id % (8 * tiles_n)), high = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+        n0 = in / high * TO;
+        return band * 8 + in % high;
+    };
+    MxTile t;
     if (p.offsets) {
-        t = groups.find(tm);
+        t = MxTiles{p.offsets, p.E, p.M, TM}.place(p.clear_rest, take);
         if (t.group < 0) {
             mx_clear(p.y, p.y_bf16, p.N, t, n0, TO);
             return;
         }
+    } else {
+        const int tm = take((p.M + TM - 1) / TM);
+        if (tm < 0) return;
+        t = {0, tm * TM, p.M - tm * TM < TM ? p.M - tm * TM : TM, 0, 0};
     }
     t = {uniform(t.group), uniform(t.row0), uniform(t.rows), 0, 0};
 
@@ -398,14 +405,11 @@ bool mx_tile_ok(const MxProduct &p) {
     return row * 256 < INT32_MAX && (!p.rows || row * p.x_rows < INT32_MAX);
 }
 
-#ifndef MXT_FORCE
-#define MXT_FORCE -1
-#endif
+// ---- which tile, and K in how many parts
 enum Tile { T64x32, T64x64, T128x64, T256x64, T128x128, T256x128, T256x256, T256x96, T128x96, T256x32, TILES };  // weight rows x activation rows
 
 static int launch_tile(const MxProduct &p, int tile, hipStream_t st) {
     using namespace mxt;
-    if (MXT_FORCE >= 0) tile = MXT_FORCE;
     //                                                       WN WM WK NB MB BPS ST
     if (p.w2) {
         switch (tile) {
@@ -446,10 +450,90 @@ static int launch_tile(const MxProduct &p, int tile, hipStream_t st) {
     }
 }
 
-int mx_tile_launch(const MxProduct &p, hipStream_t st) {
-    const int per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;
-    const int tile = per <= 32 ? T64x32 : per <= 64 ? T64x64 : p.xs && per > 1024 ? T256x256 : T128x128;
+// Time of a product by tile: `start` us once, and for each round of the compute units' workgroups `round` us and `few` (64 workgroups, at the clock that they leave) to
+// `full` (256) us per 1024 k.  Measured at 64, 256 and 512 workgroups and K = 1024 and 4096.
+struct TileTime {
+    int tn, tm;
+    float start, round, few, full;
+};
+static const TileTime kBf16[TILES] = {{64, 32, 1.5f, 2.7f, 1.46f, 1.55f},   {64, 64, 1.7f, 3.0f, 2.21f, 2.35f},  {128, 64, 1.4f, 1.8f, 4.82f, 5.1f},
+                                      {256, 64, 1.7f, 2.3f, 7.31f, 7.85f},  {128, 128, 2.4f, 2.5f, 6.07f, 7.5f}, {256, 128, 0.6f, 4.7f, 9.29f, 13.2f},
+                                      {256, 256, 0.f, 1e9f, 0.f, 0.f},      {256, 96, 2.3f, 3.1f, 8.0f, 10.5f},  {128, 96, 2.8f, 2.0f, 4.33f, 6.05f},
+                                      {256, 32, 0.7f, 2.0f, 6.65f, 6.1f}};
+static const TileTime kMx[TILES] = {{64, 32, 1.5f, 2.5f, 1.33f, 1.31f},  {64, 64, 1.4f, 3.2f, 1.26f, 1.29f},  {128, 64, 1.6f, 2.5f, 2.88f, 2.5f},
+                                    {256, 64, 1.7f, 2.3f, 4.54f, 4.15f}, {128, 128, 2.2f, 3.0f, 3.21f, 3.1f}, {256, 128, 3.0f, 2.5f, 5.05f, 5.15f},
+                                    {256, 256, 1.8f, 6.8f, 7.34f, 8.1f}, {256, 96, 2.4f, 3.3f, 5.0f, 4.6f},   {128, 96, 2.1f, 2.9f, 3.05f, 2.77f},
+                                    {256, 32, 1.3f, 1.6f, 4.41f, 3.8f}};
+
+static MxTilePick pick(int M, int N, int K, int E, bool x_mx, bool gated, int most_parts) {
+    MxTilePick best = {T128x128, 0};
+    float least = 1e30f;
+    for (int i = 0; i < TILES; ++i) {
+        const TileTime &t = (x_mx ? kMx : kBf16)[i];
+        const int tn = gated ? (t.tn < 128 ? 64 : t.tn / 2) : t.tn;
+        if (t.round > 1e8f || (gated && t.tn < 128)) continue;
+        // rows by group: between the tiles of groups of one size and those of exponentially distributed sizes
+        const float mean = (float)M / E > 1.f ? (float)M / E : 1.f, hit = E * (1.f - expf(-(float)M / E)), even = mean / t.tm + 0.3f;
+        const float tm = E > 1 ? hit * 0.5f * ((even > 1.f ? even : 1.f) + 1.f / (1.f - expf(-t.tm / mean))) : (float)((M + t.tm - 1) / t.tm);
+        const float tiles = tm * ((N + tn - 1) / tn);
+        for (int parts = 1; parts <= most_parts; ++parts) {
+            const int part_k = parts > 1 ? ((K + parts - 1) / parts + 511) / 512 * 512 : K;
+            if (parts > 1 && (part_k < 1024 || (int64_t)part_k * (parts - 1) >= K)) continue;
+            const float wgs = tiles * parts, full = wgs >= 256.f ? 1.f : wgs <= 64.f ? 0.f : (wgs - 64.f) / 192.f;
+            const float rounds = E > 1 && wgs > 256.f ? wgs / 256.f + 0.3f : ceilf(wgs / 256.f);
+            float us = t.start + rounds * (t.round + (t.few + (t.full - t.few) * full) * (part_k / 1024.f));
+            if (parts > 1) us += 3.f + (8.f * parts + 2.f) * M * (float)N * 2.5e-7f;  // the sums written, read again and joined by another launch
+            if (us < least * (parts > 1 ? 0.95f : 1.f)) {
+                least = us;
+                best = {i, parts > 1 ? part_k : 0};
+            }
+        }
+    }
+    return best;
+}
+
+MxTilePick mx_tile_pick(const MxProduct &p, int most_parts) { return pick(p.M, p.N, p.K, p.offsets ? p.E : 1, p.xs != nullptr, p.w2 != nullptr, most_parts); }
+int mx_tile_part_k(int M, int N, int K, int E, bool x_mx, int most_parts) { return pick(M, N, K, E, x_mx, false, most_parts).part_k; }
+
+int mx_tile_launch(const MxProduct &p, int tile, hipStream_t st) {
+#ifdef MXT_FORCE
+    tile = MXT_FORCE;
+#endif
     return launch_tile(p, tile, st);
+}
+
+// y = the parts' sums, added in their order; four values to a thread where the rows allow
+__global__ __launch_bounds__(256) void mx_join_kernel(const float *__restrict__ part, void *__restrict__ y, int64_t n, int parts, bool y_bf16, bool quads) {
+    const int64_t stride = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (quads) {
+        for (int64_t i = at; i < n / 4; i += stride) {
+            f32x4 v = reinterpret_cast<const f32x4 *>(part)[i];
+            for (int k = 1; k < parts; ++k) v += reinterpret_cast<const f32x4 *>(part + k * n)[i];
+            if (y_bf16) reinterpret_cast<u32x2 *>(y)[i] = u32x2{pack_bf16_rne(v.x, v.y), pack_bf16_rne(v.z, v.w)};
+            else reinterpret_cast<f32x4 *>(y)[i] = v;
+        }
+    } else {
+        for (int64_t i = at; i < n; i += stride) {
+            float v = part[i];
+            for (int k = 1; k < parts; ++k) v += part[k * n + i];
+            store_sum(reinterpret_cast<float *>(y), i, v, y_bf16);
+        }
+    }
+}
+
+// The product in parts of K: fp32 sums to `part`, joined into y
+int mx_tile_parts_launch(const MxProduct &p, const MxTilePick &pick, float *part, hipStream_t st) {
+    MxProduct q = p;
+    q.y = part;
+    q.y_bf16 = false;
+    q.part_k = pick.part_k;
+    const int rc = mx_tile_launch(q, pick.tile, st);
+    if (rc) return rc;
+    const int64_t n = (int64_t)p.M * p.N;
+    const bool quads = n % 4 == 0 && aligned16(p.y);
+    const int64_t items = quads ? n / 4 : n;
+    hipLaunchKernelGGL(mx_join_kernel, dim3((int)(items < 2048 * 256 ? (items + 255) / 256 : 2048)), dim3(256), 0, st, part, p.y, n, q.parts(), p.y_bf16, quads);
+    return hip_check(hipGetLastError(), "mxfp4 join launch");
 }
 
 }  // namespace chadq
