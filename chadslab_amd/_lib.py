@@ -136,6 +136,8 @@ _NATIVE_ENTRIES = ("chadq_gemv_i4g32", "chadq_gemv_i4g32_bf16", "chadq_gemm_i4g3
                    "chadq_gemm_i8row_bf16", "chadq_gemm_bf16_workspace_bytes", "chadq_gemm_i4g32_bf16_ws", "chadq_gemm_i8row_bf16_ws",
                    "chadq_gemv_workspace_bytes", "chadq_gemv_i4g32_ws", "chadq_gemv_i8row_ws",
                    "chadq_moe_ffn_i4g32_workspace_bytes", "chadq_moe_ffn_i4g32", "chadq_moe_ffn_i4g32_tiled")
+_NATIVE_MX_ENTRIES = ("chadq_quantize_mxfp4", "chadq_dequant_mxfp4", "chadq_product_mxfp4_workspace_bytes", "chadq_product_mxfp4", "chadq_product_mxfp4_grouped",
+                      "chadq_moe_ffn_mxfp4_workspace_bytes", "chadq_moe_ffn_mxfp4")
 
 
 HOST_PATH = Path(__file__).resolve().parent / "_host_call.so"
@@ -150,11 +152,31 @@ class _NoHostModule:
         pass
 
     @staticmethod
+    def bind_mx(addresses, containers):
+        pass
+
+    @staticmethod
     def linear(x, weight, out_dtype):
         return None
 
     @staticmethod
     def moe_ffn(x, logits, experts, top_k, renorm):
+        return None
+
+    @staticmethod
+    def quantize(x):
+        return None
+
+    @staticmethod
+    def dequantize(qw):
+        return None
+
+    @staticmethod
+    def grouped(x, experts, offsets):
+        return None
+
+    @staticmethod
+    def moe_ffn_mx(x, logits, experts, top_k, renorm):
         return None
 
     @staticmethod
@@ -188,10 +210,13 @@ def native():
             warnings.warn("calls take some 3 us longer without the host module (`python -m chadslab_amd.build` builds it): %s" % e,
                           RuntimeWarning, stacklevel=3)
             _native = _NoHostModule
-    from .formats import QWeightInt4G32, QWeightInt4G32Tiles, QWeightInt8
+    from .formats import QExpertsMXFP4, QWeightInt4G32, QWeightInt4G32Tiles, QWeightInt8, QWeightMXFP4
 
-    _native.bind(tuple(ctypes.cast(getattr(lib, n), c_void_p).value for n in _NATIVE_ENTRIES), (QWeightInt4G32, QWeightInt8, QWeightInt4G32Tiles),
-                 check)
+    def addresses(names):
+        return tuple(ctypes.cast(getattr(lib, n), c_void_p).value for n in names)
+
+    _native.bind(addresses(_NATIVE_ENTRIES), (QWeightInt4G32, QWeightInt8, QWeightInt4G32Tiles), check)
+    _native.bind_mx(addresses(_NATIVE_MX_ENTRIES), (QWeightMXFP4, QExpertsMXFP4))
     _native_lib = lib
     return _native
 

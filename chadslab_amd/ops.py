@@ -88,6 +88,9 @@ def quantize_mxfp4(x: torch.Tensor) -> Union[QWeightMXFP4, QExpertsMXFP4]:
 
     Per block of 32 values along K the scale is 2^(floor(log2(largest magnitude)) - 2), at least 2^-127; each value goes to the nearest code,
     ties to the even one, beyond 6 scales to 6.  A block that holds a NaN or an infinity becomes NaN."""
+    q = _lib.native().quantize(x)
+    if q is not None:
+        return q
     if x.dtype not in _MX_TYPES:
         raise ValueError("x must be float32, bfloat16 or float16, got %s" % x.dtype)
     if x.dim() not in (2, 3) or x.size(-1) % GROUP:
@@ -105,6 +108,9 @@ def dequantize(qw: Union[QWeight, QExpertsMXFP4]) -> torch.Tensor:
     """fp32 [N,K] dequantised weights (exact); [E,N,K] of QExpertsMXFP4."""
     lib = _lib.load()
     if isinstance(qw, (QWeightMXFP4, QExpertsMXFP4)):
+        out = _lib.native().dequantize(qw)
+        if out is not None:
+            return out
         p, s = _mxfp4(qw, "qw")
         out = torch.empty(*p.shape[:-1], qw.K, dtype=torch.float32, device=p.device)
         if out.numel():
@@ -161,6 +167,10 @@ def qgemm_grouped(x: Union[torch.Tensor, QWeightMXFP4], experts: QExpertsMXFP4, 
     x bf16 [R,K] or QWeightMXFP4 of R rows; offsets int32 [E+1] on the GPU, read there (groups of any size, empty ones too, no host round trip); y bf16
     [R,N], fp32 sums.  Rows in front of offsets[0] and behind offsets[E] are 0 in a fresh result and left as they are in `out`.  Offsets beyond [0, R] count as its ends, one
     that descends as the largest before it."""
+    if out is None:
+        y = _lib.native().grouped(x, experts, offsets)
+        if y is not None:
+            return y
     x_mx = isinstance(x, QWeightMXFP4)
     if not isinstance(experts, QExpertsMXFP4):
         raise TypeError("qgemm_grouped wants QExpertsMXFP4, got %r" % type(experts))
@@ -287,13 +297,13 @@ def qlinear(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, *, out_dtype: Opt
     out_dtype picks the result type.  The GEMV writes bf16 itself if that is asked for (the same sums rounded once); any
     other type than the kernel's native one is a cast.  x may be a QWeightMXFP4 where the weights are.
     """
-    if isinstance(x, QWeightMXFP4):
-        y = _qlinear_2d(x, qw, out_dtype if out_dtype == torch.bfloat16 else None)
-        return y if out_dtype is None or y.dtype == out_dtype else y.to(out_dtype)
     native = _lib.native()
     y = native.linear(x, qw, out_dtype)
     if y is not None:
         return y
+    if isinstance(x, QWeightMXFP4):
+        y = _qlinear_2d(x, qw, out_dtype if out_dtype == torch.bfloat16 else None)
+        return y if out_dtype is None or y.dtype == out_dtype else y.to(out_dtype)
     # more dimensions, strides and a cast at the end are dealt with here, around the native call (8.7 -> 6.2 us of host time for an x of three
     # dimensions, 12.2 -> 9.8 with a cast)
     x2 = (x if x.dim() == 2 else x.reshape(-1, x.shape[-1])).contiguous()
@@ -406,6 +416,9 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, experts, *, top_k: int = 2, r
 
 
 def _moe_ffn_mxfp4(x: torch.Tensor, logits: torch.Tensor, experts, top_k: int, renorm: bool) -> torch.Tensor:
+    y = _lib.native().moe_ffn_mx(x, logits, experts, top_k, renorm)
+    if y is not None:
+        return y
     if len(experts) != 3 or not all(isinstance(m, QExpertsMXFP4) for m in experts):
         raise TypeError("MXFP4 experts are one (gate, up, down) triple of QExpertsMXFP4")
     x, z = _dev(x, "x", torch.bfloat16), _dev(logits, "logits", torch.float32)
