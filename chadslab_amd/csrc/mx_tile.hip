@@ -51,41 +51,16 @@ __device__ __forceinline__ int key(int r) {
     return ROW == 64 ? (r >> 2) & 3 : (r >> 1) & 7;
 }
 
+// The tile t, n0 by MB blocks of rows per wave
 template <bool X4, bool GATED, int WN, int WM, int WK, int NB, int MB, int BPS, int ST>
-__global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_eu(WN * WM * WK / 4, WN * WM * WK / 4))) void mx_tile_kernel(MxProduct p) {
+__device__ __forceinline__ void tile_body(const MxProduct &p, const MxTile &t, int n0, uint8_t *lds) {
     typedef Cfg<X4, WN, WM, WK, NB, MB, BPS, ST> C;
     constexpr int TN = C::TN, TM = C::TM, TO = GATED ? TN / 2 : TN, NW = C::NW;  // TO: result columns
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, kq = lane >> 5, wn = wave % WN, wm = wave / WN % WM, wk = wave / (WN * WM);
     // K of this workgroup: the scale blocks of its part, from step s0 on
     const int G = p.K >> 5, s0 = p.part_k ? (int)blockIdx.y * (p.part_k / (32 * BPS)) : 0, gend = p.part_k && (s0 * BPS + p.part_k / 32) < G ? s0 * BPS + p.part_k / 32 : G;
     const int steps = (gend - s0 * BPS + BPS - 1) / BPS;
-
-    // ---- which tile: workgroup i runs on XCD i % 8; each XCD takes consecutive tiles, which go through 8 row tiles before the next columns, so
-    // that what runs on it at one time shares rows and columns through its L2
-    const int tiles_n = (p.N + TO - 1) / TO;
-    int n0 = 0;
-    auto take = [&](int tiles_m) {
-        const int64_t total = (int64_t)tiles_m * tiles_n, per_xcd = (total + 7) >> 3, id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-        if ((blockIdx.x >> 3) >= per_xcd || id >= total) return -1;
-        const int band = (int)(id / (8 * tiles_n)), in = (int)(id % (8 * tiles_n)), high = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
-        n0 = in / high * TO;
-        return band * 8 + in % high;
-    };
-    MxTile t;
-    if (p.offsets) {
-        t = MxTiles{p.offsets, p.E, p.M, TM}.place(p.clear_rest, take);
-        if (t.group < 0) {
-            mx_clear(p.y, p.y_bf16, p.N, t, n0, TO);
-            return;
-        }
-    } else {
-        const int tm = take((p.M + TM - 1) / TM);
-        if (tm < 0) return;
-        t = {0, tm * TM, p.M - tm * TM < TM ? p.M - tm * TM : TM, 0, 0};
-    }
-    t = {uniform(t.group), uniform(t.row0), uniform(t.rows), 0, 0};
 
     // ---- requests
     const int wbytes = p.K >> 1, xbytes = X4 ? wbytes : p.K * 2;  // of a row
@@ -380,6 +355,44 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
 }
 
 template <bool X4, bool GATED, int WN, int WM, int WK, int NB, int MB, int BPS, int ST>
+__global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_eu(WN * WM * WK / 4, WN * WM * WK / 4))) void mx_tile_kernel(MxProduct p) {
+    typedef Cfg<X4, WN, WM, WK, NB, MB, BPS, ST> C;
+    constexpr int TM = C::TM, TO = GATED ? C::TN / 2 : C::TN;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    // Which tile: workgroup i runs on XCD i % 8; each XCD takes consecutive tiles, which go through 8 row tiles before the next columns, so
+    // that what runs on it at one time shares rows and columns through its L2
+    const int tiles_n = (p.N + TO - 1) / TO;
+    int n0 = 0;
+    auto take = [&](int tiles_m) {
+        const int64_t total = (int64_t)tiles_m * tiles_n, per_xcd = (total + 7) >> 3, id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+        if ((blockIdx.x >> 3) >= per_xcd || id >= total) return -1;
+        const int band = (int)(id / (8 * tiles_n)), in = (int)(id % (8 * tiles_n)), high = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+        n0 = in / high * TO;
+        return band * 8 + in % high;
+    };
+    MxTile t;
+    if (p.offsets) {
+        t = MxTiles{p.offsets, p.E, p.M, TM}.place(p.clear_rest, take);
+        if (t.group < 0) {
+            mx_clear(p.y, p.y_bf16, p.N, t, n0, TO);
+            return;
+        }
+    } else {
+        const int tm = take((p.M + TM - 1) / TM);
+        if (tm < 0) return;
+        t = {0, tm * TM, p.M - tm * TM < TM ? p.M - tm * TM : TM, 0, 0};
+    }
+    t = {uniform(t.group), uniform(t.row0), uniform(t.rows), 0, 0};
+    // A cut tile takes as many blocks of 32 rows as it has
+    if constexpr (WM == 1 && MB > 1) {
+        if (t.rows <= 32) return tile_body<X4, GATED, WN, WM, WK, NB, 1, BPS, ST>(p, t, n0, lds);
+        if constexpr (MB > 2)
+            if (t.rows <= 64) return tile_body<X4, GATED, WN, WM, WK, NB, 2, BPS, ST>(p, t, n0, lds);
+    }
+    tile_body<X4, GATED, WN, WM, WK, NB, MB, BPS, ST>(p, t, n0, lds);
+}
+
+template <bool X4, bool GATED, int WN, int WM, int WK, int NB, int MB, int BPS, int ST>
 static int launch(const MxProduct &p, hipStream_t st) {
     typedef Cfg<X4, WN, WM, WK, NB, MB, BPS, ST> C;
     constexpr int TO = GATED ? C::TN / 2 : C::TN, LDS = C::lds(TO);
@@ -481,7 +494,9 @@ static MxTilePick pick(int M, int N, int K, int E, bool x_mx, bool gated, int mo
             if (parts > 1 && (part_k < 1024 || (int64_t)part_k * (parts - 1) >= K)) continue;
             const float wgs = tiles * parts, full = wgs >= 256.f ? 1.f : wgs <= 64.f ? 0.f : (wgs - 64.f) / 192.f;
             const float rounds = E > 1 && wgs > 256.f ? wgs / 256.f + 0.3f : ceilf(wgs / 256.f);
-            float us = t.start + rounds * (t.round + (t.few + (t.full - t.few) * full) * (part_k / 1024.f));
+            // (a cut tile one wave high takes fewer blocks of rows; one block costs this share of two or three)
+            const float one = E == 1 ? 1.f : t.tm == 96 ? 0.6f : t.tm == 64 ? 0.8f : 1.f, rows = (float)M / (tm * t.tm);
+            float us = t.start + rounds * (t.round + (t.few + (t.full - t.few) * full) * (one + (1.f - one) * (rows < 1.f ? rows : 1.f)) * (part_k / 1024.f));
             if (parts > 1) us += 3.f + (8.f * parts + 2.f) * M * (float)N * 2.5e-7f;  // the sums written, read again and joined by another launch
             if (us < least * (parts > 1 ? 0.95f : 1.f)) {
                 least = us;
