@@ -649,13 +649,14 @@ int chadq_dequant_mxfp4(const uint8_t *codes, const uint8_t *scale, float *w, in
 }
 
 size_t chadq_product_mxfp4_workspace_bytes(int M, int N, int K, int x_mxfp4) {
-    return M > 0 && N > 0 && K >= 32 && K % 32 == 0 ? mx_product_workspace_bytes(M, N, K, x_mxfp4 != 0) : 0;
+    return M > 0 && N > 0 && K >= 32 && K % 32 == 0 && K <= kMxMostK ? mx_product_workspace_bytes(M, N, K, x_mxfp4 != 0) : 0;
 }
 
 int chadq_product_mxfp4(const void *x, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, void *y, int y_bf16, int M, int N, int K,
                         void *workspace, size_t workspace_bytes, void *stream) {
     ENTER();
-    CHADQ_REQUIRE(M >= 0 && N >= 0 && K >= 32 && K % 32 == 0, CHADQ_ERR_SHAPE, "chadq_product_mxfp4: M=%d N=%d K=%d (K must be a positive multiple of 32)", M, N, K);
+    CHADQ_REQUIRE(M >= 0 && N >= 0 && K >= 32 && K % 32 == 0 && K <= kMxMostK, CHADQ_ERR_SHAPE,
+                  "chadq_product_mxfp4: M=%d N=%d K=%d (K must be a positive multiple of 32 up to 2^26)", M, N, K);
     if (M == 0 || N == 0) return 0;
     CHADQ_REQUIRE(x && w && w_scale && y, CHADQ_ERR_NULL, "chadq_product_mxfp4: null pointer");
     CHADQ_REQUIRE(aligned16(x) && aligned16(w) && aligned16(workspace), CHADQ_ERR_ALIGN, "chadq_product_mxfp4: x, w and workspace must be 16-byte aligned");
@@ -666,8 +667,8 @@ int chadq_product_mxfp4(const void *x, const uint8_t *x_scale, const uint8_t *w,
 int chadq_product_mxfp4_grouped(const void *x, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const int32_t *offsets,
                                 uint16_t *y_bf16, int M, int E, int N, int K, int clear_rest, void *stream) {
     ENTER();
-    CHADQ_REQUIRE(M >= 0 && E >= 1 && N >= 0 && K >= 32 && K % 32 == 0, CHADQ_ERR_SHAPE,
-                  "chadq_product_mxfp4_grouped: M=%d E=%d N=%d K=%d (E at least 1, K a positive multiple of 32)", M, E, N, K);
+    CHADQ_REQUIRE(M >= 0 && E >= 1 && N >= 0 && K >= 32 && K % 32 == 0 && K <= kMxMostK, CHADQ_ERR_SHAPE,
+                  "chadq_product_mxfp4_grouped: M=%d E=%d N=%d K=%d (E at least 1, K a positive multiple of 32 up to 2^26)", M, E, N, K);
     if (M == 0 || N == 0) return 0;
     CHADQ_REQUIRE(x && w && w_scale && offsets && y_bf16, CHADQ_ERR_NULL, "chadq_product_mxfp4_grouped: null pointer");
     CHADQ_REQUIRE(aligned16(x) && aligned16(w), CHADQ_ERR_ALIGN, "chadq_product_mxfp4_grouped: x and w must be 16-byte aligned");
@@ -678,7 +679,7 @@ int chadq_product_mxfp4_grouped(const void *x, const uint8_t *x_scale, const uin
 
 // (the rows of the products, T * top_k, are counted in 32 bits)
 static bool moe_mxfp4_sizes_ok(int T, int H, int F, int E, int top_k) {
-    return moe_sizes_ok(T, H, F, E, top_k) && (int64_t)T * top_k <= INT32_MAX;
+    return moe_sizes_ok(T, H, F, E, top_k) && (int64_t)T * top_k <= INT32_MAX && H <= kMxMostK && F <= kMxMostK;
 }
 
 size_t chadq_moe_ffn_mxfp4_workspace_bytes(int T, int H, int F, int E, int top_k) {

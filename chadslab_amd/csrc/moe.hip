@@ -498,11 +498,17 @@ int moe_ffn_i4g32_launch(const uint16_t *x, const float *logits, const chadq_moe
 
 // ---- the same on MXFP4 experts, E matrices of each kind one behind the other: router, gate and up with the SiLU gate in one product by
 // group that reads the activations through the sorted token list, down to fp32, combine.
-// Parts of K of the down product, which the combine adds as it does those of the int4 experts
-static int moe_mx_parts(int P, int H, int F, int E, int *part_k) {
-    const int k = (P + E - 1) / E > 16 ? mx_tile_part_k(P, H, F, E, false, MOE_KSPLIT) : 0;
-    if (part_k) *part_k = k;
-    return k ? (F + k - 1) / k : 1;
+// The down product of the MXFP4 experts, K in parts where that is quicker: the combine adds them as it does those of the int4 experts
+static MxProduct moe_mx_down(int P, int H, int F, int E, const int32_t *offsets) {
+    static const int32_t any = 0;
+    MxProduct p = {};
+    p.offsets = offsets ? offsets : &any;
+    p.M = P;
+    p.N = H;
+    p.K = F;
+    p.E = E;
+    p.part_k = mx_product_part_k(p, kMxGroupParts);
+    return p;
 }
 
 static size_t moe_mx_layout(uint8_t *base, int T, int H, int F, int E, int top_k, MoeWs *ws) {
@@ -522,7 +528,7 @@ static size_t moe_mx_layout(uint8_t *base, int T, int H, int F, int E, int top_k
     w.groups = (GemmGroup *)take((size_t)3 * E * sizeof(GemmGroup));  // the router's, read by nobody here
     w.tiles = (int32_t *)take((size_t)E * 4);
     w.h = (uint16_t *)take(P * F * 2);
-    w.yp = (float *)take(P * H * 4 * moe_mx_parts((int)P, H, F, E, nullptr));
+    w.yp = (float *)take(P * H * 4 * moe_mx_down((int)P, H, F, E, nullptr).parts());
     if (ws) *ws = w;
     return o;
 }
@@ -547,12 +553,15 @@ int moe_ffn_mxfp4_launch(const uint16_t *x, const float *logits, const chadq_moe
     gu.w2s = ex->up_scale;
     rc = mx_product_launch(gu, nullptr, 0, st);
     if (rc) return rc;
-    MxProduct down = {ws.h, nullptr, ex->down, ex->down_scale, ws.yp, ws.cnt + E, P, H, F, E, false, false};
-    const int parts = moe_mx_parts(P, H, F, E, &down.part_k);
-    rc = parts > 1 ? mx_tile_launch(down, mx_tile_pick(down, MOE_KSPLIT).tile, st) : mx_product_launch(down, nullptr, 0, st);
+    MxProduct down = moe_mx_down(P, H, F, E, ws.cnt + E);
+    down.x = ws.h;
+    down.w = ex->down;
+    down.ws = ex->down_scale;
+    down.y = ws.yp;
+    rc = mx_product_launch(down, nullptr, 0, st);
     if (rc) return rc;
     const int64_t quads = (int64_t)T * (H / 4);
-    hipLaunchKernelGGL(moe_combine_kernel, dim3(quads < 1024 * 256 ? (int)((quads + 255) / 256) : 1024), dim3(256), 0, st, ws.yp, ws.pos, ws.w, y, T, H, top_k, parts,
+    hipLaunchKernelGGL(moe_combine_kernel, dim3(quads < 1024 * 256 ? (int)((quads + 255) / 256) : 1024), dim3(256), 0, st, ws.yp, ws.pos, ws.w, y, T, H, top_k, down.parts(),
                        (size_t)P * H);
     return hip_check(hipGetLastError(), "moe combine launch");
 }

@@ -172,11 +172,12 @@ bool mx_tile_ok(const MxProduct &p);
 struct MxTilePick {
     int tile, part_k;  // 0: one part
 };
-constexpr int kMxParts = 8;  // parts of K at most
+constexpr int kMxMostK = 1 << 26;  // bytes of an activation row are counted in 32 bits
+constexpr int kMxParts = 8, kMxGroupParts = 4;  // parts of K at most, of a product by group (which its caller joins)
 MxTilePick mx_tile_pick(const MxProduct &p, int most_parts);
-int mx_tile_part_k(int M, int N, int K, int E, bool x_mx, int most_parts);
 int mx_tile_launch(const MxProduct &p, int tile, hipStream_t st);
-int mx_tile_parts_launch(const MxProduct &p, const MxTilePick &pick, float *part, hipStream_t st);
+int mx_tile_parts_launch(const MxProduct &p, int tile, float *part, hipStream_t st);
+int mx_product_part_k(const MxProduct &p, int most_parts);
 int mx_product_launch(const MxProduct &p, void *workspace, size_t workspace_bytes, hipStream_t st);
 size_t mx_product_workspace_bytes(int M, int N, int K, bool x_mxfp4);
 

@@ -69,17 +69,25 @@ __global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const T *__restrict
     }
 }
 
-// w[i] = value(code i) * scale of its block as fp32, exact (beyond fp32's range: infinity); 8 codes to a lane
-__global__ __launch_bounds__(256) void dequant_mxfp4_kernel(const uint32_t *__restrict__ codes, const uint8_t *__restrict__ scale,
-                                                            float *__restrict__ w, int64_t n8) {
-    const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += stride) {
-        const uint32_t c = codes[i];
-        const float s = mx_scale(scale[i >> 2]);
-        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
-        const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
-        reinterpret_cast<f32x4 *>(w)[2 * i] = f32x4{a.x, a.y, b.x, b.y};
-        reinterpret_cast<f32x4 *>(w)[2 * i + 1] = f32x4{d.x, d.y, e.x, e.y};
+// w[i] = value(code i) * scale of its block as fp32, exact (beyond fp32's range: infinity); 4 codes to a lane, so that a wave stores 1 KiB in a row, four
+// times in flight.  Bound by what it writes, four bytes a value (14336 x 4096: us and TB/s in the file's head).
+__global__ __launch_bounds__(256) void dequant_mxfp4_kernel(const uint16_t *__restrict__ codes, const uint8_t *__restrict__ scale,
+                                                            float *__restrict__ w, int64_t n4) {
+    const int64_t stride = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += 4 * stride) {
+        uint32_t c[4], s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t at = i + j * stride < n4 ? i + j * stride : i;
+            c[j] = codes[at];
+            s[j] = scale[at >> 3];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (i + j * stride >= n4) break;
+            const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[j], mx_scale(s[j]), 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[j], mx_scale(s[j]), 1);
+            __builtin_nontemporal_store(f32x4{a.x, a.y, b.x, b.y}, reinterpret_cast<f32x4 *>(w) + i + j * stride);
+        }
     }
 }
 
@@ -98,8 +106,8 @@ int quantize_mxfp4_launch(const void *x, int dtype, uint8_t *codes, uint8_t *sca
 }
 
 int dequant_mxfp4_launch(const uint8_t *codes, const uint8_t *scale, float *w, int64_t rows, int K, hipStream_t st) {
-    const int64_t n8 = rows * (K / 8);
-    hipLaunchKernelGGL(dequant_mxfp4_kernel, dim3(grid_for(n8)), dim3(256), 0, st, reinterpret_cast<const uint32_t *>(codes), scale, w, n8);
+    const int64_t n4 = rows * (K / 4);
+    hipLaunchKernelGGL(dequant_mxfp4_kernel, dim3(grid_for((n4 + 3) / 4)), dim3(256), 0, st, reinterpret_cast<const uint16_t *>(codes), scale, w, n4);
     return hip_check(hipGetLastError(), "dequant_mxfp4 launch");
 }
 

@@ -224,7 +224,7 @@ static int launch(const MxProduct &p, int RT, int wk, hipStream_t st) {
     const size_t lds = SCALES + (part > xb ? part : xb);
     if (lds > 163840) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: %zu bytes of LDS", lds);
     const int64_t nwg = (int64_t)(W >> wk) * RT, tiles = p.offsets ? mx_most_tiles(p.M, p.E, 8 * MT) : (p.M + 8 * MT - 1) / (8 * MT), cols = (p.N + nwg - 1) / nwg;
-    if (tiles > INT32_MAX || cols > 65535) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
+    if (tiles > (1 << 22) || cols > 65535) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
     const auto kernel = &mx_stream_kernel<X4, GATED, GROUPED, MT, D>;
     static std::atomic<bool> set[64];  // more LDS than the default limit: once per device
     int dev = 0;
@@ -258,31 +258,40 @@ static int launch_rows(const MxProduct &p, hipStream_t st) {
     }
 }
 
-template <bool X4, bool GATED, bool GROUPED>
-static int launch_kind(const MxProduct &p, hipStream_t st) {
-    const int per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;
-    return per <= 8 ? launch_rows<X4, GATED, GROUPED, 1>(p, st) : launch_rows<X4, GATED, GROUPED, 2>(p, st);
-}
-
 int mx_stream_launch(const MxProduct &p, hipStream_t st) {
-    if (p.w2) return launch_kind<false, true, true>(p, st);
-    if (p.offsets) return p.xs ? launch_kind<true, false, true>(p, st) : launch_kind<false, false, true>(p, st);
-    return p.xs ? launch_kind<true, false, false>(p, st) : launch_kind<false, false, false>(p, st);
+    if (p.w2) return launch_rows<false, true, true, 1>(p, st);
+    if (p.offsets) return p.xs ? launch_rows<true, false, true, 1>(p, st) : launch_rows<false, false, true, 1>(p, st);
+    if (p.M <= 8) return p.xs ? launch_rows<true, false, false, 1>(p, st) : launch_rows<false, false, false, 1>(p, st);
+    return p.xs ? launch_rows<true, false, false, 2>(p, st) : launch_rows<false, false, false, 2>(p, st);
 }
 
-// Up to 16 rows (of a group, on average) stream the weights, more go through the tiles
-static bool streams(int M, int E) { return (M + E - 1) / E <= 16; }
+// Up to 16 rows, or 8 of a group on average, stream the weights, more go through the tiles: by group, us, streamed / tiles: 40 rows, 8 matrices of 14336 x 4096
+// 48.9 / 56.6, 64 rows 62.8 / 60.3, 96 rows 92 / 58 (a group of more than a tile's rows reads its weights twice).
+static bool streams(const MxProduct &p) { return p.offsets ? (p.M + p.E - 1) / p.E <= 8 : p.M <= 16; }
+
+int mx_product_part_k(const MxProduct &p, int most_parts) { return streams(p) || !mx_tile_ok(p) ? 0 : mx_tile_pick(p, most_parts).part_k; }
 
 size_t mx_product_workspace_bytes(int M, int N, int K, bool x_mxfp4) {
-    if (streams(M, 1)) return 0;
-    const int part_k = mx_tile_part_k(M, N, K, 1, x_mxfp4, kMxParts);
-    return part_k ? (size_t)((K + part_k - 1) / part_k) * M * N * 4 : 0;
+    MxProduct p = {};
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    p.E = 1;
+    static const uint8_t any = 0;
+    p.xs = x_mxfp4 ? &any : nullptr;
+    p.part_k = mx_product_part_k(p, kMxParts);
+    return p.part_k ? (size_t)p.parts() * M * N * 4 : 0;
 }
 
 int mx_product_launch(const MxProduct &p, void *workspace, size_t workspace_bytes, hipStream_t st) {
-    if (streams(p.M, p.offsets ? p.E : 1) || !mx_tile_ok(p)) return mx_stream_launch(p, st);
-    const size_t need = p.offsets ? 0 : mx_product_workspace_bytes(p.M, p.N, p.K, p.xs != nullptr);
-    if (need && workspace_bytes >= need) return mx_tile_parts_launch(p, mx_tile_pick(p, kMxParts), reinterpret_cast<float *>(workspace), st);
+    if (streams(p) || !mx_tile_ok(p)) return mx_stream_launch(p, st);
+    if (p.part_k) return mx_tile_launch(p, mx_tile_pick(p, kMxGroupParts).tile, st);  // (the caller, who asked for at most so many, joins the parts)
+    if (!p.offsets && workspace) {
+        MxProduct q = p;
+        const MxTilePick pick = mx_tile_pick(p, kMxParts);
+        q.part_k = pick.part_k;
+        if (pick.part_k && workspace_bytes >= (size_t)q.parts() * p.M * p.N * 4) return mx_tile_parts_launch(q, pick.tile, reinterpret_cast<float *>(workspace), st);
+    }
     return mx_tile_launch(p, mx_tile_pick(p, 1).tile, st);
 }
 

@@ -398,7 +398,7 @@ static int launch(const MxProduct &p, hipStream_t st) {
     constexpr int TO = GATED ? C::TN / 2 : C::TN, LDS = C::lds(TO);
     static_assert(LDS <= 163840, "LDS of a compute unit");
     const int64_t tm = p.offsets ? mx_most_tiles(p.M, p.E, C::TM) : (p.M + C::TM - 1) / C::TM, tiles = tm * ((p.N + TO - 1) / TO);
-    if (tiles > INT32_MAX - 8) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
+    if (tiles > (1 << 22)) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
     static std::atomic<bool> set[64];  // more LDS than the default limit: once per device
     int dev = 0;
     CHADQ_HIP(hipGetDevice(&dev));
@@ -508,7 +508,6 @@ static MxTilePick pick(int M, int N, int K, int E, bool x_mx, bool gated, int mo
 }
 
 MxTilePick mx_tile_pick(const MxProduct &p, int most_parts) { return pick(p.M, p.N, p.K, p.offsets ? p.E : 1, p.xs != nullptr, p.w2 != nullptr, most_parts); }
-int mx_tile_part_k(int M, int N, int K, int E, bool x_mx, int most_parts) { return pick(M, N, K, E, x_mx, false, most_parts).part_k; }
 
 int mx_tile_launch(const MxProduct &p, int tile, hipStream_t st) {
 #ifdef MXT_FORCE
@@ -536,13 +535,12 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const float *__restrict__ 
     }
 }
 
-// The product in parts of K: fp32 sums to `part`, joined into y
-int mx_tile_parts_launch(const MxProduct &p, const MxTilePick &pick, float *part, hipStream_t st) {
+// The product in its parts of K: fp32 sums to `part`, joined into y
+int mx_tile_parts_launch(const MxProduct &p, int tile, float *part, hipStream_t st) {
     MxProduct q = p;
     q.y = part;
     q.y_bf16 = false;
-    q.part_k = pick.part_k;
-    const int rc = mx_tile_launch(q, pick.tile, st);
+    const int rc = mx_tile_launch(q, tile, st);
     if (rc) return rc;
     const int64_t n = (int64_t)p.M * p.N;
     const bool quads = n % 4 == 0 && aligned16(p.y);

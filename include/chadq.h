@@ -426,8 +426,9 @@ int chadq_dequant_mxfp4(const uint8_t *codes, const uint8_t *scale, float *w, in
 
 /*
  * y[m,n] = sum_k x[m,k] w[n,k], fp32 sums, y fp32 or (y_bf16) the same rounded once.  x_scale NULL: x is bf16 [M,K], multiplied as it is;
- * else x holds the codes [M,K/2] of MXFP4 activations.  Any M, N >= 0; K a positive multiple of 32; x and codes 16-byte aligned.
- * A NaN block of w makes column n NaN, one of x row m.  workspace: chadq_product_mxfp4_workspace_bytes bytes (16-byte aligned; 0: none needed), for the
+ * else x holds the codes [M,K/2] of MXFP4 activations.  M, N >= 0 (y of at most 2^22 tiles, the smallest of 64 n x 32 m); K a positive multiple of
+ * 32 up to 2^26; x and codes 16-byte aligned, scales anywhere.  A NaN block of w makes column n NaN, one of x row m.  With bf16 x a weight beyond bf16's range (scale bytes
+ * 253 and 254) counts as infinite; infinities and NaN in x act as IEEE has them.  workspace: chadq_product_mxfp4_workspace_bytes bytes (16-byte aligned; 0: none needed), for the
  * sums of parts of K where that is the quicker form; without it (NULL or fewer bytes) the product is one part.
  */
 size_t chadq_product_mxfp4_workspace_bytes(int M, int N, int K, int x_mxfp4);

@@ -487,3 +487,142 @@ def test_moe_refusals(ops):
     for bad in (0, 5):
         with pytest.raises(ValueError, match="unsupported"):
             ops.moe_ffn(x, z, (gate, up, down), top_k=bad)
+
+
+# ---- the ends of the ranges ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("m", [1, 12, 40, 300])
+def test_subnormal_activations_and_weights(ops, m):
+    """bf16's subnormal numbers, as activations and as weights times their scale, count: 2^-130 against 2^100 is 2^-30."""
+    from chadslab_amd import QWeightMXFP4
+
+    r = np.random.Generator(np.random.PCG64(m + 3))
+    n, k = 40, 256
+    c, _ = weights(r, n, k)
+    w64 = dev(O.dequant_mxfp4(c, np.full((n, k // 32), 127, np.uint8)))
+    x = r.integers(-8, 9, (m, k)).astype(np.float64)
+    for xe, we in ((-133, 227), (100, 0), (100, 2), (-120, 230)):
+        xt = torch.from_numpy(x * 2.0 ** xe).to(torch.bfloat16).to(DEV)
+        y = ops.qlinear(xt, QWeightMXFP4(dev(c), torch.full((n, k // 32), we, dtype=torch.uint8, device=DEV)))
+        check((y.double() * 2.0 ** (127 - we - xe)).to(y.dtype), dev(x), w64)  # (of y's own type: the bound counts its rounding)
+
+
+@pytest.mark.parametrize("x4", [False, True], ids=["bf16", "mxfp4"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (16, 1, 4096), (17, 1, 96), (500, 1, 352), (3, 5, 20000), (33, 3, 20000), (20000, 2, 64), (1, 70000, 32), (40, 70000, 32)])
+def test_thin_products(ops, m, n, k, x4):
+    from chadslab_amd import QWeightMXFP4
+
+    r = np.random.Generator(np.random.PCG64(m + n + k))
+    c, s = weights(r, n, k)
+    x, x64 = activations(r, m, k, x4)
+    check(ops.qlinear(x, QWeightMXFP4(dev(c), dev(s))), x64, dev(O.dequant_mxfp4(c, s)))
+
+
+@pytest.mark.parametrize("m", [2, 48, 300])
+def test_scales_at_any_address(ops, m):
+    """Scales are bytes and may begin anywhere; codes want 16 bytes' alignment and are refused without."""
+    from chadslab_amd import QWeightMXFP4
+
+    r = np.random.Generator(np.random.PCG64(m))
+    n, k = 100, 1056
+    c, s = weights(r, n, k)
+    x, x64 = activations(r, m, k, False)
+    for shift in (1, 2, 7):
+        buf = torch.zeros(n * k // 32 + shift, dtype=torch.uint8, device=DEV)
+        buf[shift:] = dev(s).flatten()
+        check(ops.qlinear(x, QWeightMXFP4(dev(c), buf[shift:].view(n, k // 32))), x64, dev(O.dequant_mxfp4(c, s)))
+    codes = torch.zeros(n * k // 2 + 8, dtype=torch.uint8, device=DEV)[8:].view(n, k // 2)
+    with pytest.raises(ValueError, match="aligned"):
+        ops.qlinear(x, QWeightMXFP4(codes, dev(s)))
+
+
+def test_without_the_host_module(ops, monkeypatch):
+    """The Python road to the same kernels: the same bits."""
+    from chadslab_amd import QExpertsMXFP4, QWeightMXFP4, _lib
+
+    r = np.random.Generator(np.random.PCG64(5))
+    c, s = weights(r, 4, 128, 256)
+    qw, qe = QWeightMXFP4(dev(c[0]), dev(s[0])), QExpertsMXFP4(dev(c), dev(s))
+    down = QExpertsMXFP4(*(dev(a) for a in weights(r, 4, 256, 128)))
+    x, _ = activations(r, 40, 256, False)
+    z, offsets = dev(r.standard_normal((40, 4)).astype(np.float32)), torch.tensor([0, 7, 7, 30, 40], dtype=torch.int32, device=DEV)
+
+    def calls():
+        q = ops.quantize_mxfp4(x)
+        e = ops.quantize_mxfp4(x.float().view(2, 20, 256))
+        assert type(q) is QWeightMXFP4 and type(e) is QExpertsMXFP4 and repr(q) and (q.N, q.K, e.E) == (40, 256, 2)
+        return [q.packed, q.scale, e.packed, e.scale, ops.dequantize(q), ops.dequantize(e), ops.qlinear(x, qw), ops.qlinear(x[:3], qw), ops.qlinear(q, qw),
+                ops.qlinear(x[:3], qw, out_dtype=torch.bfloat16), ops.qgemm_grouped(x, qe, offsets), ops.qgemm_grouped(q, qe, offsets), ops.moe_ffn(x, z, (qe, qe, down))]
+
+    native = calls()
+    monkeypatch.setattr(_lib, "_native", _lib._NoHostModule)
+    for a, b in zip(native, calls()):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,x4", [(30, False), (400, False), (400, True)])
+def test_captured_groups_follow_their_offsets(ops, rows, x4):
+    """A captured product by group reads the offsets of the replay, not those of the capture."""
+    n, k = 96, 288
+    x, x64, w, w64, offsets = grouped_case(rows, [rows // 4] * 4, n, k, x4)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ops.qgemm_grouped(x, w, offsets)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        y = ops.qgemm_grouped(x, w, offsets)
+    rows = x64.shape[0]
+    for bounds in ([0, 0, 0, 0, rows], [2, 9, 9, rows - 1, rows - 1], [0, 5, rows // 2, rows, rows], [0, rows // 4, rows // 2, rows - 3, rows]):
+        offsets.copy_(torch.tensor(bounds, dtype=torch.int32))
+        eager = ops.qgemm_grouped(x, w, offsets)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager)
+        check_groups(y, x64, w64, bounds)
+        assert not y[:bounds[0]].any() and not y[bounds[-1]:].any()
+
+
+@pytest.mark.parametrize("m,n,k", [(48, 512, 8192), (100, 2048, 8192), (20, 130, 14368), (300, 256, 14336)])
+def test_products_in_parts_of_k(ops, m, n, k):
+    """Few tiles and a long K: summed in parts, by the C entry point with its workspace and without, and with one too small."""
+    from chadslab_amd import QWeightMXFP4, _lib
+
+    lib = _lib.load()
+    need = lib.chadq_product_mxfp4_workspace_bytes(m, n, k, 0)
+    assert need > 0 and need % (4 * m * n) == 0
+    r = np.random.Generator(np.random.PCG64(m))
+    c, s = weights(r, n, k)
+    qw, w64 = QWeightMXFP4(dev(c), dev(s)), dev(O.dequant_mxfp4(c, s))
+    x, x64 = activations(r, m, k, False)
+    check(ops.qlinear(x, qw), x64, w64)
+    for size in (0, need - 1, need):
+        ws = torch.full((need,), 255, dtype=torch.uint8, device=DEV)
+        for dtype in (torch.float32, torch.bfloat16):
+            y = torch.full((m, n), float("nan"), dtype=dtype, device=DEV)
+            rc = lib.chadq_product_mxfp4(x.data_ptr(), None, qw.packed.data_ptr(), qw.scale.data_ptr(), y.data_ptr(), int(dtype == torch.bfloat16), m, n, k, ws.data_ptr() if size else None,
+                                         size, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            check(y, x64, w64)
+
+
+def test_library_refuses(ops):
+    """The C entry points' own checks: status and message, no launch."""
+    from chadslab_amd import _lib
+
+    lib = _lib.load()
+    a = torch.zeros(4096, dtype=torch.uint8, device=DEV).data_ptr()
+    for call, status in (((a, None, a, a, a, 0, 1, 1, 48, None, 0, None), -2), ((a, None, a, a, a, 0, -1, 1, 32, None, 0, None), -2), ((a, None, a, a, a, 0, 1, 1, 2 ** 26 + 32, None, 0, None), -2),
+                         ((None, None, a, a, a, 0, 1, 1, 32, None, 0, None), -1), ((a, None, a, None, a, 0, 1, 1, 32, None, 0, None), -1), ((a + 8, None, a, a, a, 0, 1, 1, 32, None, 0, None), -3),
+                         ((a, None, a + 4, a, a, 0, 1, 1, 32, None, 0, None), -3), ((a, None, a, a, a, 0, 20, 1, 32, a + 4, 64, None), -3), ((a, None, a, a, a, 0, 2 ** 31 - 1, 2 ** 31 - 1, 32, None, 0, None), -2)):
+        assert lib.chadq_product_mxfp4(*call) == status, call
+    assert lib.chadq_product_mxfp4(None, None, None, None, None, 0, 0, 5, 32, None, 0, None) == 0
+    for call, status in (((a, None, a, a, a, a, 4, 0, 1, 32, 1, None), -2), ((a, None, a, a, None, a, 4, 1, 1, 32, 1, None), -1), ((a, None, a, a, a + 2, a, 4, 1, 1, 32, 1, None), -3),
+                         ((a, None, a, a, a, a, 4, 1, 1, 33, 1, None), -2)):
+        assert lib.chadq_product_mxfp4_grouped(*call) == status, call
+    for call, status in (((a, 3, a, a, 1, 32, None), -2), ((a, 0, a, a, 1, 33, None), -2), ((a, 0, a, a, -1, 32, None), -2), ((a, 0, None, a, 1, 32, None), -1), ((a + 4, 0, a, a, 1, 32, None), -3),
+                         ((a, 0, a + 1, a, 1, 32, None), -3), ((a, 0, a, a, 2 ** 62, 32, None), -2)):
+        assert lib.chadq_quantize_mxfp4(*call) == status, call
+    assert lib.chadq_dequant_mxfp4(a, a, a + 4, 1, 32, None) == -3 and lib.chadq_dequant_mxfp4(a, a, a, 1, 31, None) == -2
+    assert lib.chadq_moe_ffn_mxfp4_workspace_bytes(4, 64, 64, 17, 2) == 0 and lib.chadq_moe_ffn_mxfp4_workspace_bytes(4, 64, 48, 4, 2) == 0
+    assert lib.chadq_moe_ffn_mxfp4_workspace_bytes(4, 64, 64, 4, 2) > 0
