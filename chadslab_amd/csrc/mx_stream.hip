@@ -219,12 +219,13 @@ template <bool X4, bool GATED, bool GROUPED, int MT, int D>
 static int launch(const MxProduct &p, int RT, int wk, hipStream_t st) {
     constexpr int W = MXS_W, NB = GATED ? 2 : 1, UB = X4 ? 128 : 512, SCALES = W * (NB + X4 * MT) * 8 * (8 * D + 8);
     const int U = (p.K + 255) / 256, round = D << wk, rounds = (U + round - 1) / round, rows = p.M < 8 * MT ? p.M : 8 * MT;
-    const int most = 73728 / (rows * round * UB), chunk = most < 1 ? 1 : most > rounds ? rounds : most;  // two workgroups to a compute unit
+    const int64_t nwg = (int64_t)(W >> wk) * RT, tiles = p.offsets ? mx_most_tiles(p.M, p.E, 8 * MT) : (p.M + 8 * MT - 1) / (8 * MT), cols = (p.N + nwg - 1) / nwg;
+    if (tiles > (1 << 22) || cols > 65535) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
+    // all of K if it fits: two workgroups to a compute unit where there are so many
+    const int most = (tiles * cols <= 256 ? 147456 : 73728) / (rows * round * UB), chunk = most < 1 ? 1 : most > rounds ? rounds : most;
     const size_t per = ((size_t)chunk * round * UB + 1023) / 1024, xb = rows * (per * 1024 + 16), part = wk ? W * MT * NB * 256 : 0;
     const size_t lds = SCALES + (part > xb ? part : xb);
     if (lds > 163840) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: %zu bytes of LDS", lds);
-    const int64_t nwg = (int64_t)(W >> wk) * RT, tiles = p.offsets ? mx_most_tiles(p.M, p.E, 8 * MT) : (p.M + 8 * MT - 1) / (8 * MT), cols = (p.N + nwg - 1) / nwg;
-    if (tiles > (1 << 22) || cols > 65535) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
     const auto kernel = &mx_stream_kernel<X4, GATED, GROUPED, MT, D>;
     static std::atomic<bool> set[64];  // more LDS than the default limit: once per device
     int dev = 0;
