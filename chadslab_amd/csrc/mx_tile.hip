@@ -419,20 +419,17 @@ bool mx_tile_ok(const MxProduct &p) {
 }
 
 // ---- which tile, and K in how many parts
-enum Tile { T64x32, T64x64, T128x64, T256x64, T128x128, T256x128, T256x256, T256x96, T128x96, T256x32, TILES };  // weight rows x activation rows
+enum Tile { T64x32, T64x64, T128x64, T256x64, T128x128, T256x128, T256x256, T256x96, T128x96, T128x32, TILES };  // weight rows x activation rows
 
-static int launch_tile(const MxProduct &p, int tile, hipStream_t st) {
+int mx_tile_launch(const MxProduct &p, int tile, hipStream_t st) {
     using namespace mxt;
     //                                                       WN WM WK NB MB BPS ST
     if (p.w2) {
         switch (tile) {
-        case T64x32: case T64x64: return launch<false, true, 2, 1, 4, 2, 1, 8, 4>(p, st);  // (128 x 32)
+        case T128x32: return launch<false, true, 2, 1, 4, 2, 1, 8, 4>(p, st);
         case T128x64: return launch<false, true, 2, 1, 4, 2, 2, 8, 3>(p, st);
         case T256x64: return launch<false, true, 4, 1, 2, 2, 2, 4, 4>(p, st);
         case T256x96: return launch<false, true, 4, 1, 2, 2, 3, 4, 3>(p, st);
-        case T128x96: return launch<false, true, 2, 1, 4, 2, 3, 8, 2>(p, st);
-        case T256x32: return launch<false, true, 4, 1, 2, 2, 1, 4, 6>(p, st);
-        case T128x128: return launch<false, true, 2, 2, 2, 2, 2, 4, 3>(p, st);
         default: return launch<false, true, 4, 2, 1, 2, 2, 4, 3>(p, st);
         }
     }
@@ -444,7 +441,6 @@ static int launch_tile(const MxProduct &p, int tile, hipStream_t st) {
         case T256x64: return launch<true, false, 4, 1, 2, 2, 2, 8, 3>(p, st);
         case T256x96: return launch<true, false, 4, 1, 2, 2, 3, 8, 3>(p, st);
         case T128x96: return launch<true, false, 4, 1, 2, 1, 3, 8, 4>(p, st);
-        case T256x32: return launch<true, false, 4, 1, 2, 2, 1, 8, 3>(p, st);
         case T128x128: return launch<true, false, 2, 2, 2, 2, 2, 8, 4>(p, st);
         case T256x128: return launch<true, false, 4, 2, 1, 2, 2, 8, 3>(p, st);
         default: return launch<true, false, 2, 4, 1, 4, 2, 8, 2>(p, st);
@@ -457,7 +453,6 @@ static int launch_tile(const MxProduct &p, int tile, hipStream_t st) {
     case T256x64: return launch<false, false, 4, 1, 2, 2, 2, 4, 4>(p, st);
     case T256x96: return launch<false, false, 4, 1, 2, 2, 3, 4, 3>(p, st);
     case T128x96: return launch<false, false, 4, 1, 2, 1, 3, 4, 4>(p, st);
-    case T256x32: return launch<false, false, 4, 1, 2, 2, 1, 4, 6>(p, st);
     case T128x128: return launch<false, false, 2, 2, 2, 2, 2, 4, 3>(p, st);
     default: return launch<false, false, 4, 2, 1, 2, 2, 4, 3>(p, st);
     }
@@ -472,19 +467,20 @@ struct TileTime {
 static const TileTime kBf16[TILES] = {{64, 32, 1.5f, 2.7f, 1.46f, 1.55f},   {64, 64, 1.7f, 3.0f, 2.21f, 2.35f},  {128, 64, 1.4f, 1.8f, 4.82f, 5.1f},
                                       {256, 64, 1.7f, 2.3f, 7.31f, 7.85f},  {128, 128, 2.4f, 2.5f, 6.07f, 7.5f}, {256, 128, 0.6f, 4.7f, 9.29f, 13.2f},
                                       {256, 256, 0.f, 1e9f, 0.f, 0.f},      {256, 96, 2.3f, 3.1f, 8.0f, 10.5f},  {128, 96, 2.8f, 2.0f, 4.33f, 6.05f},
-                                      {256, 32, 0.7f, 2.0f, 6.65f, 6.1f}};
+                                      {128, 32, 1.7f, 3.0f, 3.0f, 3.2f}};
 static const TileTime kMx[TILES] = {{64, 32, 1.5f, 2.5f, 1.33f, 1.31f},  {64, 64, 1.4f, 3.2f, 1.26f, 1.29f},  {128, 64, 1.6f, 2.5f, 2.88f, 2.5f},
                                     {256, 64, 1.7f, 2.3f, 4.54f, 4.15f}, {128, 128, 2.2f, 3.0f, 3.21f, 3.1f}, {256, 128, 3.0f, 2.5f, 5.05f, 5.15f},
                                     {256, 256, 1.8f, 6.8f, 7.34f, 8.1f}, {256, 96, 2.4f, 3.3f, 5.0f, 4.6f},   {128, 96, 2.1f, 2.9f, 3.05f, 2.77f},
-                                    {256, 32, 1.3f, 1.6f, 4.41f, 3.8f}};
+                                    {128, 32, 0.f, 1e9f, 0.f, 0.f}};
 
 static MxTilePick pick(int M, int N, int K, int E, bool x_mx, bool gated, int most_parts) {
     MxTilePick best = {T128x128, 0};
     float least = 1e30f;
     for (int i = 0; i < TILES; ++i) {
         const TileTime &t = (x_mx ? kMx : kBf16)[i];
-        const int tn = gated ? (t.tn < 128 ? 64 : t.tn / 2) : t.tn;
-        if (t.round > 1e8f || (gated && t.tn < 128)) continue;
+        const int tn = gated ? t.tn / 2 : t.tn;
+        // (gated: 128 x 96 and 128 x 128 were up to 1.45x behind the fastest and never it; 128 x 32 is their tile for few rows or columns)
+        if (t.round > 1e8f || (gated ? t.tn < 128 || i == T128x96 || i == T128x128 : i == T128x32)) continue;
         // rows by group: between the tiles of groups of one size and those of exponentially distributed sizes
         const float mean = (float)M / E > 1.f ? (float)M / E : 1.f, hit = E * (1.f - expf(-(float)M / E)), even = mean / t.tm + 0.3f;
         const float tm = E > 1 ? hit * 0.5f * ((even > 1.f ? even : 1.f) + 1.f / (1.f - expf(-t.tm / mean))) : (float)((M + t.tm - 1) / t.tm);
@@ -509,12 +505,6 @@ static MxTilePick pick(int M, int N, int K, int E, bool x_mx, bool gated, int mo
 
 MxTilePick mx_tile_pick(const MxProduct &p, int most_parts) { return pick(p.M, p.N, p.K, p.offsets ? p.E : 1, p.xs != nullptr, p.w2 != nullptr, most_parts); }
 
-int mx_tile_launch(const MxProduct &p, int tile, hipStream_t st) {
-#ifdef MXT_FORCE
-    tile = MXT_FORCE;
-#endif
-    return launch_tile(p, tile, st);
-}
 
 // y = the parts' sums, added in their order; four values to a thread where the rows allow
 __global__ __launch_bounds__(256) void mx_join_kernel(const float *__restrict__ part, void *__restrict__ y, int64_t n, int parts, bool y_bf16, bool quads) {
