@@ -47,8 +47,9 @@ __device__ __forceinline__ i32x8 mx_operand(u32x4 v) {
     return __builtin_bit_cast(i32x8, w);
 }
 
-// B scale bytes (1, 2, 4 or 8, no more than the row has) from byte `at` of a row of G on, anything behind its end; any alignment.  What is loaded near the
-// end begins before `at`: the shift that puts that right is left to the reader (get), who does not want to wait for it earlier.
+// B scale bytes (1, 2, 4 or 8, no more than the row has) from byte `at` of a row of G on, zeros behind its end (2^-127: what is infinite may not
+// meet the activations there, which are zeros); any alignment.  What is loaded near the end begins before `at`: the shift that puts that right is left
+// to the reader (get), who does not want to wait for it earlier.
 template <int B>
 struct MxScales {
     typedef std::conditional_t<B == 8, uint64_t, std::conditional_t<B == 4, uint32_t, std::conditional_t<B == 2, uint16_t, uint8_t>>> bytes_t;
@@ -56,10 +57,10 @@ struct MxScales {
     int cut;
     __device__ __forceinline__ void load(const uint8_t *row, int at, int G) {
         const int o = at < G - B ? at : G - B;
-        cut = at - o < B - 1 ? at - o : B - 1;
+        cut = at - o < B ? at - o : B;
         __builtin_memcpy(&raw, row + o, B);
     }
-    __device__ __forceinline__ bytes_t get() const { return (bytes_t)(raw >> (8 * cut)); }
+    __device__ __forceinline__ bytes_t get() const { return cut < B ? (bytes_t)(raw >> (8 * cut)) : (bytes_t)0; }
 };
 
 // y[r, n] = sum_k x[r, k] w[g(r), n, k] for the rows r of group g(r) = the g with offsets[g] <= r < offsets[g + 1]

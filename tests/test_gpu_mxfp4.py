@@ -224,6 +224,26 @@ def test_infinite_activations(ops, m):
     assert y[1, 0] == float("inf") and y[1, 1] == -float("inf") and torch.isnan(y[1, 2]) and bool((y[0] == 0).all())
 
 
+@pytest.mark.parametrize("k", [32, 96, 288, 800, 1056, 4128])
+@pytest.mark.parametrize("m", [1, 3, 16, 40])
+def test_weights_beyond_bf16_in_the_last_block(ops, m, k):
+    """They count as infinite, and the activations behind the row's end, zeros, may not meet them: infinity times zero is NaN."""
+    from chadslab_amd import QExpertsMXFP4, QWeightMXFP4
+
+    c = np.zeros((2, 24, k // 2), np.uint8)
+    s = np.full((2, 24, k // 32), 127, np.uint8)
+    s[0, 5, -1], s[1, 7, -1] = 254, 253
+    c[0, 5, -16:], c[1, 7, -16:] = 0x44, 0x77  # 2 x 2^127, 6 x 2^126
+    x = torch.ones(m, k, dtype=torch.bfloat16, device=DEV)
+    want = torch.zeros(2, m, 24, device=DEV)
+    want[0, :, 5] = want[1, :, 7] = float("inf")
+    for e in range(2):
+        assert torch.equal(ops.qlinear(x, QWeightMXFP4(dev(c[e]), dev(s[e]))).float(), want[e])
+    half = m // 2
+    y = ops.qgemm_grouped(x, QExpertsMXFP4(dev(c), dev(s)), torch.tensor([0, half, m], dtype=torch.int32, device=DEV))
+    assert torch.equal(y.float(), torch.cat((want[0, :half], want[1, half:])))
+
+
 @pytest.mark.parametrize("m", [1, 33, 150])
 def test_extreme_scales(ops, m):
     """Scales at both ends of the bytes; 2^-100 against 2^100 has to come out as if neither were there."""
