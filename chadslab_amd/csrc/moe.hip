@@ -11,6 +11,9 @@
 // through the sorted token list, down split over K).  Else (row order only): the prefill dequant-GEMM kernel in grouped mode
 // on a gathered copy of the activations with a separate SiLU kernel.  The small kernels here are the router, the gather,
 // the SiLU gate and the weighted combine.
+//
+// MXFP4 experts take the router, the products by group of mx_stream.hip and mx_tile.hip, and the combine (at the end of the file): 4 tokens through 8 experts of
+// 14336 x 4096 92 us (what they read, at a large copy's rate, 99), 256 tokens 306 us (gate and up 184, down 119).
 #include "chadq_common.h"
 #include "expert_prep.h"
 #include "mx.h"
@@ -498,6 +501,7 @@ int moe_ffn_i4g32_launch(const uint16_t *x, const float *logits, const chadq_moe
 
 // ---- the same on MXFP4 experts, E matrices of each kind one behind the other: router, gate and up with the SiLU gate in one product by
 // group that reads the activations through the sorted token list, down to fp32, combine.
+
 // The down product of the MXFP4 experts, K in parts where that is quicker: the combine adds them as it does those of the int4 experts
 static MxProduct moe_mx_down(int P, int H, int F, int E, const int32_t *offsets) {
     static const int32_t any = 0;

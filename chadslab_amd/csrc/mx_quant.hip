@@ -1,6 +1,9 @@
 // MXFP4: quantisation and its inverse.  Per block of 32 values along K:  e = clamp(floor(log2 max|x|) - 2 + 127, 0, 254),
 // code = the nearest e2m1 to x / 2^(e - 127), ties to the even one, what lies beyond 6 to 6; a block that holds a NaN or an
 // infinity gets e = 255 and codes of 0.  The division by a power of two is exact, so there is nothing to round but the code.
+//
+// Both are bound by the bytes they move: quantising 14336 x 4096 fp32 47.2 us = 5.6 TB/s, 4096 x 4096 bf16 8.5 us, and dequantising 14336 x 4096 45.9 us =
+// 5.8 TB/s (a copy of 1 GiB moves 5.15 TB/s, read and written).  16 x 4096: 3.2 us, a launch and one trip to memory.
 #include "mx.h"
 
 namespace chadq {
@@ -37,7 +40,8 @@ __device__ __forceinline__ void load8<_Float16>(const _Float16 *p, float f[8]) {
     }
 }
 
-// Four lanes to a block, 8 values to a lane; rows do not matter, K is a multiple of 32.
+// Four lanes to a block, 8 values to a lane: a lane stores one word of codes, and two exchanges inside the quad give the block's largest magnitude.
+// Rows do not matter, K is a multiple of 32.
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const T *__restrict__ x, uint32_t *__restrict__ codes, uint8_t *__restrict__ scale,
                                                              int64_t n8) {
@@ -70,7 +74,7 @@ __global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const T *__restrict
 }
 
 // w[i] = value(code i) * scale of its block as fp32, exact (beyond fp32's range: infinity); 4 codes to a lane, so that a wave stores 1 KiB in a row, four
-// times in flight.  Bound by what it writes, four bytes a value (14336 x 4096: us and TB/s in the file's head).
+// times in flight.  The stores go past the caches: 14336 x 4096 65 -> 45 us with both.
 __global__ __launch_bounds__(256) void dequant_mxfp4_kernel(const uint16_t *__restrict__ codes, const uint8_t *__restrict__ scale,
                                                             float *__restrict__ w, int64_t n4) {
     const int64_t stride = (int64_t)gridDim.x * 256;

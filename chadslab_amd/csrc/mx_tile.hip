@@ -4,10 +4,17 @@
 // matrix cores' first operand, so that a lane holds four consecutive n of one activation row.
 //   MXFP4 x  v_mfma_scale_f32_32x32x64_f8f6f4: both operands and their scale bytes go in as they are stored
 //   bf16 x   the codes become bf16 with their scale, exactly (16 conversions per 32 codes), v_mfma_f32_32x32x16_bf16
-// A step is BPS scale blocks along K.  Codes and activations go global -> LDS by DMA, ST stages, requests dealt to the waves in equal numbers; a
-// piece past the end of a row or of the matrix is requested beyond the buffer's range and arrives as zeros, so nothing in the loop knows about
-// edges.  Scales are 4 or 8 bytes of a row and step, at any alignment: one thread loads those of a row a step ahead and puts them into LDS.  16-byte pieces of
-// a row are XOR-swizzled by the row so that the 16 rows that a read takes at a time cover all banks.
+// A step is BPS scale blocks along K.  Codes and activations go global -> LDS by DMA, ST stages, requests dealt to the waves in equal numbers and placed between
+// the MFMAs; a piece past the end of a row or of the matrix is requested beyond the buffer's range and arrives as zeros, so nothing in the loop knows about
+// edges.  Scales are 4 or 8 bytes of a row and step, at any alignment: a thread loads two steps' of a row, two steps ahead, and puts them into LDS.  16-byte
+// pieces of a row are XOR-swizzled by the row so that the 16 rows that a read takes at a time cover all banks.  WK > 1: waves of a workgroup split the blocks of a
+// step and add their sums at the end, so that a small tile too has eight waves to hide its reads.
+//
+// Measured, bf16 x: 48 x 14336 x 4096 16.2 us, 1000 x 4096 x 14336 109-114 us = 1.03-1.08 PFLOP/s, 4096^3 116-121 us = 1.14-1.18 PFLOP/s (a bf16 library product of 8192^3:
+// 1.40); MXFP4 x: 4096^3 42-43 us = 3.2 PFLOP/s, 4096 x 14336 x 4096 156 us = 3.1 PFLOP/s.  Matrix cores busy: 54 % of the cycles of
+// 1000 x 4096 x 14336, 39 % of 4096 x 14336 x 4096 with MXFP4 x.  bf16: the loop of 4096^3 without loads and conversions takes 71 us, at a clock that the power leaves.  MXFP4 x
+// and small tiles: what a compute unit gets by DMA, 40-60 KB per us (a step of the 256 x 256 tile is 64 KB), and a tile's first requests and its result, which nothing overlaps.  Four blocks of columns to a wave for the bf16 256 x 128 tile, scale conversion once per block, and a branch round the scales' loads (the compiler moves
+// MFMAs behind it) were no faster.
 #include <cmath>
 #include <type_traits>
 #include <utility>
