@@ -12,8 +12,10 @@
 //
 // Measured, bf16 x: 48 x 14336 x 4096 16.2 us, 1000 x 4096 x 14336 109-114 us = 1.03-1.08 PFLOP/s, 4096^3 116-121 us = 1.14-1.18 PFLOP/s (a bf16 library product of 8192^3:
 // 1.40); MXFP4 x: 4096^3 42-43 us = 3.2 PFLOP/s, 4096 x 14336 x 4096 156 us = 3.1 PFLOP/s.  Matrix cores busy: 54 % of the cycles of
-// 1000 x 4096 x 14336, 39 % of 4096 x 14336 x 4096 with MXFP4 x.  bf16: the loop of 4096^3 without loads and conversions takes 71 us, at a clock that the power leaves.  MXFP4 x
-// and small tiles: what a compute unit gets by DMA, 40-60 KB per us (a step of the 256 x 256 tile is 64 KB), and a tile's first requests and its result, which nothing overlaps.  Four blocks of columns to a wave for the bf16 256 x 128 tile, scale conversion once per block, and a branch round the scales' loads (the compiler moves
+// 1000 x 4096 x 14336, 39 % of 4096 x 14336 x 4096 with MXFP4 x.  bf16: the loop of 4096^3 without loads and conversions takes 71 us, at a clock that the power leaves.  MXFP4 x,
+// 4096 x 4096 x 14336: 124 us (3.9 PFLOP/s); without the loop's requests 101, without its fragment reads 119, without both 94, the MFMAs alone 88 (5.5 PFLOP/s);
+// at K = 4096 a tile's first requests and its result, 128 KB from each compute unit at once, are a quarter of the 43 us.  Small tiles: what a compute unit gets by
+// DMA, 40-60 KB per us.  256 x 256 in steps of 128 k with three or four stages: 5-10 % slower.  Four blocks of columns to a wave for the bf16 256 x 128 tile, scale conversion once per block, and a branch round the scales' loads (the compiler moves
 // MFMAs behind it) were no faster.
 #include <cmath>
 #include <type_traits>
@@ -496,10 +498,11 @@ static MxTilePick pick(int M, int N, int K, int E, bool x_mx, bool gated, int mo
             const int part_k = parts > 1 ? ((K + parts - 1) / parts + 511) / 512 * 512 : K;
             if (parts > 1 && (part_k < 1024 || (int64_t)part_k * (parts - 1) >= K)) continue;
             const float wgs = tiles * parts, full = wgs >= 256.f ? 1.f : wgs <= 64.f ? 0.f : (wgs - 64.f) / 192.f;
-            const float rounds = E > 1 && wgs > 256.f ? wgs / 256.f + 0.3f : ceilf(wgs / 256.f);
+            // (by group: a workgroup finds its tile first; the groups' tiles end unevenly)
+            const float rounds = E > 1 && wgs > 256.f ? wgs / 256.f + 0.6f : ceilf(wgs / 256.f), round = E > 1 ? t.round + 2.f : t.round;
             // (a cut tile one wave high takes fewer blocks of rows; one block costs this share of two or three)
             const float one = E == 1 ? 1.f : t.tm == 96 ? 0.6f : t.tm == 64 ? 0.8f : 1.f, rows = (float)M / (tm * t.tm);
-            float us = t.start + rounds * (t.round + (t.few + (t.full - t.few) * full) * (one + (1.f - one) * (rows < 1.f ? rows : 1.f)) * (part_k / 1024.f));
+            float us = t.start + rounds * (round + (t.few + (t.full - t.few) * full) * (one + (1.f - one) * (rows < 1.f ? rows : 1.f)) * (part_k / 1024.f));
             if (parts > 1) us += 3.f + (8.f * parts + 2.f) * M * (float)N * 2.5e-7f;  // the sums written, read again and joined by another launch
             if (us < least * (parts > 1 ? 0.95f : 1.f)) {
                 least = us;
