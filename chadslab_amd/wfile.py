@@ -4,12 +4,12 @@ memory map so that a multi-GB checkpoint is paged in by the copy to the GPU and 
 Layout (little endian):
     bytes 0..7    magic  b"CHADQW01"
     bytes 8..15   uint64 header length H
-    bytes 16..    H bytes of UTF-8 JSON: {"tensors": {name: {"kind": "i4g32" | "i8row" | "raw", "shape": [...],
+    bytes 16..    H bytes of UTF-8 JSON: {"tensors": {name: {"kind": "i4g32" | "i8row" | "mxfp4" | "raw", "shape": [...],
                   "arrays": {array_name: {"dtype": numpy dtype string, "shape": [...], "offset": bytes from file start,
                   "nbytes": ...}}}}, "meta": {...}}
     then the arrays, each starting on a 256-byte boundary, in the layouts of chadslab_amd.formats
     (i4g32: "packed" uint8 [N,K/2], "scale" float16 [N,K/32];  i8row: "w" int8 [N,K], "scale" float32 [N];
-     raw: "data" of any dtype, e.g. norm weights).
+     mxfp4: "packed" uint8 [N,K/2], "scale" uint8 [N,K/32], both with E in front for the matrices of experts;  raw: "data" of any dtype, e.g. norm weights).
 
 The reference snapshot defines no checkpoint format for this path; this one is the build's own.
 """
@@ -22,12 +22,12 @@ from typing import Dict, Union
 import numpy as np
 import torch
 
-from .formats import QWeightInt4G32, QWeightInt8
+from .formats import QExpertsMXFP4, QWeightInt4G32, QWeightInt8, QWeightMXFP4
 
 MAGIC = b"CHADQW01"
 ALIGN = 256
 
-Entry = Union[QWeightInt4G32, QWeightInt8, torch.Tensor, np.ndarray]
+Entry = Union[QWeightInt4G32, QWeightInt8, QWeightMXFP4, QExpertsMXFP4, torch.Tensor, np.ndarray]
 
 
 def _np(t) -> np.ndarray:
@@ -39,12 +39,20 @@ def _np(t) -> np.ndarray:
     return np.ascontiguousarray(t)
 
 
+def _shape(e: Entry):
+    return [e.E, e.N, e.K] if isinstance(e, QExpertsMXFP4) else [e.N, e.K]
+
+
 def _arrays(e: Entry):
     if isinstance(e, QWeightInt4G32):
         return "i4g32", [e.N, e.K], {"packed": _np(e.packed), "scale": _np(e.scale)}
     if isinstance(e, QWeightInt8):
         return "i8row", [e.N, e.K], {"w": _np(e.w), "scale": _np(e.scale)}
+    if isinstance(e, (QWeightMXFP4, QExpertsMXFP4)):
+        return "mxfp4", _shape(e), {"packed": _np(e.packed), "scale": _np(e.scale)}
     a = _np(e)
+    if a.dtype.hasobject:
+        raise TypeError("a weight file holds quantized weights and plain tensors, got %r" % type(e))
     return "raw", list(a.shape), {"data": a}
 
 
@@ -109,7 +117,7 @@ def _copy_out(m: np.ndarray, shape, device) -> torch.Tensor:
 
 
 def load(path: str, device="cpu") -> Dict[str, Entry]:
-    """Memory-maps `path` and returns name -> QWeightInt4G32 / QWeightInt8 / tensor on `device`.  Every array is
+    """Memory-maps `path` and returns name -> quantized weight or tensor on `device`.  Every array is
     copied out of the map in slabs of 64 MiB (to the GPU for a GPU device), so a multi-GB file is never held whole
     in host memory; the map is closed on return."""
     hdr = read_header(path)
@@ -129,10 +137,12 @@ def load(path: str, device="cpu") -> Dict[str, Entry]:
             out[name] = QWeightInt4G32(arrs["packed"], arrs["scale"])
         elif t["kind"] == "i8row":
             out[name] = QWeightInt8(arrs["w"], arrs["scale"])
+        elif t["kind"] == "mxfp4":
+            out[name] = (QExpertsMXFP4 if arrs["packed"].dim() == 3 else QWeightMXFP4)(arrs["packed"], arrs["scale"])
         elif t["kind"] == "raw":
             out[name] = arrs["data"]
         else:
             raise ValueError("%s: unknown tensor kind %r" % (path, t["kind"]))
-        if t["kind"] != "raw" and [out[name].N, out[name].K] != t["shape"]:
-            raise ValueError("%s: %s has shape %s, header says %s" % (path, name, [out[name].N, out[name].K], t["shape"]))
+        if t["kind"] != "raw" and _shape(out[name]) != t["shape"]:
+            raise ValueError("%s: %s has shape %s, header says %s" % (path, name, _shape(out[name]), t["shape"]))
     return out

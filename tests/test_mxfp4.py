@@ -93,3 +93,21 @@ def test_library_refuses_bad_sizes_without_a_launch():
     f = _lib.load().chadq_product_mxfp4_workspace_bytes
     for m, n, k in ((0, 64, 64), (4, 0, 64), (4, 64, 0), (4, 64, 48), (-1, 64, 64)):
         assert f(m, n, k, 0) == 0 and f(m, n, k, 1) == 0
+
+
+def test_weight_file_holds_them(tmp_path):
+    """One matrix and those of experts come back as they were; what a file cannot hold is refused instead of written as addresses."""
+    from chadslab_amd import QExpertsMXFP4, QWeightMXFP4, wfile
+    from chadslab_amd.formats import QWeightInt4G32Tiles
+
+    r = np.random.Generator(np.random.PCG64(8))
+    q, e = (c(*(torch.from_numpy(r.integers(0, 256, (*s, n), dtype=np.uint8)) for n in (48, 3))) for c, s in ((QWeightMXFP4, (5,)), (QExpertsMXFP4, (2, 5))))
+    path = str(tmp_path / "w.chadq")
+    wfile.save(path, {"one": q, "experts": e, "norm": torch.arange(4.0)})
+    back = wfile.load(path)
+    for name, want in (("one", q), ("experts", e)):
+        assert type(back[name]) is type(want) and torch.equal(back[name].packed, want.packed) and torch.equal(back[name].scale, want.scale)
+    assert torch.equal(back["norm"], torch.arange(4.0)) and wfile.read_header(path)["tensors"]["experts"]["shape"] == [2, 5, 96]
+    for bad in (object(), QWeightInt4G32Tiles.__new__(QWeightInt4G32Tiles)):
+        with pytest.raises(TypeError):
+            wfile.save(path, {"w": bad})
