@@ -509,6 +509,37 @@ def test_moe_refusals(ops):
             ops.moe_ffn(x, z, (gate, up, down), top_k=bad)
 
 
+# ---- sizes for which the rule takes each of the tiles, with K that ends inside a step -------------------------------------
+@pytest.mark.parametrize("x4,m,n,k", [(False, 19, 32, 608), (False, 135, 3466, 576), (False, 2919, 139, 640), (False, 2798, 2060, 608), (False, 523, 3762, 576),
+                                      (False, 1063, 2698, 576), (False, 803, 4884, 608), (False, 2340, 1553, 640), (True, 2864, 146, 640), (True, 2524, 1594, 608),
+                                      (True, 18, 36, 608), (True, 331, 2753, 576), (True, 2887, 652, 704), (True, 2358, 1683, 608), (True, 1608, 1183, 608),
+                                      (True, 2347, 1550, 608), (True, 2188, 3702, 608)])
+def test_every_tile(ops, x4, m, n, k):
+    from chadslab_amd import QWeightMXFP4
+
+    r = np.random.Generator(np.random.PCG64(m + n))
+    c, s = weights(r, n, k)
+    x, x64 = activations(r, m, k, x4)
+    check(ops.qlinear(x, QWeightMXFP4(dev(c), dev(s))), x64, dev(O.dequant_mxfp4(c, s)))
+
+
+@pytest.mark.parametrize("x4,m,n,k,e", [(False, 17, 32, 608, 2), (False, 69, 4062, 800, 8), (False, 115, 1277, 640, 13), (False, 88, 3552, 608, 10), (False, 129, 1436, 800, 11),
+                                        (False, 202, 4169, 640, 15), (False, 710, 4513, 800, 13), (False, 2827, 1386, 608, 2), (True, 17, 33, 672, 2), (True, 67, 2089, 576, 8),
+                                        (True, 113, 2567, 608, 14), (True, 348, 4184, 736, 15), (True, 18, 36, 2176, 2), (True, 1958, 3084, 576, 11), (True, 245, 4573, 1568, 7),
+                                        (True, 209, 4216, 1056, 15), (True, 79, 3988, 928, 8)])
+def test_every_tile_by_group(ops, x4, m, n, k, e):
+    """Groups of any sizes, the first one empty."""
+    r = np.random.Generator(np.random.PCG64(m * 3 + n))
+    counts = [0, *r.multinomial(m, r.dirichlet(np.ones(e - 1)))]
+    x, x64, w, w64, offsets = grouped_case(m + n + k, counts, n, k, x4)
+    check_groups(ops.qgemm_grouped(x, w, offsets), x64, w64, offsets.tolist())
+
+
+@pytest.mark.parametrize("tokens,h,f,experts", [(19, 1568, 64, 2), (22, 704, 32, 2), (92, 576, 1824, 11), (200, 672, 2080, 15), (303, 640, 2848, 11)])
+def test_every_tile_of_gate_and_up(ops, tokens, h, f, experts):
+    test_moe(ops, tokens, h, f, experts, 1, False)
+
+
 # ---- the ends of the ranges ------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("m", [1, 12, 40, 300])
 def test_subnormal_activations_and_weights(ops, m):
