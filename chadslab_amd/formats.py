@@ -101,7 +101,7 @@ class QWeightInt4G32Tiles:
         return self.packed.size(1) * 2
 
 
-def _check_mxfp4(name: str, packed: torch.Tensor, scale: torch.Tensor, dim: int) -> None:
+def check_mxfp4(name: str, packed: torch.Tensor, scale: torch.Tensor, dim: int) -> None:
     lead = "E,N" if dim == 3 else "N"
     if packed.dtype != torch.uint8 or packed.dim() != dim:
         raise ValueError("%s.packed must be uint8 [%s,K/2]" % (name, lead))
@@ -117,7 +117,7 @@ class QWeightMXFP4:
     scale: torch.Tensor   # uint8 [N, K/32]
 
     def __post_init__(self):
-        _check_mxfp4("QWeightMXFP4", self.packed, self.scale, 2)
+        check_mxfp4("QWeightMXFP4", self.packed, self.scale, 2)
 
     @property
     def N(self) -> int:
@@ -138,7 +138,7 @@ class QExpertsMXFP4:
     scale: torch.Tensor   # uint8 [E, N, K/32]
 
     def __post_init__(self):
-        _check_mxfp4("QExpertsMXFP4", self.packed, self.scale, 3)
+        check_mxfp4("QExpertsMXFP4", self.packed, self.scale, 3)
 
     @property
     def E(self) -> int:

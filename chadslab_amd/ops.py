@@ -12,7 +12,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .formats import GROUP, QExpertsMXFP4, QWeightInt4G32, QWeightInt4G32Tiles, QWeightInt8, QWeightMXFP4
+from .formats import GROUP, QExpertsMXFP4, QWeightInt4G32, QWeightInt4G32Tiles, QWeightInt8, QWeightMXFP4, check_mxfp4
 
 QWeight = Union[QWeightInt4G32, QWeightInt8, QWeightMXFP4]
 GEMV_MAX_M = 16  # decode batch sizes served by the bandwidth kernel
@@ -71,9 +71,17 @@ def _launch(device: torch.device, name: str, *args) -> None:
             _lib.check(fn(*args, _stream()), name)
 
 
-def _mxfp4(q: Union[QWeightMXFP4, QExpertsMXFP4], name: str, device: Optional[torch.device] = None):
-    """Codes and scales of a container, checked before their addresses go to the library."""
-    p, s = _dev(q.packed, name + ".packed", torch.uint8), _dev(q.scale, name + ".scale", torch.uint8)
+def _arrays(q: Union[QWeightMXFP4, QExpertsMXFP4]):
+    """Codes and scales of a container, which may hold other arrays by now than those it was made of: the kernels read as far as the codes' shape
+    says, so the scales have to fit it."""
+    p, s = q.packed, q.scale
+    check_mxfp4(type(q).__name__, p, s, 3 if isinstance(q, QExpertsMXFP4) else 2)
+    return p, s
+
+
+def _mxfp4(p: torch.Tensor, s: torch.Tensor, name: str, device: Optional[torch.device] = None):
+    """Codes and scales (of _arrays), checked before their addresses go to the library."""
+    p, s = _dev(p, name + ".packed", torch.uint8), _dev(s, name + ".scale", torch.uint8)
     for t in (p, s):
         if t.device != (p.device if device is None else device):
             raise ValueError("%s must live on %s, got %s" % (name, p.device if device is None else device, t.device))
@@ -111,10 +119,11 @@ def dequantize(qw: Union[QWeight, QExpertsMXFP4]) -> torch.Tensor:
         out = _lib.native().dequantize(qw)
         if out is not None:
             return out
-        p, s = _mxfp4(qw, "qw")
-        out = torch.empty(*p.shape[:-1], qw.K, dtype=torch.float32, device=p.device)
+        p, s = _mxfp4(*_arrays(qw), "qw")
+        k = p.size(-1) * 2
+        out = torch.empty(*p.shape[:-1], k, dtype=torch.float32, device=p.device)
         if out.numel():
-            _launch(p.device, "chadq_dequant_mxfp4", p.data_ptr(), s.data_ptr(), out.data_ptr(), out.numel() // qw.K, qw.K)
+            _launch(p.device, "chadq_dequant_mxfp4", p.data_ptr(), s.data_ptr(), out.data_ptr(), out.numel() // k, k)
         return out
     if isinstance(qw, QWeightInt4G32):
         p, s = _dev(qw.packed, "packed", torch.uint8), _dev(qw.scale, "scale", torch.float16)
@@ -134,15 +143,17 @@ def dequantize(qw: Union[QWeight, QExpertsMXFP4]) -> torch.Tensor:
 def _product_mxfp4(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeightMXFP4, out: Optional[torch.Tensor], y_dtype: torch.dtype) -> torch.Tensor:
     """x (bf16 or MXFP4) [M,K] times MXFP4 weights -> fp32 or bf16 [M,N]."""
     x_mx = isinstance(x, QWeightMXFP4)
-    if (not x_mx and x.dim() != 2) or (x.K if x_mx else x.size(1)) != qw.K:
-        raise ValueError("x must be [M,%d], got %s" % (qw.K, (x.N, x.K) if x_mx else tuple(x.shape)))
+    p, s = _arrays(qw)
+    xt, xs = _arrays(x) if x_mx else (x, None)
+    m, n, k = xt.size(0) if xt.dim() else 0, p.size(0), p.size(1) * 2
+    if xt.dim() != 2 or xt.size(1) * (2 if x_mx else 1) != k:
+        raise ValueError("x must be [M,%d], got %s" % (k, (m, xt.size(1) * 2) if x_mx else tuple(x.shape)))
     if x_mx:
-        xt, xs = _mxfp4(x, "x")
+        xt, xs = _mxfp4(xt, xs, "x")
         xs_ptr = xs.data_ptr()
     else:
         xt, xs_ptr = _dev(x, "x", torch.bfloat16), None
-    p, s = _mxfp4(qw, "weights", xt.device)
-    m, n, k = xt.size(0), qw.N, qw.K
+    p, s = _mxfp4(p, s, "weights", xt.device)
     y = _out(out, (m, n), y_dtype, xt.device)
     if m == 0 or n == 0:
         return y
@@ -174,15 +185,17 @@ def qgemm_grouped(x: Union[torch.Tensor, QWeightMXFP4], experts: QExpertsMXFP4, 
     x_mx = isinstance(x, QWeightMXFP4)
     if not isinstance(experts, QExpertsMXFP4):
         raise TypeError("qgemm_grouped wants QExpertsMXFP4, got %r" % type(experts))
-    e, n, k = experts.E, experts.N, experts.K
-    if (not x_mx and x.dim() != 2) or (x.K if x_mx else x.size(1)) != k:
-        raise ValueError("x must be [R,%d], got %s" % (k, (x.N, x.K) if x_mx else tuple(x.shape)))
+    p, s = _arrays(experts)
+    xt, xs = _arrays(x) if x_mx else (x, None)
+    e, n, k = p.size(0), p.size(1), p.size(2) * 2
+    if xt.dim() != 2 or xt.size(1) * (2 if x_mx else 1) != k:
+        raise ValueError("x must be [R,%d], got %s" % (k, (xt.size(0), xt.size(1) * 2) if x_mx else tuple(x.shape)))
     if x_mx:
-        xt, xs = _mxfp4(x, "x")
+        xt, xs = _mxfp4(xt, xs, "x")
         xs_ptr = xs.data_ptr()
     else:
         xt, xs_ptr = _dev(x, "x", torch.bfloat16), None
-    p, s = _mxfp4(experts, "experts", xt.device)
+    p, s = _mxfp4(p, s, "experts", xt.device)
     offsets = _dev(offsets, "offsets", torch.int32)
     if e < 1 or tuple(offsets.shape) != (e + 1,) or offsets.device != xt.device:
         raise ValueError("offsets must be int32 [%d] on %s, one more than there are experts (at least one), got %s on %s"
@@ -421,21 +434,22 @@ def _moe_ffn_mxfp4(x: torch.Tensor, logits: torch.Tensor, experts, top_k: int, r
         return y
     if len(experts) != 3 or not all(isinstance(m, QExpertsMXFP4) for m in experts):
         raise TypeError("MXFP4 experts are one (gate, up, down) triple of QExpertsMXFP4")
+    arrays = [_arrays(m) for m in experts]
     x, z = _dev(x, "x", torch.bfloat16), _dev(logits, "logits", torch.float32)
     if x.dim() != 2:
         raise ValueError("x must be [T,H], got %s" % (tuple(x.shape),))
-    gate, up, down = experts
-    (t, h), e, f = x.shape, gate.E, gate.N
+    (e, f, kh), up, down = ((p.size(0), p.size(1), p.size(2) * 2) for p, _ in arrays)  # [E,F,H], the same, [E,H,F]
+    t, h = x.shape
     if tuple(z.shape) != (t, e) or z.device != x.device:
         raise ValueError("logits must be [%d,%d] on %s" % (t, e, x.device))
-    if (gate.K, up.E, up.N, up.K) != (h, e, f, h) or (down.E, down.N, down.K) != (e, h, f):
+    if kh != h or up != (e, f, h) or down != (e, h, f):
         raise ValueError("gate and up must be [%d,%d,%d] and down [%d,%d,%d]" % (e, f, h, e, h, f))
     lib = _lib.load()
     y = torch.empty(t, h, dtype=torch.bfloat16, device=x.device)
     need = lib.chadq_moe_ffn_mxfp4_workspace_bytes(t, h, f, e, top_k)
     if need == 0:
         raise ValueError("unsupported MoE sizes T=%d H=%d F=%d E=%d top_k=%d" % (t, h, f, e, top_k))
-    ts = [v for name, m in (("gate", gate), ("up", up), ("down", down)) for v in _mxfp4(m, name, x.device)]
+    ts = [v for name, ps in zip(("gate", "up", "down"), arrays) for v in _mxfp4(*ps, name, x.device)]
     arr = _lib.MoeMXFP4(*[v.data_ptr() for v in ts])
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)  # as moe_ffn's
     _launch(x.device, "chadq_moe_ffn_mxfp4", x.data_ptr(), z.data_ptr(), ctypes.byref(arr), y.data_ptr(), t, h, f, e, top_k, int(renorm), ws.data_ptr(), need)

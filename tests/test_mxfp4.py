@@ -111,3 +111,34 @@ def test_weight_file_holds_them(tmp_path):
     for bad in (object(), QWeightInt4G32Tiles.__new__(QWeightInt4G32Tiles)):
         with pytest.raises(TypeError):
             wfile.save(path, {"w": bad})
+
+
+def test_operators_look_at_a_containers_arrays_again():
+    """Arrays exchanged since a container was made: those that no longer fit each other are refused, not read as far as the other's shape says."""
+    from chadslab_amd import QExpertsMXFP4, QWeightMXFP4, ops
+
+    p, s = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    x, off, z = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32), torch.zeros(4, 2)
+
+    def weight(packed=p, scale=s):
+        q = QWeightMXFP4(p, s)
+        q.packed, q.scale = packed, scale
+        return q
+
+    def experts(packed=p.view(2, 2, 32), scale=s.view(2, 2, 2)):
+        e = QExpertsMXFP4(p.view(2, 2, 32), s.view(2, 2, 2))
+        e.packed, e.scale = packed, scale
+        return e
+
+    whole, group = weight(), experts()
+    for bad, message in ((weight(scale=s[:, :1]), "scale must be uint8"), (weight(scale=s[:3]), "scale must be uint8"), (weight(scale=s.float()), "scale must be uint8"),
+                         (weight(packed=p.view(2, 2, 32)), "packed must be uint8"), (weight(packed=p.flatten()), "packed must be uint8"), (weight(packed=p[:, :8]), "multiple of 32")):
+        for call in (lambda: ops.dequantize(bad), lambda: ops.qgemv(x, bad), lambda: ops.qgemm(x, bad), lambda: ops.qlinear(x, bad), lambda: ops.qlinear(bad, whole),
+                     lambda: ops.qgemm(bad, whole), lambda: ops.qgemm_grouped(bad, group, off)):
+            with pytest.raises(ValueError, match=message):
+                call()
+    for bad, message in ((experts(scale=s.view(2, 2, 2)[:, :1]), "scale must be uint8"), (experts(scale=s.view(2, 2, 2)[:1]), "scale must be uint8"),
+                         (experts(packed=p), "packed must be uint8"), (experts(packed=p.view(2, 2, 32)[..., :8]), "multiple of 32")):
+        for call in (lambda: ops.dequantize(bad), lambda: ops.qgemm_grouped(x, bad, off), lambda: ops.moe_ffn(x, z, (bad, group, group), top_k=1), lambda: ops.moe_ffn(x, z, (group, group, bad), top_k=1)):
+            with pytest.raises(ValueError, match=message):
+                call()
