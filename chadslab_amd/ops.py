@@ -88,6 +88,21 @@ def _mxfp4(p: torch.Tensor, s: torch.Tensor, name: str, device: Optional[torch.d
     return p, s
 
 
+def _int4(qw: Union[QWeightInt4G32, QWeightInt4G32Tiles], name: str = ""):
+    """Packed bytes and scales of an int4 matrix, looked at as _arrays does (0.15 us)."""
+    p, s = qw.packed, qw.scale
+    if p.dim() != 2 or s.shape != (p.size(0), p.size(1) // 16):
+        raise ValueError("%sscale must be float16 [N,K/32] beside packed [N,K/2], got %s and %s" % (name, tuple(s.shape), tuple(p.shape)))
+    return _dev(p, name + "packed", torch.uint8), _dev(s, name + "scale", torch.float16)
+
+
+def _int8(qw: QWeightInt8):
+    w, s = qw.w, qw.scale
+    if w.dim() != 2 or s.shape != (w.size(0),):
+        raise ValueError("scale must be float32 [N] beside w [N,K], got %s and %s" % (tuple(s.shape), tuple(w.shape)))
+    return _dev(w, "w", torch.int8), _dev(s, "scale", torch.float32)
+
+
 _MX_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # chadq_dtype
 
 
@@ -126,13 +141,13 @@ def dequantize(qw: Union[QWeight, QExpertsMXFP4]) -> torch.Tensor:
             _launch(p.device, "chadq_dequant_mxfp4", p.data_ptr(), s.data_ptr(), out.data_ptr(), out.numel() // k, k)
         return out
     if isinstance(qw, QWeightInt4G32):
-        p, s = _dev(qw.packed, "packed", torch.uint8), _dev(qw.scale, "scale", torch.float16)
+        p, s = _int4(qw)
         out = torch.empty(qw.N, qw.K, dtype=torch.float32, device=p.device)
         _lib.check(lib.chadq_dequant_i4g32(p.data_ptr(), s.data_ptr(), out.data_ptr(), qw.N, qw.K, _stream()),
                    "chadq_dequant_i4g32")
         return out
     if isinstance(qw, QWeightInt8):
-        w, s = _dev(qw.w, "w", torch.int8), _dev(qw.scale, "scale", torch.float32)
+        w, s = _int8(qw)
         out = torch.empty(qw.N, qw.K, dtype=torch.float32, device=w.device)
         _lib.check(lib.chadq_dequant_i8row(w.data_ptr(), s.data_ptr(), out.data_ptr(), qw.N, qw.K, _stream()),
                    "chadq_dequant_i8row")
@@ -240,7 +255,7 @@ def _gemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor], fp32_elemen
         raise ValueError("fp32_elements applies to int8 weights (fp32 activations) only")
     if isinstance(qw, QWeightInt4G32):
         x = _dev(x, "x", torch.bfloat16)
-        p, s = _dev(qw.packed, "packed", torch.uint8), _dev(qw.scale, "scale", torch.float16)
+        p, s = _int4(qw)
         y = _out(out, (m, n), y_dtype, x.device)
         name = "chadq_gemv_i4g32_bf16" if bf16_out else "chadq_gemv_i4g32"
         need = _lib.native().gemv_bytes(m, n, k, 0)  # as in qgemm
@@ -253,7 +268,7 @@ def _gemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor], fp32_elemen
         return y
     if isinstance(qw, QWeightInt8):
         x = _dev(x, "x", torch.float32)
-        w, s = _dev(qw.w, "w", torch.int8), _dev(qw.scale, "scale", torch.float32)
+        w, s = _int8(qw)
         y = _out(out, (m, n), y_dtype, x.device)
         name = "chadq_gemv_i8row_fp32" if fp32_elements else "chadq_gemv_i8row_bf16" if bf16_out else "chadq_gemv_i8row"
         need = 0 if fp32_elements else _lib.native().gemv_bytes(m, n, k, 1)
@@ -281,7 +296,7 @@ def qgemm(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, out: Optional[torch
     y = _out(out, (m, n), torch.bfloat16, x.device)
     # Scratch for the K parts of a product of few tiles (0 bytes where one part is the quicker form): a fresh one per call, as moe_ffn's.
     if isinstance(qw, QWeightInt4G32):
-        p, s = _dev(qw.packed, "packed", torch.uint8), _dev(qw.scale, "scale", torch.float16)
+        p, s = _int4(qw)
         need = _lib.native().gemm_bytes(m, n, k, 0)
         if need:
             ws = x.new_empty(need, dtype=torch.uint8)
@@ -291,7 +306,7 @@ def qgemm(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, out: Optional[torch
         _lib.check(lib.chadq_gemm_i4g32_bf16(x.data_ptr(), p.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, _stream()), "chadq_gemm_i4g32_bf16")
         return y
     if isinstance(qw, QWeightInt8):
-        w, s = _dev(qw.w, "w", torch.int8), _dev(qw.scale, "scale", torch.float32)
+        w, s = _int8(qw)
         need = _lib.native().gemm_bytes(m, n, k, 1)
         if need:
             ws = x.new_empty(need, dtype=torch.uint8)
@@ -355,7 +370,7 @@ def moe_route(logits: torch.Tensor, top_k: int = 2, renorm: bool = True):
 
 def _repack(w, to_tiles: bool):
     lib = _lib.load()
-    p, s = _dev(w.packed, "packed", torch.uint8), _dev(w.scale, "scale", torch.float16)
+    p, s = _int4(w)
     if w.N % 32 or w.K % 256:
         raise ValueError("tile order needs N % 32 == 0 and K % 256 == 0 (N=%d, K=%d)" % (w.N, w.K))
     po, so = torch.empty_like(p), torch.empty_like(s)
@@ -408,9 +423,7 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, experts, *, top_k: int = 2, r
     for i, (g, u, d) in enumerate(experts):
         if (g.N, g.K) != (f, h) or (u.N, u.K) != (f, h) or (d.N, d.K) != (h, f):
             raise ValueError("expert %d: gate/up must be [%d,%d] and down [%d,%d]" % (i, f, h, h, f))
-        ts = [_dev(g.packed, "gate", torch.uint8), _dev(g.scale, "gate scale", torch.float16),
-              _dev(u.packed, "up", torch.uint8), _dev(u.scale, "up scale", torch.float16),
-              _dev(d.packed, "down", torch.uint8), _dev(d.scale, "down scale", torch.float16)]
+        ts = [*_int4(g, "gate "), *_int4(u, "up "), *_int4(d, "down ")]
         keep.append(ts)
         arr[i] = _lib.MoeExpertI4G32(*[v.data_ptr() for v in ts])
     need = lib.chadq_moe_ffn_i4g32_workspace_bytes(t, h, f, e, top_k)

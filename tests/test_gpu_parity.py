@@ -1447,3 +1447,21 @@ def test_gemv_in_parts_of_k(ops, m, n, k):
             assert ws(x.data_ptr(), wp.data_ptr(), sc.data_ptr(), again.data_ptr(), m, n, k, 0, ptr, size, stream) == 0
             assert torch.equal(again.view(torch.int32), one.view(torch.int32))
         assert ws(x.data_ptr(), wp.data_ptr(), sc.data_ptr(), again.data_ptr(), m, n, k, 0, scratch.data_ptr() + 4, need, stream) == -3
+
+
+def test_exchanged_scales_are_looked_at_again(ops):
+    """Scales put into a container after it was made, of another shape than its weights want: refused on every road to the kernels."""
+    from chadslab_amd import QWeightInt4G32, QWeightInt8
+
+    n, k = 64, 256
+    x, xf, z = torch.zeros(3, k, dtype=torch.bfloat16, device="cuda:0"), torch.zeros(3, k, device="cuda:0"), torch.zeros(3, 1, device="cuda:0")
+    q = QWeightInt4G32(torch.zeros(n, k // 2, dtype=torch.uint8, device="cuda:0"), torch.zeros(n, k // 32, dtype=torch.float16, device="cuda:0"))
+    down = QWeightInt4G32(torch.zeros(k, n // 2, dtype=torch.uint8, device="cuda:0"), torch.zeros(k, n // 32, dtype=torch.float16, device="cuda:0"))
+    i8 = QWeightInt8(torch.zeros(n, k, dtype=torch.int8, device="cuda:0"), torch.zeros(n, device="cuda:0"))
+    assert not ops.qlinear(x, q).any() and not ops.qlinear(xf, i8).any() and not ops.moe_ffn(x, z, [(q, q, down)], top_k=1).any()
+    q.scale, i8.scale = q.scale[:, :4], i8.scale[:32]
+    for call in (lambda: ops.qlinear(x, q), lambda: ops.qgemv(x, q), lambda: ops.qgemm(x, q), lambda: ops.dequantize(q), lambda: ops.to_tiles(q),
+                 lambda: ops.moe_ffn(x, z, [(q, q, down)], top_k=1), lambda: ops.qlinear(xf, i8), lambda: ops.qgemv(xf, i8), lambda: ops.qgemv(xf, i8, fp32_elements=True),
+                 lambda: ops.qgemm(x, i8), lambda: ops.dequantize(i8)):
+        with pytest.raises(ValueError, match="scale must be"):
+            call()

@@ -129,3 +129,25 @@ def test_the_library_is_linked_before_the_host_module_can_fail(monkeypatch, tmp_
         build.build(verbose=False)
     assert (tmp_path / "libchadq.so").exists() and "libchadq.so.tmp" in linked
     assert build.build(verbose=False, host=False) == tmp_path / "libchadq.so"
+
+
+def test_operators_look_at_a_containers_arrays_again():
+    """Scales exchanged since a container was made, that no longer fit its weights, are refused before anything is read as far as the weights' shape says."""
+    import torch
+
+    from chadslab_amd import QWeightInt4G32, QWeightInt8, ops
+    from chadslab_amd.formats import QWeightInt4G32Tiles
+
+    for kind in (QWeightInt4G32, QWeightInt4G32Tiles):
+        q = kind(torch.zeros(64, 128, dtype=torch.uint8), torch.zeros(64, 8, dtype=torch.float16))
+        convert = ops.to_tiles if kind is QWeightInt4G32 else ops.to_rows
+        for bad in (q.scale[:, :4], q.scale[:32], q.scale.flatten()):
+            q.scale = bad
+            for call in (convert, ops.dequantize) if kind is QWeightInt4G32 else (convert,):
+                with pytest.raises(ValueError, match="scale must be"):
+                    call(q)
+    q = QWeightInt8(torch.zeros(4, 32, dtype=torch.int8), torch.zeros(4))
+    for bad in (q.scale[:3], q.scale.view(4, 1)):
+        q.scale = bad
+        with pytest.raises(ValueError, match="scale must be"):
+            ops.dequantize(q)
