@@ -103,6 +103,15 @@ def _int8(qw: QWeightInt8):
     return _dev(w, "w", torch.int8), _dev(s, "scale", torch.float32)
 
 
+def _rows(x: Union[torch.Tensor, QWeightMXFP4]):
+    """The activations of a product on MXFP4 weights: a tensor and None, or codes and scales of one matrix."""
+    if isinstance(x, torch.Tensor):
+        return x, None
+    if not isinstance(x, QWeightMXFP4):
+        raise TypeError("x must be a tensor or a QWeightMXFP4 (of activations of more dimensions: quantize_mxfp4(x.flatten(0, -2))), got %r" % type(x))
+    return _arrays(x)
+
+
 _MX_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # chadq_dtype
 
 
@@ -157,9 +166,9 @@ def dequantize(qw: Union[QWeight, QExpertsMXFP4]) -> torch.Tensor:
 
 def _product_mxfp4(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeightMXFP4, out: Optional[torch.Tensor], y_dtype: torch.dtype) -> torch.Tensor:
     """x (bf16 or MXFP4) [M,K] times MXFP4 weights -> fp32 or bf16 [M,N]."""
-    x_mx = isinstance(x, QWeightMXFP4)
+    xt, xs = _rows(x)
+    x_mx = xs is not None
     p, s = _arrays(qw)
-    xt, xs = _arrays(x) if x_mx else (x, None)
     m, n, k = xt.size(0) if xt.dim() else 0, p.size(0), p.size(1) * 2
     if xt.dim() != 2 or xt.size(1) * (2 if x_mx else 1) != k:
         raise ValueError("x must be [M,%d], got %s" % (k, (m, xt.size(1) * 2) if x_mx else tuple(x.shape)))
@@ -182,7 +191,7 @@ def _product_mxfp4(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeightMXFP4, out: 
 
 
 def _no_mxfp4(x, qw) -> None:
-    if isinstance(x, QWeightMXFP4):
+    if isinstance(x, (QWeightMXFP4, QExpertsMXFP4)):
         raise TypeError("MXFP4 activations go with MXFP4 weights, got %r" % type(qw))
 
 
@@ -197,11 +206,11 @@ def qgemm_grouped(x: Union[torch.Tensor, QWeightMXFP4], experts: QExpertsMXFP4, 
         y = _lib.native().grouped(x, experts, offsets)
         if y is not None:
             return y
-    x_mx = isinstance(x, QWeightMXFP4)
     if not isinstance(experts, QExpertsMXFP4):
         raise TypeError("qgemm_grouped wants QExpertsMXFP4, got %r" % type(experts))
+    xt, xs = _rows(x)
+    x_mx = xs is not None
     p, s = _arrays(experts)
-    xt, xs = _arrays(x) if x_mx else (x, None)
     e, n, k = p.size(0), p.size(1), p.size(2) * 2
     if xt.dim() != 2 or xt.size(1) * (2 if x_mx else 1) != k:
         raise ValueError("x must be [R,%d], got %s" % (k, (xt.size(0), xt.size(1) * 2) if x_mx else tuple(x.shape)))
@@ -242,7 +251,8 @@ def _gemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor], fp32_elemen
     if isinstance(qw, QWeightMXFP4):
         if fp32_elements:
             raise ValueError("fp32_elements applies to int8 weights (fp32 activations) only")
-        m = x.N if isinstance(x, QWeightMXFP4) else x.size(0) if x.dim() == 2 else 0
+        xt = _rows(x)[0]
+        m = xt.size(0) if xt.dim() == 2 else 0
         if m > GEMV_MAX_M:
             raise ValueError("qgemv takes at most %d rows, got %d" % (GEMV_MAX_M, m))
         return _product_mxfp4(x, qw, out, y_dtype)
@@ -323,13 +333,13 @@ def qlinear(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, *, out_dtype: Opt
 
     Up to 16 rows go to the bandwidth-bound GEMV (fp32 result); more rows go to the MFMA GEMM (bf16 result).
     out_dtype picks the result type.  The GEMV writes bf16 itself if that is asked for (the same sums rounded once); any
-    other type than the kernel's native one is a cast.  x may be a QWeightMXFP4 where the weights are.
+    other type than the kernel's native one is a cast.  x may be a QWeightMXFP4, [M,K], where the weights are one.
     """
     native = _lib.native()
     y = native.linear(x, qw, out_dtype)
     if y is not None:
         return y
-    if isinstance(x, QWeightMXFP4):
+    if not isinstance(x, torch.Tensor):
         y = _qlinear_2d(x, qw, out_dtype if out_dtype == torch.bfloat16 else None)
         return y if out_dtype is None or y.dtype == out_dtype else y.to(out_dtype)
     # more dimensions, strides and a cast at the end are dealt with here, around the native call (8.7 -> 6.2 us of host time for an x of three
@@ -347,7 +357,7 @@ def qlinear(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, *, out_dtype: Opt
 def _qlinear_2d(x2: torch.Tensor, qw: QWeight, written: Optional[torch.dtype]) -> torch.Tensor:
     """What the native call leaves: misplaced or strided weights, other types, everything that raises."""
     if isinstance(qw, QWeightMXFP4):  # (no rows at all: an empty result, of the type that few rows have)
-        few = (x2.N if isinstance(x2, QWeightMXFP4) else x2.size(0)) <= GEMV_MAX_M
+        few = _rows(x2)[0].size(0) <= GEMV_MAX_M
         return _product_mxfp4(x2, qw, None, torch.float32 if few and written is None else torch.bfloat16)
     _no_mxfp4(x2, qw)
     m = x2.size(0)

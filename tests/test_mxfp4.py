@@ -142,3 +142,20 @@ def test_operators_look_at_a_containers_arrays_again():
         for call in (lambda: ops.dequantize(bad), lambda: ops.qgemm_grouped(x, bad, off), lambda: ops.moe_ffn(x, z, (bad, group, group), top_k=1), lambda: ops.moe_ffn(x, z, (group, group, bad), top_k=1)):
             with pytest.raises(ValueError, match=message):
                 call()
+
+
+def test_quantised_activations_of_more_than_two_dimensions_are_refused():
+    """quantize_mxfp4 takes three dimensions for the matrices of experts; as activations these are refused by name."""
+    from chadslab_amd import QExpertsMXFP4, QWeightInt4G32, QWeightInt8, QWeightMXFP4, ops
+
+    p, s = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    q, e, off = QWeightMXFP4(p, s), QExpertsMXFP4(p.view(2, 2, 32), s.view(2, 2, 2)), torch.zeros(3, dtype=torch.int32)
+    for call in (ops.qlinear, ops.qgemv, ops.qgemm, lambda x, _: ops.qgemm_grouped(x, e, off), lambda x, w: ops.qlinear(x, w, out_dtype=torch.bfloat16)):
+        with pytest.raises(TypeError, match="quantize_mxfp4"):
+            call(e, q)
+        with pytest.raises(TypeError, match="x must be"):
+            call(p.numpy(), q)
+    for w in (QWeightInt4G32(p, torch.ones(4, 2, dtype=torch.float16)), QWeightInt8(p.to(torch.int8), torch.ones(4))):
+        for call in (ops.qlinear, ops.qgemv, ops.qgemm):
+            with pytest.raises(TypeError, match="MXFP4 activations"):
+                call(e, w)
