@@ -411,11 +411,14 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, experts, *, top_k: int = 2, r
     rounding; at most 16 tokens take exact weights in row order and, where the experts hit hold at most 64 MB, in tile order
     too, with the same bits from both.  Or experts is one triple of QExpertsMXFP4, gate and up [E,F,H] and down [E,H,F]: weights multiplied as
     they are.  Returns bf16 [T,H]."""
-    if isinstance(experts, (tuple, list)) and any(isinstance(m, QExpertsMXFP4) for m in experts):
+    several = isinstance(experts, (tuple, list))
+    if several and experts and isinstance(experts[0], QExpertsMXFP4):
         return _moe_ffn_mxfp4(x, logits, experts, top_k, renorm)
     y = _lib.native().moe_ffn(x, logits, experts, top_k, renorm)
     if y is not None:
         return y
+    if several and any(isinstance(m, QExpertsMXFP4) for m in experts):  # (not a triple: refused there.  Here, as a look at each of 16 experts takes 1 us)
+        return _moe_ffn_mxfp4(x, logits, experts, top_k, renorm)
     lib = _lib.load()  # (as in qlinear)
     x = _dev(x, "x", torch.bfloat16)
     z = _dev(logits, "logits", torch.float32)
