@@ -89,18 +89,20 @@ def _mxfp4(p: torch.Tensor, s: torch.Tensor, name: str, device: Optional[torch.d
 
 
 def _int4(qw: Union[QWeightInt4G32, QWeightInt4G32Tiles], name: str = ""):
-    """Packed bytes and scales of an int4 matrix, looked at as _arrays does (0.15 us)."""
+    """Packed bytes, scales, N and K of an int4 matrix, looked at as _arrays does (no slower than asking the container for N and K)."""
     p, s = qw.packed, qw.scale
-    if p.dim() != 2 or s.shape != (p.size(0), p.size(1) // 16):
+    n, kb = p.shape if p.dim() == 2 else (-1, -1)
+    if s.shape != (n, kb >> 4):
         raise ValueError("%sscale must be float16 [N,K/32] beside packed [N,K/2], got %s and %s" % (name, tuple(s.shape), tuple(p.shape)))
-    return _dev(p, name + "packed", torch.uint8), _dev(s, name + "scale", torch.float16)
+    return p, s, n, kb * 2
 
 
 def _int8(qw: QWeightInt8):
     w, s = qw.w, qw.scale
-    if w.dim() != 2 or s.shape != (w.size(0),):
+    n, k = w.shape if w.dim() == 2 else (-1, -1)
+    if s.shape != (n,):
         raise ValueError("scale must be float32 [N] beside w [N,K], got %s and %s" % (tuple(s.shape), tuple(w.shape)))
-    return _dev(w, "w", torch.int8), _dev(s, "scale", torch.float32)
+    return w, s, n, k
 
 
 def _rows(x: Union[torch.Tensor, QWeightMXFP4]):
@@ -150,15 +152,17 @@ def dequantize(qw: Union[QWeight, QExpertsMXFP4]) -> torch.Tensor:
             _launch(p.device, "chadq_dequant_mxfp4", p.data_ptr(), s.data_ptr(), out.data_ptr(), out.numel() // k, k)
         return out
     if isinstance(qw, QWeightInt4G32):
-        p, s = _int4(qw)
-        out = torch.empty(qw.N, qw.K, dtype=torch.float32, device=p.device)
-        _lib.check(lib.chadq_dequant_i4g32(p.data_ptr(), s.data_ptr(), out.data_ptr(), qw.N, qw.K, _stream()),
+        p, s, n, k = _int4(qw)
+        p, s = _dev(p, "packed", torch.uint8), _dev(s, "scale", torch.float16)
+        out = torch.empty(n, k, dtype=torch.float32, device=p.device)
+        _lib.check(lib.chadq_dequant_i4g32(p.data_ptr(), s.data_ptr(), out.data_ptr(), n, k, _stream()),
                    "chadq_dequant_i4g32")
         return out
     if isinstance(qw, QWeightInt8):
-        w, s = _int8(qw)
-        out = torch.empty(qw.N, qw.K, dtype=torch.float32, device=w.device)
-        _lib.check(lib.chadq_dequant_i8row(w.data_ptr(), s.data_ptr(), out.data_ptr(), qw.N, qw.K, _stream()),
+        w, s, n, k = _int8(qw)
+        w, s = _dev(w, "w", torch.int8), _dev(s, "scale", torch.float32)
+        out = torch.empty(n, k, dtype=torch.float32, device=w.device)
+        _lib.check(lib.chadq_dequant_i8row(w.data_ptr(), s.data_ptr(), out.data_ptr(), n, k, _stream()),
                    "chadq_dequant_i8row")
         return out
     raise TypeError("unknown weight container %r" % type(qw))
@@ -193,6 +197,18 @@ def _product_mxfp4(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeightMXFP4, out: 
 def _no_mxfp4(x, qw) -> None:
     if isinstance(x, (QWeightMXFP4, QExpertsMXFP4)):
         raise TypeError("MXFP4 activations go with MXFP4 weights, got %r" % type(qw))
+
+
+def _rows_of(x: torch.Tensor, k: int, qw: QWeight) -> int:
+    """M of activations [M,k]."""
+    try:
+        m, xk = x.shape
+    except (AttributeError, ValueError):
+        _no_mxfp4(x, qw)
+        m, xk = 0, -1
+    if xk != k:
+        raise ValueError("x must be [M,%d], got %s" % (k, tuple(x.shape)))
+    return m
 
 
 def qgemm_grouped(x: Union[torch.Tensor, QWeightMXFP4], experts: QExpertsMXFP4, offsets: torch.Tensor,
@@ -248,7 +264,11 @@ def _gemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor], fp32_elemen
     """qgemv with the sums as fp32 or, bf16_out, rounded to bf16 by the kernel that forms them."""
     lib = _lib.load()
     y_dtype = torch.bfloat16 if bf16_out else torch.float32
-    if isinstance(qw, QWeightMXFP4):
+    if isinstance(qw, QWeightInt4G32):
+        w, s, n, k = _int4(qw)
+    elif isinstance(qw, QWeightInt8):
+        w, s, n, k = _int8(qw)
+    elif isinstance(qw, QWeightMXFP4):
         if fp32_elements:
             raise ValueError("fp32_elements applies to int8 weights (fp32 activations) only")
         xt = _rows(x)[0]
@@ -256,16 +276,14 @@ def _gemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor], fp32_elemen
         if m > GEMV_MAX_M:
             raise ValueError("qgemv takes at most %d rows, got %d" % (GEMV_MAX_M, m))
         return _product_mxfp4(x, qw, out, y_dtype)
-    _no_mxfp4(x, qw)
-    n, k = qw.N, qw.K
-    if x.dim() != 2 or x.size(1) != k:
-        raise ValueError("x must be [M,%d], got %s" % (k, tuple(x.shape)))
-    m = x.size(0)
+    else:
+        raise TypeError("unknown weight container %r" % type(qw))
+    m = _rows_of(x, k, qw)
     if fp32_elements and not isinstance(qw, QWeightInt8):
         raise ValueError("fp32_elements applies to int8 weights (fp32 activations) only")
     if isinstance(qw, QWeightInt4G32):
         x = _dev(x, "x", torch.bfloat16)
-        p, s = _int4(qw)
+        p, s = _dev(w, "packed", torch.uint8), _dev(s, "scale", torch.float16)
         y = _out(out, (m, n), y_dtype, x.device)
         name = "chadq_gemv_i4g32_bf16" if bf16_out else "chadq_gemv_i4g32"
         need = _lib.native().gemv_bytes(m, n, k, 0)  # as in qgemm
@@ -276,37 +294,37 @@ def _gemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor], fp32_elemen
             return y
         _lib.check(getattr(lib, name)(x.data_ptr(), p.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, _stream()), name)
         return y
-    if isinstance(qw, QWeightInt8):
-        x = _dev(x, "x", torch.float32)
-        w, s = _int8(qw)
-        y = _out(out, (m, n), y_dtype, x.device)
-        name = "chadq_gemv_i8row_fp32" if fp32_elements else "chadq_gemv_i8row_bf16" if bf16_out else "chadq_gemv_i8row"
-        need = 0 if fp32_elements else _lib.native().gemv_bytes(m, n, k, 1)
-        if need:
-            ws = x.new_empty(need, dtype=torch.uint8)
-            _lib.check(lib.chadq_gemv_i8row_ws(x.data_ptr(), w.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, int(bf16_out), ws.data_ptr(), need,
-                                               _stream()), name)
-            return y
-        _lib.check(getattr(lib, name)(x.data_ptr(), w.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, _stream()), name)
+    x = _dev(x, "x", torch.float32)
+    w, s = _dev(w, "w", torch.int8), _dev(s, "scale", torch.float32)
+    y = _out(out, (m, n), y_dtype, x.device)
+    name = "chadq_gemv_i8row_fp32" if fp32_elements else "chadq_gemv_i8row_bf16" if bf16_out else "chadq_gemv_i8row"
+    need = 0 if fp32_elements else _lib.native().gemv_bytes(m, n, k, 1)
+    if need:
+        ws = x.new_empty(need, dtype=torch.uint8)
+        _lib.check(lib.chadq_gemv_i8row_ws(x.data_ptr(), w.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, int(bf16_out), ws.data_ptr(), need,
+                                           _stream()), name)
         return y
-    raise TypeError("unknown weight container %r" % type(qw))
+    _lib.check(getattr(lib, name)(x.data_ptr(), w.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, _stream()), name)
+    return y
 
 
 def qgemm(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Prefill product on the matrix cores: x bf16 [M,K], or QWeightMXFP4 for MXFP4 weights, -> bf16 [M,N], fp32 accumulate."""
     lib = _lib.load()
-    if isinstance(qw, QWeightMXFP4):
+    if isinstance(qw, QWeightInt4G32):
+        w, s, n, k = _int4(qw)
+    elif isinstance(qw, QWeightInt8):
+        w, s, n, k = _int8(qw)
+    elif isinstance(qw, QWeightMXFP4):
         return _product_mxfp4(x, qw, out, torch.bfloat16)
-    _no_mxfp4(x, qw)
-    n, k = qw.N, qw.K
-    if x.dim() != 2 or x.size(1) != k:
-        raise ValueError("x must be [M,%d], got %s" % (k, tuple(x.shape)))
+    else:
+        raise TypeError("unknown weight container %r" % type(qw))
+    m = _rows_of(x, k, qw)
     x = _dev(x, "x", torch.bfloat16)
-    m = x.size(0)
     y = _out(out, (m, n), torch.bfloat16, x.device)
     # Scratch for the K parts of a product of few tiles (0 bytes where one part is the quicker form): a fresh one per call, as moe_ffn's.
     if isinstance(qw, QWeightInt4G32):
-        p, s = _int4(qw)
+        p, s = _dev(w, "packed", torch.uint8), _dev(s, "scale", torch.float16)
         need = _lib.native().gemm_bytes(m, n, k, 0)
         if need:
             ws = x.new_empty(need, dtype=torch.uint8)
@@ -315,17 +333,15 @@ def qgemm(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, out: Optional[torch
             return y
         _lib.check(lib.chadq_gemm_i4g32_bf16(x.data_ptr(), p.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, _stream()), "chadq_gemm_i4g32_bf16")
         return y
-    if isinstance(qw, QWeightInt8):
-        w, s = _int8(qw)
-        need = _lib.native().gemm_bytes(m, n, k, 1)
-        if need:
-            ws = x.new_empty(need, dtype=torch.uint8)
-            _lib.check(lib.chadq_gemm_i8row_bf16_ws(x.data_ptr(), w.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, ws.data_ptr(), need, _stream()),
-                       "chadq_gemm_i8row_bf16")
-            return y
-        _lib.check(lib.chadq_gemm_i8row_bf16(x.data_ptr(), w.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, _stream()), "chadq_gemm_i8row_bf16")
+    w, s = _dev(w, "w", torch.int8), _dev(s, "scale", torch.float32)
+    need = _lib.native().gemm_bytes(m, n, k, 1)
+    if need:
+        ws = x.new_empty(need, dtype=torch.uint8)
+        _lib.check(lib.chadq_gemm_i8row_bf16_ws(x.data_ptr(), w.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, ws.data_ptr(), need, _stream()),
+                   "chadq_gemm_i8row_bf16")
         return y
-    raise TypeError("unknown weight container %r" % type(qw))
+    _lib.check(lib.chadq_gemm_i8row_bf16(x.data_ptr(), w.data_ptr(), s.data_ptr(), y.data_ptr(), m, n, k, _stream()), "chadq_gemm_i8row_bf16")
+    return y
 
 
 def qlinear(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -380,12 +396,13 @@ def moe_route(logits: torch.Tensor, top_k: int = 2, renorm: bool = True):
 
 def _repack(w, to_tiles: bool):
     lib = _lib.load()
-    p, s = _int4(w)
-    if w.N % 32 or w.K % 256:
-        raise ValueError("tile order needs N % 32 == 0 and K % 256 == 0 (N=%d, K=%d)" % (w.N, w.K))
+    p, s, n, k = _int4(w)
+    p, s = _dev(p, "packed", torch.uint8), _dev(s, "scale", torch.float16)
+    if n % 32 or k % 256:
+        raise ValueError("tile order needs N %% 32 == 0 and K %% 256 == 0 (N=%d, K=%d)" % (n, k))
     po, so = torch.empty_like(p), torch.empty_like(s)
     fn = lib.chadq_repack_i4g32_tiles if to_tiles else lib.chadq_unrepack_i4g32_tiles
-    _lib.check(fn(p.data_ptr(), s.data_ptr(), po.data_ptr(), so.data_ptr(), w.N, w.K, _stream()),
+    _lib.check(fn(p.data_ptr(), s.data_ptr(), po.data_ptr(), so.data_ptr(), n, k, _stream()),
                "chadq_repack_i4g32_tiles" if to_tiles else "chadq_unrepack_i4g32_tiles")
     return po, so
 
@@ -436,7 +453,10 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, experts, *, top_k: int = 2, r
     for i, (g, u, d) in enumerate(experts):
         if (g.N, g.K) != (f, h) or (u.N, u.K) != (f, h) or (d.N, d.K) != (h, f):
             raise ValueError("expert %d: gate/up must be [%d,%d] and down [%d,%d]" % (i, f, h, h, f))
-        ts = [*_int4(g, "gate "), *_int4(u, "up "), *_int4(d, "down ")]
+        ts = []
+        for m, name in ((g, "gate "), (u, "up "), (d, "down ")):
+            p, s, _, _ = _int4(m, name)
+            ts += [_dev(p, name + "packed", torch.uint8), _dev(s, name + "scale", torch.float16)]
         keep.append(ts)
         arr[i] = _lib.MoeExpertI4G32(*[v.data_ptr() for v in ts])
     need = lib.chadq_moe_ffn_i4g32_workspace_bytes(t, h, f, e, top_k)
