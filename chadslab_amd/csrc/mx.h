@@ -156,6 +156,8 @@ struct MxTiles {
         return place(false, [t](int) { return t; });
     }
 };
+// a / b rounded up; rows and columns up to 2^31 - 1 with a tile more do not fit 32 bits
+inline int64_t mx_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Row tiles that suffice for any offsets: full tiles of M rows, one cut per group that can have a row, one of the rest.
 inline int64_t mx_most_tiles(int M, int E, int TR) { return (int64_t)M / TR + (E < M ? E : M) + 2; }
 

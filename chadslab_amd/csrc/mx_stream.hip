@@ -224,7 +224,7 @@ template <bool X4, bool GATED, bool GROUPED, int MT, int D>
 static int launch(const MxProduct &p, int RT, int wk, hipStream_t st) {
     constexpr int W = MXS_W, NB = GATED ? 2 : 1, UB = X4 ? 128 : 512, SCALES = W * (NB + X4 * MT) * 8 * (8 * D + 8);
     const int U = (p.K + 255) / 256, round = D << wk, rounds = (U + round - 1) / round, rows = p.M < 8 * MT ? p.M : 8 * MT;
-    const int64_t nwg = (int64_t)(W >> wk) * RT, tiles = p.offsets ? mx_most_tiles(p.M, p.E, 8 * MT) : (p.M + 8 * MT - 1) / (8 * MT), cols = (p.N + nwg - 1) / nwg;
+    const int64_t nwg = (int64_t)(W >> wk) * RT, tiles = p.offsets ? mx_most_tiles(p.M, p.E, 8 * MT) : mx_ceil(p.M, 8 * MT), cols = mx_ceil(p.N, nwg);
     if (tiles > (1 << 22) || cols > 65535) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
     // all of K if it fits: two workgroups to a compute unit where there are so many
     const int most = (tiles * cols <= 256 ? 147456 : 73728) / (rows * round * UB), chunk = most < 1 ? 1 : most > rounds ? rounds : most;
@@ -273,7 +273,7 @@ int mx_stream_launch(const MxProduct &p, hipStream_t st) {
 
 // Up to 16 rows, or 8 of a group on average, stream the weights, more go through the tiles: by group, us, streamed / tiles: 40 rows, 8 matrices of 14336 x 4096
 // 48.9 / 56.6, 64 rows 62.8 / 60.3, 96 rows 92 / 58 (a group of more than a tile's rows reads its weights twice).
-static bool streams(const MxProduct &p) { return p.offsets ? (p.M + p.E - 1) / p.E <= 8 : p.M <= 16; }
+static bool streams(const MxProduct &p) { return p.offsets ? p.M <= (int64_t)8 * p.E : p.M <= 16; }
 
 int mx_product_part_k(const MxProduct &p, int most_parts) { return streams(p) || !mx_tile_ok(p) ? 0 : mx_tile_pick(p, most_parts).part_k; }
 

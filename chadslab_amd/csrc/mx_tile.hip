@@ -406,7 +406,7 @@ static int launch(const MxProduct &p, hipStream_t st) {
     typedef Cfg<X4, WN, WM, WK, NB, MB, BPS, ST> C;
     constexpr int TO = GATED ? C::TN / 2 : C::TN, LDS = C::lds(TO);
     static_assert(LDS <= 163840, "LDS of a compute unit");
-    const int64_t tm = p.offsets ? mx_most_tiles(p.M, p.E, C::TM) : (p.M + C::TM - 1) / C::TM, tiles = tm * ((p.N + TO - 1) / TO);
+    const int64_t tm = p.offsets ? mx_most_tiles(p.M, p.E, C::TM) : mx_ceil(p.M, C::TM), tiles = tm * mx_ceil(p.N, TO);
     if (tiles > (1 << 22)) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
     static std::atomic<bool> set[64];  // more LDS than the default limit: once per device
     int dev = 0;
@@ -492,8 +492,8 @@ static MxTilePick pick(int M, int N, int K, int E, bool x_mx, bool gated, int mo
         if (t.round > 1e8f || (gated ? t.tn < 128 || i == T128x96 || i == T128x128 : i == T128x32)) continue;
         // rows by group: between the tiles of groups of one size and those of exponentially distributed sizes
         const float mean = (float)M / E > 1.f ? (float)M / E : 1.f, hit = E * (1.f - expf(-(float)M / E)), even = mean / t.tm + 0.3f;
-        const float tm = E > 1 ? hit * 0.5f * ((even > 1.f ? even : 1.f) + 1.f / (1.f - expf(-t.tm / mean))) : (float)((M + t.tm - 1) / t.tm);
-        const float tiles = tm * ((N + tn - 1) / tn);
+        const float tm = E > 1 ? hit * 0.5f * ((even > 1.f ? even : 1.f) + 1.f / (1.f - expf(-t.tm / mean))) : (float)mx_ceil(M, t.tm);
+        const float tiles = tm * mx_ceil(N, tn);
         for (int parts = 1; parts <= most_parts; ++parts) {
             const int part_k = parts > 1 ? ((K + parts - 1) / parts + 511) / 512 * 512 : K;
             if (parts > 1 && (part_k < 1024 || (int64_t)part_k * (parts - 1) >= K)) continue;

@@ -32,3 +32,18 @@ def test_exchanged_arrays_are_looked_at_again(ops):
         qw.scale = dev(s2)
         check(ops.qlinear(x, qw), x64, dev(O.dequant_mxfp4(c2, s2)))
         check(ops.qgemm(x, qw), x64, dev(O.dequant_mxfp4(c2, s2)))
+
+
+def test_too_many_tiles_are_refused(ops):
+    """Rows or columns up to the last 32-bit number, the other few: the status of a size that is refused, and no launch."""
+    from chadslab_amd import _lib
+
+    lib = _lib.load()
+    a = torch.zeros(4096, dtype=torch.uint8, device=DEV).data_ptr()
+    for most in (2 ** 31 - 1, 2 ** 31 - 32, 2 ** 31 - 300):
+        for m, n in ((most, 1), (17, most), (40, most), (most, 17)):
+            for k in (32, 4096):
+                for xs in (None, a):
+                    assert lib.chadq_product_mxfp4(a, xs, a, a, a, 1, m, n, k, None, 0, None) == -2 and b"too many tiles" in lib.chadq_last_error()
+                    assert lib.chadq_product_mxfp4_grouped(a, xs, a, a, a, a, m, 1, n, k, 1, None) == -2 and b"too many tiles" in lib.chadq_last_error()
+    assert lib.chadq_product_mxfp4_grouped(a, None, a, a, a, a, 2 ** 31 - 1, 2 ** 31 - 2, 1, 32, 1, None) == -2  # (rows and groups)

@@ -186,3 +186,15 @@ def test_int4_experts_are_not_looked_at_one_by_one_for_mxfp4(monkeypatch):
     for bad in ([e], [e, e], (None, e, e), [e, e, e, e], (e, None, e)):
         with pytest.raises(TypeError, match="triple"):
             ops.moe_ffn(None, None, bad)
+
+
+def test_tiles_of_the_largest_sizes_are_counted():
+    """Rows or columns within a tile of 2^31: their tiles are too many, not fewer than none, so K in parts (gigabytes of workspace) is not what the rule wants."""
+    from chadslab_amd import _lib
+
+    f = _lib.load().chadq_product_mxfp4_workspace_bytes
+    for most in (2 ** 31 - 1, 2 ** 31 - 32, 2 ** 31 - 300):
+        for small in (1, 17, 100):
+            for k in (1024, 4096, 14336):
+                assert f(most, small, k, 0) == f(most, small, k, 1) == 0
+                assert f(small, most, k, 0) == f(small, most, k, 1) == 0
