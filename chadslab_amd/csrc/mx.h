@@ -170,6 +170,7 @@ __device__ __forceinline__ void mx_clear(void *y, bool y_bf16, int N, const MxTi
     }
 }
 
+bool mx_streams(const MxProduct &p);
 int mx_stream_launch(const MxProduct &p, hipStream_t st);
 bool mx_tile_ok(const MxProduct &p);
 struct MxTilePick {

@@ -22,6 +22,7 @@
 namespace chadq {
 
 constexpr int MXS_W = 8;  // waves
+constexpr int kStreamCols = 65535;  // workgroups along n: a grid's second dimension
 
 // What the first requests need comes first in the arguments, where it arrives in registers with the wave.
 // RT: weight rows of a wave in use (<= 8); wk: log2 WK; chunk: rounds of a chunk of activations; inv: 65536 / KiB of its rows, rounded up
@@ -220,12 +221,26 @@ __global__ __launch_bounds__(64 * MXS_W) __attribute__((amdgpu_waves_per_eu(4)))
     }
 }
 
+// Weight rows of a wave, and how many waves split K (log2): as many rows to a workgroup as give every compute unit the same number of them; waves that
+// they leave split K
+struct StreamShape {
+    int RT, wk;
+    int64_t cols(int N) const { return mx_ceil(N, (MXS_W >> wk) * RT); }  // workgroups along n
+};
+static StreamShape stream_shape(const MxProduct &p) {
+    if (p.offsets) return {8, 0};
+    const int64_t turns = mx_ceil(p.N, 256 * 64);
+    const int rows = (int)mx_ceil(p.N, 256 * turns), wk = rows > 32 ? 0 : rows > 16 ? 1 : rows > 8 ? 2 : 3, s = MXS_W >> wk;
+    return {(rows + s - 1) / s, wk};
+}
+
 template <bool X4, bool GATED, bool GROUPED, int MT, int D>
-static int launch(const MxProduct &p, int RT, int wk, hipStream_t st) {
+static int launch(const MxProduct &p, StreamShape shape, hipStream_t st) {
     constexpr int W = MXS_W, NB = GATED ? 2 : 1, UB = X4 ? 128 : 512, SCALES = W * (NB + X4 * MT) * 8 * (8 * D + 8);
+    const int RT = shape.RT, wk = shape.wk;
     const int U = (p.K + 255) / 256, round = D << wk, rounds = (U + round - 1) / round, rows = p.M < 8 * MT ? p.M : 8 * MT;
-    const int64_t nwg = (int64_t)(W >> wk) * RT, tiles = p.offsets ? mx_most_tiles(p.M, p.E, 8 * MT) : mx_ceil(p.M, 8 * MT), cols = mx_ceil(p.N, nwg);
-    if (tiles > (1 << 22) || cols > 65535) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
+    const int64_t tiles = p.offsets ? mx_most_tiles(p.M, p.E, 8 * MT) : mx_ceil(p.M, 8 * MT), cols = shape.cols(p.N);
+    if (tiles > (1 << 22) || cols > kStreamCols) return fail(CHADQ_ERR_SHAPE, "mxfp4 product: M=%d N=%d are too many tiles", p.M, p.N);
     // all of K if it fits: two workgroups to a compute unit where there are so many
     const int most = (tiles * cols <= 256 ? 147456 : 73728) / (rows * round * UB), chunk = most < 1 ? 1 : most > rounds ? rounds : most;
     const size_t per = ((size_t)chunk * round * UB + 1023) / 1024, xb = rows * (per * 1024 + 16), part = wk ? W * MT * NB * 256 : 0;
@@ -247,20 +262,18 @@ static int launch(const MxProduct &p, int RT, int wk, hipStream_t st) {
 template <bool X4, bool GATED, bool GROUPED, int MT>
 static int launch_rows(const MxProduct &p, hipStream_t st) {
     const int U = (p.K + 255) / 256;
+    const StreamShape shape = stream_shape(p);
     if constexpr (GROUPED) {
-        return U > 2 ? launch<X4, GATED, true, MT, 4>(p, 8, 0, st) : launch<X4, GATED, true, MT, 1>(p, 8, 0, st);
+        return U > 2 ? launch<X4, GATED, true, MT, 4>(p, shape, st) : launch<X4, GATED, true, MT, 1>(p, shape, st);
     } else {
-        // As many weight rows to a workgroup as give every compute unit the same number of them; waves that they leave split K
-        const int64_t turns = ((int64_t)p.N + 256 * 64 - 1) / (256 * 64);
-        const int rows = (int)((p.N + 256 * turns - 1) / (256 * turns));
-        const int wk = rows > 32 ? 0 : rows > 16 ? 1 : rows > 8 ? 2 : 3, s = MXS_W >> wk, RT = (rows + s - 1) / s, own = (U + (1 << wk) - 1) >> wk;
+        const int wk = shape.wk, own = (U + (1 << wk) - 1) >> wk;
         const int fit = 131072 / ((p.M < 16 ? p.M : 16) * (X4 ? 128 : 512) << wk), most = own < fit ? own : fit;
         // (MXFP4 x: eight registers for an operand that uses four, so eight units ahead would not fit)
         if constexpr (!X4)
-            if (most > 4) return launch<X4, GATED, GROUPED, MT, 8>(p, RT, wk, st);
-        return most > 2   ? launch<X4, GATED, GROUPED, MT, 4>(p, RT, wk, st)
-               : most > 1 ? launch<X4, GATED, GROUPED, MT, 2>(p, RT, wk, st)
-                          : launch<X4, GATED, GROUPED, MT, 1>(p, RT, wk, st);
+            if (most > 4) return launch<X4, GATED, GROUPED, MT, 8>(p, shape, st);
+        return most > 2   ? launch<X4, GATED, GROUPED, MT, 4>(p, shape, st)
+               : most > 1 ? launch<X4, GATED, GROUPED, MT, 2>(p, shape, st)
+                          : launch<X4, GATED, GROUPED, MT, 1>(p, shape, st);
     }
 }
 
@@ -273,9 +286,10 @@ int mx_stream_launch(const MxProduct &p, hipStream_t st) {
 
 // Up to 16 rows, or 8 of a group on average, stream the weights, more go through the tiles: by group, us, streamed / tiles: 40 rows, 8 matrices of 14336 x 4096
 // 48.9 / 56.6, 64 rows 62.8 / 60.3, 96 rows 92 / 58 (a group of more than a tile's rows reads its weights twice).
-static bool streams(const MxProduct &p) { return p.offsets ? p.M <= (int64_t)8 * p.E : p.M <= 16; }
+// Columns beyond what the streaming grid holds (4194240) go through the tiles whatever the rows.
+bool mx_streams(const MxProduct &p) { return (p.offsets ? p.M <= (int64_t)8 * p.E : p.M <= 16) && stream_shape(p).cols(p.N) <= kStreamCols; }
 
-int mx_product_part_k(const MxProduct &p, int most_parts) { return streams(p) || !mx_tile_ok(p) ? 0 : mx_tile_pick(p, most_parts).part_k; }
+int mx_product_part_k(const MxProduct &p, int most_parts) { return mx_streams(p) || !mx_tile_ok(p) ? 0 : mx_tile_pick(p, most_parts).part_k; }
 
 size_t mx_product_workspace_bytes(int M, int N, int K, bool x_mxfp4) {
     MxProduct p = {};
@@ -290,7 +304,7 @@ size_t mx_product_workspace_bytes(int M, int N, int K, bool x_mxfp4) {
 }
 
 int mx_product_launch(const MxProduct &p, void *workspace, size_t workspace_bytes, hipStream_t st) {
-    if (streams(p) || !mx_tile_ok(p)) return mx_stream_launch(p, st);
+    if (mx_streams(p) || !mx_tile_ok(p)) return mx_stream_launch(p, st);
     if (p.part_k) return mx_tile_launch(p, mx_tile_pick(p, kMxGroupParts).tile, st);  // (the caller, who asked for at most so many, joins the parts)
     if (!p.offsets && workspace) {
         MxProduct q = p;

@@ -208,3 +208,31 @@ def test_host_module_answers_as_the_library_does():
     assert native.gemm_bytes(1 << 40, 512, 16384, 0) == 0  # (the product refuses it)
     with pytest.raises(TypeError):
         native.gemv_bytes(1, 512, 16384)
+
+
+class MxProduct(ctypes.Structure):
+    """The product as the MXFP4 rules see it (csrc/mx.h); pointers are looked at for being there only."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "xs", "w", "ws", "y", "offsets")] + [(n, ctypes.c_int) for n in "MNKE"] +
+                [("y_bf16", ctypes.c_bool), ("clear_rest", ctypes.c_bool), ("rows", ctypes.c_void_p), ("x_rows", ctypes.c_int), ("w2", ctypes.c_void_p),
+                 ("w2s", ctypes.c_void_p), ("part_k", ctypes.c_int)])
+
+
+def _mx(m, n, k, groups=0, x4=False, gated=False):
+    return MxProduct(M=m, N=n, K=k, E=groups or 1, offsets=1 if groups else None, xs=1 if x4 else None, w2=1 if gated else None, rows=1 if gated else None, x_rows=m)
+
+
+def _mx_streams(p):
+    fn = _rule("_ZN5chadq10mx_streamsERKNS_9MxProductE", ctypes.c_bool)
+    fn.argtypes = [ctypes.c_void_p]
+    return fn(ctypes.byref(p))
+
+
+def test_mxfp4_products_stream_only_what_the_grid_holds():
+    """Few rows stream their weights, as long as the columns are no more than a grid's second dimension holds."""
+    for n in (1, 4096, 14336, 32000, 10 ** 6, 4194240):
+        for m in (1, 16):
+            assert _mx_streams(_mx(m, n, 64))
+        assert not _mx_streams(_mx(17, n, 64))
+        assert _mx_streams(_mx(64, n, 64, groups=8)) and _mx_streams(_mx(64, n, 64, groups=8, gated=True)) and not _mx_streams(_mx(65, n, 64, groups=8))
+    for n in (4194241, 5 * 10 ** 6, 2 ** 31 - 1):
+        assert not any(_mx_streams(_mx(m, n, 32, groups=g)) for m in (1, 16) for g in (0, 4))

@@ -47,3 +47,46 @@ def test_too_many_tiles_are_refused(ops):
                     assert lib.chadq_product_mxfp4(a, xs, a, a, a, 1, m, n, k, None, 0, None) == -2 and b"too many tiles" in lib.chadq_last_error()
                     assert lib.chadq_product_mxfp4_grouped(a, xs, a, a, a, a, m, 1, n, k, 1, None) == -2 and b"too many tiles" in lib.chadq_last_error()
     assert lib.chadq_product_mxfp4_grouped(a, None, a, a, a, a, 2 ** 31 - 1, 2 ** 31 - 2, 1, 32, 1, None) == -2  # (rows and groups)
+
+
+@pytest.mark.parametrize("x4", [False, True], ids=["bf16", "mxfp4"])
+@pytest.mark.parametrize("n", [4194240, 4194241, 5000000])
+def test_few_rows_of_millions_of_columns(ops, n, x4):
+    """On both sides of what the streaming grid holds; one matrix and by group."""
+    from chadslab_amd import QExpertsMXFP4, QWeightMXFP4
+
+    k = 32
+    g = torch.Generator(device=DEV).manual_seed(n)
+    c = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device=DEV, generator=g)
+    s = torch.randint(118, 124, (n, 1), dtype=torch.uint8, device=DEV, generator=g)
+    w64 = ops.dequantize(QWeightMXFP4(c, s)).double()
+    for m in (1, 16):
+        x, x64 = activations(np.random.Generator(np.random.PCG64(m)), m, k, x4)
+        check(ops.qlinear(x, QWeightMXFP4(c, s)), x64, w64)
+        check(ops.qlinear(x, QWeightMXFP4(c, s), out_dtype=torch.bfloat16), x64, w64)
+    off = torch.tensor([1, 14], dtype=torch.int32, device=DEV)
+    y = ops.qgemm_grouped(x, QExpertsMXFP4(c[None], s[None]), off)
+    check(y[1:14], x64[1:14], w64)
+    assert not y[0].any() and not y[14:].any()
+
+
+def test_moe_of_millions_of_hidden_columns(ops):
+    """Gate and up beyond the streaming grid's columns; their product is then the down product's K, beyond what the tiles' offsets hold."""
+    from chadslab_amd import QExpertsMXFP4
+
+    h, f, t = 32, 4194240 + 96, 2
+    g = torch.Generator(device=DEV).manual_seed(1)
+
+    def experts(n, k):
+        return QExpertsMXFP4(torch.randint(0, 256, (1, n, k // 2), dtype=torch.uint8, device=DEV, generator=g),
+                             torch.randint(118, 124, (1, n, k // 32), dtype=torch.uint8, device=DEV, generator=g))
+
+    gate, up, down = experts(f, h), experts(f, h), experts(h, f)
+    x = torch.randn(t, h, device=DEV, generator=g).to(torch.bfloat16)
+    y = ops.moe_ffn(x, torch.zeros(t, 1, device=DEV), (gate, up, down), top_k=1)
+    a, b, d = (ops.dequantize(m)[0].double() for m in (gate, up, down))
+    u = x.double() @ a.T
+    want = (u * torch.sigmoid(u) * (x.double() @ b.T)) @ d.T
+    # h and the result are rounded to bf16 (as in test_moe); down adds 131075 instructions' worth of products in fp32, each addition off by at most 2^-24 of a
+    # sum that grows with the root of their number, independently: 2^-24 sqrt(131075 / 2) = 2^-16
+    assert O.rel_l2(y.double().cpu().numpy(), want.cpu().numpy()) <= 2 * 2.0 ** -8 + 2.0 ** -16
