@@ -236,3 +236,52 @@ def test_mxfp4_products_stream_only_what_the_grid_holds():
         assert _mx_streams(_mx(64, n, 64, groups=8)) and _mx_streams(_mx(64, n, 64, groups=8, gated=True)) and not _mx_streams(_mx(65, n, 64, groups=8))
     for n in (4194241, 5 * 10 ** 6, 2 ** 31 - 1):
         assert not any(_mx_streams(_mx(m, n, 32, groups=g)) for m in (1, 16) for g in (0, 4))
+
+
+MX_TILES = ["64x32", "64x64", "128x64", "256x64", "128x128", "256x128", "256x256", "256x96", "128x96", "128x32"]
+
+
+def mx_pick(p, most_parts):
+    """Tile and parts of K of an MXFP4 product of many rows."""
+    class Pick(ctypes.Structure):
+        _fields_ = [("tile", ctypes.c_int), ("part_k", ctypes.c_int)]
+
+    fn = _rule("_ZN5chadq12mx_tile_pickERKNS_9MxProductEi", Pick)
+    fn.argtypes = [ctypes.c_void_p, ctypes.c_int]
+    got = fn(ctypes.byref(p), most_parts)
+    return MX_TILES[got.tile], -(-p.K // got.part_k) if got.part_k else 1
+
+
+def _sizes_of(test):
+    return next(m for m in test.pytestmark if m.name == "parametrize").args[1]
+
+
+def test_sizes_of_the_mxfp4_tile_tests_take_every_tile():
+    """The sizes that the GPU tests run for each tile's sake do take it (the rule's times are fitted: with others they may not)."""
+    from tests import test_gpu_mxfp4 as G
+
+    def seen(x4, products):
+        return {mx_pick(p, most)[0] for q, p, most in products if q == x4}
+
+    dense = [(x4, _mx(m, n, k, x4=x4), 8) for x4, m, n, k in _sizes_of(G.test_every_tile)]
+    groups = [(x4, _mx(m, n, k, e, x4=x4), 1) for x4, m, n, k, e in _sizes_of(G.test_every_tile_by_group)]
+    gated = [(False, _mx(t, f, h, e, gated=True), 1) for t, h, f, e in _sizes_of(G.test_every_tile_of_gate_and_up)]
+    for x4, p, _ in dense + groups + gated:
+        assert not _mx_streams(p), (p.M, p.N, p.K, p.E)
+    for products in (dense, groups):
+        assert seen(False, products) == set(MX_TILES) - {"256x256", "128x32"} and seen(True, products) == set(MX_TILES) - {"128x32"}
+    assert seen(False, gated) == {"128x32", "128x64", "256x64", "256x96", "256x128"}
+
+
+def test_sizes_of_the_mxfp4_tests_in_parts_of_k_take_them():
+    from tests import test_gpu_mxfp4_edges as G
+
+    for x4, m, n, k, want in _sizes_of(G.test_every_tile_in_parts_of_k):
+        p = _mx(m, n, k, x4=x4)
+        assert not _mx_streams(p) and mx_pick(p, 8) == want and k % 512
+    assert {w[0] for x4, *_, w in _sizes_of(G.test_every_tile_in_parts_of_k) if not x4} == set(MX_TILES) - {"256x256", "128x32"}
+    assert {w[0] for x4, *_, w in _sizes_of(G.test_every_tile_in_parts_of_k) if x4} == set(MX_TILES) - {"128x32"}
+    for tokens, h, f, experts, top_k, want in _sizes_of(G.test_moe_down_in_parts_of_k):
+        p = _mx(tokens * top_k, h, f, experts)
+        assert not _mx_streams(p) and mx_pick(p, 4) == want and f % 512
+    assert {w[0] for *_, w in _sizes_of(G.test_moe_down_in_parts_of_k)} == set(MX_TILES) - {"256x256", "128x32"}

@@ -90,3 +90,81 @@ def test_moe_of_millions_of_hidden_columns(ops):
     # h and the result are rounded to bf16 (as in test_moe); down adds 131075 instructions' worth of products in fp32, each addition off by at most 2^-24 of a
     # sum that grows with the root of their number, independently: 2^-24 sqrt(131075 / 2) = 2^-16
     assert O.rel_l2(y.double().cpu().numpy(), want.cpu().numpy()) <= 2 * 2.0 ** -8 + 2.0 ** -16
+
+
+# ---- K in parts, the last one shorter; (the rule, asked on the host, is held to the tile and the number of parts given here) ----
+@pytest.mark.parametrize("x4,m,n,k,want", [(False, 93, 16, 7392, ("64x32", 8)), (False, 1392, 65, 6592, ("64x64", 5)), (False, 1409, 77, 7904, ("128x64", 8)),
+                                           (False, 1869, 130, 24384, ("256x64", 8)), (False, 1488, 338, 10592, ("128x128", 7)), (False, 2044, 641, 12672, ("256x128", 5)),
+                                           (False, 1901, 663, 11872, ("256x96", 4)), (False, 1812, 276, 12256, ("128x96", 4)), (True, 49, 16, 3712, ("64x32", 4)),
+                                           (True, 1680, 65, 5792, ("64x64", 3)), (True, 1393, 202, 22112, ("128x64", 5)), (True, 1063, 1225, 16640, ("256x64", 3)),
+                                           (True, 1871, 153, 22592, ("128x128", 8)), (True, 2021, 684, 25344, ("256x128", 5)), (True, 2039, 2091, 16800, ("256x256", 3)),
+                                           (True, 670, 2161, 24416, ("256x96", 4)), (True, 1362, 195, 18880, ("128x96", 8))])
+def test_every_tile_in_parts_of_k(ops, x4, m, n, k, want):
+    """Through Python, and through the C entry point into fp32 and bf16 with a workspace full of NaN."""
+    from chadslab_amd import QWeightMXFP4, _lib
+
+    lib = _lib.load()
+    need = lib.chadq_product_mxfp4_workspace_bytes(m, n, k, int(x4))
+    assert need == want[1] * m * n * 4
+    r = np.random.Generator(np.random.PCG64(m + n))
+    c, s = weights(r, n, k)
+    qw, w64 = QWeightMXFP4(dev(c), dev(s)), dev(O.dequant_mxfp4(c, s))
+    x, x64 = activations(r, m, k, x4)
+    y = ops.qlinear(x, qw)
+    check(y, x64, w64)
+    xt, xs = (x.packed, x.scale.data_ptr()) if x4 else (x, None)
+    for dtype in (torch.float32, torch.bfloat16):
+        ws = torch.full((need,), 255, dtype=torch.uint8, device=DEV)
+        out = torch.full((m, n), float("nan"), dtype=dtype, device=DEV)
+        assert lib.chadq_product_mxfp4(xt.data_ptr(), xs, qw.packed.data_ptr(), qw.scale.data_ptr(), out.data_ptr(), int(dtype == torch.bfloat16), m, n, k, ws.data_ptr(),
+                                       need, torch.cuda.current_stream().cuda_stream) == 0
+        check(out, x64, w64)
+    assert torch.equal(out, y)
+
+
+def moe_in_64_bits(x64, logits, mats, top_k, renorm):
+    idx, w = O.moe_route(logits, top_k, renorm)
+    idx, w = dev(idx.astype(np.int64)), dev(w.astype(np.float64))
+    y = torch.zeros_like(x64)
+    for e in range(len(mats[0][0])):
+        gate, up, down = (dev(O.dequant_mxfp4(c[e], s[e])) for c, s in mats)
+        g, u = x64 @ gate.T, x64 @ up.T
+        y += (w * (idx == e)).sum(1, keepdim=True) * ((g * torch.sigmoid(g) * u) @ down.T)
+    return y
+
+
+@pytest.mark.parametrize("tokens,h,f,experts,top_k,want", [(57, 320, 5568, 4, 2, ("64x32", 4)), (60, 384, 11808, 8, 2, ("64x32", 4)), (824, 32, 6112, 4, 4, ("64x32", 2)),
+                                                           (973, 32, 7232, 4, 4, ("64x64", 4)), (541, 224, 12096, 4, 4, ("128x64", 3)),
+                                                           (1021, 608, 10656, 2, 2, ("128x128", 3)), (1015, 96, 16000, 4, 4, ("128x96", 4)),
+                                                           (789, 416, 13760, 4, 4, ("256x128", 4)), (855, 1504, 6080, 1, 1, ("256x64", 3)), (664, 448, 11904, 4, 4, ("256x96", 4))])
+def test_moe_down_in_parts_of_k(ops, tokens, h, f, experts, top_k, want):
+    """The experts' down product summed in parts that the weighted sum joins: against 64 bits (bound: as in test_moe), the same bits twice and from a graph."""
+    from chadslab_amd import QExpertsMXFP4, _lib
+
+    pairs = tokens * top_k
+    need = _lib.load().chadq_moe_ffn_mxfp4_workspace_bytes(tokens, h, f, experts, top_k)
+    assert 0 <= need - pairs * (2 * f + 4 * want[1] * h) <= 16 * pairs + 4096  # h as bf16, every part as fp32, and the router's four words to a pair
+    r = np.random.Generator(np.random.PCG64(tokens + f))
+    mats = [weights(r, experts, *shape, spread=0.5) for shape in ((f, h), (f, h), (h, f))]
+    x, x64 = activations(r, tokens, h, False)
+    logits = r.standard_normal((tokens, experts)).astype(np.float32)
+    if experts > top_k:
+        logits[:, 1] = -50.0  # nobody's choice
+    triple, z = tuple(QExpertsMXFP4(dev(c), dev(s)) for c, s in mats), dev(logits)
+    y = ops.moe_ffn(x, z, triple, top_k=top_k)
+    assert torch.isfinite(y).all()
+    assert O.rel_l2(y.double().cpu().numpy(), moe_in_64_bits(x64, logits, mats, top_k, True).cpu().numpy()) <= 2 * 2.0 ** -8 + 2.0 ** -18
+    assert torch.equal(ops.moe_ffn(x, z, triple, top_k=top_k), y)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        captured = ops.moe_ffn(x, z, triple, top_k=top_k)
+    for turn in range(3):
+        x.copy_(activations(r, tokens, h, False)[0])
+        z.copy_(torch.randn_like(z))
+        eager = ops.moe_ffn(x, z, triple, top_k=top_k)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, eager)
