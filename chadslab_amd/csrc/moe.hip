@@ -12,6 +12,10 @@
 // on a gathered copy of the activations with a separate SiLU kernel.  The small kernels here are the router, the gather,
 // the SiLU gate and the weighted combine.
 //
+// Between the products h = silu(gate) up is bf16 in every order of weights: the matrix cores multiply exact bf16 weights by bf16 activations, and h in 32 bits would be
+// two such operands, twice the down product's instructions and activation bytes.  Its rounding, at most 2^-8 of a value, comes out of the down product's sums at the size
+// of the one that the bf16 result has anyway: MXFP4 results are 2.3e-3 from those in 64 bits, relative, instead of 1.65e-3.
+//
 // MXFP4 experts take the router, the products by group of mx_stream.hip and mx_tile.hip, and the combine (at the end of the file): 4 tokens through 8 experts of
 // 14336 x 4096 92 us (what they read, at a large copy's rate, 99), 256 tokens 306 us (gate and up 184, down 119).
 #include "chadq_common.h"

@@ -2,8 +2,9 @@
 // code = the nearest e2m1 to x / 2^(e - 127), ties to the even one, what lies beyond 6 to 6; a block that holds a NaN or an
 // infinity gets e = 255 and codes of 0.  The division by a power of two is exact, so there is nothing to round but the code.
 //
-// Both are bound by the bytes they move: quantising 14336 x 4096 fp32 47.2 us = 5.6 TB/s, 4096 x 4096 bf16 8.5 us, and dequantising 14336 x 4096 45.9 us =
-// 5.8 TB/s (a copy of 1 GiB moves 5.15 TB/s, read and written).  16 x 4096: 3.2 us, a launch and one trip to memory.
+// Both are bound by the bytes they move.  Over inputs and results that do not fit the 256 MB cache: quantising 14336 x 4096 fp32 46.6 us = 5.7 TB/s, seven eighths of
+// it read, 4096 x 4096 bf16 9.1 us = 4.7 TB/s, and dequantising 14336 x 4096 55.9 us = 4.8 TB/s, seven eighths written (a copy of 1 GiB moves 5.2 TB/s, read and written, filling it
+// 6.8); with results that the cache holds 8.5 and 45.5 us.  16 x 4096: 3.2 us, a launch and one trip to memory.
 #include "mx.h"
 
 namespace chadq {
@@ -74,7 +75,7 @@ __global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const T *__restrict
 }
 
 // w[i] = value(code i) * scale of its block as fp32, exact (beyond fp32's range: infinity); 4 codes to a lane, so that a wave stores 1 KiB in a row, four
-// times in flight.  The stores go past the caches: 14336 x 4096 65 -> 45 us with both.
+// times in flight.  The stores go past the caches: 14336 x 4096, into a result that the last cache holds, 65 -> 45 us with both.
 __global__ __launch_bounds__(256) void dequant_mxfp4_kernel(const uint16_t *__restrict__ codes, const uint8_t *__restrict__ scale,
                                                             float *__restrict__ w, int64_t n4) {
     const int64_t stride = (int64_t)gridDim.x * 256;

@@ -284,8 +284,10 @@ int mx_stream_launch(const MxProduct &p, hipStream_t st) {
     return p.xs ? launch_rows<true, false, false, 2>(p, st) : launch_rows<false, false, false, 2>(p, st);
 }
 
-// Up to 16 rows, or 8 of a group on average, stream the weights, more go through the tiles: by group, us, streamed / tiles: 40 rows, 8 matrices of 14336 x 4096
-// 48.9 / 56.6, 64 rows 62.8 / 60.3, 96 rows 92 / 58 (a group of more than a tile's rows reads its weights twice).
+// Up to 16 rows, or 8 of a group on average, stream the weights, more go through the tiles.  By group, 8 matrices of 14336 x 4096, us, streamed / tiles, bf16 x: 40
+// rows evenly 45 / 59, 64 evenly 48 / 59, 72 evenly 81 / 60 (a group of more than eight rows reads its weights again).  Of the groups the rule knows the mean alone:
+// drawn at random 40 rows take 53 / 59, 56 rows 63 / 59, 64 rows 64 / 57, 80 rows 79 / 60; all in one group 40 rows 34 / 26, 64 rows 49 / 26.  MXFP4 x, 16 matrices of
+// 4096 x 2048, 64 of 1024 x 2048 and 4 of 4096 x 4096 cross between 6 and 8 rows a group too.
 // Columns beyond what the streaming grid holds (4194240) go through the tiles whatever the rows.
 bool mx_streams(const MxProduct &p) { return (p.offsets ? p.M <= (int64_t)8 * p.E : p.M <= 16) && stream_shape(p).cols(p.N) <= kStreamCols; }
 

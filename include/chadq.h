@@ -429,7 +429,7 @@ int chadq_dequant_mxfp4(const uint8_t *codes, const uint8_t *scale, float *w, in
  * else x holds the codes [M,K/2] of MXFP4 activations.  M, N >= 0 (y of at most 2^22 tiles, the smallest of 64 n x 32 m); K a positive multiple of
  * 32 up to 2^26; x and codes 16-byte aligned, scales anywhere.  A NaN block of w makes column n NaN, one of x row m.  With bf16 x a weight beyond bf16's range (scale bytes
  * 253 and 254) counts as infinite; infinities and NaN in x act as IEEE has them.  workspace: chadq_product_mxfp4_workspace_bytes bytes (16-byte aligned; 0: none needed), for the
- * sums of parts of K where that is the quicker form; without it (NULL or fewer bytes) the product is one part.
+ * sums of parts of K where that is the quicker form (a size that is refused has none); without it (NULL or fewer bytes) the product is one part.
  */
 size_t chadq_product_mxfp4_workspace_bytes(int M, int N, int K, int x_mxfp4);
 int chadq_product_mxfp4(const void *x, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, void *y, int y_bf16, int M, int N, int K,
@@ -439,7 +439,8 @@ int chadq_product_mxfp4(const void *x, const uint8_t *x_scale, const uint8_t *w,
  * The same for rows sorted by group, each group times its own matrix: w [E,N,K/2], w_scale [E,N,K/32], offsets int32 [E+1] on the device;
  * rows offsets[e] .. offsets[e+1] - 1 of x and y belong to group e.  Groups may be empty.  Rows of no group (in front of offsets[0], behind
  * offsets[E]) become 0 where clear_rest is set and are left as they are otherwise.  Offsets are taken as clamped into [0, M], one that descends as the
- * largest before it.  y bf16 [M,N].  E >= 1.
+ * largest before it.  y bf16 [M,N].  E >= 1.  Row tiles are cut by the groups: up to M / 8 + min(E, M) + 2 of them where M <= 8 E, else M / 32 + min(E, M) + 2 for every 64 columns;
+ * 2^22 at most.
  */
 int chadq_product_mxfp4_grouped(const void *x, const uint8_t *x_scale, const uint8_t *w, const uint8_t *w_scale, const int32_t *offsets,
                                 uint16_t *y_bf16, int M, int E, int N, int K, int clear_rest, void *stream);
