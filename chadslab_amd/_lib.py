@@ -79,6 +79,14 @@ SIGNATURES = {
     "chadq_product_mxfp4_grouped": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "chadq_moe_ffn_mxfp4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "chadq_moe_ffn_mxfp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "chadq_quantize_fp8": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]),
+    "chadq_dequant_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]),
+    "chadq_product_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "chadq_product_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "chadq_product_fp8_grouped": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "chadq_moe_route_experts": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "chadq_moe_ffn_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "chadq_moe_ffn_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "chadq_sample_topk_f32": (c_int, [c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
 }
 
@@ -91,6 +99,16 @@ class MoeExpertI4G32(ctypes.Structure):
 class MoeMXFP4(ctypes.Structure):
     """Mirror of chadq_moe_mxfp4: six device pointers."""
     _fields_ = [(n, c_void_p) for n in ("gate", "gate_scale", "up", "up_scale", "down", "down_scale")]
+
+
+class MoeFP8(ctypes.Structure):
+    """Mirror of chadq_moe_fp8: six device pointers."""
+    _fields_ = [(n, c_void_p) for n in ("gate", "up", "down", "gate_scale", "up_scale", "down_scale")]
+
+
+class Routing(ctypes.Structure):
+    """Mirror of chadq_routing."""
+    _fields_ = [("bias", c_void_p), *((n, c_int) for n in ("sigmoid", "renorm", "groups", "top_groups", "group_sum", "top_k")), ("scale", c_float)]
 
 
 class PromptLayerI4G32(ctypes.Structure):
@@ -138,6 +156,8 @@ _NATIVE_ENTRIES = ("chadq_gemv_i4g32", "chadq_gemv_i4g32_bf16", "chadq_gemm_i4g3
                    "chadq_moe_ffn_i4g32_workspace_bytes", "chadq_moe_ffn_i4g32", "chadq_moe_ffn_i4g32_tiled")
 _NATIVE_MX_ENTRIES = ("chadq_quantize_mxfp4", "chadq_dequant_mxfp4", "chadq_product_mxfp4_workspace_bytes", "chadq_product_mxfp4", "chadq_product_mxfp4_grouped",
                       "chadq_moe_ffn_mxfp4_workspace_bytes", "chadq_moe_ffn_mxfp4")
+_NATIVE_FP8_ENTRIES = ("chadq_quantize_fp8", "chadq_dequant_fp8", "chadq_product_fp8_workspace_bytes", "chadq_product_fp8", "chadq_product_fp8_grouped",
+                       "chadq_moe_route_experts", "chadq_moe_ffn_fp8_workspace_bytes", "chadq_moe_ffn_fp8")
 
 
 HOST_PATH = Path(__file__).resolve().parent / "_host_call.so"
@@ -180,6 +200,22 @@ class _NoHostModule:
         return None
 
     @staticmethod
+    def bind_fp8(addresses, containers):
+        pass
+
+    @staticmethod
+    def quantize_fp8(x, rows):
+        return None
+
+    @staticmethod
+    def route(logits, *routing):
+        return None
+
+    @staticmethod
+    def moe_ffn_fp8(x, logits, experts, *routing):
+        return None
+
+    @staticmethod
     def gemv_bytes(m, n, k, int8):
         return load().chadq_gemv_workspace_bytes(m, n, k, int8)
 
@@ -210,13 +246,14 @@ def native():
             warnings.warn("calls take some 3 us longer without the host module (`python -m chadslab_amd.build` builds it): %s" % e,
                           RuntimeWarning, stacklevel=3)
             _native = _NoHostModule
-    from .formats import QExpertsMXFP4, QWeightInt4G32, QWeightInt4G32Tiles, QWeightInt8, QWeightMXFP4
+    from .formats import QExpertsFP8, QExpertsMXFP4, QRowsFP8, QWeightFP8, QWeightInt4G32, QWeightInt4G32Tiles, QWeightInt8, QWeightMXFP4
 
     def addresses(names):
         return tuple(ctypes.cast(getattr(lib, n), c_void_p).value for n in names)
 
     _native.bind(addresses(_NATIVE_ENTRIES), (QWeightInt4G32, QWeightInt8, QWeightInt4G32Tiles), check)
     _native.bind_mx(addresses(_NATIVE_MX_ENTRIES), (QWeightMXFP4, QExpertsMXFP4))
+    _native.bind_fp8(addresses(_NATIVE_FP8_ENTRIES), (QWeightFP8, QExpertsFP8, QRowsFP8))
     _native_lib = lib
     return _native
 

@@ -5,7 +5,9 @@
 #include <cstring>
 
 #include "chadq_common.h"
+#include "fp8.h"
 #include "mx.h"
+#include "route.h"
 
 namespace chadq {
 
@@ -110,6 +112,10 @@ int quantize_mxfp4_launch(const void *, int, uint8_t *, uint8_t *, int64_t, int,
 int dequant_mxfp4_launch(const uint8_t *, const uint8_t *, float *, int64_t, int, hipStream_t);
 size_t moe_mxfp4_workspace_bytes(int, int, int, int, int);
 int moe_ffn_mxfp4_launch(const uint16_t *, const float *, const chadq_moe_mxfp4 *, uint16_t *, int, int, int, int, int, int, void *, hipStream_t);
+int quantize_fp8_launch(const void *, int, uint8_t *, float *, int64_t, int, int, bool, hipStream_t);
+int dequant_fp8_launch(const uint8_t *, const float *, float *, int64_t, int, int, bool, hipStream_t);
+size_t moe_fp8_workspace_bytes(int, int, int, int, int, bool);
+int moe_ffn_fp8_launch(const void *, const float *, const float *, const Routing &, const chadq_moe_fp8 *, uint16_t *, int, int, int, int, void *, hipStream_t);
 int sample_topk_launch(const float *, int, int, float, const float *, float *, int32_t *, int32_t *, int32_t *, int, hipStream_t);
 
 }  // namespace chadq
@@ -700,6 +706,118 @@ int chadq_moe_ffn_mxfp4(const uint16_t *x_bf16, const float *logits, const chadq
     CHADQ_REQUIRE(aligned16(x_bf16) && aligned16(experts->gate) && aligned16(experts->up) && aligned16(experts->down) && aligned16(workspace) && aligned16(y_bf16),
                   CHADQ_ERR_ALIGN, "chadq_moe_ffn_mxfp4: x, y, codes and workspace must be 16-byte aligned");
     return moe_ffn_mxfp4_launch(x_bf16, logits, experts, y_bf16, T, H, F, E, top_k, renorm, workspace, st);
+}
+
+static int fp8_sizes(const char *name, int64_t matrices, int N, int K) {
+    CHADQ_REQUIRE(matrices >= 0 && N >= 0 && K >= 0 && K % 16 == 0, CHADQ_ERR_SHAPE, "%s: matrices=%lld N=%d K=%d (K %% 16 != 0?)", name, (long long)matrices, N, K);
+    CHADQ_REQUIRE(K == 0 || N == 0 || matrices <= INT64_MAX / 16 / K / N, CHADQ_ERR_SHAPE, "%s: matrices=%lld N=%d K=%d are too many values", name,
+                  (long long)matrices, N, K);
+    return 0;
+}
+
+int chadq_quantize_fp8(const void *x, int dtype, uint8_t *values, float *scale, int64_t matrices, int N, int K, int by_row, void *stream) {
+    ENTER();
+    CHADQ_REQUIRE(dtype == CHADQ_F32 || dtype == CHADQ_BF16 || dtype == CHADQ_F16, CHADQ_ERR_SHAPE, "chadq_quantize_fp8: unknown type %d", dtype);
+    const int rc = fp8_sizes("chadq_quantize_fp8", matrices, N, K);
+    if (rc != 0) return rc;
+    if (matrices == 0 || N == 0 || K == 0) return 0;
+    CHADQ_REQUIRE(x && values && scale, CHADQ_ERR_NULL, "chadq_quantize_fp8: null pointer");
+    CHADQ_REQUIRE(aligned16(x) && aligned16(values) && (reinterpret_cast<uintptr_t>(scale) & 3) == 0, CHADQ_ERR_ALIGN,
+                  "chadq_quantize_fp8: x and values must be 16-byte, scales 4-byte aligned");
+    return quantize_fp8_launch(x, dtype, values, scale, matrices, N, K, by_row != 0, st);
+}
+
+int chadq_dequant_fp8(const uint8_t *values, const float *scale, float *w, int64_t matrices, int N, int K, int by_row, void *stream) {
+    ENTER();
+    const int rc = fp8_sizes("chadq_dequant_fp8", matrices, N, K);
+    if (rc != 0) return rc;
+    if (matrices == 0 || N == 0 || K == 0) return 0;
+    CHADQ_REQUIRE(values && scale && w, CHADQ_ERR_NULL, "chadq_dequant_fp8: null pointer");
+    CHADQ_REQUIRE(aligned16(w) && aligned16(values) && (reinterpret_cast<uintptr_t>(scale) & 3) == 0, CHADQ_ERR_ALIGN,
+                  "chadq_dequant_fp8: w and values must be 16-byte, scales 4-byte aligned");
+    return dequant_fp8_launch(values, scale, w, matrices, N, K, by_row != 0, st);
+}
+
+size_t chadq_product_fp8_workspace_bytes(int M, int N, int K, int x_fp8) {
+    return M > 0 && N > 0 && K >= 16 && K % 16 == 0 && K <= kFp8MostK ? fp8_product_workspace_bytes(M, N, K, x_fp8 != 0) : 0;
+}
+
+static bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+int chadq_product_fp8(const void *x, const float *x_scale, const uint8_t *w, const float *w_scale, void *y, int y_bf16, int M, int N, int K, void *workspace,
+                      size_t workspace_bytes, void *stream) {
+    ENTER();
+    CHADQ_REQUIRE(M >= 0 && N >= 0 && K >= 16 && K % 16 == 0 && K <= kFp8MostK, CHADQ_ERR_SHAPE,
+                  "chadq_product_fp8: M=%d N=%d K=%d (K must be a positive multiple of 16 up to 2^26)", M, N, K);
+    if (M == 0 || N == 0) return 0;
+    CHADQ_REQUIRE(x && w && w_scale && y, CHADQ_ERR_NULL, "chadq_product_fp8: null pointer");
+    CHADQ_REQUIRE(aligned16(x) && aligned16(w) && aligned16(workspace) && aligned4(x_scale) && aligned4(w_scale), CHADQ_ERR_ALIGN,
+                  "chadq_product_fp8: x, w and workspace must be 16-byte, scales 4-byte aligned");
+    const Fp8Product p = {x, x_scale, w, w_scale, y, nullptr, M, N, K, 1, y_bf16 != 0, false};
+    return fp8_product_launch(p, workspace, workspace ? workspace_bytes : 0, st);
+}
+
+int chadq_product_fp8_grouped(const void *x, const float *x_scale, const uint8_t *w, const float *w_scale, const int32_t *offsets, uint16_t *y_bf16, int M, int E,
+                              int N, int K, int clear_rest, void *stream) {
+    ENTER();
+    CHADQ_REQUIRE(M >= 0 && E >= 1 && N >= 0 && K >= 16 && K % 16 == 0 && K <= kFp8MostK, CHADQ_ERR_SHAPE,
+                  "chadq_product_fp8_grouped: M=%d E=%d N=%d K=%d (E at least 1, K a positive multiple of 16 up to 2^26)", M, E, N, K);
+    if (M == 0 || N == 0) return 0;
+    CHADQ_REQUIRE(x && w && w_scale && offsets && y_bf16, CHADQ_ERR_NULL, "chadq_product_fp8_grouped: null pointer");
+    CHADQ_REQUIRE(aligned16(x) && aligned16(w) && aligned4(x_scale) && aligned4(w_scale) && aligned4(offsets), CHADQ_ERR_ALIGN,
+                  "chadq_product_fp8_grouped: x and w must be 16-byte, scales and offsets 4-byte aligned");
+    const Fp8Product p = {x, x_scale, w, w_scale, y_bf16, offsets, M, N, K, E, true, clear_rest != 0};
+    return fp8_product_launch(p, nullptr, 0, st);
+}
+
+static bool routing_ok(const chadq_routing &r, int E) {
+    return E >= 1 && E <= kRouteExperts && r.groups >= 1 && r.groups <= kRouteGroups && r.groups <= E && E % r.groups == 0 && r.group_sum >= 1 && r.group_sum <= 2 &&
+           r.group_sum <= E / r.groups && r.top_groups >= 1 && r.top_groups <= r.groups && r.top_k >= 1 && r.top_k <= kRouteTopK &&
+           r.top_k <= r.top_groups * (E / r.groups);
+}
+static const char kRoutingRule[] = "E <= 512; groups <= 64, a divisor of E; group_sum 1 or 2, at most E / groups; top_groups <= groups; top_k <= min(32, top_groups * E / groups)";
+static Routing routing_of(const chadq_routing &r) { return Routing{r.bias, r.sigmoid != 0, r.renorm != 0, r.groups, r.top_groups, r.group_sum, r.top_k, r.scale}; }
+
+int chadq_moe_route_experts(const float *logits, const chadq_routing *routing, int32_t *idx, float *w, int T, int E, void *stream) {
+    ENTER();
+    CHADQ_REQUIRE(routing, CHADQ_ERR_NULL, "chadq_moe_route_experts: null pointer");
+    const chadq_routing &r = *routing;
+    CHADQ_REQUIRE(T >= 0 && routing_ok(r, E), CHADQ_ERR_SHAPE, "chadq_moe_route_experts: T=%d E=%d top_k=%d groups=%d top_groups=%d group_sum=%d (%s)", T, E, r.top_k,
+                  r.groups, r.top_groups, r.group_sum, kRoutingRule);
+    if (T == 0) return 0;
+    CHADQ_REQUIRE(logits && idx && w, CHADQ_ERR_NULL, "chadq_moe_route_experts: null pointer");
+    CHADQ_REQUIRE(aligned4(logits) && aligned4(r.bias) && aligned4(idx) && aligned4(w), CHADQ_ERR_ALIGN, "chadq_moe_route_experts: arrays must be 4-byte aligned");
+    return route_experts_launch(logits, idx, w, T, E, routing_of(r), st);
+}
+
+// (the rows of the products, T * top_k, are counted in 32 bits)
+static bool moe_fp8_sizes_ok(int T, int H, int F, int E, int top_k) {
+    return T >= 1 && H >= 16 && F >= 16 && H % 16 == 0 && F % 16 == 0 && H <= kFp8MostK && F <= kFp8MostK && E >= 1 && E <= kRouteExperts && top_k >= 1 &&
+           top_k <= kRouteTopK && top_k <= E && (int64_t)T * top_k <= INT32_MAX;
+}
+
+size_t chadq_moe_ffn_fp8_workspace_bytes(int T, int H, int F, int E, int top_k, int x_fp8) {
+    return moe_fp8_sizes_ok(T, H, F, E, top_k) ? moe_fp8_workspace_bytes(T, H, F, E, top_k, x_fp8 != 0) : 0;
+}
+
+int chadq_moe_ffn_fp8(const void *x, const float *x_scale, const float *logits, const chadq_routing *routing, const chadq_moe_fp8 *experts, uint16_t *y_bf16, int T,
+                      int H, int F, int E, void *workspace, size_t workspace_bytes, void *stream) {
+    ENTER();
+    CHADQ_REQUIRE(routing, CHADQ_ERR_NULL, "chadq_moe_ffn_fp8: null pointer");
+    const chadq_routing &r = *routing;
+    CHADQ_REQUIRE(moe_fp8_sizes_ok(T, H, F, E, r.top_k) && routing_ok(r, E), CHADQ_ERR_SHAPE,
+                  "chadq_moe_ffn_fp8: T=%d H=%d F=%d E=%d top_k=%d groups=%d top_groups=%d group_sum=%d (H, F multiples of 16; %s)", T, H, F, E, r.top_k, r.groups,
+                  r.top_groups, r.group_sum, kRoutingRule);
+    CHADQ_REQUIRE(x && logits && experts && y_bf16 && experts->gate && experts->gate_scale && experts->up && experts->up_scale && experts->down && experts->down_scale,
+                  CHADQ_ERR_NULL, "chadq_moe_ffn_fp8: null pointer");
+    const size_t need = moe_fp8_workspace_bytes(T, H, F, E, r.top_k, x_scale != nullptr);
+    CHADQ_REQUIRE(workspace && workspace_bytes >= need, CHADQ_ERR_WORKSPACE, "chadq_moe_ffn_fp8: workspace of %zu bytes needed, %zu given", need,
+                  workspace ? workspace_bytes : (size_t)0);
+    CHADQ_REQUIRE(aligned16(x) && aligned16(experts->gate) && aligned16(experts->up) && aligned16(experts->down) && aligned16(workspace) && aligned16(y_bf16) &&
+                      aligned4(x_scale) && aligned4(logits) && aligned4(r.bias) && aligned4(experts->gate_scale) && aligned4(experts->up_scale) &&
+                      aligned4(experts->down_scale),
+                  CHADQ_ERR_ALIGN, "chadq_moe_ffn_fp8: x, y, values and workspace must be 16-byte, everything else 4-byte aligned");
+    return moe_ffn_fp8_launch(x, x_scale, logits, routing_of(r), experts, y_bf16, T, H, F, E, workspace, st);
 }
 
 }  // extern "C"

@@ -1,0 +1,43 @@
+// 8-bit floating point (FP8) with a scale for each block of 128: what its kernels share.
+//   values e4m3: sign, 4 bits of exponent (bias 7), 3 of mantissa; largest 448, 0x7F and 0xFF are NaN; one to a byte
+//   scales fp32: of activations one per row and 128 k, of weights one per 128 rows and 128 k; the last block of rows and of k may be cut
+// A product's sum of a block, of values alone, is multiplied by the block's scales and added to the result, all in fp32.
+#pragma once
+#include "mx.h"
+
+namespace chadq {
+
+constexpr int kFp8Block = 128;
+inline __host__ __device__ int fp8_blocks(int n) { return (int)(((int64_t)n + 127) >> 7); }
+
+// 4 values (one word) -> 4 bf16 in order, exact
+__device__ __forceinline__ u32x2 fp8_to_bf16(uint32_t w) {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true))};
+}
+
+// y[r, n] = sum over blocks b of xs[r, b] ws[g(r), n / 128, b] sum_{k in b} x[r, k] w[g(r), n, k] for the rows r of group g(r) = the g with
+// offsets[g] <= r < offsets[g + 1]
+struct Fp8Product {
+    const void *x;            // bf16 [M,K] (xs null), or values [M,K]
+    const float *xs;          // scales of the values [M,ceil(K/128)]
+    const uint8_t *w;         // values [E,N,K]
+    const float *ws;          // [E,ceil(N/128),ceil(K/128)]
+    void *y;                  // fp32 or bf16 [M,N]
+    const int32_t *offsets;   // [E+1] on the device, or null: one group, all rows
+    int M, N, K, E;
+    bool y_bf16, clear_rest;  // clear_rest: rows of no group become 0 (else they are left as they are)
+    // mixture of experts: row r of the groups is row rows[r] of x (null: r); with a second matrix per group, of w's shape, the result
+    // is silu(x w) (x w2)
+    const int32_t *rows = nullptr;
+    int x_rows = 0;           // ... which has so many
+    const uint8_t *w2 = nullptr;
+    const float *w2s = nullptr;
+};
+
+constexpr int kFp8MostK = 1 << 26;  // bytes of an activation row are counted in 32 bits
+
+int fp8_product_launch(const Fp8Product &p, void *workspace, size_t workspace_bytes, hipStream_t st);
+size_t fp8_product_workspace_bytes(int M, int N, int K, bool x_fp8);
+
+}  // namespace chadq

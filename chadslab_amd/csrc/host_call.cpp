@@ -1,4 +1,4 @@
-// The plain calls of chadslab_amd.ops (qlinear, moe_ffn, and those on MXFP4) from the Python object to the C ABI in one native function.
+// The plain calls of chadslab_amd.ops (qlinear, moe_ffn, and those on MXFP4 and FP8) from the Python object to the C ABI in one native function.
 //
 // What bounds a small call is the host: a product of 2048 x 2048 on one token takes 2.9 us on the GPU and took 7.2 us of Python
 // (attribute look-ups, checks, the result's allocation, eight arguments through ctypes), a mixture of experts with sixteen experts
@@ -36,10 +36,15 @@ enum MxEntry { MX_QUANTIZE, MX_DEQUANT, MX_BYTES, MX_PRODUCT, MX_GROUPED, MX_MOE
 const char *const kMxNames[MX_ENTRIES] = {"chadq_quantize_mxfp4", "chadq_dequant_mxfp4", "chadq_product_mxfp4_workspace_bytes", "chadq_product_mxfp4", "chadq_product_mxfp4_grouped",
                                           "chadq_moe_ffn_mxfp4_workspace_bytes", "chadq_moe_ffn_mxfp4"};
 void *g_mx_entry[MX_ENTRIES];                          // (bind_mx)
+enum Fp8Entry { FP8_QUANTIZE, FP8_DEQUANT, FP8_BYTES, FP8_PRODUCT, FP8_GROUPED, FP8_ROUTE, FP8_MOE_BYTES, FP8_MOE, FP8_ENTRIES };
+const char *const kFp8Names[FP8_ENTRIES] = {"chadq_quantize_fp8", "chadq_dequant_fp8", "chadq_product_fp8_workspace_bytes", "chadq_product_fp8", "chadq_product_fp8_grouped",
+                                            "chadq_moe_route_experts", "chadq_moe_ffn_fp8_workspace_bytes", "chadq_moe_ffn_fp8"};
+void *g_fp8_entry[FP8_ENTRIES];                        // (bind_fp8)
+PyObject *g_fp8 = nullptr, *g_fp8_experts = nullptr, *g_fp8_rows = nullptr;
 PyObject *g_int4 = nullptr, *g_int8 = nullptr, *g_tiles = nullptr, *g_mx = nullptr, *g_mx_experts = nullptr;  // the weight containers
 PyObject *g_check = nullptr;                           // _lib.check(status, name): raises
 PyObject *s_packed, *s_scale, *s_w;
-constexpr int kGemvRows = 16, kMaxExperts = 16;
+constexpr int kGemvRows = 16, kMaxExperts = 16, kRouteExperts = 512;
 
 // a dense GPU tensor that may be handed on as it is
 const at::Tensor *plain(PyObject *o, at::ScalarType type, int dim, int device) {
@@ -120,8 +125,10 @@ struct MxRows {
 // the device of a tensor or of a container's codes, if that is the current one; else -1
 int device_of(PyObject *o) {
     if (!THPVariable_CheckExact(o)) {
-        if ((PyObject *)Py_TYPE(o) != g_mx && (PyObject *)Py_TYPE(o) != g_mx_experts) return -1;
-        const Ref po(PyObject_GetAttr(o, s_packed));
+        PyObject *const kind = (PyObject *)Py_TYPE(o);
+        const bool fp8 = kind == g_fp8 || kind == g_fp8_rows || kind == g_fp8_experts;
+        if (kind != g_mx && kind != g_mx_experts && !fp8) return -1;
+        const Ref po(PyObject_GetAttr(o, fp8 ? s_w : s_packed));
         return po.p && THPVariable_CheckExact(po.p) ? device_of(po.p) : -1;
     }
     const at::Tensor &t = THPVariable_Unpack(o);
@@ -133,12 +140,12 @@ int device_of(PyObject *o) {
 void *stream_of(int dev) { return c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev).stream(); }
 
 // a container of these arrays, which fit each other by construction
-PyObject *container(PyObject *kind, at::Tensor &&p, at::Tensor &&s) {
+PyObject *container(PyObject *kind, at::Tensor &&p, at::Tensor &&s, PyObject *first) {
     PyTypeObject *const type = reinterpret_cast<PyTypeObject *>(kind);
     PyObject *const o = type->tp_alloc(type, 0);
     if (!o) return nullptr;
     const Ref po(THPVariable_Wrap(std::move(p))), so(THPVariable_Wrap(std::move(s)));
-    if (!po.p || !so.p || PyObject_SetAttr(o, s_packed, po.p) < 0 || PyObject_SetAttr(o, s_scale, so.p) < 0) {
+    if (!po.p || !so.p || PyObject_SetAttr(o, first, po.p) < 0 || PyObject_SetAttr(o, s_scale, so.p) < 0) {
         Py_DECREF(o);
         return nullptr;
     }
@@ -172,13 +179,16 @@ PyObject *quantize(PyObject *, PyObject *x_o) {
             x.numel() / k, (int)k, stream_of(dev));
     }
     if (rc != 0) return failed(rc, kMxNames[MX_QUANTIZE]);
-    return container(dim == 3 ? g_mx_experts : g_mx, std::move(p), std::move(s));
+    return container(dim == 3 ? g_mx_experts : g_mx, std::move(p), std::move(s), s_packed);
     END_HANDLE_TH_ERRORS
 }
+
+PyObject *dequantize_fp8(PyObject *o);
 
 // dequantize(container) -> fp32 tensor, or None
 PyObject *dequantize(PyObject *, PyObject *o) {
     HANDLE_TH_ERRORS
+    if ((PyObject *)Py_TYPE(o) == g_fp8 || (PyObject *)Py_TYPE(o) == g_fp8_experts || (PyObject *)Py_TYPE(o) == g_fp8_rows) return dequantize_fp8(o);
     const bool experts = (PyObject *)Py_TYPE(o) == g_mx_experts;
     const int dev = THPVariable_CheckExact(o) ? -1 : device_of(o);
     Mx m;
@@ -229,9 +239,12 @@ PyObject *linear_mx(PyObject *x_o, PyObject *qw, PyObject *out_dtype) {
     return THPVariable_Wrap(std::move(y));
 }
 
+PyObject *grouped_fp8(PyObject *const *args);
+
 // grouped(x, experts, offsets) -> y, or None
 PyObject *grouped(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
+    if (n_args == 3 && (PyObject *)Py_TYPE(args[1]) == g_fp8_experts) return grouped_fp8(args);
     const int dev = n_args == 3 ? device_of(args[0]) : -1;
     MxRows x;
     Mx w;
@@ -294,12 +307,257 @@ PyObject *moe_ffn_mx(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- FP8
+// values and scales of a container of `dim` dimensions, on the device, that fit each other
+struct Fp8 {
+    at::Tensor w, s;
+    int64_t rows = 0, k = 0;  // rows: of a matrix
+    bool of(PyObject *o, PyObject *kind, int dim, int dev) {
+        if ((PyObject *)Py_TYPE(o) != kind) return false;
+        const Ref wo(PyObject_GetAttr(o, s_w)), so(PyObject_GetAttr(o, s_scale));
+        const at::Tensor *const wt = plain(wo.p, at::kFloat8_e4m3fn, dim, dev), *const st = plain(so.p, at::kFloat, dim, dev);
+        if (!wt || !st) return false;
+        rows = wt->size(dim - 2);
+        k = wt->size(dim - 1);
+        if (k < 16 || k % 16 || k > INT_MAX || rows < 1 || rows > INT_MAX || st->size(dim - 1) != (k + 127) / 128 ||
+            st->size(dim - 2) != (kind == g_fp8_rows ? rows : (rows + 127) / 128) || (dim == 3 && (st->size(0) != wt->size(0) || wt->size(0) < 1 || wt->size(0) > INT_MAX)))
+            return false;
+        w = *wt;
+        s = *st;
+        return true;
+    }
+    const uint8_t *values() const { return reinterpret_cast<const uint8_t *>(w.const_data_ptr()); }
+    const float *scale() const { return s.const_data_ptr<float>(); }
+};
+
+// activations: a bf16 tensor [M,K] or a QRowsFP8
+struct Fp8Rows {
+    at::Tensor x, s;
+    int64_t rows = 0, k = 0;
+    bool of(PyObject *o, int dev) {
+        if (THPVariable_CheckExact(o)) {
+            const at::Tensor *const t = plain(o, at::kBFloat16, 2, dev);
+            if (!t) return false;
+            x = *t;
+            rows = t->size(0);
+            k = t->size(1);
+        } else {
+            Fp8 m;
+            if (!m.of(o, g_fp8_rows, 2, dev)) return false;
+            x = m.w;
+            s = m.s;
+            rows = m.rows;
+            k = m.k;
+        }
+        return rows >= 1 && rows <= INT_MAX;
+    }
+    const float *scale() const { return s.defined() ? s.const_data_ptr<float>() : nullptr; }
+};
+
+bool held(const at::Tensor &t) { return t.unsafeGetTensorImpl()->has_storage(); }
+
+template <typename F>
+F fp8_entry(Fp8Entry e, F) { return reinterpret_cast<F>(g_fp8_entry[e]); }
+
+// quantize_fp8(x, rows) -> container, or None
+PyObject *quantize_fp8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    const int dev = n_args == 2 && PyBool_Check(args[1]) && THPVariable_CheckExact(args[0]) ? device_of(args[0]) : -1;
+    if (dev < 0) Py_RETURN_NONE;
+    const bool rows = args[1] == Py_True;
+    const at::ScalarType type = THPVariable_Unpack(args[0]).scalar_type();
+    const int dim = (int)THPVariable_Unpack(args[0]).dim();
+    if ((type != at::kFloat && type != at::kBFloat16 && type != at::kHalf) || (dim != 2 && (rows || dim != 3))) Py_RETURN_NONE;
+    const at::Tensor *const xt = plain(args[0], type, dim, dev);
+    if (!xt) Py_RETURN_NONE;
+    const at::Tensor x = *xt;
+    const int64_t k = x.size(dim - 1), n = x.size(dim - 2), e = dim == 3 ? x.size(0) : 1;
+    if (k < 16 || k % 16 || k > INT_MAX || n > INT_MAX || x.numel() == 0) Py_RETURN_NONE;
+    at::Tensor w, s;
+    int rc;
+    {
+        const WithoutLock free;
+        const auto wo = x.options().dtype(at::kFloat8_e4m3fn).requires_grad(false), so = x.options().dtype(at::kFloat).requires_grad(false);
+        const int64_t sn = rows ? n : (n + 127) / 128, sk = (k + 127) / 128;
+        w = dim == 3 ? at::empty({e, n, k}, wo) : at::empty({n, k}, wo);
+        s = dim == 3 ? at::empty({e, sn, sk}, so) : at::empty({sn, sk}, so);
+        if (!held(w) || !held(s)) rc = CHADQ_ERR_NULL;
+        else rc = fp8_entry(FP8_QUANTIZE, &chadq_quantize_fp8)(
+            x.const_data_ptr(), type == at::kFloat ? CHADQ_F32 : type == at::kBFloat16 ? CHADQ_BF16 : CHADQ_F16, reinterpret_cast<uint8_t *>(w.mutable_data_ptr()),
+            s.mutable_data_ptr<float>(), e, (int)n, (int)k, rows, stream_of(dev));
+    }
+    if (rc != 0) return failed(rc, kFp8Names[FP8_QUANTIZE]);
+    return container(rows ? g_fp8_rows : dim == 3 ? g_fp8_experts : g_fp8, std::move(w), std::move(s), s_w);
+    END_HANDLE_TH_ERRORS
+}
+
+// dequantize() of an FP8 container
+PyObject *dequantize_fp8(PyObject *o) {
+    PyObject *const kind = (PyObject *)Py_TYPE(o);
+    const int dev = device_of(o);
+    Fp8 m;
+    if (dev < 0 || !m.of(o, kind, kind == g_fp8_experts ? 3 : 2, dev)) Py_RETURN_NONE;
+    at::Tensor y;
+    int rc;
+    {
+        const WithoutLock free;
+        y = at::empty(m.w.sizes(), m.s.options().requires_grad(false));
+        if (!held(y)) rc = CHADQ_ERR_NULL;
+        else rc = fp8_entry(FP8_DEQUANT, &chadq_dequant_fp8)(m.values(), m.scale(), y.mutable_data_ptr<float>(), m.w.dim() == 3 ? m.w.size(0) : 1, (int)m.rows, (int)m.k,
+                                                              kind == g_fp8_rows, stream_of(dev));
+    }
+    if (rc != 0) return failed(rc, kFp8Names[FP8_DEQUANT]);
+    return THPVariable_Wrap(std::move(y));
+}
+
+// linear() on QWeightFP8
+PyObject *linear_fp8(PyObject *x_o, PyObject *qw, PyObject *out_dtype) {
+    const int dev = device_of(x_o);
+    Fp8Rows x;
+    Fp8 w;
+    if (dev < 0 || !x.of(x_o, dev) || !w.of(qw, g_fp8, 2, dev) || x.k != w.k) Py_RETURN_NONE;
+    at::ScalarType y_type = x.rows <= kGemvRows ? at::kFloat : at::kBFloat16;
+    if (out_dtype != Py_None) {
+        if (!THPDtype_Check(out_dtype)) Py_RETURN_NONE;
+        const at::ScalarType want = reinterpret_cast<THPDtype *>(out_dtype)->scalar_type;
+        if (want != y_type && want != at::kBFloat16) Py_RETURN_NONE;
+        y_type = want;
+    }
+    const int m = (int)x.rows, n = (int)w.rows, k = (int)w.k;
+    const size_t need = fp8_entry(FP8_BYTES, &chadq_product_fp8_workspace_bytes)(m, n, k, x.s.defined());
+    at::Tensor y, ws;
+    int rc;
+    {
+        const WithoutLock free;
+        if (need) ws = at::empty({(int64_t)need}, w.s.options().dtype(at::kByte).requires_grad(false));
+        y = at::empty({m, n}, w.s.options().dtype(y_type).requires_grad(false));
+        if (!held(y) || (need && !held(ws))) rc = CHADQ_ERR_NULL;
+        else rc = fp8_entry(FP8_PRODUCT, &chadq_product_fp8)(x.x.const_data_ptr(), x.scale(), w.values(), w.scale(), y.mutable_data_ptr(), y_type == at::kBFloat16, m, n, k,
+                                                              need ? ws.mutable_data_ptr() : nullptr, need, stream_of(dev));
+    }
+    if (rc != 0) return failed(rc, kFp8Names[FP8_PRODUCT]);
+    return THPVariable_Wrap(std::move(y));
+}
+
+// grouped() on QExpertsFP8
+PyObject *grouped_fp8(PyObject *const *args) {
+    const int dev = device_of(args[0]);
+    Fp8Rows x;
+    Fp8 w;
+    if (dev < 0 || !x.of(args[0], dev) || !w.of(args[1], g_fp8_experts, 3, dev) || x.k != w.k) Py_RETURN_NONE;
+    const at::Tensor *const o = plain(args[2], at::kInt, 1, dev);
+    const int64_t e = w.w.size(0);
+    if (!o || o->size(0) != e + 1) Py_RETURN_NONE;
+    const at::Tensor offsets = *o;
+    at::Tensor y;
+    int rc;
+    {
+        const WithoutLock free;
+        y = at::empty({x.rows, w.rows}, w.s.options().dtype(at::kBFloat16).requires_grad(false));
+        if (!held(y)) rc = CHADQ_ERR_NULL;
+        else rc = fp8_entry(FP8_GROUPED, &chadq_product_fp8_grouped)(x.x.const_data_ptr(), x.scale(), w.values(), w.scale(), offsets.const_data_ptr<int32_t>(),
+                                                                      reinterpret_cast<uint16_t *>(y.mutable_data_ptr()), (int)x.rows, (int)e, (int)w.rows, (int)w.k, 1,
+                                                                      stream_of(dev));
+    }
+    if (rc != 0) return failed(rc, kFp8Names[FP8_GROUPED]);
+    return THPVariable_Wrap(std::move(y));
+}
+
+// bias or None, sigmoid, renorm, groups, top_groups, group_sum, top_k, scale
+struct Route {
+    at::Tensor bias;
+    chadq_routing r = {};
+    bool of(PyObject *const *a, int64_t e, int dev) {
+        if (a[0] != Py_None) {
+            const at::Tensor *const b = plain(a[0], at::kFloat, 1, dev);
+            if (!b || b->size(0) != e) return false;
+            bias = *b;
+            r.bias = b->const_data_ptr<float>();
+        }
+        int *const to[6] = {&r.sigmoid, &r.renorm, &r.groups, &r.top_groups, &r.group_sum, &r.top_k};
+        for (int i = 0; i < 6; ++i) {
+            if (!PyBool_Check(a[i + 1]) && !PyLong_CheckExact(a[i + 1])) return false;
+            int overflow = 0;
+            const long v = PyLong_AsLongAndOverflow(a[i + 1], &overflow);
+            if (overflow || v < INT_MIN || v > INT_MAX) return false;
+            *to[i] = (int)v;
+        }
+        if (!PyFloat_CheckExact(a[7])) return false;
+        r.scale = (float)PyFloat_AS_DOUBLE(a[7]);
+        return r.top_k >= 1 && r.top_k <= e;
+    }
+};
+
+// route(logits, *Route) -> (idx, w), or None
+PyObject *route(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    const int dev = n_args == 9 && THPVariable_CheckExact(args[0]) ? device_of(args[0]) : -1;
+    if (dev < 0) Py_RETURN_NONE;
+    const at::Tensor *const zt = plain(args[0], at::kFloat, 2, dev);
+    Route how;
+    if (!zt || zt->size(0) < 1 || zt->size(0) > INT_MAX || zt->size(1) < 1 || zt->size(1) > kRouteExperts || !how.of(args + 1, zt->size(1), dev)) Py_RETURN_NONE;
+    const at::Tensor z = *zt;
+    at::Tensor idx, w;
+    int rc;
+    {
+        const WithoutLock free;
+        idx = at::empty({z.size(0), how.r.top_k}, z.options().dtype(at::kInt).requires_grad(false));
+        w = at::empty({z.size(0), how.r.top_k}, z.options().requires_grad(false));
+        if (!held(idx) || !held(w)) rc = CHADQ_ERR_NULL;
+        else rc = fp8_entry(FP8_ROUTE, &chadq_moe_route_experts)(z.const_data_ptr<float>(), &how.r, idx.mutable_data_ptr<int32_t>(), w.mutable_data_ptr<float>(),
+                                                                  (int)z.size(0), (int)z.size(1), stream_of(dev));
+    }
+    if (rc != 0) return failed(rc, kFp8Names[FP8_ROUTE]);
+    const Ref io(THPVariable_Wrap(std::move(idx))), wo(THPVariable_Wrap(std::move(w)));
+    if (!io.p || !wo.p) return PyErr_NoMemory();
+    return PyTuple_Pack(2, io.p, wo.p);
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_ffn_fp8(x, logits, (gate, up, down), *Route) -> y, or None
+PyObject *moe_ffn_fp8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 11 || !(PyList_CheckExact(args[2]) || PyTuple_CheckExact(args[2])) || PySequence_Fast_GET_SIZE(args[2]) != 3) Py_RETURN_NONE;
+    const int dev = device_of(args[0]);
+    if (dev < 0) Py_RETURN_NONE;
+    Fp8Rows x;
+    Fp8 w[3];
+    Route how;
+    const at::Tensor *const zt = plain(args[1], at::kFloat, 2, dev);
+    if (!zt || !x.of(args[0], dev)) Py_RETURN_NONE;
+    const at::Tensor z = *zt;
+    for (int i = 0; i < 3; ++i)
+        if (!w[i].of(PySequence_Fast_GET_ITEM(args[2], i), g_fp8_experts, 3, dev)) Py_RETURN_NONE;
+    const int64_t t = x.rows, h = x.k, e = w[0].w.size(0), f = w[0].rows;
+    if (e > kRouteExperts || z.size(0) != t || z.size(1) != e || !how.of(args + 3, e, dev)) Py_RETURN_NONE;
+    for (int i = 0; i < 3; ++i)
+        if (w[i].w.size(0) != e || w[i].rows != (i < 2 ? f : h) || w[i].k != (i < 2 ? h : f)) Py_RETURN_NONE;
+    const size_t need = fp8_entry(FP8_MOE_BYTES, &chadq_moe_ffn_fp8_workspace_bytes)((int)t, (int)h, (int)f, (int)e, how.r.top_k, x.s.defined());
+    if (need == 0) Py_RETURN_NONE;
+    const chadq_moe_fp8 experts = {w[0].values(), w[1].values(), w[2].values(), w[0].scale(), w[1].scale(), w[2].scale()};
+    at::Tensor ws, y;
+    int rc;
+    {
+        const WithoutLock free;
+        ws = at::empty({(int64_t)need}, z.options().dtype(at::kByte).requires_grad(false));
+        y = at::empty({t, h}, z.options().dtype(at::kBFloat16).requires_grad(false));
+        if (!held(ws) || !held(y)) rc = CHADQ_ERR_NULL;
+        else rc = fp8_entry(FP8_MOE, &chadq_moe_ffn_fp8)(x.x.const_data_ptr(), x.scale(), z.const_data_ptr<float>(), &how.r, &experts,
+                                                          reinterpret_cast<uint16_t *>(y.mutable_data_ptr()), (int)t, (int)h, (int)f, (int)e, ws.mutable_data_ptr(), need,
+                                                          stream_of(dev));
+    }
+    if (rc != 0) return failed(rc, kFp8Names[FP8_MOE]);
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
 // linear(x, weight, out_dtype) -> y, or None
 PyObject *linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
     if (n_args != 3) Py_RETURN_NONE;
     PyObject *const qw = args[1];
     if ((PyObject *)Py_TYPE(qw) == g_mx) return linear_mx(args[0], qw, args[2]);
+    if ((PyObject *)Py_TYPE(qw) == g_fp8) return linear_fp8(args[0], qw, args[2]);
     const bool int4 = (PyObject *)Py_TYPE(qw) == g_int4;
     if (!int4 && (PyObject *)Py_TYPE(qw) != g_int8) Py_RETURN_NONE;
     if (!THPVariable_CheckExact(args[0])) Py_RETURN_NONE;
@@ -486,12 +744,25 @@ PyObject *bind_mx(PyObject *, PyObject *args) {
     Py_RETURN_NONE;
 }
 
+// bind_fp8(addresses of the entry points in the order of Fp8Entry, (QWeightFP8, QExpertsFP8, QRowsFP8))
+PyObject *bind_fp8(PyObject *, PyObject *args) {
+    PyObject *addr, *kinds;
+    if (!PyArg_ParseTuple(args, "O!O!", &PyTuple_Type, &addr, &PyTuple_Type, &kinds)) return nullptr;
+    PyObject **const slots[3] = {&g_fp8, &g_fp8_experts, &g_fp8_rows};
+    if (!keep(addr, FP8_ENTRIES, g_fp8_entry, kinds, 3, slots)) return nullptr;
+    Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {{"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, "linear(x, weight, out_dtype) -> y, or None where the Python path has to look"},
                          {"moe_ffn", (PyCFunction)(void (*)(void))moe_ffn, METH_FASTCALL, "moe_ffn(x, logits, experts, top_k, renorm) -> y, or None"},
                          {"quantize", quantize, METH_O, "quantize(x) -> MXFP4 container, or None"},
                          {"dequantize", dequantize, METH_O, "dequantize(MXFP4 container) -> fp32 tensor, or None"},
                          {"grouped", (PyCFunction)(void (*)(void))grouped, METH_FASTCALL, "grouped(x, experts, offsets) -> y, or None"},
                          {"moe_ffn_mx", (PyCFunction)(void (*)(void))moe_ffn_mx, METH_FASTCALL, "moe_ffn_mx(x, logits, experts, top_k, renorm) -> y, or None"},
+                         {"quantize_fp8", (PyCFunction)(void (*)(void))quantize_fp8, METH_FASTCALL, "quantize_fp8(x, rows) -> FP8 container, or None"},
+                         {"route", (PyCFunction)(void (*)(void))route, METH_FASTCALL, "route(logits, bias, ...) -> (idx, w), or None"},
+                         {"moe_ffn_fp8", (PyCFunction)(void (*)(void))moe_ffn_fp8, METH_FASTCALL, "moe_ffn_fp8(x, logits, experts, bias, ...) -> y, or None"},
+                         {"bind_fp8", bind_fp8, METH_VARARGS, "bind_fp8(addresses, containers)"},
                          {"gemv_bytes", (PyCFunction)(void (*)(void))bytes_of<GEMV_BYTES>, METH_FASTCALL, "gemv_bytes(M, N, K, int8) -> bytes"},
                          {"gemm_bytes", (PyCFunction)(void (*)(void))bytes_of<GEMM_BYTES>, METH_FASTCALL, "gemm_bytes(M, N, K, int8) -> bytes"},
                          {"bind", bind, METH_VARARGS, "bind(addresses, containers, check)"},

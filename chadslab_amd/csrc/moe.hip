@@ -20,7 +20,9 @@
 // 14336 x 4096 92 us (what they read, at a large copy's rate, 99), 256 tokens 306 us (gate and up 184, down 119).
 #include "chadq_common.h"
 #include "expert_prep.h"
+#include "fp8.h"
 #include "mx.h"
+#include "route.h"
 
 namespace chadq {
 
@@ -570,6 +572,73 @@ int moe_ffn_mxfp4_launch(const uint16_t *x, const float *logits, const chadq_moe
     if (rc) return rc;
     const int64_t quads = (int64_t)T * (H / 4);
     hipLaunchKernelGGL(moe_combine_kernel, dim3(quads < 1024 * 256 ? (int)((quads + 255) / 256) : 1024), dim3(256), 0, st, ws.yp, ws.pos, ws.w, y, T, H, top_k, down.parts(),
+                       (size_t)P * H);
+    return hip_check(hipGetLastError(), "moe combine launch");
+}
+
+// ---- the same on FP8 experts, routed as route.hip does it: gate and up with the SiLU gate in one product by group, down to fp32, combine.  With 8-bit
+// activations h becomes 8-bit too, from its fp32 values.
+struct MoeFp8Ws {
+    int32_t *idx, *pos, *tok, *offsets, *hist;
+    float *w;
+    void *h;       // bf16 [P,F], or fp32 for 8-bit activations
+    uint8_t *h8;   // [P,F]
+    float *h8s;    // [P,ceil(F/128)]
+    float *yp;     // [P,H]
+};
+
+static size_t moe_fp8_layout(uint8_t *base, int T, int H, int F, int E, int top_k, bool x_fp8, MoeFp8Ws *ws) {
+    const size_t P = (size_t)T * top_k;
+    size_t o = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t *p = base ? base + o : nullptr;
+        o += align_up(bytes);
+        return p;
+    };
+    MoeFp8Ws w = {};
+    w.idx = (int32_t *)take(P * 4);
+    w.w = (float *)take(P * 4);
+    w.pos = (int32_t *)take(P * 4);
+    w.tok = (int32_t *)take(P * 4);
+    w.offsets = (int32_t *)take(((size_t)E + 1) * 4);
+    w.hist = (int32_t *)take(sort_chunks(P) > 1 ? (size_t)sort_chunks(P) * E * 4 : 0);
+    w.h = take(P * F * (x_fp8 ? 4 : 2));
+    w.h8 = take(x_fp8 ? P * F : 0);
+    w.h8s = (float *)take(x_fp8 ? P * fp8_blocks(F) * 4 : 0);
+    w.yp = (float *)take(P * H * 4);
+    if (ws) *ws = w;
+    return o;
+}
+
+size_t moe_fp8_workspace_bytes(int T, int H, int F, int E, int top_k, bool x_fp8) { return moe_fp8_layout(nullptr, T, H, F, E, top_k, x_fp8, nullptr); }
+
+int quantize_fp8_launch(const void *x, int dtype, uint8_t *q, float *scale, int64_t matrices, int N, int K, bool rows, hipStream_t st);
+
+int moe_ffn_fp8_launch(const void *x, const float *xs, const float *logits, const Routing &r, const chadq_moe_fp8 *ex, uint16_t *y, int T, int H, int F, int E,
+                       void *workspace, hipStream_t st) {
+    MoeFp8Ws ws;
+    moe_fp8_layout(reinterpret_cast<uint8_t *>(workspace), T, H, F, E, r.top_k, xs != nullptr, &ws);
+    const int P = T * r.top_k;
+    int rc = route_sort_launch(logits, ws.idx, ws.w, T, E, r, RouteSort{ws.pos, ws.tok, ws.offsets, ws.hist}, st);
+    if (rc) return rc;
+    Fp8Product gu = {x, xs, ex->gate, ex->gate_scale, ws.h, ws.offsets, P, F, H, E, xs == nullptr, false};
+    gu.rows = ws.tok;
+    gu.x_rows = T;
+    gu.w2 = ex->up;
+    gu.w2s = ex->up_scale;
+    rc = fp8_product_launch(gu, nullptr, 0, st);
+    if (rc) return rc;
+    Fp8Product down = {ws.h, nullptr, ex->down, ex->down_scale, ws.yp, ws.offsets, P, H, F, E, false, false};
+    if (xs) {
+        rc = quantize_fp8_launch(ws.h, CHADQ_F32, ws.h8, ws.h8s, 1, P, F, true, st);
+        if (rc) return rc;
+        down.x = ws.h8;
+        down.xs = ws.h8s;
+    }
+    rc = fp8_product_launch(down, nullptr, 0, st);
+    if (rc) return rc;
+    const int64_t quads = (int64_t)T * (H / 4);
+    hipLaunchKernelGGL(moe_combine_kernel, dim3(quads < 1024 * 256 ? (int)((quads + 255) / 256) : 1024), dim3(256), 0, st, ws.yp, ws.pos, ws.w, y, T, H, r.top_k, 1,
                        (size_t)P * H);
     return hip_check(hipGetLastError(), "moe combine launch");
 }

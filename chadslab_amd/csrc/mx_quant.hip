@@ -5,41 +5,10 @@
 // Both are bound by the bytes they move.  Over inputs and results that do not fit the 256 MB cache: quantising 14336 x 4096 fp32 46.6 us = 5.7 TB/s, seven eighths of
 // it read, 4096 x 4096 bf16 9.1 us = 4.7 TB/s, and dequantising 14336 x 4096 55.9 us = 4.8 TB/s, seven eighths written (a copy of 1 GiB moves 5.2 TB/s, read and written, filling it
 // 6.8); with results that the cache holds 8.5 and 45.5 us.  16 x 4096: 3.2 us, a launch and one trip to memory.
+#include "load8.h"
 #include "mx.h"
 
 namespace chadq {
-
-// the bits of 8 consecutive values as fp32
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, float f[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float *p, float f[8]) {
-    const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[i] = a[i];
-        f[4 + i] = b[i];
-    }
-}
-template <>
-__device__ __forceinline__ void load8<__bf16>(const __bf16 *p, float f[8]) {
-    const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(v[i] << 16);
-        f[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
-    }
-}
-template <>
-__device__ __forceinline__ void load8<_Float16>(const _Float16 *p, float f[8]) {
-    const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const f16x2 h = as_f16x2(v[i]);
-        f[2 * i] = (float)h.x;
-        f[2 * i + 1] = (float)h.y;
-    }
-}
 
 // Four lanes to a block, 8 values to a lane: a lane stores one word of codes, and two exchanges inside the quad give the block's largest magnitude.
 // Rows do not matter, K is a multiple of 32.

@@ -1,0 +1,360 @@
+// Routing to experts.  Token t with logits z over E experts in `groups` groups of consecutive ones:
+//   score s = softmax(z) or 1 / (1 + exp(-z));  an expert is chosen by c = s + bias, or by z where there is neither a bias nor a sum over a group
+//   a group's value is the sum of its group_sum largest c; the experts of the top_groups largest groups are open
+//   the top_k open experts with the largest c, ties to the lowest index;  weights s, divided by their sum if asked (0 where that is 0), times scale
+// An expert whose logit is -infinity or NaN comes behind all others that are open and has the score 0.
+//
+// c and the sums of groups are formed in 64 bits: in 32 two experts whose scores differ by less than a rounding change places, which happens to a few of some
+// thousand tokens, and then another expert's output is added.  By z alone, 32 bits are exact.
+//
+// A token takes L lanes of a wave (8 to 64), each with PER consecutive experts: a lane's best is found among its own, the token's by a reduction over the lanes,
+// and the lowest lane that holds it wins, so that equal ones go to the lowest index with no index in the keys.
+#include <type_traits>
+
+#include "route.h"
+
+namespace chadq {
+
+__device__ __forceinline__ uint32_t route_key(float v) { return order_key(v); }
+__device__ __forceinline__ uint64_t route_key(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);
+    return b ^ ((b >> 63) ? ~0ull : 1ull << 63);
+}
+
+template <int L, typename T, typename F>
+__device__ __forceinline__ T over_lanes(T v, F f) {
+#pragma unroll
+    for (int s = 1; s < L; s *= 2) v = f(v, __shfl_xor(v, s));
+    return v;
+}
+
+// All lanes of the wave; the token's choices come back in its lanes 0 .. top_k - 1.  lds: [tokens of the workgroup][L * PER] choice values (groups > 1)
+template <int L, int PER, bool WIDE>
+__device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, int E, const Routing &r, void *lds, int &chosen, float &weight) {
+    typedef std::conditional_t<WIDE, double, float> V;
+    typedef std::conditional_t<WIDE, uint64_t, uint32_t> K;
+    const int lane = threadIdx.x & 63, ls = lane % L, seg = lane - ls;
+    const unsigned long long seg_mask = (L == 64 ? ~0ull : ((1ull << L) - 1)) << seg;
+    const auto larger = [](auto a, auto b) { return a > b ? a : b; };
+    float zr[PER];
+    bool masked[PER];
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int e = ls * PER + i;
+        zr[i] = e < E ? z[e] : -INFINITY;
+        masked[i] = !(zr[i] > -INFINITY);  // NaN too
+        top = masked[i] ? top : fmaxf(top, zr[i]);
+    }
+    top = over_lanes<L>(top, larger);
+    V c[PER];      // what chooses
+    double s[WIDE ? PER : 1];
+    V total = 0;   // of the softmax
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            s[i] = masked[i] ? 0.0 : r.sigmoid ? 1.0 / (1.0 + exp(-(double)zr[i])) : exp((double)zr[i] - (double)top);
+            total += s[i];
+        }
+        if (!r.sigmoid) {
+            total = over_lanes<L>(total, [](double a, double b) { return a + b; });
+#pragma unroll
+            for (int i = 0; i < PER; ++i) s[i] = masked[i] ? 0.0 : s[i] / total;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = ls * PER + i;
+            c[i] = masked[i] ? -1e300 : s[i] + (r.bias && e < E ? (double)r.bias[e] : 0.0);
+        }
+    } else {
+        if (!r.sigmoid && !r.renorm) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) total += masked[i] ? 0.f : expf(zr[i] - top);
+            total = over_lanes<L>(total, [](float a, float b) { return a + b; });
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) c[i] = masked[i] ? -INFINITY : zr[i];
+    }
+    uint32_t open = 0;  // bit i: expert i of the lane may still be chosen
+#pragma unroll
+    for (int i = 0; i < PER; ++i) open |= (ls * PER + i < E ? 1u : 0u) << i;
+    if (r.groups > 1) {
+        const int G = r.groups, per = E / G;
+        int q = L;  // lanes that share a group: a power of two
+        while (q * G > L) q >>= 1;
+        V *const mine = reinterpret_cast<V *>(lds) + (threadIdx.x / L) * (L * PER);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) mine[ls * PER + i] = c[i];
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's own: its LDS accesses keep their order
+        const int g = ls / q, j = ls % q;
+        V a = -INFINITY, b = -INFINITY;  // the two largest
+        if (g < G)
+            for (int i = j; i < per; i += q) {
+                const V v = mine[g * per + i];
+                b = v > a ? a : v > b ? v : b;
+                a = v > a ? v : a;
+            }
+        for (int d = 1; d < q; d *= 2) {
+            const V oa = __shfl_xor(a, d), ob = __shfl_xor(b, d);
+            const V low = a > oa ? oa : a, second = b > ob ? b : ob;
+            a = a > oa ? a : oa;
+            b = low > second ? low : second;
+        }
+        const V value = r.group_sum == 2 ? a + b : a;
+        int rank = 0;
+        for (int h = 0; h < G; ++h) {
+            const V o = __shfl(value, seg + h * q);
+            rank += o > value || (o == value && h < g);
+        }
+        const unsigned long long kept = __ballot(g < G && rank < r.top_groups) >> seg;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = ls * PER + i;
+            if (e < E && !(kept >> (e / per * q) & 1)) open &= ~(1u << i);
+        }
+    }
+    K key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = open >> i & 1 ? route_key(c[i]) : 0;
+    K best;
+    int at;
+    auto own = [&] {
+        best = key[0];
+        at = 0;
+#pragma unroll
+        for (int i = 1; i < PER; ++i)
+            if (key[i] > best) {  // strict: the lowest index
+                best = key[i];
+                at = i;
+            }
+    };
+    own();
+    float zc = -INFINITY;
+    double sc = 0.0;
+    chosen = 0;
+    for (int k = 0; k < r.top_k; ++k) {
+        const K most = over_lanes<L>(best, larger);
+        const unsigned long long hold = __ballot(best == most) & seg_mask;
+        const int winner = __ffsll((long long)hold) - 1;
+        const int e = __shfl(ls * PER + at, winner);
+        float zw = zr[0];
+        double sw = 0.0;
+        if constexpr (WIDE) sw = s[0];
+#pragma unroll
+        for (int i = 1; i < PER; ++i)
+            if (at == i) {
+                zw = zr[i];
+                if constexpr (WIDE) sw = s[i];
+            }
+        zw = __shfl(zw, winner);
+        if constexpr (WIDE) sw = __shfl(sw, winner);
+        if (ls == k) {
+            chosen = e;
+            zc = zw;
+            sc = sw;
+        }
+        if (lane == winner) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (at == i) key[i] = 0;
+            own();
+        }
+    }
+    const bool has = ls < r.top_k, none = !(zc > -INFINITY);
+    if constexpr (!WIDE) {
+        const float from = r.renorm ? over_lanes<L>(has && !none ? zc : -INFINITY, larger) : top;
+        sc = !has || none ? 0.0 : r.sigmoid ? 1.0 / (1.0 + exp(-(double)zc)) : exp((double)zc - (double)from);
+        if (!r.sigmoid && !r.renorm && !none) sc /= (double)total;
+    }
+    if (!has) sc = 0.0;
+    if (r.renorm) {
+        const double sum = over_lanes<L>(sc, [](double a, double b) { return a + b; });
+        if (sum > 0) sc /= sum;
+    }
+    weight = (float)(sc * (double)r.scale);
+}
+
+template <int L, int PER, bool WIDE>
+__global__ __launch_bounds__(256) void route_experts_kernel(const float *__restrict__ logits, int32_t *__restrict__ idx, float *__restrict__ w, int T, int E,
+                                                            Routing r) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int ls = threadIdx.x % L;
+    const int64_t t = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L, from = t < T ? t : T - 1;
+    int chosen;
+    float weight;
+    route_token_lanes<L, PER, WIDE>(logits + from * E, E, r, lds, chosen, weight);
+    if (t < T && ls < r.top_k) {
+        idx[t * r.top_k + ls] = chosen;
+        w[t * r.top_k + ls] = weight;
+    }
+}
+
+// ---- sorting: each workgroup a chunk of pairs.  e: the thread's expert, or -1.  Returns how many pairs of the chunk in front of it have the same expert;
+// s_cnt [16][E]: left as the counts of each wave's predecessors, s_total [E]: the chunk's pairs of each expert
+__device__ __forceinline__ int chunk_rank(int e, int E, uint16_t *s_cnt, int32_t *s_total) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    for (int i = tid; i < waves * E; i += blockDim.x) s_cnt[i] = 0;
+    __syncthreads();
+    unsigned long long same = __ballot(e >= 0);
+    for (int b = 0; 1 << b < E; ++b) {
+        const unsigned long long m = __ballot(e >> b & 1);
+        same &= e >> b & 1 ? m : ~m;
+    }
+    int rank = __popcll(same & ((1ull << lane) - 1));
+    if (e >= 0 && rank == 0) s_cnt[wave * E + e] = (uint16_t)__popcll(same);
+    __syncthreads();
+    if (tid < E) {
+        int n = 0;
+        for (int i = 0; i < waves; ++i) {
+            const int c = s_cnt[i * E + tid];
+            s_cnt[i * E + tid] = (uint16_t)n;
+            n += c;
+        }
+        s_total[tid] = n;
+    }
+    __syncthreads();
+    return e >= 0 ? rank + s_cnt[wave * E + e] : 0;
+}
+// s_first[e] = sum of s_total in front of e, s_first[E] = all; by the first wave
+__device__ __forceinline__ void experts_first(int E, const int32_t *s_total, int32_t *s_first) {
+    if (threadIdx.x < 64) {
+        const int lane = threadIdx.x;
+        int before = 0;
+        for (int c = 0; c < E; c += 64) {
+            const int v = c + lane < E ? s_total[c + lane] : 0;
+            int upto = v;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const int o = __shfl_up(upto, d);
+                upto += lane >= d ? o : 0;
+            }
+            if (c + lane < E) s_first[c + lane] = before + upto - v;
+            before += __shfl(upto, 63);
+        }
+        if (lane == 0) s_first[E] = before;
+    }
+    __syncthreads();
+}
+
+// One chunk: everything.  Several: FIRST writes each chunk's counts and its pairs' ranks, and then each workgroup adds what is in front of its own.
+enum SortStep { SORT_ALL, SORT_COUNT, SORT_PLACE };
+template <SortStep STEP>
+__global__ __launch_bounds__(kSortChunk) void sort_pairs_kernel(const int32_t *__restrict__ idx, RouteSort s, int P, int E, int top_k) {
+    __shared__ uint16_t s_cnt[16 * kRouteExperts];
+    __shared__ int32_t s_total[kRouteExperts], s_first[kRouteExperts + 1];
+    const int tid = threadIdx.x;
+    const int64_t p = (int64_t)blockIdx.x * blockDim.x + tid;
+    const int e = p < P ? idx[p] : -1;
+    int row = 0;
+    if (STEP != SORT_PLACE) row = chunk_rank(e, E, s_cnt, s_total);
+    if (STEP == SORT_COUNT) {
+        if (tid < E) s.hist[(int64_t)blockIdx.x * E + tid] = s_total[tid];
+        if (p < P) s.pos[p] = row;
+        return;
+    }
+    if (STEP == SORT_PLACE) {
+        int32_t *const s_before = reinterpret_cast<int32_t *>(s_cnt);
+        if (tid < E) {
+            int before = 0, all = 0;
+            for (int c = 0; c < (int)gridDim.x; ++c) {
+                const int n = s.hist[(int64_t)c * E + tid];
+                before += c < (int)blockIdx.x ? n : 0;
+                all += n;
+            }
+            s_before[tid] = before;
+            s_total[tid] = all;
+        }
+        __syncthreads();
+        if (p < P) row = s.pos[p] + s_before[e];
+    }
+    experts_first(E, s_total, s_first);
+    if (blockIdx.x == 0)
+        for (int i = tid; i <= E; i += blockDim.x) s.offsets[i] = s_first[i];
+    if (p < P) {
+        row += s_first[e];
+        s.pos[p] = row;
+        s.tok[row] = (int32_t)(p / top_k);
+    }
+}
+
+// Few tokens: one workgroup routes them and sorts their pairs.
+template <int L, int PER, bool WIDE>
+__global__ __launch_bounds__(1024) void route_few_kernel(const float *__restrict__ logits, int32_t *__restrict__ idx, float *__restrict__ w, int T, int E, Routing r,
+                                                         RouteSort s) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ uint16_t s_cnt[16 * kRouteExperts];
+    __shared__ int32_t s_total[kRouteExperts], s_first[kRouteExperts + 1];
+    __shared__ int16_t s_e[1024];
+    const int tid = threadIdx.x, ls = tid % L, t = tid / L;
+    s_e[tid] = -1;
+    __syncthreads();
+    int chosen;
+    float weight;
+    route_token_lanes<L, PER, WIDE>(logits + (int64_t)(t < T ? t : T - 1) * E, E, r, lds, chosen, weight);
+    if (t < T && ls < r.top_k) {
+        idx[t * r.top_k + ls] = chosen;
+        w[t * r.top_k + ls] = weight;
+        s_e[t * r.top_k + ls] = (int16_t)chosen;
+    }
+    __syncthreads();
+    const int e = s_e[tid];
+    int row = chunk_rank(e, E, s_cnt, s_total);
+    experts_first(E, s_total, s_first);
+    for (int i = tid; i <= E; i += blockDim.x) s.offsets[i] = s_first[i];
+    if (e >= 0) {
+        row += s_first[e];
+        s.pos[tid] = row;
+        s.tok[row] = tid / r.top_k;
+    }
+}
+
+template <typename F>
+static int with_shape(int E, bool wide, F f) {
+    auto go = [&](auto l, auto per) {
+        return wide ? f(l, per, std::true_type{}) : f(l, per, std::false_type{});
+    };
+#define CHADQ_INT(N) std::integral_constant<int, N>{}
+    if (E <= 8) return go(CHADQ_INT(8), CHADQ_INT(1));
+    if (E <= 16) return go(CHADQ_INT(16), CHADQ_INT(1));
+    if (E <= 32) return go(CHADQ_INT(32), CHADQ_INT(1));
+    if (E <= 64) return go(CHADQ_INT(64), CHADQ_INT(1));
+    if (E <= 128) return go(CHADQ_INT(64), CHADQ_INT(2));
+    if (E <= 256) return go(CHADQ_INT(64), CHADQ_INT(4));
+    return go(CHADQ_INT(64), CHADQ_INT(8));
+#undef CHADQ_INT
+}
+
+int route_experts_launch(const float *logits, int32_t *idx, float *w, int T, int E, const Routing &r, hipStream_t st) {
+    return with_shape(E, r.bias || r.group_sum == 2, [&](auto l, auto per, auto wide) {
+        constexpr int L = decltype(l)::value, PER = decltype(per)::value;
+        constexpr bool WIDE = decltype(wide)::value;
+        const int tokens = 256 / L, lds = r.groups > 1 ? 256 * PER * (WIDE ? 8 : 4) : 0;
+        hipLaunchKernelGGL((route_experts_kernel<L, PER, WIDE>), dim3((int)(((int64_t)T + tokens - 1) / tokens)), dim3(256), lds, st, logits, idx, w, T, E, r);
+        return hip_check(hipGetLastError(), "moe route launch");
+    });
+}
+
+int route_sort_launch(const float *logits, int32_t *idx, float *w, int T, int E, const Routing &r, const RouteSort &s, hipStream_t st) {
+    const int P = T * r.top_k, lanes = E <= 8 ? 8 : E <= 16 ? 16 : E <= 32 ? 32 : 64, most = E > 256 ? 512 : 1024;  // (threads: the groups' LDS)
+    if ((int64_t)T * lanes <= most)
+        return with_shape(E, r.bias || r.group_sum == 2, [&](auto l, auto per, auto wide) {
+            constexpr int L = decltype(l)::value, PER = decltype(per)::value;
+            constexpr bool WIDE = decltype(wide)::value;
+            const int threads = T * L <= 256 && E <= 256 ? 256 : most, lds = r.groups > 1 ? threads * PER * (WIDE ? 8 : 4) : 0;
+            hipLaunchKernelGGL((route_few_kernel<L, PER, WIDE>), dim3(1), dim3(threads), lds, st, logits, idx, w, T, E, r, s);
+            return hip_check(hipGetLastError(), "moe route launch");
+        });
+    int rc = route_experts_launch(logits, idx, w, T, E, r, st);
+    if (rc) return rc;
+    const int chunks = sort_chunks(P);
+    if (chunks == 1) {
+        hipLaunchKernelGGL(sort_pairs_kernel<SORT_ALL>, dim3(1), dim3(kSortChunk), 0, st, idx, s, P, E, r.top_k);
+    } else {
+        hipLaunchKernelGGL(sort_pairs_kernel<SORT_COUNT>, dim3(chunks), dim3(kSortChunk), 0, st, idx, s, P, E, r.top_k);
+        hipLaunchKernelGGL(sort_pairs_kernel<SORT_PLACE>, dim3(chunks), dim3(kSortChunk), 0, st, idx, s, P, E, r.top_k);
+    }
+    return hip_check(hipGetLastError(), "moe sort launch");
+}
+
+}  // namespace chadq

@@ -14,6 +14,10 @@ Layouts (this build's choices; the benchmark text fixes only "2 per byte", "grou
                   scale  uint8 [N, K/32]                    value(c) * 2^(scale[n, k // 32] - 127); 255: the block is NaN
                   (microscaled 4-bit floating point; the same container holds quantised activations)
   QExpertsMXFP4   the same for E matrices of one shape: packed [E, N, K/2], scale [E, N, K/32]
+  QWeightFP8      w      e4m3  [N, K]    row-major          value = w[n,k] * scale[n // 128, k // 128]
+                  scale  fp32  [ceil(N/128), ceil(K/128)]   (K a multiple of 16; the last blocks are cut)
+  QExpertsFP8     the same for E matrices of one shape: w [E, N, K], scale [E, ceil(N/128), ceil(K/128)]
+  QRowsFP8        activations: w e4m3 [M, K], scale fp32 [M, ceil(K/128)], one for each row and 128 k
 
 The tensors live wherever the caller puts them; the operators in chadslab_amd.ops want them on the GPU.
 Quantising and packing are load-time tools, not the hot path, and are written with torch tensor ops.
@@ -25,6 +29,8 @@ from dataclasses import dataclass
 import torch
 
 GROUP = 32
+FP8_BLOCK = 128
+FP8 = torch.float8_e4m3fn
 ZERO_POINT = 8
 FP16_MAX = 65504.0
 
@@ -158,6 +164,87 @@ class QExpertsMXFP4:
 
     def to(self, device) -> "QExpertsMXFP4":
         return QExpertsMXFP4(self.packed.to(device).contiguous(), self.scale.to(device).contiguous())
+
+
+def check_fp8(name: str, w: torch.Tensor, scale: torch.Tensor, dim: int, by_row: bool = False) -> None:
+    lead = "E,N" if dim == 3 else "M" if by_row else "N"
+    if w.dtype != FP8 or w.dim() != dim:
+        raise ValueError("%s.w must be float8_e4m3fn [%s,K]" % (name, lead))
+    *first, n, k = w.shape
+    if k % 16:
+        raise ValueError("K must be a multiple of 16")
+    if scale.dtype != torch.float32 or scale.shape != (*first, n if by_row else -(-n // FP8_BLOCK), -(-k // FP8_BLOCK)):
+        raise ValueError("%s.scale must be float32 [%s,ceil(K/128)]" % (name, "M" if by_row else lead[:-1] + "ceil(N/128)"))
+
+
+@dataclass
+class QWeightFP8:
+    w: torch.Tensor      # float8_e4m3fn [N, K]
+    scale: torch.Tensor  # float32 [ceil(N/128), ceil(K/128)]
+
+    def __post_init__(self):
+        check_fp8("QWeightFP8", self.w, self.scale, 2)
+
+    @property
+    def N(self) -> int:
+        return self.w.size(0)
+
+    @property
+    def K(self) -> int:
+        return self.w.size(1)
+
+    def to(self, device) -> "QWeightFP8":
+        return QWeightFP8(self.w.to(device).contiguous(), self.scale.to(device).contiguous())
+
+
+@dataclass
+class QExpertsFP8:
+    """E matrices of one shape in FP8, one behind the other: what ops.qgemm_grouped and ops.moe_ffn take."""
+    w: torch.Tensor      # float8_e4m3fn [E, N, K]
+    scale: torch.Tensor  # float32 [E, ceil(N/128), ceil(K/128)]
+
+    def __post_init__(self):
+        check_fp8("QExpertsFP8", self.w, self.scale, 3)
+
+    @property
+    def E(self) -> int:
+        return self.w.size(0)
+
+    @property
+    def N(self) -> int:
+        return self.w.size(1)
+
+    @property
+    def K(self) -> int:
+        return self.w.size(2)
+
+    def expert(self, e: int) -> QWeightFP8:
+        """Matrix e (the same memory)."""
+        return QWeightFP8(self.w[e], self.scale[e])
+
+    def to(self, device) -> "QExpertsFP8":
+        return QExpertsFP8(self.w.to(device).contiguous(), self.scale.to(device).contiguous())
+
+
+@dataclass
+class QRowsFP8:
+    """Activations in FP8, a scale for each row and 128 k: ops.quantize_fp8 makes them, products on FP8 weights take them."""
+    w: torch.Tensor      # float8_e4m3fn [M, K]
+    scale: torch.Tensor  # float32 [M, ceil(K/128)]
+
+    def __post_init__(self):
+        check_fp8("QRowsFP8", self.w, self.scale, 2, by_row=True)
+
+    @property
+    def M(self) -> int:
+        return self.w.size(0)
+
+    @property
+    def K(self) -> int:
+        return self.w.size(1)
+
+    def to(self, device) -> "QRowsFP8":
+        return QRowsFP8(self.w.to(device).contiguous(), self.scale.to(device).contiguous())
 
 
 def pack_int4(q: torch.Tensor) -> torch.Tensor:

@@ -12,9 +12,11 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .formats import GROUP, QExpertsMXFP4, QWeightInt4G32, QWeightInt4G32Tiles, QWeightInt8, QWeightMXFP4, check_mxfp4
+from .formats import (FP8, FP8_BLOCK, GROUP, QExpertsFP8, QExpertsMXFP4, QRowsFP8, QWeightFP8, QWeightInt4G32, QWeightInt4G32Tiles, QWeightInt8,
+                      QWeightMXFP4, check_fp8, check_mxfp4)
 
-QWeight = Union[QWeightInt4G32, QWeightInt8, QWeightMXFP4]
+QWeight = Union[QWeightInt4G32, QWeightInt8, QWeightMXFP4, QWeightFP8]
+QRows = Union[torch.Tensor, QWeightMXFP4, QRowsFP8]
 GEMV_MAX_M = 16  # decode batch sizes served by the bandwidth kernel
 
 
@@ -138,9 +140,52 @@ def quantize_mxfp4(x: torch.Tensor) -> Union[QWeightMXFP4, QExpertsMXFP4]:
     return QWeightMXFP4(p, s) if len(lead) == 1 else QExpertsMXFP4(p, s)
 
 
-def dequantize(qw: Union[QWeight, QExpertsMXFP4]) -> torch.Tensor:
-    """fp32 [N,K] dequantised weights (exact); [E,N,K] of QExpertsMXFP4."""
+def _fp8(q: Union[QWeightFP8, QExpertsFP8, QRowsFP8], name: str, device: Optional[torch.device] = None):
+    """Values and scales of a container, looked at as _arrays does, checked before their addresses go to the library."""
+    w, s = q.w, q.scale
+    check_fp8(type(q).__name__, w, s, 3 if isinstance(q, QExpertsFP8) else 2, isinstance(q, QRowsFP8))
+    w, s = _dev(w, name + ".w", FP8), _dev(s, name + ".scale", torch.float32)
+    for t in (w, s):
+        if t.device != (w.device if device is None else device):
+            raise ValueError("%s must live on %s, got %s" % (name, w.device if device is None else device, t.device))
+    return w, s
+
+
+def quantize_fp8(x: torch.Tensor, *, rows: bool = True) -> Union[QRowsFP8, QWeightFP8, QExpertsFP8]:
+    """fp32, bf16 or fp16 -> e4m3 with an fp32 scale for each block of 128; K a multiple of 16.  rows: activations [M,K], a block is 128 k of one row
+    -> QRowsFP8.  Else weights, a block is 128 rows x 128 k: [N,K] -> QWeightFP8, [E,N,K] -> QExpertsFP8.
+
+    With a = max(largest magnitude, 448 * 2^-126) of a block: scale = a / 448, r = 448 / a, each value goes to the nearest of x * r, ties to the even one (all in
+    fp32).  A block that holds a NaN or an infinity becomes NaN."""
+    q = _lib.native().quantize_fp8(x, rows)
+    if q is not None:
+        return q
+    if x.dtype not in _MX_TYPES:
+        raise ValueError("x must be float32, bfloat16 or float16, got %s" % x.dtype)
+    if x.dim() not in ((2,) if rows else (2, 3)) or x.size(-1) % 16:
+        raise ValueError("x must be %s with K a multiple of 16, got %s" % ("[M,K] (of more dimensions: x.flatten(0, -2))" if rows else "[N,K] or [E,N,K]", tuple(x.shape)))
+    x = _dev(x, "x", x.dtype)
+    *lead, n, k = x.shape
+    w = torch.empty(x.shape, dtype=FP8, device=x.device)
+    s = torch.empty(*lead, n if rows else -(-n // FP8_BLOCK), -(-k // FP8_BLOCK), dtype=torch.float32, device=x.device)
+    if x.numel():
+        _launch(x.device, "chadq_quantize_fp8", x.data_ptr(), _MX_TYPES[x.dtype], w.data_ptr(), s.data_ptr(), lead[0] if lead else 1, n, k, int(rows))
+    return QRowsFP8(w, s) if rows else QExpertsFP8(w, s) if lead else QWeightFP8(w, s)
+
+
+def dequantize(qw: Union[QWeight, QExpertsMXFP4, QExpertsFP8, QRowsFP8]) -> torch.Tensor:
+    """fp32 [N,K] dequantised weights (exact; FP8: value times scale, rounded once); [E,N,K] of QExpertsMXFP4 and QExpertsFP8."""
     lib = _lib.load()
+    if isinstance(qw, (QWeightFP8, QExpertsFP8, QRowsFP8)):
+        out = _lib.native().dequantize(qw)
+        if out is not None:
+            return out
+        w, s = _fp8(qw, "qw")
+        out = torch.empty(w.shape, dtype=torch.float32, device=w.device)
+        if out.numel():
+            *lead, n, k = w.shape
+            _launch(w.device, "chadq_dequant_fp8", w.data_ptr(), s.data_ptr(), out.data_ptr(), lead[0] if lead else 1, n, k, int(isinstance(qw, QRowsFP8)))
+        return out
     if isinstance(qw, (QWeightMXFP4, QExpertsMXFP4)):
         out = _lib.native().dequantize(qw)
         if out is not None:
@@ -194,9 +239,66 @@ def _product_mxfp4(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeightMXFP4, out: 
     return y
 
 
-def _no_mxfp4(x, qw) -> None:
+def _fp8_rows(x: Union[torch.Tensor, QRowsFP8], k: int, lead: str):
+    """The activations of a product on FP8 weights: a bf16 tensor or values, the address of their scales, and what has to live as long."""
+    if isinstance(x, torch.Tensor):
+        xt, xs = x, None
+    elif isinstance(x, QRowsFP8):
+        xt, xs = _fp8(x, "x")
+    else:
+        raise TypeError("x must be a tensor or a QRowsFP8 (of activations of more dimensions: quantize_fp8(x.flatten(0, -2))), got %r" % type(x))
+    if xt.dim() != 2 or xt.size(1) != k:
+        raise ValueError("x must be [%s,%d], got %s" % (lead, k, tuple(xt.shape)))
+    if xs is None:
+        return _dev(xt, "x", torch.bfloat16), None, None
+    return xt, xs.data_ptr(), xs
+
+
+def _product_fp8(x: Union[torch.Tensor, QRowsFP8], qw: QWeightFP8, out: Optional[torch.Tensor], y_dtype: torch.dtype) -> torch.Tensor:
+    """x (bf16 or FP8) [M,K] times FP8 weights -> fp32 or bf16 [M,N]."""
+    n, k = qw.w.shape if qw.w.dim() == 2 else (0, -1)
+    xt, xs, _keep = _fp8_rows(x, k, "M")
+    m = xt.size(0)
+    w, s = _fp8(qw, "weights", xt.device)
+    y = _out(out, (m, n), y_dtype, xt.device)
+    if m == 0 or n == 0:
+        return y
+    if k == 0:
+        return y.zero_()
+    need = _lib.load().chadq_product_fp8_workspace_bytes(m, n, k, int(xs is not None))
+    ws = torch.empty(need, dtype=torch.uint8, device=xt.device) if need else None  # a fresh one per call, as moe_ffn's
+    _launch(xt.device, "chadq_product_fp8", xt.data_ptr(), xs, w.data_ptr(), s.data_ptr(), y.data_ptr(), int(y_dtype == torch.bfloat16), m, n, k,
+            ws.data_ptr() if need else None, need)
+    return y
+
+
+def _grouped_fp8(x: Union[torch.Tensor, QRowsFP8], experts: QExpertsFP8, offsets: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+    e, n, k = experts.w.shape if experts.w.dim() == 3 else (0, 0, -1)
+    xt, xs, _keep = _fp8_rows(x, k, "R")
+    w, s = _fp8(experts, "experts", xt.device)
+    offsets = _offsets(offsets, e, xt.device)
+    y = _out(out, (xt.size(0), n), torch.bfloat16, xt.device)
+    if y.numel() == 0:
+        return y
+    if k == 0:
+        raise ValueError("K must be at least 16")
+    _launch(xt.device, "chadq_product_fp8_grouped", xt.data_ptr(), xs, w.data_ptr(), s.data_ptr(), offsets.data_ptr(), y.data_ptr(), xt.size(0), e, n, k, int(out is None))
+    return y
+
+
+def _no_quantised(x, qw) -> None:
     if isinstance(x, (QWeightMXFP4, QExpertsMXFP4)):
-        raise TypeError("MXFP4 activations go with MXFP4 weights, got %r" % type(qw))
+        raise TypeError("MXFP4 activations go with MXFP4 weights, got %r" % (qw if isinstance(qw, type) else type(qw)))
+    if isinstance(x, (QRowsFP8, QWeightFP8, QExpertsFP8)):
+        raise TypeError("FP8 activations go with FP8 weights, got %r" % (qw if isinstance(qw, type) else type(qw)))
+
+
+def _offsets(offsets: torch.Tensor, e: int, device: torch.device) -> torch.Tensor:
+    offsets = _dev(offsets, "offsets", torch.int32)
+    if e < 1 or tuple(offsets.shape) != (e + 1,) or offsets.device != device:
+        raise ValueError("offsets must be int32 [%d] on %s, one more than there are experts (at least one), got %s on %s"
+                         % (e + 1, device, tuple(offsets.shape), offsets.device))
+    return offsets
 
 
 def _rows_of(x: torch.Tensor, k: int, qw: QWeight) -> int:
@@ -204,26 +306,27 @@ def _rows_of(x: torch.Tensor, k: int, qw: QWeight) -> int:
     try:
         m, xk = x.shape
     except (AttributeError, ValueError):
-        _no_mxfp4(x, qw)
+        _no_quantised(x, qw)
         m, xk = 0, -1
     if xk != k:
         raise ValueError("x must be [M,%d], got %s" % (k, tuple(x.shape)))
     return m
 
 
-def qgemm_grouped(x: Union[torch.Tensor, QWeightMXFP4], experts: QExpertsMXFP4, offsets: torch.Tensor,
-                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+def qgemm_grouped(x: QRows, experts: Union[QExpertsMXFP4, QExpertsFP8], offsets: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rows sorted by expert, each group times its own matrix: y[r] = x[r] @ dequant(experts[e]).T for offsets[e] <= r < offsets[e+1].
 
-    x bf16 [R,K] or QWeightMXFP4 of R rows; offsets int32 [E+1] on the GPU, read there (groups of any size, empty ones too, no host round trip); y bf16
+    x bf16 [R,K] or, of R rows, QWeightMXFP4 (QRowsFP8 for QExpertsFP8); offsets int32 [E+1] on the GPU, read there (groups of any size, empty ones too, no host round trip); y bf16
     [R,N], fp32 sums.  Rows in front of offsets[0] and behind offsets[E] are 0 in a fresh result and left as they are in `out`.  Offsets beyond [0, R] count as its ends, one
     that descends as the largest before it."""
     if out is None:
         y = _lib.native().grouped(x, experts, offsets)
         if y is not None:
             return y
+    if isinstance(experts, QExpertsFP8):
+        return _grouped_fp8(x, experts, offsets, out)
     if not isinstance(experts, QExpertsMXFP4):
-        raise TypeError("qgemm_grouped wants QExpertsMXFP4, got %r" % type(experts))
+        raise TypeError("qgemm_grouped wants QExpertsMXFP4 or QExpertsFP8, got %r" % type(experts))
     xt, xs = _rows(x)
     x_mx = xs is not None
     p, s = _arrays(experts)
@@ -236,10 +339,7 @@ def qgemm_grouped(x: Union[torch.Tensor, QWeightMXFP4], experts: QExpertsMXFP4, 
     else:
         xt, xs_ptr = _dev(x, "x", torch.bfloat16), None
     p, s = _mxfp4(p, s, "experts", xt.device)
-    offsets = _dev(offsets, "offsets", torch.int32)
-    if e < 1 or tuple(offsets.shape) != (e + 1,) or offsets.device != xt.device:
-        raise ValueError("offsets must be int32 [%d] on %s, one more than there are experts (at least one), got %s on %s"
-                         % (e + 1, xt.device, tuple(offsets.shape), offsets.device))
+    offsets = _offsets(offsets, e, xt.device)
     y = _out(out, (xt.size(0), n), torch.bfloat16, xt.device)
     if y.numel() == 0:
         return y
@@ -250,9 +350,9 @@ def qgemm_grouped(x: Union[torch.Tensor, QWeightMXFP4], experts: QExpertsMXFP4, 
     return y
 
 
-def qgemv(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, out: Optional[torch.Tensor] = None, *, fp32_elements: bool = False) -> torch.Tensor:
+def qgemv(x: QRows, qw: QWeight, out: Optional[torch.Tensor] = None, *, fp32_elements: bool = False) -> torch.Tensor:
     """Decode product, fp32 out [M,N], M <= 16.  x is bf16 [M,K] for int4 weights, fp32 [M,K] for int8 weights, bf16 [M,K] or
-    QWeightMXFP4 for MXFP4 weights.
+    QWeightMXFP4 for MXFP4 weights, bf16 [M,K] or QRowsFP8 for FP8 weights.
 
     fp32_elements (int8 weights only): fp32 arithmetic on every activation (chadq_gemv_i8row_fp32) instead of the
     matrix-core kernel's per-block fixed point, whose error on a small activation grows with the largest one of its
@@ -276,6 +376,13 @@ def _gemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor], fp32_elemen
         if m > GEMV_MAX_M:
             raise ValueError("qgemv takes at most %d rows, got %d" % (GEMV_MAX_M, m))
         return _product_mxfp4(x, qw, out, y_dtype)
+    elif isinstance(qw, QWeightFP8):
+        if fp32_elements:
+            raise ValueError("fp32_elements applies to int8 weights (fp32 activations) only")
+        xt = x.w if isinstance(x, QRowsFP8) else x
+        if isinstance(xt, torch.Tensor) and xt.dim() == 2 and xt.size(0) > GEMV_MAX_M:
+            raise ValueError("qgemv takes at most %d rows, got %d" % (GEMV_MAX_M, xt.size(0)))
+        return _product_fp8(x, qw, out, y_dtype)
     else:
         raise TypeError("unknown weight container %r" % type(qw))
     m = _rows_of(x, k, qw)
@@ -308,8 +415,8 @@ def _gemv(x: torch.Tensor, qw: QWeight, out: Optional[torch.Tensor], fp32_elemen
     return y
 
 
-def qgemm(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Prefill product on the matrix cores: x bf16 [M,K], or QWeightMXFP4 for MXFP4 weights, -> bf16 [M,N], fp32 accumulate."""
+def qgemm(x: QRows, qw: QWeight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Prefill product on the matrix cores: x bf16 [M,K], or QWeightMXFP4 for MXFP4 weights, QRowsFP8 for FP8 ones, -> bf16 [M,N], fp32 accumulate."""
     lib = _lib.load()
     if isinstance(qw, QWeightInt4G32):
         w, s, n, k = _int4(qw)
@@ -317,6 +424,8 @@ def qgemm(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, out: Optional[torch
         w, s, n, k = _int8(qw)
     elif isinstance(qw, QWeightMXFP4):
         return _product_mxfp4(x, qw, out, torch.bfloat16)
+    elif isinstance(qw, QWeightFP8):
+        return _product_fp8(x, qw, out, torch.bfloat16)
     else:
         raise TypeError("unknown weight container %r" % type(qw))
     m = _rows_of(x, k, qw)
@@ -344,12 +453,12 @@ def qgemm(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, out: Optional[torch
     return y
 
 
-def qlinear(x: Union[torch.Tensor, QWeightMXFP4], qw: QWeight, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+def qlinear(x: QRows, qw: QWeight, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y = x @ dequant(W).T over the last axis of x.
 
     Up to 16 rows go to the bandwidth-bound GEMV (fp32 result); more rows go to the MFMA GEMM (bf16 result).
     out_dtype picks the result type.  The GEMV writes bf16 itself if that is asked for (the same sums rounded once); any
-    other type than the kernel's native one is a cast.  x may be a QWeightMXFP4, [M,K], where the weights are one.
+    other type than the kernel's native one is a cast.  x may be a QWeightMXFP4, [M,K], where the weights are one, and a QRowsFP8 where they are a QWeightFP8.
     """
     native = _lib.native()
     y = native.linear(x, qw, out_dtype)
@@ -375,7 +484,10 @@ def _qlinear_2d(x2: torch.Tensor, qw: QWeight, written: Optional[torch.dtype]) -
     if isinstance(qw, QWeightMXFP4):  # (no rows at all: an empty result, of the type that few rows have)
         few = _rows(x2)[0].size(0) <= GEMV_MAX_M
         return _product_mxfp4(x2, qw, None, torch.float32 if few and written is None else torch.bfloat16)
-    _no_mxfp4(x2, qw)
+    if isinstance(qw, QWeightFP8):
+        few = (x2.w if isinstance(x2, QRowsFP8) else x2).size(0) <= GEMV_MAX_M if isinstance(x2, (torch.Tensor, QRowsFP8)) else False
+        return _product_fp8(x2, qw, None, torch.float32 if few and written is None else torch.bfloat16)
+    _no_quantised(x2, qw)
     m = x2.size(0)
     use_gemv = m <= GEMV_MAX_M and not (isinstance(qw, QWeightInt8) and x2.dtype == torch.bfloat16)
     if isinstance(qw, QWeightInt8) and x2.dtype == torch.float32 and not use_gemv:
@@ -383,14 +495,55 @@ def _qlinear_2d(x2: torch.Tensor, qw: QWeight, written: Optional[torch.dtype]) -
     return _gemv(x2, qw, None, False, written is not None) if use_gemv else qgemm(x2, qw)
 
 
-def moe_route(logits: torch.Tensor, top_k: int = 2, renorm: bool = True):
-    """softmax over experts, top_k by logit (lowest index wins ties) -> (idx int32 [T,top_k], w fp32 [T,top_k])."""
+def _routing(top_k, renorm, score, bias, groups, top_groups, group_sum, scale):
+    """The arguments of a routing, as the library's struct has them behind the bias."""
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError("score must be 'softmax' or 'sigmoid', got %r" % (score,))
+    if bias is not None and not isinstance(bias, torch.Tensor):
+        raise TypeError("bias must be a tensor or None, got %r" % type(bias))
+    return score == "sigmoid", renorm, groups, groups if top_groups is None else top_groups, group_sum, top_k, scale
+
+
+def _bias(bias: Optional[torch.Tensor], e: int, device: torch.device) -> Optional[torch.Tensor]:
+    if bias is None:
+        return None
+    bias = _dev(bias, "bias", torch.float32)
+    if tuple(bias.shape) != (e,) or bias.device != device:
+        raise ValueError("bias must be float32 [%d] on %s, got %s on %s" % (e, device, tuple(bias.shape), bias.device))
+    return bias
+
+
+def moe_route(logits: torch.Tensor, top_k: int = 2, renorm: bool = True, *, score: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
+              top_groups: Optional[int] = None, group_sum: int = 1, scale: float = 1.0):
+    """Routing of tokens to experts, logits fp32 [T,E] -> (idx int32 [T,top_k], w fp32 [T,top_k]): the top_k experts by logit (lowest index wins
+    ties), w their softmax scores, divided by their sum if renorm.
+
+    score "sigmoid": 1 / (1 + exp(-logit)) instead.  bias fp32 [E]: the experts are chosen by score + bias, in 64 bits; w has no bias in it.  groups: E / groups
+    consecutive experts form a group, whose value is the sum of the group_sum (1 or 2) largest of what its experts are chosen by, and only the experts of the
+    top_groups largest groups may be chosen.  scale: a factor of w.  An expert whose logit is -infinity or NaN comes behind all others that may be chosen and has
+    the score 0.  E up to 512, top_k up to 32."""
+    if score == "softmax" and bias is None and groups == 1 and scale == 1.0 and logits.dim() == 2 and logits.size(1) <= 16 and top_k <= 8 and group_sum == 1 \
+            and top_groups in (None, 1):
+        z = _dev(logits, "logits", torch.float32)
+        t, e = z.shape
+        idx = torch.empty(t, top_k, dtype=torch.int32, device=z.device)
+        w = torch.empty(t, top_k, dtype=torch.float32, device=z.device)
+        _lib.check(_lib.load().chadq_moe_route(z.data_ptr(), idx.data_ptr(), w.data_ptr(), t, e, top_k, int(renorm), _stream()),
+                   "chadq_moe_route")
+        return idx, w
+    how = _routing(top_k, renorm, score, bias, groups, top_groups, group_sum, scale)
+    got = _lib.native().route(logits, bias, *how)
+    if got is not None:
+        return got
     z = _dev(logits, "logits", torch.float32)
+    if z.dim() != 2:
+        raise ValueError("logits must be [T,E], got %s" % (tuple(z.shape),))
     t, e = z.shape
-    idx = torch.empty(t, top_k, dtype=torch.int32, device=z.device)
-    w = torch.empty(t, top_k, dtype=torch.float32, device=z.device)
-    _lib.check(_lib.load().chadq_moe_route(z.data_ptr(), idx.data_ptr(), w.data_ptr(), t, e, top_k, int(renorm), _stream()),
-               "chadq_moe_route")
+    bias = _bias(bias, e, z.device)
+    idx = torch.empty(t, max(0, top_k), dtype=torch.int32, device=z.device)
+    w = torch.empty(t, max(0, top_k), dtype=torch.float32, device=z.device)
+    r = _lib.Routing(None if bias is None else bias.data_ptr(), *how)
+    _launch(z.device, "chadq_moe_route_experts", z.data_ptr(), ctypes.byref(r), idx.data_ptr(), w.data_ptr(), t, e)
     return idx, w
 
 
@@ -421,14 +574,20 @@ def to_rows(w: QWeightInt4G32Tiles) -> QWeightInt4G32:
     return QWeightInt4G32(*_repack(w, False))
 
 
-def moe_ffn(x: torch.Tensor, logits: torch.Tensor, experts, *, top_k: int = 2, renorm: bool = True) -> torch.Tensor:
+def moe_ffn(x: Union[torch.Tensor, QRowsFP8], logits: torch.Tensor, experts, *, top_k: int = 2, renorm: bool = True, score: str = "softmax",
+            bias: Optional[torch.Tensor] = None, groups: int = 1, top_groups: Optional[int] = None, group_sum: int = 1, scale: float = 1.0) -> torch.Tensor:
     """SiLU-gated mixture of experts.  x bf16 [T,H], logits fp32 [T,E]; experts: sequence of (gate, up, down)
     triples with gate/up [F,H] and down [H,F], all QWeightInt4G32 or all QWeightInt4G32Tiles (to_tiles(): faster from
     some 16 tokens on).  Dequantised weights are rounded to bf16 (row order) or fp16 (tile order), so the two orders agree within
     rounding; at most 16 tokens take exact weights in row order and, where the experts hit hold at most 64 MB, in tile order
     too, with the same bits from both.  Or experts is one triple of QExpertsMXFP4, gate and up [E,F,H] and down [E,H,F]: weights multiplied as
-    they are.  Returns bf16 [T,H]."""
+    they are.  Or one triple of QExpertsFP8, up to 512 experts, which alone take the routings of moe_route beyond softmax and top_k, and for which x may be
+    a QRowsFP8: then the hidden activations become 8-bit too, as quantize_fp8 makes them.  Returns bf16 [T,H]."""
     several = isinstance(experts, (tuple, list))
+    if several and experts and isinstance(experts[0], QExpertsFP8):
+        return _moe_ffn_fp8(x, logits, experts, _routing(top_k, renorm, score, bias, groups, top_groups, group_sum, scale), bias)
+    if score != "softmax" or bias is not None or groups != 1 or scale != 1.0 or group_sum != 1 or top_groups not in (None, 1):
+        raise ValueError("score, bias, groups and scale go with QExpertsFP8")
     if several and experts and isinstance(experts[0], QExpertsMXFP4):
         return _moe_ffn_mxfp4(x, logits, experts, top_k, renorm)
     y = _lib.native().moe_ffn(x, logits, experts, top_k, renorm)
@@ -436,6 +595,9 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, experts, *, top_k: int = 2, r
         return y
     if several and any(isinstance(m, QExpertsMXFP4) for m in experts):  # (not a triple: refused there.  Here, as a look at each of 16 experts takes 1 us)
         return _moe_ffn_mxfp4(x, logits, experts, top_k, renorm)
+    if several and any(isinstance(m, QExpertsFP8) for m in experts):
+        raise TypeError("FP8 experts are one (gate, up, down) triple of QExpertsFP8")
+    _no_quantised(x, QWeightInt4G32)
     lib = _lib.load()  # (as in qlinear)
     x = _dev(x, "x", torch.bfloat16)
     z = _dev(logits, "logits", torch.float32)
@@ -480,6 +642,7 @@ def _moe_ffn_mxfp4(x: torch.Tensor, logits: torch.Tensor, experts, top_k: int, r
         return y
     if len(experts) != 3 or not all(isinstance(m, QExpertsMXFP4) for m in experts):
         raise TypeError("MXFP4 experts are one (gate, up, down) triple of QExpertsMXFP4")
+    _no_quantised(x, type(experts[0]))
     arrays = [_arrays(m) for m in experts]
     x, z = _dev(x, "x", torch.bfloat16), _dev(logits, "logits", torch.float32)
     if x.dim() != 2:
@@ -499,4 +662,32 @@ def _moe_ffn_mxfp4(x: torch.Tensor, logits: torch.Tensor, experts, top_k: int, r
     arr = _lib.MoeMXFP4(*[v.data_ptr() for v in ts])
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)  # as moe_ffn's
     _launch(x.device, "chadq_moe_ffn_mxfp4", x.data_ptr(), z.data_ptr(), ctypes.byref(arr), y.data_ptr(), t, h, f, e, top_k, int(renorm), ws.data_ptr(), need)
+    return y
+
+
+def _moe_ffn_fp8(x: Union[torch.Tensor, QRowsFP8], logits: torch.Tensor, experts, how, bias: Optional[torch.Tensor]) -> torch.Tensor:
+    y = _lib.native().moe_ffn_fp8(x, logits, experts, bias, *how)
+    if y is not None:
+        return y
+    if len(experts) != 3 or not all(isinstance(m, QExpertsFP8) for m in experts):
+        raise TypeError("FP8 experts are one (gate, up, down) triple of QExpertsFP8")
+    (e, f, h), up, down = (tuple(m.w.shape) if m.w.dim() == 3 else (0, 0, 0) for m in experts)  # [E,F,H], the same, [E,H,F]
+    xt, xs, _keep = _fp8_rows(x, h, "T")
+    z, t = _dev(logits, "logits", torch.float32), xt.size(0)
+    if tuple(z.shape) != (t, e) or z.device != xt.device:
+        raise ValueError("logits must be [%d,%d] on %s" % (t, e, xt.device))
+    if up != (e, f, h) or down != (e, h, f):
+        raise ValueError("gate and up must be [%d,%d,%d] and down [%d,%d,%d]" % (e, f, h, e, h, f))
+    bias = _bias(bias, e, xt.device)
+    lib = _lib.load()
+    ts = [_fp8(m, name, xt.device) for name, m in zip(("gate", "up", "down"), experts)]
+    y = torch.empty(t, h, dtype=torch.bfloat16, device=xt.device)
+    top_k = how[5]
+    need = lib.chadq_moe_ffn_fp8_workspace_bytes(t, h, f, e, top_k, int(xs is not None))
+    if need == 0:
+        raise ValueError("unsupported MoE sizes T=%d H=%d F=%d E=%d top_k=%d" % (t, h, f, e, top_k))
+    arr = _lib.MoeFP8(*[w.data_ptr() for w, _ in ts], *[s.data_ptr() for _, s in ts])
+    r = _lib.Routing(None if bias is None else bias.data_ptr(), *how)
+    ws = torch.empty(need, dtype=torch.uint8, device=xt.device)  # as moe_ffn's
+    _launch(xt.device, "chadq_moe_ffn_fp8", xt.data_ptr(), xs, z.data_ptr(), ctypes.byref(r), ctypes.byref(arr), y.data_ptr(), t, h, f, e, ws.data_ptr(), need)
     return y

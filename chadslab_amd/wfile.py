@@ -4,12 +4,13 @@ memory map so that a multi-GB checkpoint is paged in by the copy to the GPU and 
 Layout (little endian):
     bytes 0..7    magic  b"CHADQW01"
     bytes 8..15   uint64 header length H
-    bytes 16..    H bytes of UTF-8 JSON: {"tensors": {name: {"kind": "i4g32" | "i8row" | "mxfp4" | "raw", "shape": [...],
+    bytes 16..    H bytes of UTF-8 JSON: {"tensors": {name: {"kind": "i4g32" | "i8row" | "mxfp4" | "fp8" | "raw", "shape": [...],
                   "arrays": {array_name: {"dtype": numpy dtype string, "shape": [...], "offset": bytes from file start,
                   "nbytes": ...}}}}, "meta": {...}}
     then the arrays, each starting on a 256-byte boundary, in the layouts of chadslab_amd.formats
     (i4g32: "packed" uint8 [N,K/2], "scale" float16 [N,K/32];  i8row: "w" int8 [N,K], "scale" float32 [N];
-     mxfp4: "packed" uint8 [N,K/2], "scale" uint8 [N,K/32], both with E in front for the matrices of experts;  raw: "data" of any dtype, e.g. norm weights).
+     mxfp4: "packed" uint8 [N,K/2], "scale" uint8 [N,K/32], both with E in front for the matrices of experts;
+     fp8: "w" [N,K] as its bytes, uint8, "scale" float32 [ceil(N/128),ceil(K/128)], experts as there;  raw: "data" of any dtype, e.g. norm weights).
 
 The reference snapshot defines no checkpoint format for this path; this one is the build's own.
 """
@@ -22,12 +23,12 @@ from typing import Dict, Union
 import numpy as np
 import torch
 
-from .formats import QExpertsMXFP4, QWeightInt4G32, QWeightInt8, QWeightMXFP4
+from .formats import FP8, QExpertsFP8, QExpertsMXFP4, QWeightFP8, QWeightInt4G32, QWeightInt8, QWeightMXFP4
 
 MAGIC = b"CHADQW01"
 ALIGN = 256
 
-Entry = Union[QWeightInt4G32, QWeightInt8, QWeightMXFP4, QExpertsMXFP4, torch.Tensor, np.ndarray]
+Entry = Union[QWeightInt4G32, QWeightInt8, QWeightMXFP4, QExpertsMXFP4, QWeightFP8, QExpertsFP8, torch.Tensor, np.ndarray]
 
 
 def _np(t) -> np.ndarray:
@@ -40,7 +41,7 @@ def _np(t) -> np.ndarray:
 
 
 def _shape(e: Entry):
-    return [e.E, e.N, e.K] if isinstance(e, QExpertsMXFP4) else [e.N, e.K]
+    return [e.E, e.N, e.K] if isinstance(e, (QExpertsMXFP4, QExpertsFP8)) else [e.N, e.K]
 
 
 def _arrays(e: Entry):
@@ -50,6 +51,8 @@ def _arrays(e: Entry):
         return "i8row", [e.N, e.K], {"w": _np(e.w), "scale": _np(e.scale)}
     if isinstance(e, (QWeightMXFP4, QExpertsMXFP4)):
         return "mxfp4", _shape(e), {"packed": _np(e.packed), "scale": _np(e.scale)}
+    if isinstance(e, (QWeightFP8, QExpertsFP8)):
+        return "fp8", _shape(e), {"w": _np(e.w.view(torch.uint8)), "scale": _np(e.scale)}
     a = _np(e)
     if a.dtype.hasobject:
         raise TypeError("a weight file holds quantized weights and plain tensors, got %r" % type(e))
@@ -139,6 +142,8 @@ def load(path: str, device="cpu") -> Dict[str, Entry]:
             out[name] = QWeightInt8(arrs["w"], arrs["scale"])
         elif t["kind"] == "mxfp4":
             out[name] = (QExpertsMXFP4 if arrs["packed"].dim() == 3 else QWeightMXFP4)(arrs["packed"], arrs["scale"])
+        elif t["kind"] == "fp8":
+            out[name] = (QExpertsFP8 if arrs["w"].dim() == 3 else QWeightFP8)(arrs["w"].view(FP8), arrs["scale"])
         elif t["kind"] == "raw":
             out[name] = arrs["data"]
         else:

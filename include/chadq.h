@@ -456,6 +456,69 @@ size_t chadq_moe_ffn_mxfp4_workspace_bytes(int T, int H, int F, int E, int top_k
 int chadq_moe_ffn_mxfp4(const uint16_t *x_bf16, const float *logits, const chadq_moe_mxfp4 *experts, uint16_t *y_bf16, int T, int H, int F, int E, int top_k,
                         int renorm, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- 8-bit floating point (FP8) with a scale for each block of 128 ----------------------- */
+
+/*
+ * Format: values e4m3, one to a byte, row-major [N,K], K % 16 == 0: sign, 4 bits of exponent (bias 7), 3 of mantissa; largest 448, 0x7F and 0xFF NaN.
+ * Scales fp32, by blocks of 128 from the first row and the first k on, the last ones cut: of weights [ceil(N/128), ceil(K/128)], of activations, by_row,
+ * [N, ceil(K/128)].  A number is its value times its block's scale.
+ */
+
+/*
+ * x [matrices,N,K] of the given chadq_dtype -> values and scales.  Per block, a = max(max |x|, 448 * 2^-126): scale = a / 448, r = 448 / a, value = the nearest
+ * e4m3 to x r, ties to the even one, each of the three operations in fp32.  A block with a NaN or an infinity: scale NaN, values 0.  x and values 16-byte aligned.
+ */
+int chadq_quantize_fp8(const void *x, int dtype, uint8_t *values, float *scale, int64_t matrices, int N, int K, int by_row, void *stream);
+
+/* fp32 [matrices,N,K] of values and scales, one rounding.  w and values 16-byte aligned. */
+int chadq_dequant_fp8(const uint8_t *values, const float *scale, float *w, int64_t matrices, int N, int K, int by_row, void *stream);
+
+/*
+ * y[m,n] = sum over blocks b of x_scale[m,b] w_scale[n/128,b] sum_{k in b} x[m,k] w[n,k]: a block's sum in fp32 of exact products, its scales multiplied with each
+ * other in fp32, one FMA to the result; y fp32 or (y_bf16) the same rounded once.  x_scale NULL: x is bf16 [M,K], multiplied as it is, with no scale; else x holds
+ * values [M,K].  M, N >= 0; K a positive multiple of 16 up to 2^26; x and w 16-byte aligned.  NaN and infinities act as IEEE has them.  workspace:
+ * chadq_product_fp8_workspace_bytes bytes (16-byte aligned; 0: none needed), for the sums of parts of K where that is the quicker form; without it (NULL or
+ * fewer bytes) the product is one part.
+ */
+size_t chadq_product_fp8_workspace_bytes(int M, int N, int K, int x_fp8);
+int chadq_product_fp8(const void *x, const float *x_scale, const uint8_t *w, const float *w_scale, void *y, int y_bf16, int M, int N, int K, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/*
+ * The same for rows sorted by group, each group times its own matrix: w [E,N,K], w_scale [E,ceil(N/128),ceil(K/128)]; offsets, rows of no group, clear_rest and
+ * the number of tiles as in chadq_product_mxfp4_grouped.  y bf16 [M,N].
+ */
+int chadq_product_fp8_grouped(const void *x, const float *x_scale, const uint8_t *w, const float *w_scale, const int32_t *offsets, uint16_t *y_bf16, int M, int E,
+                              int N, int K, int clear_rest, void *stream);
+
+/*
+ * Routing of tokens to up to 512 experts.  The score s of an expert is softmax(logits) or, sigmoid, 1 / (1 + exp(-logit)).  It is chosen by c = s + bias[e] (bias
+ * NULL: 0), in 64 bits; by its logit where bias is NULL and group_sum is 1.  The experts form `groups` groups of consecutive ones; a group's value is the sum of its
+ * group_sum (1 or 2) largest c, and the experts of the top_groups groups of the largest value may be chosen: the top_k of the largest c among them, in that order.
+ * Ties go to the lowest index.  weight = s, divided by the sum of the chosen ones if renorm (0 where that is 0), times scale.  An expert whose logit is -infinity
+ * or NaN comes behind all others that may be chosen and has the score 0.
+ * E <= 512, groups <= 64 and a divisor of E, group_sum <= E / groups, top_groups <= groups, top_k <= min(32, top_groups * E / groups).
+ */
+typedef struct chadq_routing {
+    const float *bias; /* [E] on the device, or NULL */
+    int sigmoid, renorm, groups, top_groups, group_sum, top_k;
+    float scale;
+} chadq_routing;
+int chadq_moe_route_experts(const float *logits, const chadq_routing *routing, int32_t *idx, float *w, int T, int E, void *stream);
+
+/*
+ * Mixture-of-experts FFN on FP8 experts: routing as above, y[t] = bf16( sum_j w[t,j] down_e( h ) ), h = silu(gate_e x_t) * (up_e x_t).  gate, up [E,F,H], down
+ * [E,H,F], values and scales of the E matrices one behind the other.  x_scale NULL: x bf16 [T,H] and h rounded to bf16; else x holds values [T,H] and h becomes
+ * 8-bit as chadq_quantize_fp8 by_row does it.  H, F multiples of 16.  workspace: chadq_moe_ffn_fp8_workspace_bytes bytes (0: sizes that are not served).
+ */
+typedef struct chadq_moe_fp8 {
+    const uint8_t *gate, *up, *down;
+    const float *gate_scale, *up_scale, *down_scale;
+} chadq_moe_fp8;
+size_t chadq_moe_ffn_fp8_workspace_bytes(int T, int H, int F, int E, int top_k, int x_fp8);
+int chadq_moe_ffn_fp8(const void *x, const float *x_scale, const float *logits, const chadq_routing *routing, const chadq_moe_fp8 *experts, uint16_t *y_bf16, int T,
+                      int H, int F, int E, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -303,6 +303,75 @@ def dequant_mxfp4(codes: np.ndarray, scale: np.ndarray) -> np.ndarray:
     return v * np.repeat(s, 32, axis=-1)
 
 
+def e4m3_values() -> np.ndarray:
+    """float64 [256]: the value of each byte."""
+    b = np.arange(256)
+    e, m = (b >> 3) & 15, (b & 7) / 8.0
+    v = np.where(e == 0, np.ldexp(m, -6), np.ldexp(1 + m, e - 7))
+    return np.where(b & 127 == 127, np.nan, np.where(b & 128, -v, v))
+
+
+def _blocks(x: np.ndarray, high: int):
+    """[N,K] -> the block of each element: row of blocks, column of blocks."""
+    n, k = x.shape
+    return np.arange(n)[:, None] // high, np.arange(k)[None, :] // 128
+
+
+def quantize_fp8(x: np.ndarray, high: int):
+    """Floats [N,K] -> (bytes uint8 [N,K], scales fp32 [ceil(N/high),ceil(K/128)]), blocks of `high` rows and 128 k.  a = max(max |x|, 448 * 2^-126), scale = a / 448,
+    value = nearest e4m3 of x * (448 / a), ties to the even byte; divisions and product in fp32.  A block with a NaN or an infinity: scale NaN, bytes 0."""
+    x = np.asarray(x, dtype=np.float32)
+    n, k = x.shape
+    a = np.zeros((-(-n // high), -(-k // 128)), np.float32)
+    for i in range(a.shape[0]):
+        for j in range(a.shape[1]):
+            a[i, j] = np.abs(x[i * high:(i + 1) * high, j * 128:(j + 1) * 128]).max()  # (a NaN stays one)
+    bad = ~np.isfinite(a)
+    a = np.where(bad, np.float32(1), np.maximum(a, np.float32(448 * 2.0 ** -126)))
+    r = np.float32(448) / a
+    i, j = _blocks(x, high)
+    v = (np.where(bad[i, j], np.float32(0), x) * r[i, j]).astype(np.float64)
+    values = e4m3_values()[:127]
+    up = np.searchsorted(values, np.abs(v)).clip(1, 126)
+    low, high_ = np.abs(v) - values[up - 1], values[up] - np.abs(v)
+    c = np.where((low < high_) | ((low == high_) & ((up - 1) % 2 == 0)), up - 1, up)
+    c = np.where(bad[i, j], 0, c | (np.signbit(v).astype(np.int64) << 7)).astype(np.uint8)
+    return c, np.where(bad, np.float32(np.nan), a / np.float32(448)).astype(np.float32)
+
+
+def dequant_fp8(b: np.ndarray, scale: np.ndarray, high: int) -> np.ndarray:
+    """float64 [N,K] of bytes and scales."""
+    i, j = _blocks(b, high)
+    return e4m3_values()[b] * scale.astype(np.float64)[i, j]
+
+
+def moe_route_experts(logits, top_k, renorm=True, score="softmax", bias=None, groups=1, top_groups=1, group_sum=1, scale=1.0):
+    """Token by token in 64 bits, as chadq.h defines it -> (idx int32 [T,top_k], w float64 [T,top_k])."""
+    logits = np.asarray(logits, dtype=np.float64)
+    t, e = logits.shape
+    idx, w = np.zeros((t, top_k), np.int32), np.zeros((t, top_k))
+    for i, z in enumerate(logits):
+        masked = ~(z > -np.inf)
+        z = np.where(masked, -np.inf, z)
+        with np.errstate(over="ignore", invalid="ignore"):
+            s = np.exp(z - z.max()) if score == "softmax" else 1 / (1 + np.exp(-z))
+            if score == "softmax":
+                s = s / s[~masked].sum() if not masked.all() else s
+        s = np.where(masked, 0.0, s)
+        c = z if bias is None and group_sum == 1 else s + (0 if bias is None else np.asarray(bias, np.float64))
+        per = e // groups
+        # (masked first, so that a plain sort puts them behind everything)
+        order = lambda members: sorted(members, key=lambda j: (masked[j], -c[j] if not masked[j] else 0.0, j))
+        value = [tuple((not masked[j], c[j] if not masked[j] else 0.0) for j in order(range(g * per, (g + 1) * per))[:group_sum]) for g in range(groups)]
+        size = lambda v: (sum(a for a, _ in v), sum(b for _, b in v))
+        kept = sorted(range(groups), key=lambda g: (tuple(-x for x in size(value[g])), g))[:top_groups]
+        taken = order(j for g in kept for j in range(g * per, (g + 1) * per))[:top_k]
+        idx[i], w[i] = taken, s[taken]
+        if renorm and w[i].sum() > 0:
+            w[i] /= w[i].sum()
+    return idx, w * scale
+
+
 def rel_l2(a: np.ndarray, ref: np.ndarray) -> float:
     a = np.asarray(a, dtype=np.float64)
     ref = np.asarray(ref, dtype=np.float64)
