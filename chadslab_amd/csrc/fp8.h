@@ -37,6 +37,8 @@ struct Fp8Product {
 
 constexpr int kFp8MostK = 1 << 26;  // bytes of an activation row are counted in 32 bits
 
+bool fp8_streams(const Fp8Product &p);
+int fp8_stream_launch(const Fp8Product &p, hipStream_t st);
 int fp8_product_launch(const Fp8Product &p, void *workspace, size_t workspace_bytes, hipStream_t st);
 size_t fp8_product_workspace_bytes(int M, int N, int K, bool x_fp8);
 

@@ -64,6 +64,7 @@ __global__ __launch_bounds__(256) void fp8_product_kernel(Fp8Product p) {
 }
 
 int fp8_product_launch(const Fp8Product &p, void *workspace, size_t workspace_bytes, hipStream_t st) {
+    if (fp8_streams(p)) return fp8_stream_launch(p, st);
     const int64_t tiles = p.offsets ? mx_most_tiles(p.M, p.E, 16) : mx_ceil(p.M, 16), cols = mx_ceil(p.N, 64);
     if (tiles > (1 << 22) || cols > 65535) return fail(CHADQ_ERR_SHAPE, "fp8 product: M=%d N=%d are too many tiles", p.M, p.N);
     const dim3 grid((int)tiles, (int)cols);
