@@ -33,12 +33,18 @@ struct Fp8Product {
     int x_rows = 0;           // ... which has so many
     const uint8_t *w2 = nullptr;
     const float *w2s = nullptr;
+    // K in parts of part_k (a multiple of 1024; 0: one part), the sums of part i as fp32 [M,N] from y + i M N on
+    int part_k = 0;
+    int parts() const { return part_k ? (K + part_k - 1) / part_k : 1; }
 };
 
 constexpr int kFp8MostK = 1 << 26;  // bytes of an activation row are counted in 32 bits
 
 bool fp8_streams(const Fp8Product &p);
 int fp8_stream_launch(const Fp8Product &p, hipStream_t st);
+enum Fp8Tile { F8_64x32, F8_64x64, F8_128x64, F8_256x64, F8_128x128, F8_256x128, F8_256x256, F8_TILES };  // weight rows x activation rows
+bool fp8_tile_ok(const Fp8Product &p);
+int fp8_tile_launch(const Fp8Product &p, int tile, hipStream_t st);
 int fp8_product_launch(const Fp8Product &p, void *workspace, size_t workspace_bytes, hipStream_t st);
 size_t fp8_product_workspace_bytes(int M, int N, int K, bool x_fp8);
 

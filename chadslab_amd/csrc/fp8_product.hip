@@ -1,4 +1,5 @@
 // Products on FP8 weights: a wave takes 16 weight rows and 16 activation rows, its operands straight from memory, as bf16 (exact).
+#include <cstdlib>
 #include "fp8.h"
 
 namespace chadq {
@@ -64,7 +65,9 @@ __global__ __launch_bounds__(256) void fp8_product_kernel(Fp8Product p) {
 }
 
 int fp8_product_launch(const Fp8Product &p, void *workspace, size_t workspace_bytes, hipStream_t st) {
-    if (fp8_streams(p)) return fp8_stream_launch(p, st);
+    static const char *const tile = getenv("F8TILE");
+    if (!(tile && atoi(tile) >= 100) && fp8_streams(p)) return fp8_stream_launch(p, st);
+    if (fp8_tile_ok(p) && !(tile && atoi(tile) < 0)) return fp8_tile_launch(p, tile ? atoi(tile) % 100 : p.M > 256 ? F8_256x256 : p.M > 64 ? F8_256x128 : F8_128x64, st);
     const int64_t tiles = p.offsets ? mx_most_tiles(p.M, p.E, 16) : mx_ceil(p.M, 16), cols = mx_ceil(p.N, 64);
     if (tiles > (1 << 22) || cols > 65535) return fail(CHADQ_ERR_SHAPE, "fp8 product: M=%d N=%d are too many tiles", p.M, p.N);
     const dim3 grid((int)tiles, (int)cols);
