@@ -65,8 +65,8 @@ struct Source {
     int tid, lane, wave, s0, kend, steps, nrows;  // s0: first step of the workgroup's part of K; nrows: result columns that there are
     __amdgpu_buffer_rsrc_t wrsrc, w2rsrc, xrsrc;
     uint32_t off[C::REQ];
-    int place[C::REQ];  // of the lane's piece in its row and step
-    const float *srow;
+    int wplace, xplace;  // of the lane's piece in a part of a row: the rows of a wave's requests of a kind are a multiple of 16 apart
+    const __attribute__((address_space(1))) float *srow;
     int whole;
     float sv[C::GE], tail[C::GE];
     static constexpr uint32_t kOut = 0x80000000u;
@@ -85,28 +85,30 @@ struct Source {
         w2rsrc = C::GATED ? __builtin_amdgcn_make_buffer_rsrc(uniform(p.w2 + wfirst * wbytes), 0, uniform(nrows * wbytes), 0x00020000) : wrsrc;
         xrsrc = __builtin_amdgcn_make_buffer_rsrc(uniform(reinterpret_cast<const uint8_t *>(p.x) + (p.rows ? (size_t)0 : (size_t)t.row0 * xbytes)), 0,
                                                   uniform((p.rows ? p.x_rows : t.rows) * xbytes), 0x00020000);
+        static_assert(C::NW * 64 / (C::WROW / 16) % 16 == 0 && C::NW * 8 % 16 == 0, "rows of a wave's requests");
+        wplace = 16 * ((lane % (C::WROW / 16)) ^ key<C::WROW>(row_of(0)));
+        xplace = 16 * ((lane % 8) ^ key<128>(row_of(C::WI)));
 #pragma unroll
         for (int q = 0; q < C::REQ; ++q) {
-            const bool isw = q < C::WI;
-            const int row = isw ? C::WROW : 128, ppr = row / 16, height = isw ? C::TN : C::TM;
-            const int e = ((isw ? q : q - C::WI) * C::NW + wave) * (64 / ppr) + lane / ppr, r = e % height;
-            place[q] = e / height * (isw || C::X8 ? 128 : 256) + 16 * ((lane % ppr) ^ (isw ? key<C::WROW>(r) : key<128>(r)));
-            if (isw) {
-                off[q] = wrow(r) < nrows ? (uint32_t)wrow(r) * (uint32_t)wbytes + place[q] : kOut;
+            const int e = row_of(q);
+            if (q < C::WI) {
+                const int r = wrow(e % C::TN);
+                off[q] = r < nrows ? (uint32_t)r * (uint32_t)wbytes + wplace : kOut;
             } else {
-                const int src = r < t.rows ? (p.rows ? p.rows[t.row0 + r] : r) : 0;
-                off[q] = r < t.rows && e < C::TM * C::XPARTS ? (uint32_t)src * (uint32_t)xbytes + place[q] : kOut;
+                const int r = e % C::TM, src = r < t.rows ? (p.rows ? p.rows[t.row0 + r] : r) : 0;
+                off[q] = r < t.rows && e < C::TM * C::XPARTS ? (uint32_t)src * (uint32_t)xbytes + xplace : kOut;
             }
         }
         // scales.  Those of the last group, if it is no whole one, are loaded one by one before the loop (zeros behind the end of the row, where the activations
         // are zeros too).  No branch: a thread without a row loads another one's and writes where nobody reads, and so does the loop behind the last whole group.
         const int G = fp8_blocks(p.K), GN = fp8_blocks(p.N), r = tid < C::SROWS ? tid : 0;
+        auto global = [](const float *p) { return (const __attribute__((address_space(1))) float *)p; };
         if (C::X8 && r < C::TM) {
             const int m = t.row0 + (r < t.rows ? r : t.rows - 1);
-            srow = p.xs + (size_t)(p.rows ? p.rows[m] : m) * G;
+            srow = global(p.xs) + (size_t)(p.rows ? p.rows[m] : m) * G;
         } else {
             const int j = r - (C::X8 ? C::TM : 0), nb = (n0 >> 7) + (C::GATED ? 0 : j);
-            srow = (C::GATED && j ? p.w2s : p.ws) + ((size_t)t.group * GN + (nb < GN ? nb : GN - 1)) * G;
+            srow = global(C::GATED && j ? p.w2s : p.ws) + ((size_t)t.group * GN + (nb < GN ? nb : GN - 1)) * G;
         }
         whole = G / C::GE;
 #pragma unroll
@@ -115,7 +117,11 @@ struct Source {
 #pragma unroll
             for (int e = 0; e < C::GE; ++e)
                 if (whole * C::GE + e < G) tail[e] = srow[whole * C::GE + e];
-        if (whole == 0) srow = kNoScales;  // (readable, for the loop)
+        if (whole == 0) srow = global(kNoScales);  // (readable, for the loop)
+    }
+    // the lane's row of request q, all parts' rows counted
+    __device__ __forceinline__ int row_of(int q) const {
+        return q < C::WI ? (q * C::NW + wave) * (1024 / C::WROW) + lane / (C::WROW / 16) : ((q - C::WI) * C::NW + wave) * 8 + lane / 8;
     }
     // row r of the tile's weights: of which matrix, which row behind n0
     __device__ __forceinline__ static bool second(int r) { return C::GATED && (r >> 5 & 1); }
@@ -123,9 +129,9 @@ struct Source {
 
     __device__ __forceinline__ void request(int q, int step, uint8_t *stage) const {
         const bool isw = q < C::WI;
-        const int k0 = C::X8 ? (s0 + step) * C::SK : (s0 + step) / 2 * (2 * C::SK) + (step & 1) * 64, soff = isw || C::X8 ? k0 : k0 * 2;
-        const uint32_t o = soff + place[q] < kend * (isw || C::X8 ? 1 : 2) ? off[q] : kOut;
-        const int row = ((isw ? q : q - C::WI) * C::NW + wave) * (1024 / (isw ? C::WROW : 128));
+        const int row = ((isw ? q : q - C::WI) * C::NW + wave) * (1024 / (isw ? C::WROW : 128)), part = row / (isw ? C::TN : C::TM);  // (the same for the wave)
+        const int k0 = C::X8 ? (s0 + step) * C::SK + part * 128 : (s0 + step) / 2 * (2 * C::SK) + (step & 1) * 64 + part * 128, soff = isw || C::X8 ? k0 : k0 * 2;
+        const uint32_t o = (isw ? wplace : xplace) < (isw || C::X8 ? kend : kend * 2) - soff ? off[q] : kOut;
         const bool two = isw && C::GATED && second(row % C::TN);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(isw ? (two ? w2rsrc : wrsrc) : xrsrc, (__attribute__((address_space(3))) void *)(stage + (q * C::NW + wave) * 1024), 16, o, soff,
                                                  0, 0);
@@ -133,7 +139,10 @@ struct Source {
     // group: of two steps, counted from the part's first
     __device__ __forceinline__ void scales(int group) {
         const int g = s0 / 2 + group, at = (g < whole ? g : whole > 0 ? whole - 1 : 0) * C::GE;
-        __builtin_memcpy(sv, srow + at, 4 * C::GE);
+        typedef float group_t __attribute__((ext_vector_type(C::GE), aligned(4)));
+        const group_t v = *(const __attribute__((address_space(1))) group_t *)(srow + at);
+#pragma unroll
+        for (int e = 0; e < C::GE; ++e) sv[e] = v[e];
     }
     __device__ __forceinline__ void keep(int group) const {
         float *const d = reinterpret_cast<float *>(lds + (tid < C::SROWS ? C::S_OFF + (group & 1) * C::S_GROUP + tid * 4 : C::DUMP + lane * 4));
@@ -180,19 +189,22 @@ __device__ __forceinline__ void sum_fp8(Source<C> &src, f32x4 (&acc)[2 * C::NB][
     float s[2][SW][M];
     auto read_w = [&](int pair, int j, int buf, const uint8_t *stage) { wf[buf][j] = fragment(stage + wl + (pair * 2 + j) * 2048); };
     auto read_x = [&](int b, const uint8_t *stage) { xf[b] = fragment(stage + xl + b * 2048); };
-    auto read_s = [&](int step, int par) {
+    float sw[SW], sx[M];  // of the next step
+    auto read_s = [&](int step) {
         const int e = (step & 1) * C::WK + wk;
-        float w[SW];
 #pragma unroll
-        for (int j = 0; j < SW; ++j) w[j] = src.scale(step >> 1, e, C::TM + (C::GATED ? j : (wn * C::NB * 32) >> 7));
+        for (int j = 0; j < SW; ++j) sw[j] = src.scale(step >> 1, e, C::TM + (C::GATED ? j : (wn * C::NB * 32) >> 7));
 #pragma unroll
-        for (int b = 0; b < M; ++b) {
-            const float x = src.scale(step >> 1, e, wm * C::MB * 32 + b * 16 + l16);
-#pragma unroll
-            for (int j = 0; j < SW; ++j) s[par][j][b] = x * w[j];
-        }
+        for (int b = 0; b < M; ++b) sx[b] = src.scale(step >> 1, e, wm * C::MB * 32 + b * 16 + l16);
     };
-    read_s(0, 0);
+    auto multiply_s = [&](int par) {
+#pragma unroll
+        for (int b = 0; b < M; ++b)
+#pragma unroll
+            for (int j = 0; j < SW; ++j) s[par][j][b] = sx[b] * sw[j];
+    };
+    read_s(0);
+    multiply_s(0);
 #pragma unroll
     for (int b = 0; b < M; ++b) read_x(b, lds);
 #pragma unroll
@@ -220,8 +232,9 @@ __device__ __forceinline__ void sum_fp8(Source<C> &src, f32x4 (&acc)[2 * C::NB][
     constexpr int LATE = (PAIRS - 1) * NE;  // MFMAs of a step in front of its barrier
     auto step = [&](int i, auto par_c) {
         constexpr int par = decltype(par_c)::value;
-        uint8_t *const cur = lds + slot * C::STAGE, *const nxt = lds + (slot + 1 == ST ? 0 : slot + 1) * C::STAGE;
-        uint8_t *const prv = lds + (slot == 0 ? ST - 1 : slot - 1) * C::STAGE;
+        const int at_slot = ST == 2 ? par : slot;
+        uint8_t *const cur = lds + at_slot * C::STAGE, *const nxt = lds + (at_slot + 1 == ST ? 0 : at_slot + 1) * C::STAGE;
+        uint8_t *const prv = lds + (at_slot == 0 ? ST - 1 : at_slot - 1) * C::STAGE;
         auto pair = [&](auto pc) {
             constexpr int P = decltype(pc)::value, buf = (par * PAIRS + P) & 1;
             constexpr bool late = P == PAIRS - 1;
@@ -242,7 +255,8 @@ __device__ __forceinline__ void sum_fp8(Source<C> &src, f32x4 (&acc)[2 * C::NB][
                 } else {
                     if constexpr (e == 0 || e == M) read_w(0, e / M, buf ^ 1, nxt);
                     if constexpr (j == 1) read_x(b, nxt);
-                    if constexpr (e == LAG) read_s(i + 1, par ^ 1);
+                    if constexpr (e == 0) read_s(i + 1);
+                    if constexpr (e == NE - 1) multiply_s(par ^ 1);  // (the last use of the step before's was LAG MFMAs into this one)
                 }
                 const int pos = at + (late ? -LATE : NP - LATE);
 #pragma unroll
@@ -334,8 +348,9 @@ __device__ __forceinline__ void sum_bf16(Source<C> &src, f32x16 (&acc)[C::NB][C:
     constexpr int NE = NB * MB, NP = SL * NE, LATE = (SL - AH) * NE;  // MFMAs of a slice, of a step, of a step in front of its barrier
     auto step = [&](int i, auto par_c) {
         constexpr int par = decltype(par_c)::value;
-        uint8_t *const cur = lds + slot * C::STAGE, *const nxt = lds + (slot + 1 == ST ? 0 : slot + 1) * C::STAGE;
-        uint8_t *const prv = lds + (slot == 0 ? ST - 1 : slot - 1) * C::STAGE;
+        const int at_slot = ST == 2 ? par : slot;
+        uint8_t *const cur = lds + at_slot * C::STAGE, *const nxt = lds + (at_slot + 1 == ST ? 0 : at_slot + 1) * C::STAGE;
+        uint8_t *const prv = lds + (at_slot == 0 ? ST - 1 : at_slot - 1) * C::STAGE;
         auto slice = [&](auto sc) {
             constexpr int s = decltype(sc)::value, at = par * SL + s;  // (fragment buffers in turn over two steps)
             constexpr bool first = s == 0 && par == 0;                 // of a block
