@@ -40,11 +40,17 @@ struct Fp8Product {
 
 constexpr int kFp8MostK = 1 << 26;  // bytes of an activation row are counted in 32 bits
 
+enum Fp8Tile { F8_64x32, F8_64x64, F8_128x64, F8_256x64, F8_128x128, F8_256x128, F8_256x256, F8_TILES };  // weight rows x activation rows
+struct Fp8TilePick {
+    int tile, part_k;  // 0: one part
+};
+constexpr int kFp8Parts = 8, kFp8GroupParts = 4;  // parts of K at most, of a product by group (which its caller joins)
 bool fp8_streams(const Fp8Product &p);
 int fp8_stream_launch(const Fp8Product &p, hipStream_t st);
-enum Fp8Tile { F8_64x32, F8_64x64, F8_128x64, F8_256x64, F8_128x128, F8_256x128, F8_256x256, F8_TILES };  // weight rows x activation rows
 bool fp8_tile_ok(const Fp8Product &p);
+Fp8TilePick fp8_tile_pick(const Fp8Product &p, int most_parts);
 int fp8_tile_launch(const Fp8Product &p, int tile, hipStream_t st);
+int fp8_product_part_k(const Fp8Product &p, int most_parts);
 int fp8_product_launch(const Fp8Product &p, void *workspace, size_t workspace_bytes, hipStream_t st);
 size_t fp8_product_workspace_bytes(int M, int N, int K, bool x_fp8);
 

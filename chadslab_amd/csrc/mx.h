@@ -181,6 +181,7 @@ constexpr int kMxParts = 8, kMxGroupParts = 4;  // parts of K at most, of a prod
 MxTilePick mx_tile_pick(const MxProduct &p, int most_parts);
 int mx_tile_launch(const MxProduct &p, int tile, hipStream_t st);
 int mx_tile_parts_launch(const MxProduct &p, int tile, float *part, hipStream_t st);
+int mx_join_launch(const float *part, void *y, int64_t n, int parts, bool y_bf16, hipStream_t st);
 int mx_product_part_k(const MxProduct &p, int most_parts);
 int mx_product_launch(const MxProduct &p, void *workspace, size_t workspace_bytes, hipStream_t st);
 size_t mx_product_workspace_bytes(int M, int N, int K, bool x_mxfp4);

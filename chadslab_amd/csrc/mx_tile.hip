@@ -535,6 +535,13 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const float *__restrict__ 
     }
 }
 
+int mx_join_launch(const float *part, void *y, int64_t n, int parts, bool y_bf16, hipStream_t st) {
+    const bool quads = n % 4 == 0 && aligned16(y);
+    const int64_t items = quads ? n / 4 : n;
+    hipLaunchKernelGGL(mx_join_kernel, dim3((int)(items < 2048 * 256 ? (items + 255) / 256 : 2048)), dim3(256), 0, st, part, y, n, parts, y_bf16, quads);
+    return hip_check(hipGetLastError(), "join launch");
+}
+
 // The product in its parts of K: fp32 sums to `part`, joined into y
 int mx_tile_parts_launch(const MxProduct &p, int tile, float *part, hipStream_t st) {
     MxProduct q = p;
@@ -542,11 +549,7 @@ int mx_tile_parts_launch(const MxProduct &p, int tile, float *part, hipStream_t 
     q.y_bf16 = false;
     const int rc = mx_tile_launch(q, tile, st);
     if (rc) return rc;
-    const int64_t n = (int64_t)p.M * p.N;
-    const bool quads = n % 4 == 0 && aligned16(p.y);
-    const int64_t items = quads ? n / 4 : n;
-    hipLaunchKernelGGL(mx_join_kernel, dim3((int)(items < 2048 * 256 ? (items + 255) / 256 : 2048)), dim3(256), 0, st, part, p.y, n, q.parts(), p.y_bf16, quads);
-    return hip_check(hipGetLastError(), "mxfp4 join launch");
+    return mx_join_launch(part, p.y, (int64_t)p.M * p.N, q.parts(), p.y_bf16, st);
 }
 
 }  // namespace chadq
