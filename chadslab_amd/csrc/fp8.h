@@ -16,6 +16,56 @@ __device__ __forceinline__ u32x2 fp8_to_bf16(uint32_t w) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true))};
 }
 
+// Quantisation of a block with a = max(max |x|, 448 * 2^-126):
+//   scale = a / 448,  r = 448 / a  (fp32 divisions),  value = the nearest e4m3 to x r (one fp32 product), ties to the even one.
+// |x r| <= 448 (1 + 2^-23), which goes to 448: nothing saturates.  The least a keeps scale and r normal numbers.  A block that holds a NaN or an
+// infinity gets a NaN for its scale and values of 0.
+constexpr float kFp8Least = 448.f * 0x1p-126f;
+
+__device__ __forceinline__ uint32_t absmax8(const float f[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t b = __float_as_uint(f[j]) & 0x7FFFFFFFu;  // as integers: a NaN is larger than infinity
+        m = b > m ? b : m;
+    }
+    return m;
+}
+
+struct Fp8Scale {
+    float scale, r;
+    bool bad;
+    __device__ __forceinline__ explicit Fp8Scale(uint32_t most) {
+        bad = most >= 0x7F800000u;
+        const float m = __uint_as_float(most), a = m > kFp8Least ? m : kFp8Least;
+        scale = bad ? __uint_as_float(0x7FC00000u) : a / 448.f;
+        r = 448.f / a;
+    }
+    __device__ __forceinline__ u32x2 values(const float f[8]) const {
+        int lo = 0, hi = 0;
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * r, f[1] * r, lo, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * r, f[3] * r, lo, true);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * r, f[5] * r, hi, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * r, f[7] * r, hi, true);
+        return bad ? u32x2{0, 0} : u32x2{(uint32_t)lo, (uint32_t)hi};
+    }
+};
+
+// over 16 lanes next to each other
+__device__ __forceinline__ uint32_t max_of_16(uint32_t m) {
+#define CHADQ_MAX_STEP(CTRL)                                                                                \
+    {                                                                                                       \
+        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, CTRL, 0xF, 0xF, false);         \
+        m = o > m ? o : m;                                                                                  \
+    }
+    CHADQ_MAX_STEP(0xB1)   // quad_perm [1,0,3,2]
+    CHADQ_MAX_STEP(0x4E)   // quad_perm [2,3,0,1]
+    CHADQ_MAX_STEP(0x141)  // row_half_mirror
+    CHADQ_MAX_STEP(0x140)  // row_mirror
+#undef CHADQ_MAX_STEP
+    return m;
+}
+
 // y[r, n] = sum over blocks b of xs[r, b] ws[g(r), n / 128, b] sum_{k in b} x[r, k] w[g(r), n, k] for the rows r of group g(r) = the g with
 // offsets[g] <= r < offsets[g + 1]
 struct Fp8Product {
@@ -33,6 +83,9 @@ struct Fp8Product {
     int x_rows = 0;           // ... which has so many
     const uint8_t *w2 = nullptr;
     const float *w2s = nullptr;
+    // ... with 8-bit x and more rows than are streamed also in 8 bits: values [M,N], scales [M,ceil(N/128)] (then y is not written)
+    uint8_t *h8 = nullptr;
+    float *h8s = nullptr;
     // K in parts of part_k (a multiple of 1024; 0: one part), the sums of part i as fp32 [M,N] from y + i M N on
     int part_k = 0;
     int parts() const { return part_k ? (K + part_k - 1) / part_k : 1; }
@@ -40,13 +93,15 @@ struct Fp8Product {
 
 constexpr int kFp8MostK = 1 << 26;  // bytes of an activation row are counted in 32 bits
 
-enum Fp8Tile { F8_64x32, F8_64x64, F8_128x64, F8_256x64, F8_128x128, F8_256x128, F8_256x256, F8_TILES };  // weight rows x activation rows
+// weight rows x activation rows; P: two workgroups to a compute unit
+enum Fp8Tile { F8_64x32, F8_64x64, F8_128x64, F8_128x64P, F8_256x64, F8_256x64P, F8_128x128, F8_128x128P, F8_256x128, F8_256x256, F8_TILES };
 struct Fp8TilePick {
     int tile, part_k;  // 0: one part
 };
 constexpr int kFp8Parts = 8, kFp8GroupParts = 4;  // parts of K at most, of a product by group (which its caller joins)
 bool fp8_streams(const Fp8Product &p);
 int fp8_stream_launch(const Fp8Product &p, hipStream_t st);
+bool fp8_product_streams(const Fp8Product &p);
 bool fp8_tile_ok(const Fp8Product &p);
 Fp8TilePick fp8_tile_pick(const Fp8Product &p, int most_parts);
 int fp8_tile_launch(const Fp8Product &p, int tile, hipStream_t st);

@@ -5,24 +5,25 @@
 
 namespace chadq {
 
-// Time of a product by tile: `start` us once, and for each round of the compute units' workgroups `round` us and `few` (64 workgroups, at the clock that they leave) to
-// `full` (256) us per 1024 k.
+// Time of a product by tile: `start` us once, and for each round of the compute units' workgroups (`wgs` to each) `round` us and `few` (a quarter of that many, at the clock
+// that they leave) to `full` us per 1024 k.  Fitted to the times of every tile.
 struct TileTime {
-    int tn, tm;
+    int tn, tm, wgs;
     float start, round, few, full;
 };
-static const TileTime kBf16[F8_TILES] = {{64, 32, 1.43f, 3.38f, 1.77f, 2.51f}, {64, 64, 1.25f, 4.1f, 2.46f, 3.5f}, {128, 64, 1.15f, 3.7f, 3.87f, 5.58f}, {256, 64, 0.92f, 5.05f, 6.43f, 9.74f},
-                                         {128, 128, 0.57f, 5.56f, 6.05f, 8.52f}, {256, 128, 0.5f, 5.73f, 10.42f, 15.42f}, {256, 256, 0.f, 1e9f, 0.f, 0.f}};
-static const TileTime kFp8[F8_TILES] = {{64, 32, 1.29f, 3.91f, 1.26f, 1.49f}, {64, 64, 0.87f, 4.66f, 1.93f, 2.4f}, {128, 64, 0.78f, 4.51f, 2.83f, 3.46f}, {256, 64, 1.04f, 3.74f, 5.09f, 6.73f},
-                                        {128, 128, 0.44f, 5.13f, 4.24f, 5.92f}, {256, 128, 0.0f, 5.59f, 6.56f, 9.49f}, {256, 256, 0.43f, 6.25f, 10.36f, 19.67f}};
-
-static Fp8TilePick pick(int M, int N, int K, int E, bool x_fp8, bool gated, int most_parts) {
+static const TileTime kBf16[F8_TILES] = {{64, 32, 1, 1.44f, 3.34f, 1.8f, 2.53f}, {64, 64, 1, 1.21f, 4.03f, 2.49f, 3.58f}, {128, 64, 1, 1.14f, 3.66f, 3.9f, 5.55f}, {128, 64, 2, 1.5f, 2.95f, 5.72f, 10.44f},
+                                         {256, 64, 1, 0.73f, 4.98f, 6.76f, 9.67f}, {256, 64, 2, 2.29f, 2.78f, 8.27f, 20.63f}, {128, 128, 1, 0.63f, 5.37f, 6.14f, 8.53f}, {128, 128, 2, 2.15f, 2.96f, 8.34f, 19.24f},
+                                         {256, 128, 1, 0.13f, 5.91f, 10.51f, 15.82f}, {256, 256, 1, 0.0f, 1e9f, 0.0f, 0.0f}};
+static const TileTime kFp8[F8_TILES] = {{64, 32, 1, 1.49f, 3.78f, 1.19f, 1.49f}, {64, 64, 1, 1.28f, 4.48f, 1.77f, 2.35f}, {128, 64, 1, 0.69f, 4.73f, 2.77f, 3.42f}, {128, 64, 2, 0.47f, 3.99f, 3.46f, 6.55f},
+                                        {256, 64, 1, 0.01f, 4.83f, 5.1f, 6.36f}, {256, 64, 2, 0.0f, 1e9f, 0.0f, 0.0f}, {128, 128, 1, 0.0f, 5.67f, 4.2f, 5.59f}, {128, 128, 2, 0.0f, 4.46f, 5.46f, 10.58f},
+                                        {256, 128, 1, 0.0f, 5.74f, 6.48f, 9.41f}, {256, 256, 1, 0.0f, 6.9f, 10.4f, 18.19f}};
+static Fp8TilePick pick(int M, int N, int K, int E, bool x_fp8, bool gated, bool h8, int most_parts) {
     Fp8TilePick best = {F8_128x128, 0};
     float least = 1e30f;
     for (int i = 0; i < F8_TILES; ++i) {
         const TileTime &t = (x_fp8 ? kFp8 : kBf16)[i];
         const int tn = gated ? t.tn / 2 : t.tn;
-        if (t.round > 1e8f || (gated && (t.tn < 128 || i == F8_128x128 || i == F8_256x256))) continue;
+        if (t.round > 1e8f || (gated && (t.tn < 128 || i == F8_128x128 || i == F8_256x256 || (h8 && t.tn < 256)))) continue;
         // rows by group: between the tiles of groups of one size and those of exponentially distributed sizes
         const float mean = (float)M / E > 1.f ? (float)M / E : 1.f, hit = E * (1.f - expf(-(float)M / E)), even = mean / t.tm + 0.3f;
         const float tm = E > 1 ? hit * 0.5f * ((even > 1.f ? even : 1.f) + 1.f / (1.f - expf(-t.tm / mean))) : (float)mx_ceil(M, t.tm);
@@ -30,9 +31,9 @@ static Fp8TilePick pick(int M, int N, int K, int E, bool x_fp8, bool gated, int 
         for (int parts = 1; parts <= most_parts; ++parts) {
             const int part_k = parts > 1 ? ((K + parts - 1) / parts + 1023) / 1024 * 1024 : K;
             if (parts > 1 && (int64_t)part_k * (parts - 1) >= K) continue;
-            const float wgs = tiles * parts, full = wgs >= 256.f ? 1.f : wgs <= 64.f ? 0.f : (wgs - 64.f) / 192.f;
+            const float at_once = 256.f * t.wgs, w = tiles * parts / at_once, full = w >= 1.f ? 1.f : w <= 0.25f ? 0.f : (w - 0.25f) / 0.75f;
             // (by group: a workgroup finds its tile first; the groups' tiles end unevenly)
-            const float rounds = E > 1 && wgs > 256.f ? wgs / 256.f + 0.6f : ceilf(wgs / 256.f), round = E > 1 ? t.round + 2.f : t.round;
+            const float rounds = E > 1 && w > 1.f ? w + 0.6f : ceilf(w), round = E > 1 ? t.round + 2.f : t.round;
             float us = t.start + rounds * (round + (t.few + (t.full - t.few) * full) * (part_k / 1024.f));
             if (parts > 1) us += 3.f + (8.f * parts + 2.f) * M * (float)N * 2.5e-7f;  // the sums written, read again and joined by another launch
             if (us < least * (parts > 1 ? 0.95f : 1.f)) {
@@ -45,10 +46,13 @@ static Fp8TilePick pick(int M, int N, int K, int E, bool x_fp8, bool gated, int 
 }
 
 Fp8TilePick fp8_tile_pick(const Fp8Product &p, int most_parts) {
-    return pick(p.M, p.N, p.K, p.offsets ? p.E : 1, p.xs != nullptr, p.w2 != nullptr, most_parts);
+    return pick(p.M, p.N, p.K, p.offsets ? p.E : 1, p.xs != nullptr, p.w2 != nullptr, p.h8 != nullptr, most_parts);
 }
 
-int fp8_product_part_k(const Fp8Product &p, int most_parts) { return fp8_streams(p) || !fp8_tile_ok(p) ? 0 : fp8_tile_pick(p, most_parts).part_k; }
+// Which of the two: the tiles' requests do not reach over rows as long as the streams' do
+bool fp8_product_streams(const Fp8Product &p) { return fp8_streams(p) || !fp8_tile_ok(p); }
+
+int fp8_product_part_k(const Fp8Product &p, int most_parts) { return fp8_product_streams(p) ? 0 : fp8_tile_pick(p, most_parts).part_k; }
 
 size_t fp8_product_workspace_bytes(int M, int N, int K, bool x_fp8) {
     Fp8Product p = {};
@@ -63,7 +67,7 @@ size_t fp8_product_workspace_bytes(int M, int N, int K, bool x_fp8) {
 }
 
 int fp8_product_launch(const Fp8Product &p, void *workspace, size_t workspace_bytes, hipStream_t st) {
-    if (fp8_streams(p) || !fp8_tile_ok(p)) return fp8_stream_launch(p, st);
+    if (fp8_product_streams(p)) return fp8_stream_launch(p, st);
     if (p.part_k) return fp8_tile_launch(p, fp8_tile_pick(p, kFp8GroupParts).tile, st);  // (the caller, who asked for at most so many, joins the parts)
     if (!p.offsets && workspace) {
         Fp8Product q = p;

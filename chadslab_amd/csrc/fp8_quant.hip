@@ -1,42 +1,8 @@
-// FP8: quantisation and its inverse.  Per block (128 k of a row, or 128 rows x 128 k) with a = max(max |x|, 448 * 2^-126):
-//   scale = a / 448,  r = 448 / a  (fp32 divisions),  value = the nearest e4m3 to x r (one fp32 product), ties to the even one.
-// |x r| <= 448 (1 + 2^-23), which goes to 448: nothing saturates.  The least a keeps scale and r normal numbers.  A block that holds a NaN or an
-// infinity gets a NaN for its scale and values of 0.
+// FP8: quantisation (of a block: fp8.h) and its inverse.
 #include "fp8.h"
 #include "load8.h"
 
 namespace chadq {
-
-constexpr float kFp8Least = 448.f * 0x1p-126f;
-
-__device__ __forceinline__ uint32_t absmax8(const float f[8]) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t b = __float_as_uint(f[j]) & 0x7FFFFFFFu;  // as integers: a NaN is larger than infinity
-        m = b > m ? b : m;
-    }
-    return m;
-}
-
-struct Fp8Scale {
-    float scale, r;
-    bool bad;
-    __device__ __forceinline__ explicit Fp8Scale(uint32_t most) {
-        bad = most >= 0x7F800000u;
-        const float m = __uint_as_float(most), a = m > kFp8Least ? m : kFp8Least;
-        scale = bad ? __uint_as_float(0x7FC00000u) : a / 448.f;
-        r = 448.f / a;
-    }
-    __device__ __forceinline__ u32x2 values(const float f[8]) const {
-        int lo = 0, hi = 0;
-        lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * r, f[1] * r, lo, false);
-        lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * r, f[3] * r, lo, true);
-        hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * r, f[5] * r, hi, false);
-        hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * r, f[7] * r, hi, true);
-        return bad ? u32x2{0, 0} : u32x2{(uint32_t)lo, (uint32_t)hi};
-    }
-};
 
 // Rows: 16 lanes to a block, 8 values to a lane.  K is a multiple of 16: pieces of 8 are whole.
 template <typename T>
@@ -49,13 +15,8 @@ __global__ __launch_bounds__(256) void quantize_fp8_rows_kernel(const T *__restr
         const int g = (int)(b - row * G), k = g * 128 + l * 8;
         float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (k < K) load8<T>(x + row * K + k, f);
-        uint32_t m = absmax8(f);
-#pragma unroll
-        for (int s = 1; s < 16; s *= 2) {
-            const uint32_t o = (uint32_t)__shfl_xor((int)m, s);
-            m = o > m ? o : m;
-        }
-        const Fp8Scale c(m);
+        const uint32_t m = absmax8(f);
+        const Fp8Scale c(max_of_16(m));
         if (k < K) *reinterpret_cast<u32x2 *>(q + row * K + k) = c.values(f);
         if (l == 0) scale[b] = c.scale;
     }

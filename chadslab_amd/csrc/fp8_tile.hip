@@ -38,7 +38,8 @@ struct Cfg {
     static constexpr int SROWS = (X8 ? TM : 0) + 2, SPITCH = (SROWS + 31) / 32 * 32;  // rows of scales: of x, of the tile's two blocks of weight rows (gate and up)
     static_assert(SROWS <= T && WPARTS == WK, "a thread to a row of scales; each wave a part");
     static constexpr int S_OFF = ST * STAGE, S_GROUP = GE * SPITCH * 4, DUMP = S_OFF + 2 * S_GROUP, OPER = DUMP + 64 * GE * 4, RED = WN * WM * (WK - 1) * NB * MB * 4096;
-    static constexpr int EPI = TM * (TO * 2 + 16), MOST = OPER > RED ? OPER : RED, LDS = MOST > EPI ? MOST : EPI;
+    static constexpr bool H8 = X8 && GATED && TO == 128;  // results in 8 bits: a tile has whole blocks of them
+    static constexpr int EPI = TM * (TO * (H8 ? 4 : 2) + 16), MOST = OPER > RED ? OPER : RED, LDS = MOST > EPI ? MOST : EPI;
     static_assert(LDS <= 163840, "LDS of a compute unit");
     static_assert(!GATED || (NB % 2 == 0 && 1024 / WROW <= 32), "gate and up blocks side by side; a DMA instruction's rows are of one block");
 };
@@ -472,6 +473,31 @@ __device__ __forceinline__ void tile_body(const Fp8Product &p, const MxTile &t, 
             for (int g = 0; g < 4; ++g)
 #pragma unroll
                 for (int v = 0; v < 4; ++v) out[a][b][g][v] = C::GATED ? silu_mul(sum[2 * a][b][g][v], sum[2 * a + 1][b][g][v]) : sum[C::GATED ? 2 * a : a][b][g][v];
+    if constexpr (C::H8) {
+        if (p.h8) {  // through LDS in fp32, 16 lanes to a row's block
+            static_assert(C::WK == 1, "every wave has results");
+            constexpr int PITCH = TO * 4 + 16;
+            __syncthreads();
+#pragma unroll
+            for (int a = 0; a < NO; ++a)
+#pragma unroll
+                for (int b = 0; b < MB; ++b)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<f32x4 *>(lds + ((wm * MB + b) * 32 + quad_m(g)) * PITCH + ((wn * NO + a) * 32 + quad_n(g)) * 4) = out[a][b][g];
+            __syncthreads();
+            const int l = tid & 15, G = fp8_blocks(p.N);
+            for (int m = tid >> 4; m < t.rows; m += C::T / 16) {  // (columns behind N are sums of zeros)
+                const f32x4 lo = reinterpret_cast<const f32x4 *>(lds + m * PITCH)[2 * l], hi = reinterpret_cast<const f32x4 *>(lds + m * PITCH)[2 * l + 1];
+                const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                const Fp8Scale c(max_of_16(absmax8(f)));
+                const size_t row = (size_t)(t.row0 + m);
+                if (l * 8 < src.nrows) *reinterpret_cast<u32x2 *>(p.h8 + row * p.N + n0 + l * 8) = c.values(f);
+                if (l == 0) p.h8s[row * G + (n0 >> 7)] = c.scale;
+            }
+            return;
+        }
+    }
     if (!p.y_bf16) {
         if (wk > 0) return;
         float *const y = reinterpret_cast<float *>(p.y) + (size_t)blockIdx.y * p.M * p.N;
@@ -524,7 +550,7 @@ __device__ __forceinline__ void tile_body(const Fp8Product &p, const MxTile &t, 
 }
 
 template <bool X8, bool GATED, int WN, int WM, int WK, int NB, int MB, int SK, int ST>
-__global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_eu(WN * WM * WK / 4, WN * WM * WK / 4))) void fp8_tile_kernel(Fp8Product p) {
+__global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_tile_kernel(Fp8Product p) {
     typedef Cfg<X8, GATED, WN, WM, WK, NB, MB, SK, ST> C;
     constexpr int TM = C::TM, TO = C::TO;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -585,6 +611,8 @@ bool fp8_tile_ok(const Fp8Product &p) {
     return (int64_t)p.K * 256 < INT32_MAX && row * 256 < INT32_MAX && (!p.rows || row * p.x_rows < INT32_MAX);
 }
 
+// Tiles with a P have four waves and half a compute unit's LDS: two workgroups to a unit, of which one computes while the other waits at its barrier, begins or ends.  us,
+// 8-bit x, eight waves / four: 4096^3 92 / 70 at 128 x 128 and 132 / 94 at 128 x 64, but where there is one workgroup to a unit 79 / 103 (1000 x 4096 x 14336).
 int fp8_tile_launch(const Fp8Product &p, int tile, hipStream_t st) {
     using namespace f8t;
     //                                                       WN WM WK NB MB SK ST
@@ -592,13 +620,18 @@ int fp8_tile_launch(const Fp8Product &p, int tile, hipStream_t st) {
         if (p.xs) {
             switch (tile) {
             case F8_128x64: return launch<true, true, 2, 2, 2, 2, 1, 256, 3>(p, st);
+            case F8_128x64P: return launch<true, true, 2, 2, 1, 2, 1, 128, 3>(p, st);
             case F8_256x64: return launch<true, true, 4, 2, 1, 2, 1, 128, 3>(p, st);
+            case F8_128x128P: return launch<true, true, 2, 2, 1, 2, 2, 128, 2>(p, st);
             default: return launch<true, true, 4, 2, 1, 2, 2, 128, 3>(p, st);
             }
         }
         switch (tile) {
         case F8_128x64: return launch<false, true, 2, 2, 2, 2, 1, 128, 4>(p, st);
+        case F8_128x64P: return launch<false, true, 2, 2, 1, 2, 1, 64, 4>(p, st);
         case F8_256x64: return launch<false, true, 4, 1, 2, 2, 2, 128, 3>(p, st);
+        case F8_256x64P: return launch<false, true, 4, 1, 1, 2, 2, 64, 3>(p, st);
+        case F8_128x128P: return launch<false, true, 2, 2, 1, 2, 2, 64, 3>(p, st);
         default: return launch<false, true, 4, 2, 1, 2, 2, 64, 4>(p, st);
         }
     }
@@ -607,8 +640,10 @@ int fp8_tile_launch(const Fp8Product &p, int tile, hipStream_t st) {
         case F8_64x32: return launch<true, false, 2, 1, 4, 1, 1, 512, 3>(p, st);
         case F8_64x64: return launch<true, false, 2, 1, 4, 1, 2, 512, 2>(p, st);
         case F8_128x64: return launch<true, false, 4, 1, 2, 1, 2, 256, 3>(p, st);
+        case F8_128x64P: return launch<true, false, 2, 2, 1, 2, 1, 128, 3>(p, st);
         case F8_256x64: return launch<true, false, 8, 1, 1, 1, 2, 128, 3>(p, st);
         case F8_128x128: return launch<true, false, 2, 2, 2, 2, 2, 256, 2>(p, st);
+        case F8_128x128P: return launch<true, false, 2, 2, 1, 2, 2, 128, 2>(p, st);
         case F8_256x128: return launch<true, false, 4, 2, 1, 2, 2, 128, 3>(p, st);
         default: return launch<true, false, 2, 4, 1, 4, 2, 128, 2>(p, st);
         }
@@ -617,8 +652,11 @@ int fp8_tile_launch(const Fp8Product &p, int tile, hipStream_t st) {
     case F8_64x32: return launch<false, false, 2, 1, 4, 1, 1, 256, 4>(p, st);
     case F8_64x64: return launch<false, false, 2, 1, 4, 1, 2, 256, 3>(p, st);
     case F8_128x64: return launch<false, false, 4, 1, 2, 1, 2, 128, 4>(p, st);
+    case F8_128x64P: return launch<false, false, 2, 2, 1, 2, 1, 64, 4>(p, st);
     case F8_256x64: return launch<false, false, 4, 1, 2, 2, 2, 128, 3>(p, st);
+    case F8_256x64P: return launch<false, false, 4, 1, 1, 2, 2, 64, 3>(p, st);
     case F8_128x128: return launch<false, false, 2, 2, 2, 2, 2, 128, 3>(p, st);
+    case F8_128x128P: return launch<false, false, 2, 2, 1, 2, 2, 64, 3>(p, st);
     default: return launch<false, false, 4, 2, 1, 2, 2, 64, 4>(p, st);
     }
 }

@@ -581,14 +581,31 @@ int moe_ffn_mxfp4_launch(const uint16_t *x, const float *logits, const chadq_moe
 struct MoeFp8Ws {
     int32_t *idx, *pos, *tok, *offsets, *hist;
     float *w;
-    void *h;       // bf16 [P,F], or fp32 for 8-bit activations
+    void *h;       // bf16 [P,F]; with 8-bit activations fp32, where the product does not write 8 bits itself
     uint8_t *h8;   // [P,F]
     float *h8s;    // [P,ceil(F/128)]
-    float *yp;     // [P,H]
+    float *yp;     // [parts of the down product][P,H]
 };
+
+// The two products; what their rules look at without the addresses, for the sizes of the workspace
+static Fp8Product moe_fp8_gateup(int T, int H, int F, int E, int top_k, const void *x, const float *xs) {
+    static const int32_t any = 0;
+    Fp8Product p = {x, xs, nullptr, nullptr, nullptr, &any, T * top_k, F, H, E, xs == nullptr, false};
+    p.rows = &any;
+    p.x_rows = T;
+    return p;
+}
+static Fp8Product moe_fp8_down(int T, int H, int F, int E, int top_k, const void *h, const float *hs) {
+    static const int32_t any = 0;
+    Fp8Product p = {h, hs, nullptr, nullptr, nullptr, &any, T * top_k, H, F, E, false, false};
+    p.part_k = fp8_product_part_k(p, kFp8GroupParts);
+    return p;
+}
 
 static size_t moe_fp8_layout(uint8_t *base, int T, int H, int F, int E, int top_k, bool x_fp8, MoeFp8Ws *ws) {
     const size_t P = (size_t)T * top_k;
+    static const float any = 0.f;
+    const float *const xs = x_fp8 ? &any : nullptr;
     size_t o = 0;
     auto take = [&](size_t bytes) {
         uint8_t *p = base ? base + o : nullptr;
@@ -601,11 +618,11 @@ static size_t moe_fp8_layout(uint8_t *base, int T, int H, int F, int E, int top_
     w.pos = (int32_t *)take(P * 4);
     w.tok = (int32_t *)take(P * 4);
     w.offsets = (int32_t *)take(((size_t)E + 1) * 4);
-    w.hist = (int32_t *)take(sort_chunks(P) > 1 ? (size_t)sort_chunks(P) * E * 4 : 0);
-    w.h = take(P * F * (x_fp8 ? 4 : 2));
+    w.hist = (int32_t *)take(sort_chunks(P) > kSortAlone ? (size_t)sort_chunks(P) * E * 4 : 0);
+    w.h = take(!x_fp8 ? P * F * 2 : fp8_product_streams(moe_fp8_gateup(T, H, F, E, top_k, nullptr, xs)) ? P * F * 4 : 0);
     w.h8 = take(x_fp8 ? P * F : 0);
     w.h8s = (float *)take(x_fp8 ? P * fp8_blocks(F) * 4 : 0);
-    w.yp = (float *)take(P * H * 4);
+    w.yp = (float *)take(P * H * 4 * moe_fp8_down(T, H, F, E, top_k, nullptr, xs).parts());
     if (ws) *ws = w;
     return o;
 }
@@ -621,24 +638,34 @@ int moe_ffn_fp8_launch(const void *x, const float *xs, const float *logits, cons
     const int P = T * r.top_k;
     int rc = route_sort_launch(logits, ws.idx, ws.w, T, E, r, RouteSort{ws.pos, ws.tok, ws.offsets, ws.hist}, st);
     if (rc) return rc;
-    Fp8Product gu = {x, xs, ex->gate, ex->gate_scale, ws.h, ws.offsets, P, F, H, E, xs == nullptr, false};
-    gu.rows = ws.tok;
-    gu.x_rows = T;
+    Fp8Product gu = moe_fp8_gateup(T, H, F, E, r.top_k, x, xs);
+    const bool streams = fp8_product_streams(gu);
+    gu.w = ex->gate;
+    gu.ws = ex->gate_scale;
     gu.w2 = ex->up;
     gu.w2s = ex->up_scale;
+    gu.offsets = ws.offsets;
+    gu.rows = ws.tok;
+    gu.y = ws.h;
+    if (xs && !streams) {
+        gu.h8 = ws.h8;
+        gu.h8s = ws.h8s;
+    }
     rc = fp8_product_launch(gu, nullptr, 0, st);
     if (rc) return rc;
-    Fp8Product down = {ws.h, nullptr, ex->down, ex->down_scale, ws.yp, ws.offsets, P, H, F, E, false, false};
-    if (xs) {
+    if (xs && streams) {
         rc = quantize_fp8_launch(ws.h, CHADQ_F32, ws.h8, ws.h8s, 1, P, F, true, st);
         if (rc) return rc;
-        down.x = ws.h8;
-        down.xs = ws.h8s;
     }
+    Fp8Product down = moe_fp8_down(T, H, F, E, r.top_k, xs ? (const void *)ws.h8 : ws.h, xs ? ws.h8s : nullptr);
+    down.w = ex->down;
+    down.ws = ex->down_scale;
+    down.offsets = ws.offsets;
+    down.y = ws.yp;
     rc = fp8_product_launch(down, nullptr, 0, st);
     if (rc) return rc;
     const int64_t quads = (int64_t)T * (H / 4);
-    hipLaunchKernelGGL(moe_combine_kernel, dim3(quads < 1024 * 256 ? (int)((quads + 255) / 256) : 1024), dim3(256), 0, st, ws.yp, ws.pos, ws.w, y, T, H, r.top_k, 1,
+    hipLaunchKernelGGL(moe_combine_kernel, dim3(quads < 1024 * 256 ? (int)((quads + 255) / 256) : 1024), dim3(256), 0, st, ws.yp, ws.pos, ws.w, y, T, H, r.top_k, down.parts(),
                        (size_t)P * H);
     return hip_check(hipGetLastError(), "moe combine launch");
 }

@@ -5,7 +5,7 @@
 namespace chadq {
 
 constexpr int kRouteExperts = 512, kRouteTopK = 32, kRouteGroups = 64;
-constexpr int kSortChunk = 1024;  // pairs to a workgroup
+constexpr int kSortChunk = 1024, kSortAlone = 12;  // pairs to a workgroup; workgroups up to which each counts all pairs
 
 struct Routing {
     const float *bias;  // [E] or null
@@ -17,7 +17,7 @@ struct RouteSort {
     int32_t *pos;      // [P] row of the pair
     int32_t *tok;      // [P] token of the row
     int32_t *offsets;  // [E+1] first row of each expert
-    int32_t *hist;     // [chunks,E], for more than one chunk
+    int32_t *hist;     // [chunks,E], for more than kSortAlone chunks
 };
 inline int sort_chunks(int64_t P) { return (int)((P + kSortChunk - 1) / kSortChunk); }
 

@@ -21,12 +21,79 @@ __device__ __forceinline__ uint64_t route_key(double v) {
     return b ^ ((b >> 63) ? ~0ull : 1ull << 63);
 }
 
+// f(v, the value of the lane that differs in one bit of its number) for a value that is the same in all lanes with the same number without the lower bits
+template <int S, typename T, typename F>
+__device__ __forceinline__ T across(T v, F f) {
+    static_assert(sizeof(T) == 4 || sizeof(T) == 8, "one or two registers");
+    constexpr int N = sizeof(T) / 4;
+    struct words_t { uint32_t w[N]; };
+    words_t a = __builtin_bit_cast(words_t, v), b = a;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if constexpr (S < 16) {  // quad_perm [1,0,3,2] and [2,3,0,1], row_half_mirror, row_mirror
+            constexpr int CTRL = S == 1 ? 0xB1 : S == 2 ? 0x4E : S == 4 ? 0x141 : 0x140;
+            b.w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a.w[i], CTRL, 0xF, 0xF, false);
+        } else {  // the rows, or halves, of both, one beside the other: every lane gets either
+            const auto r = S == 16 ? __builtin_amdgcn_permlane16_swap(a.w[i], a.w[i], false, false) : __builtin_amdgcn_permlane32_swap(a.w[i], a.w[i], false, false);
+            a.w[i] = r[0];
+            b.w[i] = r[1];
+        }
+    }
+    return f(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+}
+// f over L lanes next to each other, the result in all of them
 template <int L, typename T, typename F>
 __device__ __forceinline__ T over_lanes(T v, F f) {
-#pragma unroll
-    for (int s = 1; s < L; s *= 2) v = f(v, __shfl_xor(v, s));
+    if constexpr (L > 1) v = across<1>(v, f);
+    if constexpr (L > 2) v = across<2>(v, f);
+    if constexpr (L > 4) v = across<4>(v, f);
+    if constexpr (L > 8) v = across<8>(v, f);
+    if constexpr (L > 16) v = across<16>(v, f);
+    if constexpr (L > 32) v = across<32>(v, f);
     return v;
 }
+template <int L>
+__device__ __forceinline__ uint32_t most_of(uint32_t v) {
+    return over_lanes<L>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+// the largest key, by its upper word and then by the lower one: a comparison of two words is no single instruction
+template <int L>
+__device__ __forceinline__ uint64_t most_of(uint64_t v) {
+    const uint32_t hi = most_of<L>((uint32_t)(v >> 32)), lo = most_of<L>((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+    return (uint64_t)hi << 32 | lo;
+}
+// the value of lane `from`, one for the whole wave where a token takes all of it
+template <int L, typename T>
+__device__ __forceinline__ T from_lane(T v, int from) {
+    if constexpr (L < 64) return __shfl(v, from);
+    constexpr int N = sizeof(T) / 4;
+    struct words_t { uint32_t w[N]; };
+    words_t a = __builtin_bit_cast(words_t, v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) a.w[i] = (uint32_t)__builtin_amdgcn_readlane((int)a.w[i], from);
+    return __builtin_bit_cast(T, a);
+}
+// the two largest values of some
+template <typename V>
+struct Two {
+    V a, b;
+    __device__ __forceinline__ void take(V v) {
+        b = v > a ? a : v > b ? v : b;
+        a = v > a ? v : a;
+    }
+    template <int S>
+    __device__ __forceinline__ void join() {
+        const auto pick = [](V x, V y) { return x > y ? x : y; };
+        // of the lane's own and the other's: the larger first, and of its loser and the seconds the largest
+        V oa, ob;
+        across<S>(a, [&](V x, V y) { oa = x, ob = y; return x; });
+        const V first = pick(oa, ob), loser = oa > ob ? ob : oa;
+        V sa, sb;
+        across<S>(b, [&](V x, V y) { sa = x, sb = y; return x; });
+        a = first;
+        b = pick(loser, pick(sa, sb));
+    }
+};
 
 // All lanes of the wave; the token's choices come back in its lanes 0 .. top_k - 1.  lds: [tokens of the workgroup][L * PER] choice values (groups > 1)
 template <int L, int PER, bool WIDE>
@@ -80,31 +147,32 @@ __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, i
     for (int i = 0; i < PER; ++i) open |= (ls * PER + i < E ? 1u : 0u) << i;
     if (r.groups > 1) {
         const int G = r.groups, per = E / G;
-        int q = L;  // lanes that share a group: a power of two
-        while (q * G > L) q >>= 1;
-        V *const mine = reinterpret_cast<V *>(lds) + (threadIdx.x / L) * (L * PER);
+        int q;  // lanes that share a group: a power of two
+        Two<V> two = {-INFINITY, -INFINITY};
+        if (E == L * PER && per % PER == 0 && ((per / PER) & (per / PER - 1)) == 0) {  // whole lanes to a group: as they are
+            q = per / PER;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) mine[ls * PER + i] = c[i];
-        __builtin_amdgcn_wave_barrier();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's own: its LDS accesses keep their order
-        const int g = ls / q, j = ls % q;
-        V a = -INFINITY, b = -INFINITY;  // the two largest
-        if (g < G)
-            for (int i = j; i < per; i += q) {
-                const V v = mine[g * per + i];
-                b = v > a ? a : v > b ? v : b;
-                a = v > a ? v : a;
-            }
-        for (int d = 1; d < q; d *= 2) {
-            const V oa = __shfl_xor(a, d), ob = __shfl_xor(b, d);
-            const V low = a > oa ? oa : a, second = b > ob ? b : ob;
-            a = a > oa ? a : oa;
-            b = low > second ? low : second;
+            for (int i = 0; i < PER; ++i) two.take(c[i]);
+        } else {  // through LDS, each of a group's lanes every q-th
+            for (q = L; q * G > L;) q >>= 1;
+            V *const mine = reinterpret_cast<V *>(lds) + (threadIdx.x / L) * (L * PER);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) mine[ls * PER + i] = c[i];
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's own: its LDS accesses keep their order
+            if (ls / q < G)
+                for (int i = ls % q; i < per; i += q) two.take(mine[ls / q * per + i]);
         }
-        const V value = r.group_sum == 2 ? a + b : a;
+        if (q > 1) two.template join<1>();
+        if (q > 2) two.template join<2>();
+        if (q > 4) two.template join<4>();
+        if (q > 8) two.template join<8>();
+        if (q > 16) two.template join<16>();
+        const int g = ls / q;
+        const V value = r.group_sum == 2 ? two.a + two.b : two.a;
         int rank = 0;
         for (int h = 0; h < G; ++h) {
-            const V o = __shfl(value, seg + h * q);
+            const V o = from_lane<L>(value, seg + h * q);
             rank += o > value || (o == value && h < g);
         }
         const unsigned long long kept = __ballot(g < G && rank < r.top_groups) >> seg;
@@ -134,10 +202,10 @@ __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, i
     double sc = 0.0;
     chosen = 0;
     for (int k = 0; k < r.top_k; ++k) {
-        const K most = over_lanes<L>(best, larger);
+        const K most = most_of<L>(best);
         const unsigned long long hold = __ballot(best == most) & seg_mask;
         const int winner = __ffsll((long long)hold) - 1;
-        const int e = __shfl(ls * PER + at, winner);
+        const int e = from_lane<L>(ls * PER + at, winner);
         float zw = zr[0];
         double sw = 0.0;
         if constexpr (WIDE) sw = s[0];
@@ -147,8 +215,8 @@ __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, i
                 zw = zr[i];
                 if constexpr (WIDE) sw = s[i];
             }
-        zw = __shfl(zw, winner);
-        if constexpr (WIDE) sw = __shfl(sw, winner);
+        zw = from_lane<L>(zw, winner);
+        if constexpr (WIDE) sw = from_lane<L>(sw, winner);
         if (ls == k) {
             chosen = e;
             zc = zw;
@@ -237,24 +305,27 @@ __device__ __forceinline__ void experts_first(int E, const int32_t *s_total, int
     __syncthreads();
 }
 
-// One chunk: everything.  Several: FIRST writes each chunk's counts and its pairs' ranks, and then each workgroup adds what is in front of its own.
-enum SortStep { SORT_ALL, SORT_COUNT, SORT_PLACE };
-template <SortStep STEP>
-__global__ __launch_bounds__(kSortChunk) void sort_pairs_kernel(const int32_t *__restrict__ idx, RouteSort s, int P, int E, int top_k) {
+// Rows of the pairs.  COUNTED: the ranks inside a chunk and the chunks' counts are there (sort_count_kernel); else a workgroup counts all pairs itself, which is
+// quicker than another launch up to some ten thousand of them.
+__global__ __launch_bounds__(kSortChunk) void sort_count_kernel(const int32_t *__restrict__ idx, RouteSort s, int P, int E) {
     __shared__ uint16_t s_cnt[16 * kRouteExperts];
-    __shared__ int32_t s_total[kRouteExperts], s_first[kRouteExperts + 1];
+    __shared__ int32_t s_total[kRouteExperts];
     const int tid = threadIdx.x;
-    const int64_t p = (int64_t)blockIdx.x * blockDim.x + tid;
+    const int64_t p = (int64_t)blockIdx.x * kSortChunk + tid;
+    const int rank = chunk_rank(p < P ? idx[p] : -1, E, s_cnt, s_total);
+    if (tid < E) s.hist[(int64_t)blockIdx.x * E + tid] = s_total[tid];
+    if (p < P) s.pos[p] = rank;
+}
+template <bool COUNTED>
+__global__ __launch_bounds__(kSortChunk) void sort_place_kernel(const int32_t *__restrict__ idx, RouteSort s, int P, int E, int top_k) {
+    __shared__ uint16_t s_cnt[COUNTED ? 1 : 16 * kRouteExperts];
+    __shared__ int32_t s_total[kRouteExperts], s_before[kRouteExperts], s_all[kRouteExperts], s_first[kRouteExperts + 1];
+    const int tid = threadIdx.x;
+    const int64_t chunk = (int64_t)blockIdx.x * kSortChunk, p = chunk + tid;
     const int e = p < P ? idx[p] : -1;
     int row = 0;
-    if (STEP != SORT_PLACE) row = chunk_rank(e, E, s_cnt, s_total);
-    if (STEP == SORT_COUNT) {
-        if (tid < E) s.hist[(int64_t)blockIdx.x * E + tid] = s_total[tid];
-        if (p < P) s.pos[p] = row;
-        return;
-    }
-    if (STEP == SORT_PLACE) {
-        int32_t *const s_before = reinterpret_cast<int32_t *>(s_cnt);
+    if (COUNTED) {
+        if (p < P) row = s.pos[p];
         if (tid < E) {
             int before = 0, all = 0;
             for (int c = 0; c < (int)gridDim.x; ++c) {
@@ -263,16 +334,23 @@ __global__ __launch_bounds__(kSortChunk) void sort_pairs_kernel(const int32_t *_
                 all += n;
             }
             s_before[tid] = before;
-            s_total[tid] = all;
+            s_all[tid] = all;
         }
         __syncthreads();
-        if (p < P) row = s.pos[p] + s_before[e];
+    } else {
+        if (tid < E) s_before[tid] = s_all[tid] = 0;
+        __syncthreads();
+        for (int64_t i = tid; i < P; i += kSortChunk)
+            if (i < chunk || i >= chunk + kSortChunk) atomicAdd((i < chunk ? s_before : s_all) + idx[i], 1);
+        row = chunk_rank(e, E, s_cnt, s_total);  // (its barriers are the counts' too)
+        if (tid < E) s_all[tid] += s_before[tid] + s_total[tid];
+        __syncthreads();
     }
-    experts_first(E, s_total, s_first);
+    experts_first(E, s_all, s_first);
     if (blockIdx.x == 0)
-        for (int i = tid; i <= E; i += blockDim.x) s.offsets[i] = s_first[i];
+        for (int i = tid; i <= E; i += kSortChunk) s.offsets[i] = s_first[i];
     if (p < P) {
-        row += s_first[e];
+        row += s_before[e] + s_first[e];
         s.pos[p] = row;
         s.tok[row] = (int32_t)(p / top_k);
     }
@@ -348,11 +426,11 @@ int route_sort_launch(const float *logits, int32_t *idx, float *w, int T, int E,
     int rc = route_experts_launch(logits, idx, w, T, E, r, st);
     if (rc) return rc;
     const int chunks = sort_chunks(P);
-    if (chunks == 1) {
-        hipLaunchKernelGGL(sort_pairs_kernel<SORT_ALL>, dim3(1), dim3(kSortChunk), 0, st, idx, s, P, E, r.top_k);
+    if (chunks <= kSortAlone) {
+        hipLaunchKernelGGL(sort_place_kernel<false>, dim3(chunks), dim3(kSortChunk), 0, st, idx, s, P, E, r.top_k);
     } else {
-        hipLaunchKernelGGL(sort_pairs_kernel<SORT_COUNT>, dim3(chunks), dim3(kSortChunk), 0, st, idx, s, P, E, r.top_k);
-        hipLaunchKernelGGL(sort_pairs_kernel<SORT_PLACE>, dim3(chunks), dim3(kSortChunk), 0, st, idx, s, P, E, r.top_k);
+        hipLaunchKernelGGL(sort_count_kernel, dim3(chunks), dim3(kSortChunk), 0, st, idx, s, P, E);
+        hipLaunchKernelGGL(sort_place_kernel<true>, dim3(chunks), dim3(kSortChunk), 0, st, idx, s, P, E, r.top_k);
     }
     return hip_check(hipGetLastError(), "moe sort launch");
 }
