@@ -65,8 +65,10 @@ struct Source {
     uint8_t *const lds;
     int tid, lane, wave, s0, kend, steps, nrows;  // s0: first step of the workgroup's part of K; nrows: result columns that there are
     __amdgpu_buffer_rsrc_t wrsrc, w2rsrc, xrsrc;
-    uint32_t off[C::REQ];
-    int wplace, xplace;  // of the lane's piece in a part of a row: the rows of a wave's requests of a kind are a multiple of 16 apart
+    // of the lane's piece in a part of a row (the rows of a wave's requests of a kind are a multiple of 16 apart), and in a request's rows
+    int wplace, xplace;
+    uint32_t wlane, xlane[C::GATED ? C::XI : 1];  // (GATED: rows through an index, each from x's first)
+    int wbytes, xbytes;  // of a row
     const __attribute__((address_space(1))) float *srow;
     int whole;
     float sv[C::GE], tail[C::GE];
@@ -80,25 +82,26 @@ struct Source {
         kend = p.part_k && s0 * C::SK + p.part_k < p.K ? s0 * C::SK + p.part_k : p.K;
         steps = (kend - s0 * C::SK + C::SK - 1) / C::SK;
         nrows = p.N - n0 < C::TO ? p.N - n0 : C::TO;
-        const int wbytes = p.K, xbytes = C::X8 ? p.K : p.K * 2;  // of a row
+        wbytes = p.K;
+        xbytes = C::X8 ? p.K : p.K * 2;
         const size_t wfirst = (size_t)t.group * p.N + n0;
         wrsrc = __builtin_amdgcn_make_buffer_rsrc(uniform(p.w + wfirst * wbytes), 0, uniform(nrows * wbytes), 0x00020000);
         w2rsrc = C::GATED ? __builtin_amdgcn_make_buffer_rsrc(uniform(p.w2 + wfirst * wbytes), 0, uniform(nrows * wbytes), 0x00020000) : wrsrc;
-        xrsrc = __builtin_amdgcn_make_buffer_rsrc(uniform(reinterpret_cast<const uint8_t *>(p.x) + (p.rows ? (size_t)0 : (size_t)t.row0 * xbytes)), 0,
-                                                  uniform((p.rows ? p.x_rows : t.rows) * xbytes), 0x00020000);
+        xrsrc = __builtin_amdgcn_make_buffer_rsrc(uniform(reinterpret_cast<const uint8_t *>(p.x) + (C::GATED ? (size_t)0 : (size_t)t.row0 * xbytes)), 0,
+                                                  uniform((C::GATED ? p.x_rows : t.rows) * xbytes), 0x00020000);
         static_assert(C::NW * 64 / (C::WROW / 16) % 16 == 0 && C::NW * 8 % 16 == 0, "rows of a wave's requests");
-        wplace = 16 * ((lane % (C::WROW / 16)) ^ key<C::WROW>(row_of(0)));
-        xplace = 16 * ((lane % 8) ^ key<128>(row_of(C::WI)));
+        constexpr int PPR = C::WROW / 16;  // pieces of a row of weights
+        wplace = 16 * ((lane % PPR) ^ key<C::WROW>(wave * (64 / PPR) + lane / PPR));
+        xplace = 16 * ((lane % 8) ^ key<128>(wave * 8 + lane / 8));
+        wlane = (uint32_t)(lane / PPR) * (uint32_t)wbytes + wplace;
+        if constexpr (C::GATED) {
 #pragma unroll
-        for (int q = 0; q < C::REQ; ++q) {
-            const int e = row_of(q);
-            if (q < C::WI) {
-                const int r = wrow(e % C::TN);
-                off[q] = r < nrows ? (uint32_t)r * (uint32_t)wbytes + wplace : kOut;
-            } else {
-                const int r = e % C::TM, src = r < t.rows ? (p.rows ? p.rows[t.row0 + r] : r) : 0;
-                off[q] = r < t.rows && e < C::TM * C::XPARTS ? (uint32_t)src * (uint32_t)xbytes + xplace : kOut;
+            for (int q = 0; q < C::XI; ++q) {
+                const int e = (q * C::NW + wave) * 8 + lane / 8, r = e % C::TM;
+                xlane[q] = r < t.rows && e < C::TM * C::XPARTS ? (uint32_t)p.rows[t.row0 + r] * (uint32_t)xbytes + xplace : kOut;
             }
+        } else {
+            xlane[0] = (uint32_t)(lane / 8) * (uint32_t)xbytes + xplace;
         }
         // scales.  Those of the last group, if it is no whole one, are loaded one by one before the loop (zeros behind the end of the row, where the activations
         // are zeros too).  No branch: a thread without a row loads another one's and writes where nobody reads, and so does the loop behind the last whole group.
@@ -106,7 +109,7 @@ struct Source {
         auto global = [](const float *p) { return (const __attribute__((address_space(1))) float *)p; };
         if (C::X8 && r < C::TM) {
             const int m = t.row0 + (r < t.rows ? r : t.rows - 1);
-            srow = global(p.xs) + (size_t)(p.rows ? p.rows[m] : m) * G;
+            srow = global(p.xs) + (size_t)(C::GATED ? p.rows[m] : m) * G;
         } else {
             const int j = r - (C::X8 ? C::TM : 0), nb = (n0 >> 7) + (C::GATED ? 0 : j);
             srow = global(C::GATED && j ? p.w2s : p.ws) + ((size_t)t.group * GN + (nb < GN ? nb : GN - 1)) * G;
@@ -120,20 +123,25 @@ struct Source {
                 if (whole * C::GE + e < G) tail[e] = srow[whole * C::GE + e];
         if (whole == 0) srow = global(kNoScales);  // (readable, for the loop)
     }
-    // the lane's row of request q, all parts' rows counted
-    __device__ __forceinline__ int row_of(int q) const {
-        return q < C::WI ? (q * C::NW + wave) * (1024 / C::WROW) + lane / (C::WROW / 16) : ((q - C::WI) * C::NW + wave) * 8 + lane / 8;
-    }
     // row r of the tile's weights: of which matrix, which row behind n0
     __device__ __forceinline__ static bool second(int r) { return C::GATED && (r >> 5 & 1); }
     __device__ __forceinline__ static int wrow(int r) { return C::GATED ? (r >> 6) * 32 + (r & 31) : r; }
 
+    // k of part `part` of a step
+    __device__ __forceinline__ int first_k(int step, int part) const {
+        return C::X8 ? (s0 + step) * C::SK + part * 128 : (s0 + step) / 2 * (2 * C::SK) + (step & 1) * 64 + part * 128;
+    }
+    // What of a request lies behind the last row is beyond the buffer's range, which counts the scalar offset too; what lies behind a row's end, or in a step behind the
+    // last one, is sent there.
     __device__ __forceinline__ void request(int q, int step, uint8_t *stage) const {
         const bool isw = q < C::WI;
-        const int row = ((isw ? q : q - C::WI) * C::NW + wave) * (1024 / (isw ? C::WROW : 128)), part = row / (isw ? C::TN : C::TM);  // (the same for the wave)
-        const int k0 = C::X8 ? (s0 + step) * C::SK + part * 128 : (s0 + step) / 2 * (2 * C::SK) + (step & 1) * 64 + part * 128, soff = isw || C::X8 ? k0 : k0 * 2;
-        const uint32_t o = (isw ? wplace : xplace) < (isw || C::X8 ? kend : kend * 2) - soff ? off[q] : kOut;
-        const bool two = isw && C::GATED && second(row % C::TN);
+        const int row = ((isw ? q : q - C::WI) * C::NW + wave) * (1024 / (isw ? C::WROW : 128)), height = isw ? C::TN : C::TM, part = row / height, r = row % height;  // (the wave's)
+        const int k0 = first_k(step, part), each = isw || C::X8 ? 1 : 2;
+        const bool indexed = C::GATED && !isw, surplus = !isw && !indexed && row >= C::TM * C::XPARTS;
+        const uint32_t lane_off = isw ? wlane : xlane[indexed ? q - C::WI : 0];
+        const uint32_t o = (isw ? wplace : xplace) < (kend - k0) * each && !surplus ? lane_off : kOut;
+        const int soff = k0 * each + (isw ? wrow(r) * wbytes : indexed ? 0 : r * xbytes);
+        const bool two = isw && C::GATED && second(r);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(isw ? (two ? w2rsrc : wrsrc) : xrsrc, (__attribute__((address_space(3))) void *)(stage + (q * C::NW + wave) * 1024), 16, o, soff,
                                                  0, 0);
     }
@@ -187,7 +195,7 @@ __device__ __forceinline__ void sum_fp8(Source<C> &src, f32x4 (&acc)[2 * C::NB][
         return __builtin_bit_cast(i32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     i32x8 wf[2][2], xf[M];
-    float s[2][SW][M];
+    float s[SW][M];
     auto read_w = [&](int pair, int j, int buf, const uint8_t *stage) { wf[buf][j] = fragment(stage + wl + (pair * 2 + j) * 2048); };
     auto read_x = [&](int b, const uint8_t *stage) { xf[b] = fragment(stage + xl + b * 2048); };
     float sw[SW], sx[M];  // of the next step
@@ -198,32 +206,31 @@ __device__ __forceinline__ void sum_fp8(Source<C> &src, f32x4 (&acc)[2 * C::NB][
 #pragma unroll
         for (int b = 0; b < M; ++b) sx[b] = src.scale(step >> 1, e, wm * C::MB * 32 + b * 16 + l16);
     };
-    auto multiply_s = [&](int par) {
+    auto multiply_s = [&] {
 #pragma unroll
         for (int b = 0; b < M; ++b)
 #pragma unroll
-            for (int j = 0; j < SW; ++j) s[par][j][b] = sx[b] * sw[j];
+            for (int j = 0; j < SW; ++j) s[j][b] = sx[b] * sw[j];
     };
     read_s(0);
-    multiply_s(0);
 #pragma unroll
     for (int b = 0; b < M; ++b) read_x(b, lds);
 #pragma unroll
     for (int j = 0; j < 2; ++j) read_w(0, j, 0, lds);
 
     constexpr int NE = 2 * M, NP = PAIRS * NE, DB = LAG + 1;  // MFMAs of a pair of weight rows' blocks, of a step
-    static_assert(NP % DB == 0, "results of a step in the same places");
+    static_assert(NP % DB == 0 && LAG < NE, "results of a step in the same places, its scales used before the next ones are read");
     f32x4 d[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i) d[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < M; ++b)
 #pragma unroll
-        for (int j = 0; j < SW; ++j) s[1][j][b] = 0.f;
-    auto add = [&](auto at_c, int par) {  // the result of MFMA number at of a step
+        for (int j = 0; j < SW; ++j) s[j][b] = 0.f;
+    auto add = [&](auto at_c) {  // the result of MFMA number at of a step
         constexpr int at = decltype(at_c)::value, pair = at / NE, a = 2 * pair + at % 2, b = at % NE / 2;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) acc[a][b][v] = __builtin_fmaf(d[at % DB][v], s[par][C::GATED ? pair & 1 : 0][b], acc[a][b][v]);
+        for (int v = 0; v < 4; ++v) acc[a][b][v] = __builtin_fmaf(d[at % DB][v], s[C::GATED ? pair & 1 : 0][b], acc[a][b][v]);
     };
     int slot = 0;
     // Step i, the parity of its registers (par).  In front of the last pair of blocks of weight rows, whose fragments are in registers, the wave waits for its part of
@@ -249,15 +256,14 @@ __device__ __forceinline__ void sum_fp8(Source<C> &src, f32x4 (&acc)[2 * C::NB][
             auto one = [&](auto ec) {
                 constexpr int e = decltype(ec)::value, at = P * NE + e, j = e % 2, b = e / 2;
                 d[at % DB] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[buf][j], xf[b], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-                if constexpr (at >= LAG) add(std::integral_constant<int, at - LAG>{}, par);
-                else add(std::integral_constant<int, NP + at - LAG>{}, par ^ 1);
+                if constexpr (at == LAG) multiply_s();  // (the last results of the step before have been added)
+                add(std::integral_constant<int, at >= LAG ? at - LAG : NP + at - LAG>{});
                 if constexpr (!late) {
                     if constexpr (e == 0 || e == M) read_w(P + 1, e / M, buf ^ 1, cur);
                 } else {
                     if constexpr (e == 0 || e == M) read_w(0, e / M, buf ^ 1, nxt);
                     if constexpr (j == 1) read_x(b, nxt);
-                    if constexpr (e == 0) read_s(i + 1);
-                    if constexpr (e == NE - 1) multiply_s(par ^ 1);  // (the last use of the step before's was LAG MFMAs into this one)
+                    if constexpr (e == NE - 1) read_s(i + 1);  // (behind multiply_s, which is at LAG < NE)
                 }
                 const int pos = at + (late ? -LATE : NP - LATE);
 #pragma unroll
@@ -277,7 +283,7 @@ __device__ __forceinline__ void sum_fp8(Source<C> &src, f32x4 (&acc)[2 * C::NB][
         step(i, std::integral_constant<int, 0>{});
         step(i + 1, std::integral_constant<int, 1>{});
     }
-    auto rest = [&](auto ec) { add(std::integral_constant<int, NP - LAG + decltype(ec)::value>{}, 1); };
+    auto rest = [&](auto ec) { add(std::integral_constant<int, NP - LAG + decltype(ec)::value>{}); };
     each(rest, std::make_integer_sequence<int, LAG>{});
 }
 
