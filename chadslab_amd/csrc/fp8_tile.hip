@@ -94,6 +94,9 @@ struct Source {
         wplace = 16 * ((lane % PPR) ^ key<C::WROW>(wave * (64 / PPR) + lane / PPR));
         xplace = 16 * ((lane % 8) ^ key<128>(wave * 8 + lane / 8));
         wlane = (uint32_t)(lane / PPR) * (uint32_t)wbytes + wplace;
+    }
+    // The rest, of which an index may have to be waited for
+    __device__ __forceinline__ void rows(const MxTile &t, int n0) {
         if constexpr (C::GATED) {
 #pragma unroll
             for (int q = 0; q < C::XI; ++q) {
@@ -122,6 +125,24 @@ struct Source {
             for (int e = 0; e < C::GE; ++e)
                 if (whole * C::GE + e < G) tail[e] = srow[whole * C::GE + e];
         if (whole == 0) srow = global(kNoScales);  // (readable, for the loop)
+    }
+    // What comes before the first step: stages 0 .. ST - 2, the weights of the first two in front of everything that waits for an index; ends with stage 0 and the first
+    // group's scales in LDS
+    __device__ __forceinline__ void begin(const MxTile &t, int n0) {
+        constexpr int FIRST = C::ST > 2 ? 2 : 1;
+#pragma unroll
+        for (int j = 0; j < FIRST; ++j)
+#pragma unroll
+            for (int q = 0; q < C::WI; ++q) request(q, j, lds + j * C::STAGE);
+        rows(t, n0);
+        scales(0);
+#pragma unroll
+        for (int j = 0; j < C::ST - 1; ++j)
+#pragma unroll
+            for (int q = j < FIRST ? C::WI : 0; q < C::REQ; ++q) request(q, j, lds + j * C::STAGE);
+        keep(0);
+        wait_vmcnt<C::ST == 2 ? 0 : C::XI + (C::ST - 3) * C::REQ>();  // all but the second stage's activations and what came behind them
+        wg_barrier();
     }
     // row r of the tile's weights: of which matrix, which row behind n0
     __device__ __forceinline__ static bool second(int r) { return C::GATED && (r >> 5 & 1); }
@@ -167,7 +188,7 @@ struct Source {
 
 // ---- FP8 x.  A lane's part of a block of 16 rows: row l16, two pieces of 16 k of the step's block wk; of a result: activation row l16, n = 4 kg + 0..3
 template <typename C>
-__device__ __forceinline__ void sum_fp8(Source<C> &src, f32x4 (&acc)[2 * C::NB][2 * C::MB]) {
+__device__ __forceinline__ void sum_fp8(Source<C> &src, const MxTile &t, int n0, f32x4 (&acc)[2 * C::NB][2 * C::MB]) {
     constexpr int N = 2 * C::NB, M = 2 * C::MB, PAIRS = C::NB, ST = C::ST, LAG = 3, SW = C::GATED ? 2 : 1;
     const int lane = src.lane, wave = src.wave, l16 = lane & 15, kg = lane >> 4, wn = wave % C::WN, wm = wave / C::WN % C::WM, wk = wave / (C::WN * C::WM);
     uint8_t *const lds = src.lds;
@@ -176,14 +197,7 @@ __device__ __forceinline__ void sum_fp8(Source<C> &src, f32x4 (&acc)[2 * C::NB][
 #pragma unroll
         for (int b = 0; b < M; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    src.scales(0);
-#pragma unroll
-    for (int j = 0; j < ST - 1; ++j)
-#pragma unroll
-        for (int r = 0; r < C::REQ; ++r) src.request(r, j, lds + j * C::STAGE);
-    src.keep(0);
-    wait_vmcnt<(ST - 2) * C::REQ>();
-    wg_barrier();
+    src.begin(t, n0);
 
     // (row r = 16 i + l16: key (r >> 1) & 7 = l16 >> 1)
     const uint32_t wl = (wk * C::TN + wn * C::NB * 32 + l16) * 128, xl = C::W_STAGE + (wk * C::TM + wm * C::MB * 32 + l16) * 128;
@@ -290,7 +304,7 @@ __device__ __forceinline__ void sum_fp8(Source<C> &src, f32x4 (&acc)[2 * C::NB][
 // ---- bf16 x.  A lane's part of a block of 32 rows: row l32; of the wave's 64 k of a step 32, in two pieces of 16; a slice is 8 of them, 16 bytes of x; of
 // a result: activation row l32, n = 8 g + 4 kq + 0..3 for g = 0..3
 template <typename C>
-__device__ __forceinline__ void sum_bf16(Source<C> &src, f32x16 (&acc)[C::NB][C::MB]) {
+__device__ __forceinline__ void sum_bf16(Source<C> &src, const MxTile &t, int n0, f32x16 (&acc)[C::NB][C::MB]) {
     constexpr int NB = C::NB, MB = C::MB, ST = C::ST, SL = 4, AH = NB * MB < 8 ? 2 : 1, FB = 2 * AH;  // AH: how many slices ahead fragments are read
     const int lane = src.lane, wave = src.wave, l32 = lane & 31, kq = lane >> 5, wn = wave % C::WN, wm = wave / C::WN % C::WM, wk = wave / (C::WN * C::WM);
     uint8_t *const lds = src.lds;
@@ -302,14 +316,7 @@ __device__ __forceinline__ void sum_bf16(Source<C> &src, f32x16 (&acc)[C::NB][C:
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[a][b][v] = d[a][b][v] = 0.f;
 
-    src.scales(0);
-#pragma unroll
-    for (int j = 0; j < ST - 1; ++j)
-#pragma unroll
-        for (int r = 0; r < C::REQ; ++r) src.request(r, j, lds + j * C::STAGE);
-    src.keep(0);
-    wait_vmcnt<(ST - 2) * C::REQ>();
-    wg_barrier();
+    src.begin(t, n0);
 
     // the lane's h-th piece of 16 values is 2 kq + h of the part's four; of x there are twice as many
     const uint32_t wkey = key<64>(l32), xkey = key<128>(l32);
@@ -428,7 +435,7 @@ __device__ __forceinline__ void tile_body(const Fp8Product &p, const MxTile &t, 
     f32x4 sum[NB][MB][4];
     if constexpr (C::X8) {
         f32x4 acc[2 * NB][2 * MB];
-        sum_fp8<C>(src, acc);
+        sum_fp8<C>(src, t, n0, acc);
 #pragma unroll
         for (int a = 0; a < NB; ++a)
 #pragma unroll
@@ -437,7 +444,7 @@ __device__ __forceinline__ void tile_body(const Fp8Product &p, const MxTile &t, 
                 for (int g = 0; g < 4; ++g) sum[a][b][g] = acc[2 * a + g / 2][2 * b + g % 2];
     } else {
         f32x16 acc[NB][MB];
-        sum_bf16<C>(src, acc);
+        sum_bf16<C>(src, t, n0, acc);
 #pragma unroll
         for (int a = 0; a < NB; ++a)
 #pragma unroll
