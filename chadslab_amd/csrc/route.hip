@@ -105,38 +105,57 @@ __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, i
     const auto larger = [](auto a, auto b) { return a > b ? a : b; };
     float zr[PER];
     bool masked[PER];
+    bool whole = false;
+    if constexpr (PER % 4 == 0) {  // in quads where they are whole
+        whole = E == L * PER && (reinterpret_cast<uintptr_t>(z) & 15) == 0;  // (rows of 16 bytes' multiples: all tokens alike)
+        if (whole)
+#pragma unroll
+            for (int i = 0; i < PER / 4; ++i) {
+                const f32x4 v = reinterpret_cast<const f32x4 *>(z)[ls * (PER / 4) + i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) zr[4 * i + j] = v[j];
+            }
+    }
+    float bias[WIDE ? PER : 1];
+    if constexpr (WIDE)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) bias[i] = r.bias ? r.bias[ls * PER + i < E ? ls * PER + i : E - 1] : 0.f;
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int e = ls * PER + i;
-        zr[i] = e < E ? z[e] : -INFINITY;
+        zr[i] = whole ? zr[i] : e < E ? z[e] : -INFINITY;
         masked[i] = !(zr[i] > -INFINITY);  // NaN too
         top = masked[i] ? top : fmaxf(top, zr[i]);
     }
     top = over_lanes<L>(top, larger);
     V c[PER];      // what chooses
-    double s[WIDE ? PER : 1];
     V total = 0;   // of the softmax
+    const float from_top = top > -INFINITY ? top : 0.f;
     if constexpr (WIDE) {
+        // (one loop for each, with nothing in it to branch about: the lane's exponentials run into each other)
+        if (r.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            s[i] = masked[i] ? 0.0 : r.sigmoid ? 1.0 / (1.0 + exp(-(double)zr[i])) : exp((double)zr[i] - (double)top);
-            total += s[i];
-        }
-        if (!r.sigmoid) {
+            for (int i = 0; i < PER; ++i) c[i] = 1.0 / (1.0 + exp(-(double)(masked[i] ? 0.f : zr[i])));
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                c[i] = exp((double)(masked[i] ? from_top : zr[i]) - (double)from_top);
+                total += masked[i] ? 0.0 : c[i];
+            }
             total = over_lanes<L>(total, [](double a, double b) { return a + b; });
 #pragma unroll
-            for (int i = 0; i < PER; ++i) s[i] = masked[i] ? 0.0 : s[i] / total;
+            for (int i = 0; i < PER; ++i) c[i] /= total;
         }
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = ls * PER + i;
-            c[i] = masked[i] ? -1e300 : s[i] + (r.bias && e < E ? (double)r.bias[e] : 0.0);
-        }
+        for (int i = 0; i < PER; ++i) c[i] = masked[i] ? -1e300 : c[i] + (double)bias[i];
     } else {
         if (!r.sigmoid && !r.renorm) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) total += masked[i] ? 0.f : expf(zr[i] - top);
+            for (int i = 0; i < PER; ++i) {
+                const float e = expf(masked[i] ? 0.f : zr[i] - from_top);
+                total += masked[i] ? 0.f : e;
+            }
             total = over_lanes<L>(total, [](float a, float b) { return a + b; });
         }
 #pragma unroll
@@ -169,11 +188,23 @@ __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, i
         if (q > 8) two.template join<8>();
         if (q > 16) two.template join<16>();
         const int g = ls / q;
-        const V value = r.group_sum == 2 ? two.a + two.b : two.a;
+        // (a sum of two, one of them masked: behind all sums without, by the other one)
+        const bool cut = WIDE && r.group_sum == 2 && two.a > V(-1e299) && two.b < V(-1e299);
+        const V value = cut ? two.a : r.group_sum == 2 ? two.a + two.b : two.a;
+        const unsigned long long cuts = __ballot(cut);
         int rank = 0;
-        for (int h = 0; h < G; ++h) {
-            const V o = from_lane<L>(value, seg + h * q);
-            rank += o > value || (o == value && h < g);
+        if (!cuts) {  // (one answer for the wave)
+            for (int h = 0; h < G; ++h) {
+                const V o = from_lane<L>(value, seg + h * q);
+                rank += o > value || (o == value && h < g);
+            }
+        } else {
+            for (int h = 0; h < G; ++h) {
+                const int from = seg + h * q;
+                const V o = from_lane<L>(value, from);
+                const bool ocut = cuts >> from & 1, one = ocut != cut && o > V(-1e299) && value > V(-1e299);  // (what is all masked is behind both)
+                rank += one ? cut : o > value || (o == value && h < g);
+            }
         }
         const unsigned long long kept = __ballot(g < G && rank < r.top_groups) >> seg;
 #pragma unroll
@@ -199,42 +230,30 @@ __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, i
     };
     own();
     float zc = -INFINITY;
-    double sc = 0.0;
     chosen = 0;
     for (int k = 0; k < r.top_k; ++k) {
         const K most = most_of<L>(best);
         const unsigned long long hold = __ballot(best == most) & seg_mask;
         const int winner = __ffsll((long long)hold) - 1;
         const int e = from_lane<L>(ls * PER + at, winner);
-        float zw = zr[0];
-        double sw = 0.0;
-        if constexpr (WIDE) sw = s[0];
+        if (ls == k) chosen = e;
+        if constexpr (PER <= 4) {
+            float zw = zr[0];
 #pragma unroll
-        for (int i = 1; i < PER; ++i)
-            if (at == i) {
-                zw = zr[i];
-                if constexpr (WIDE) sw = s[i];
-            }
-        zw = from_lane<L>(zw, winner);
-        if constexpr (WIDE) sw = from_lane<L>(sw, winner);
-        if (ls == k) {
-            chosen = e;
-            zc = zw;
-            sc = sw;
+            for (int i = 1; i < PER; ++i) zw = at == i ? zr[i] : zw;
+            zw = from_lane<L>(zw, winner);
+            if (ls == k) zc = zw;
         }
-        if (lane == winner) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (at == i) key[i] = 0;
-            own();
-        }
+        for (int i = 0; i < PER; ++i) key[i] = lane == winner && at == i ? 0 : key[i];
+        own();
     }
+    if constexpr (PER > 4) zc = ls < r.top_k ? z[chosen] : -INFINITY;
+    // the chosen ones' scores again, from their logits
     const bool has = ls < r.top_k, none = !(zc > -INFINITY);
-    if constexpr (!WIDE) {
-        const float from = r.renorm ? over_lanes<L>(has && !none ? zc : -INFINITY, larger) : top;
-        sc = !has || none ? 0.0 : r.sigmoid ? 1.0 / (1.0 + exp(-(double)zc)) : exp((double)zc - (double)from);
-        if (!r.sigmoid && !r.renorm && !none) sc /= (double)total;
-    }
+    const float from = !WIDE && r.renorm ? over_lanes<L>(has && !none ? zc : -INFINITY, larger) : top;
+    double sc = !has || none ? 0.0 : r.sigmoid ? 1.0 / (1.0 + exp(-(double)zc)) : exp((double)zc - (double)from);
+    if (!r.sigmoid && (WIDE || !r.renorm) && !none) sc /= (double)total;
     if (!has) sc = 0.0;
     if (r.renorm) {
         const double sum = over_lanes<L>(sc, [](double a, double b) { return a + b; });

@@ -57,6 +57,21 @@ def test_groups(ops, experts, groups):
                     check(ops, z, bias, top_k=top_k, score=score, groups=groups, top_groups=top_groups, group_sum=group_sum)
 
 
+@pytest.mark.parametrize("experts,groups,top_k", [(8, 2, 4), (16, 1, 16), (33, 3, 8), (40, 1, 6), (60, 4, 4), (64, 8, 8), (64, 1, 17), (100, 5, 12), (128, 8, 8), (160, 8, 6), (160, 20, 6),
+                                                  (256, 8, 8), (256, 1, 16), (300, 6, 8), (384, 8, 8), (512, 16, 16), (512, 1, 8)])
+def test_many_tokens(ops, experts, groups, top_k):
+    """As many as take fewer lanes each; ties and masked experts among them."""
+    r = np.random.Generator(np.random.PCG64(experts + groups))
+    z = (r.standard_normal((2500, experts)) * 2).astype(np.float32)
+    z[::7] = np.rint(z[::7])
+    z[::11][r.random(z[::11].shape) < 0.3] = -np.inf
+    bias = (r.standard_normal(experts) * 0.1).astype(np.float32)
+    top_groups = max(1, -(-top_k // (experts // groups)), groups // 2)
+    for how in (dict(), dict(score="sigmoid", renorm=False, scale=2.5)):
+        check(ops, z, None, top_k=top_k, groups=groups, top_groups=top_groups, **how)
+        check(ops, z, bias, top_k=top_k, groups=groups, top_groups=top_groups, group_sum=2 if groups > 1 and experts // groups > 1 else 1, **how)
+
+
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("experts,groups", [(8, 1), (16, 4), (40, 1), (64, 8), (256, 8), (400, 1)])
 def test_ties_go_to_the_lowest_index(ops, experts, groups, wide):
