@@ -83,7 +83,7 @@ struct Fp8Product {
     int x_rows = 0;           // ... which has so many
     const uint8_t *w2 = nullptr;
     const float *w2s = nullptr;
-    // ... with 8-bit x and more rows than are streamed also in 8 bits: values [M,N], scales [M,ceil(N/128)] (then y is not written)
+    // ... with 8-bit x and more rows than are streamed always in 8 bits: values [M,N], scales [M,ceil(N/128)] (then y is not written)
     uint8_t *h8 = nullptr;
     float *h8s = nullptr;
     // K in parts of part_k (a multiple of 1024; 0: one part), the sums of part i as fp32 [M,N] from y + i M N on

@@ -19,13 +19,14 @@ static const TileTime kBf16[F8_TILES] = {{64, 32, 1, 2.28f, 2.1f, 1.87f, 2.73f},
 static const TileTime kFp8[F8_TILES] = {{64, 32, 1, 2.13f, 2.47f, 1.18f, 1.86f}, {64, 64, 1, 2.41f, 2.64f, 1.7f, 2.86f}, {128, 64, 1, 2.14f, 2.38f, 2.61f, 4.48f}, {128, 64, 2, 2.16f, 1.72f, 3.62f, 8.51f},
                                         {256, 64, 1, 1.28f, 2.86f, 4.85f, 8.03f}, {256, 64, 2, 0.0f, 1e9f, 0.0f, 0.0f}, {128, 128, 1, 2.24f, 2.79f, 4.06f, 6.65f}, {128, 128, 2, 2.26f, 1.63f, 5.19f, 12.67f},
                                         {256, 128, 1, 1.11f, 3.87f, 6.66f, 10.62f}, {256, 256, 1, 2.73f, 3.14f, 10.74f, 16.61f}};
-static Fp8TilePick pick(int M, int N, int K, int E, bool x_fp8, bool gated, bool h8, int most_parts) {
+static Fp8TilePick pick(int M, int N, int K, int E, bool x_fp8, bool gated, int most_parts) {
     Fp8TilePick best = {F8_128x128, 0};
     float least = 1e30f;
     for (int i = 0; i < F8_TILES; ++i) {
         const TileTime &t = (x_fp8 ? kFp8 : kBf16)[i];
         const int tn = gated ? t.tn / 2 : t.tn;
-        if (t.round > 1e8f || (gated && (t.tn < 128 || i == F8_128x128 || i == F8_256x256 || (h8 && t.tn < 256)))) continue;
+        // (gate and up: half the columns of each; results of 8 bits need a whole block of 128)
+        if (t.round > 1e8f || (gated && (t.tn < (x_fp8 ? 256 : 128) || i == F8_128x128 || i == F8_256x256))) continue;
         // rows by group: between the tiles of groups of one size and those of exponentially distributed sizes
         const float mean = (float)M / E > 1.f ? (float)M / E : 1.f, hit = E * (1.f - expf(-(float)M / E)), even = mean / t.tm + 0.3f;
         const float tm = E > 1 ? hit * 0.5f * ((even > 1.f ? even : 1.f) + 1.f / (1.f - expf(-t.tm / mean))) : (float)mx_ceil(M, t.tm);
@@ -52,7 +53,7 @@ static Fp8TilePick pick(int M, int N, int K, int E, bool x_fp8, bool gated, bool
 }
 
 Fp8TilePick fp8_tile_pick(const Fp8Product &p, int most_parts) {
-    return pick(p.M, p.N, p.K, p.offsets ? p.E : 1, p.xs != nullptr, p.w2 != nullptr, p.h8 != nullptr, most_parts);
+    return pick(p.M, p.N, p.K, p.offsets ? p.E : 1, p.xs != nullptr, p.w2 != nullptr, most_parts);
 }
 
 // Which of the two: the tiles' requests do not reach over rows as long as the streams' do

@@ -487,29 +487,28 @@ __device__ __forceinline__ void tile_body(const Fp8Product &p, const MxTile &t, 
 #pragma unroll
                 for (int v = 0; v < 4; ++v) out[a][b][g][v] = C::GATED ? silu_mul(sum[2 * a][b][g][v], sum[2 * a + 1][b][g][v]) : sum[C::GATED ? 2 * a : a][b][g][v];
     if constexpr (C::H8) {
-        if (p.h8) {  // through LDS in fp32, 16 lanes to a row's block
-            static_assert(C::WK == 1, "every wave has results");
-            constexpr int PITCH = TO * 4 + 16;
-            __syncthreads();
+        // through LDS in fp32, 16 lanes to a row's block
+        static_assert(C::WK == 1, "every wave has results");
+        constexpr int PITCH = TO * 4 + 16;
+        __syncthreads();
 #pragma unroll
-            for (int a = 0; a < NO; ++a)
+        for (int a = 0; a < NO; ++a)
 #pragma unroll
-                for (int b = 0; b < MB; ++b)
+            for (int b = 0; b < MB; ++b)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g)
-                        *reinterpret_cast<f32x4 *>(lds + ((wm * MB + b) * 32 + quad_m(g)) * PITCH + ((wn * NO + a) * 32 + quad_n(g)) * 4) = out[a][b][g];
-            __syncthreads();
-            const int l = tid & 15, G = fp8_blocks(p.N);
-            for (int m = tid >> 4; m < t.rows; m += C::T / 16) {  // (columns behind N are sums of zeros)
-                const f32x4 lo = reinterpret_cast<const f32x4 *>(lds + m * PITCH)[2 * l], hi = reinterpret_cast<const f32x4 *>(lds + m * PITCH)[2 * l + 1];
-                const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                const Fp8Scale c(max_of_16(absmax8(f)));
-                const size_t row = (size_t)(t.row0 + m);
-                if (l * 8 < src.nrows) *reinterpret_cast<u32x2 *>(p.h8 + row * p.N + n0 + l * 8) = c.values(f);
-                if (l == 0) p.h8s[row * G + (n0 >> 7)] = c.scale;
-            }
-            return;
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4 *>(lds + ((wm * MB + b) * 32 + quad_m(g)) * PITCH + ((wn * NO + a) * 32 + quad_n(g)) * 4) = out[a][b][g];
+        __syncthreads();
+        const int l = tid & 15, G = fp8_blocks(p.N);
+        for (int m = tid >> 4; m < t.rows; m += C::T / 16) {  // (columns behind N are sums of zeros)
+            const f32x4 lo = reinterpret_cast<const f32x4 *>(lds + m * PITCH)[2 * l], hi = reinterpret_cast<const f32x4 *>(lds + m * PITCH)[2 * l + 1];
+            const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            const Fp8Scale c(max_of_16(absmax8(f)));
+            const size_t row = (size_t)(t.row0 + m);
+            if (l * 8 < src.nrows) *reinterpret_cast<u32x2 *>(p.h8 + row * p.N + n0 + l * 8) = c.values(f);
+            if (l == 0) p.h8s[row * G + (n0 >> 7)] = c.scale;
         }
+        return;
     }
     if (!p.y_bf16) {
         if (wk > 0) return;
@@ -631,13 +630,8 @@ int fp8_tile_launch(const Fp8Product &p, int tile, hipStream_t st) {
     //                                                       WN WM WK NB MB SK ST
     if (p.w2) {
         if (p.xs) {
-            switch (tile) {
-            case F8_128x64: return launch<true, true, 2, 2, 2, 2, 1, 256, 3>(p, st);
-            case F8_128x64P: return launch<true, true, 2, 2, 1, 2, 1, 128, 3>(p, st);
-            case F8_256x64: return launch<true, true, 4, 2, 1, 2, 1, 128, 3>(p, st);
-            case F8_128x128P: return launch<true, true, 2, 2, 1, 2, 2, 128, 2>(p, st);
-            default: return launch<true, true, 4, 2, 1, 2, 2, 128, 3>(p, st);
-            }
+            if (tile == F8_256x64) return launch<true, true, 4, 2, 1, 2, 1, 128, 3>(p, st);
+            return launch<true, true, 4, 2, 1, 2, 2, 128, 3>(p, st);
         }
         switch (tile) {
         case F8_128x64: return launch<false, true, 2, 2, 2, 2, 1, 128, 4>(p, st);

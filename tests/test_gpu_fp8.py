@@ -423,8 +423,9 @@ GROUPED = dict(score="sigmoid", groups=4, top_groups=2, group_sum=2, scale=2.5)
                                                     (9, 48, 144, 300, dict(top_k=8, score="sigmoid"))])
 def test_moe(ops, tokens, h, f, experts, how, x8):
     """What is rounded is h to bf16 (2^-8; its errors are independent, so the norm of what they do is at most that) and the result (2^-8), and the fp32 sums
-    and weights by 2^-18.  With 8-bit activations h is not rounded to bf16; it is quantised here as there, but from sums that differ by some 2^-20, so that a
-    value in about 2^16 goes to the other neighbour, a 2^-3 of itself away: 2^-3 * 2^-8 of the norm."""
+    and weights by 2^-18.  With 8-bit activations h is not rounded to bf16; it is quantised here as there, but from sums that differ: streamed by some 2^-20, so
+    that a value in about 2^16 goes to the other neighbour, a 2^-3 of itself away (2^-3 * 2^-8 of the norm); on the tiles, whose sums are cut, by some 2^-15 of the norm, so
+    that one in 2^11 does (2^-3 * 2^-5.5), and the down product's sums are cut as well (2^-15): less than the 2^-8 that h in bf16 would take."""
     r = np.random.Generator(np.random.PCG64(tokens + h + f))
     triple = tuple(weights(r, *s, experts) for s in ((f, h), (f, h), (h, f)))
     x = activations(r, tokens, h, x8)
