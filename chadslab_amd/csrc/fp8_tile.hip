@@ -293,6 +293,8 @@ __device__ __forceinline__ void sum_fp8(Source<C> &src, const MxTile &t, int n0,
 #pragma unroll
     for (int r = 0; r < C::requested(NP - LATE, NP); ++r) src.request(r, ST - 1, lds + (ST - 1) * C::STAGE);
     // (A step behind the last one works on zeros.  No branch inside the loop: the compiler would move MFMAs behind it, past the barrier.)
+    // Of a SIMD's two waves one goes first, so that one's MFMAs meet the other's FMAs and reads: 4096 x 14336 x 4096 242 us instead of 249
+    if (wave & 4) __builtin_amdgcn_s_setprio(1);
     for (int i = 0; i < src.steps; i += 2) {
         step(i, std::integral_constant<int, 0>{});
         step(i + 1, std::integral_constant<int, 1>{});
