@@ -11,6 +11,9 @@
 // edges.  Scales: a thread loads two steps' of a row of x, or of a block of weight rows, two steps ahead, and puts them into LDS.  16-byte
 // pieces of a row are XOR-swizzled by the row so that the 16 rows that a read takes at a time cover all banks.  WK > 1: waves of a workgroup split the k of a
 // step and add their sums at the end, so that a small tile too has eight waves to hide its reads.
+// us, matrix cores' busy share: 4096 x 14336 x 4096 8-bit 236, 50 % (2.0 PFLOP/s; 256 x 256); 1000 x 4096 x 14336 bf16 130, 45 % (0.9 PFLOP/s; 128 x 128, one round); 2048 rows by group on
+// 16 of 4096 x 2048 8-bit 42, 23 %; gate and up of 6000 pairs, 64 experts of 1408 x 2048, 112, 19 % (400 MB, 3.6 TB/s).  Of 4096^3 with 256 x 256 tiles, 69 us, some 8 are outside
+// the loop, 13 are the requests and 9 the scales' FMAs; the MFMAs alone take 32.
 #include <cmath>
 #include <type_traits>
 #include <utility>
