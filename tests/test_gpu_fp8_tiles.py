@@ -37,9 +37,8 @@ def test_every_tile_by_group(ops, x8):
             assert not y[:bounds[0]].any() and not y[bounds[-1]:].any()
 
 
-def layer_in_64(ops, x, logits, triple, top_k):
+def layer_in_64(ops, x, triple, idx, weight):
     """-> the result and S: per token, sum over its experts of weight * (|h| |down|^T)"""
-    idx, weight = ops.moe_route(logits, top_k=top_k)
     a, y = x64(x), torch.zeros(x.shape[0] if isinstance(x, torch.Tensor) else x.M, triple[2].N, dtype=torch.float64, device=DEV)
     s = torch.zeros_like(y)
     for e in range(triple[0].E):
@@ -77,11 +76,49 @@ def test_every_tile_of_the_layer(ops, x8, which):
         triple = (*(weights(r, f, h, e, values=narrow) for _ in range(2)), weights(r, h, f, e))
         x = activations(r, pairs // 2, h, x8, values=narrow)
         logits = torch.from_numpy(r.standard_normal((pairs // 2, e)).astype(np.float32)).to(DEV)
-        want, s = layer_in_64(ops, x, logits, triple, 2)
+        want, s = layer_in_64(ops, x, triple, *ops.moe_route(logits, top_k=2))
         off = (ops.moe_ffn(x, logits, triple, top_k=2).double() - want).norm()
         bound = (2 * 2.0 ** -8 + 2.0 ** -18) * want.norm() + (7 * 2.0 ** -13 * s.norm() if x8 else 0)
         assert off <= bound, (tile, part_k, float(off / bound))
     assert len(seen) >= (2 if x8 and which != "down" else 5)
+
+
+@KINDS
+@pytest.mark.parametrize("tokens,experts,top_k,most", [(20000, 512, 8, 0), (13000, 7, 1, 3), (1537, 300, 8, 299)])
+def test_layer_of_many_pairs(ops, tokens, experts, top_k, most, x8):
+    """Sorted in one launch and, from some ten thousand pairs on, in two; an expert that most tokens take, and ones that nobody takes.  Bounds as above."""
+    r = np.random.Generator(np.random.PCG64(tokens))
+    h, f = 144, 80
+    triple = (*(weights(r, f, h, experts, values=narrow) for _ in range(2)), weights(r, h, f, experts))
+    x = activations(r, tokens, h, x8, values=narrow)
+    logits = torch.from_numpy(r.standard_normal((tokens, experts)).astype(np.float32)).to(DEV)
+    logits[:, most] += 3
+    logits[:, experts // 2] = -float("inf")
+    how = dict(top_k=top_k, score="sigmoid")
+    idx, weight = ops.moe_route(logits, **how)
+    want, s = layer_in_64(ops, x, triple, idx, weight)
+    off = (ops.moe_ffn(x, logits, triple, **how).double() - want).norm()
+    assert off <= (2 * 2.0 ** -8 + 2.0 ** -18) * want.norm() + (7 * 2.0 ** -13 * s.norm() if x8 else 0)
+
+
+@KINDS
+@pytest.mark.parametrize("n", [136, 75])
+def test_results_at_any_address(ops, n, x8):
+    """Results that begin at any element, from either kernel; what lies around them stays."""
+    r = np.random.Generator(np.random.PCG64(n))
+    k = 272
+    w = weights(r, n, k, 3, values=narrow)
+    for m in (5, 40, 300):
+        x = activations(r, m, k, x8, values=narrow)
+        offsets = torch.tensor([0, m // 3, m - 2, m], dtype=torch.int32, device=DEV)
+        for shift in (1, 2, 3, 4, 7):
+            room = torch.full((m * n + 16,), 5.0, dtype=torch.bfloat16, device=DEV)
+            y = room[shift:shift + m * n].view(m, n)
+            assert ops.qgemm(x, w.expert(1), out=y) is y
+            check(y, x64(x), w64(w.expert(1)))
+            assert ops.qgemm_grouped(x, w, offsets, out=y) is y
+            check_groups(y, x, w, offsets.tolist(), cut=False)
+            assert bool((room[:shift] == 5).all()) and bool((room[shift + m * n:] == 5).all())
 
 
 @KINDS
