@@ -67,6 +67,7 @@ struct Source {
     const Fp8Product &p;
     uint8_t *const lds;
     int tid, lane, wave, s0, kend, steps, nrows;  // s0: first step of the workgroup's part of K; nrows: result columns that there are
+    int groups, turn;  // of two steps; which of them is the first
     __amdgpu_buffer_rsrc_t wrsrc, w2rsrc, xrsrc;
     // of the lane's piece in a part of a row (the rows of a wave's requests of a kind are a multiple of 16 apart), and in a request's rows
     int wplace, xplace;
@@ -85,6 +86,12 @@ struct Source {
         kend = p.part_k && s0 * C::SK + p.part_k < p.K ? s0 * C::SK + p.part_k : p.K;
         steps = (kend - s0 * C::SK + C::SK - 1) / C::SK;
         nrows = p.N - n0 < C::TO ? p.N - n0 : C::TO;
+        groups = (steps + 1) / 2;
+        // Groups' weights come from memory once, and rows a large power of two apart (or a multiple of it) share its channels: workgroups that all go through k alike meet in a
+        // few of them.  So by group each begins at a k of its own and goes round.  us, all from 0 / each from its own: 1000 rows, 32 of 4096 x 4096 8-bit 130 / 97, bf16 131 / 105; 600
+        // rows, 8 of 8192 x 8192 192 / 119; 400 rows, 8 of 4096 x 12288 125 / 113; 1000 rows, 32 of 8192 x 1024 67 / 62; with rows of 1536, 2560, 5120, 6144, 7168 or 14336 bytes
+        // alike.  One matrix for all rows gains up to 6 % or loses 3 % and stays as it is.
+        turn = p.offsets ? (n0 / C::TO + 3 * t.group) % groups : 0;
         wbytes = p.K;
         xbytes = C::X8 ? p.K : p.K * 2;
         const size_t wfirst = (size_t)t.group * p.N + n0;
@@ -151,9 +158,12 @@ struct Source {
     __device__ __forceinline__ static bool second(int r) { return C::GATED && (r >> 5 & 1); }
     __device__ __forceinline__ static int wrow(int r) { return C::GATED ? (r >> 6) * 32 + (r & 31) : r; }
 
+    // which group comes in turn; behind the last one itself
+    __device__ __forceinline__ int turned(int group) const { return group >= groups ? group : group + turn - (group + turn >= groups ? groups : 0); }
     // k of part `part` of a step
     __device__ __forceinline__ int first_k(int step, int part) const {
-        return C::X8 ? (s0 + step) * C::SK + part * 128 : (s0 + step) / 2 * (2 * C::SK) + (step & 1) * 64 + part * 128;
+        const int pair = s0 / 2 + turned(step >> 1);  // (s0 is even)
+        return pair * (2 * C::SK) + (step & 1) * (C::X8 ? C::SK : 64) + part * 128;
     }
     // What of a request lies behind the last row is beyond the buffer's range, which counts the scalar offset too; what lies behind a row's end, or in a step behind the
     // last one, is sent there.
@@ -171,7 +181,7 @@ struct Source {
     }
     // group: of two steps, counted from the part's first
     __device__ __forceinline__ void scales(int group) {
-        const int g = s0 / 2 + group, at = (g < whole ? g : whole > 0 ? whole - 1 : 0) * C::GE;
+        const int g = s0 / 2 + turned(group), at = (g < whole ? g : whole > 0 ? whole - 1 : 0) * C::GE;
         typedef float group_t __attribute__((ext_vector_type(C::GE), aligned(4)));
         const group_t v = *(const __attribute__((address_space(1))) group_t *)(srow + at);
 #pragma unroll
@@ -179,9 +189,9 @@ struct Source {
     }
     __device__ __forceinline__ void keep(int group) const {
         float *const d = reinterpret_cast<float *>(lds + (tid < C::SROWS ? C::S_OFF + (group & 1) * C::S_GROUP + tid * 4 : C::DUMP + lane * 4));
-        const int pitch = tid < C::SROWS ? C::SPITCH : 64;
+        const int pitch = tid < C::SROWS ? C::SPITCH : 64, g = s0 / 2 + turned(group);
 #pragma unroll
-        for (int e = 0; e < C::GE; ++e) d[e * pitch] = s0 / 2 + group < whole ? sv[e] : tail[e];
+        for (int e = 0; e < C::GE; ++e) d[e * pitch] = g < whole ? sv[e] : tail[e];
     }
     // scale of row r (of SROWS) for block e of the group
     __device__ __forceinline__ float scale(int group, int e, int r) const {
