@@ -9,8 +9,8 @@
 // A workgroup's eight waves are S = 8 / WK side by side in n and WK along K.  A round is D units of each wave; its weights are requested a round ahead.  The activations
 // and all scales wait in LDS, a chunk of rounds at a time, requested before the first weights; behind K the activations are zeros, and a lane past the end of its weight
 // row reads that row's last bytes again.
-// us: 1 x 14336 x 4096 9.4-11 (the weights in turn with others: 5.2 TB/s, what a copy reaches), 6 x 11008 x 4096 with 8-bit x 9.1, 32 rows by group on 8 of 14336 x 4096 73 (470 MB,
-// 6.4 TB/s, some from the last-level cache).  The first form, a row's weights by one lane each, took 35.7, 36.5 and 223.
+// us: 1 x 14336 x 4096 10.6 (the weights in turn with others: 5.5 TB/s), 6 x 11008 x 4096 with 8-bit x 9.5, 32 rows by group on 8 of 14336 x 4096 73 (470 MB, 6.4 TB/s, some from the
+// last-level cache).  The first form, a row's weights by one lane each, took 35.7, 36.5 and 223.
 #include "fp8.h"
 
 namespace chadq {
@@ -95,8 +95,14 @@ __global__ __launch_bounds__(64 * F8S_W) __attribute__((amdgpu_waves_per_eu(4)))
     };
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
+    // Workgroups that all go through k alike meet in a few of the memory's channels where rows are a large power of two apart: each begins a chunk at a round of its own and
+    // goes round (where the last round is a whole one).  us, all from 0 / each from its own, weights from memory: 1 x 14336 x 4096 11.8 / 10.6, 8 x 8192 x 8192 17.8 / 13.0, 16 x 4096 x 4096
+    // 7.4 / 6.8, 64 rows by group with 8-bit x on 32 of 4096 x 8192 199 / 156; with rows of 2048, 7168 and 14336 bytes alike
+    int base = 0, len = rounds < chunk ? rounds : chunk, at = 0;  // the chunk's first round, its rounds, the round in it
+    const int first = U % (D << wk) == 0 ? (int)((blockIdx.y + 3 * t.group) % len) : 0;
+    at = first;
 #pragma unroll
-    for (int d = 0; d < D; ++d) load_w(0, d);
+    for (int d = 0; d < D; ++d) load_w(at, d);
     __builtin_amdgcn_sched_barrier(0);
 
     // the sums of lane (kg, m < 8): weight rows 2 kg and 2 kg + 1, activation row m
@@ -122,9 +128,8 @@ __global__ __launch_bounds__(64 * F8S_W) __attribute__((amdgpu_waves_per_eu(4)))
     }
     wait_vmcnt<D * NB>();  // what has been requested since the activations
     wg_barrier();
-    int at = 0;  // of the round in its chunk
-    auto turn = [&](int round, bool more) {
-        const int left = U - first_unit(round);  // units of the wave in this round
+    auto turn = [&](int next, bool more) {
+        const int left = U - first_unit(base + at);  // units of the wave in this round
 #pragma unroll
         for (int d = 0; d < D; ++d) {
             if (more || d < left) {
@@ -164,23 +169,29 @@ __global__ __launch_bounds__(64 * F8S_W) __attribute__((amdgpu_waves_per_eu(4)))
                     }
                 }
             }
-            if (more) load_w(round + 1, d);
+            if (more) load_w(next, d);
             __builtin_amdgcn_sched_barrier(0);
         }
-        ++at;
     };
-    int round = 0;
-    for (; round + 1 < rounds; ++round) {
-        turn(round, true);
-        if (at == chunk) {
-            wg_barrier();
-            stage(round + 1);
-            wait_vmcnt<0>();
-            wg_barrier();
-            at = 0;
+    for (;;) {
+        for (int i = 1; i < len; ++i) {
+            const int next = at + 1 == len ? 0 : at + 1;
+            turn(base + next, true);
+            at = next;
         }
+        const int begin = base + len;
+        if (begin == rounds) break;
+        const int size = rounds - begin < chunk ? rounds - begin : chunk, next = first < size ? first : 0;
+        turn(begin + next, true);
+        base = begin;
+        len = size;
+        at = next;
+        wg_barrier();
+        stage(base);
+        wait_vmcnt<0>();
+        wg_barrier();
     }
-    turn(round, false);
+    turn(0, false);
 
     // ---- results.  Lane (kg, m < 8): n = 2 kg and 2 kg + 1 of row m
     auto put = [&](int a, f32x2 g, f32x2 u) {
