@@ -89,9 +89,9 @@ struct Source {
         groups = (steps + 1) / 2;
         // Groups' weights come from memory once, and rows a large power of two apart (or a multiple of it) share its channels: workgroups that all go through k alike meet in a
         // few of them.  So by group each begins at a k of its own and goes round.  us, all from 0 / each from its own: 1000 rows, 32 of 4096 x 4096 8-bit 130 / 97, bf16 131 / 105; 600
-        // rows, 8 of 8192 x 8192 192 / 119; 400 rows, 8 of 4096 x 12288 125 / 113; 1000 rows, 32 of 8192 x 1024 67 / 62; with rows of 1536, 2560, 5120, 6144, 7168 or 14336 bytes
-        // alike.  One matrix for all rows gains up to 6 % or loses 3 % and stays as it is.
-        turn = p.offsets ? (n0 / C::TO + 3 * t.group) % groups : 0;
+        // rows, 8 of 8192 x 8192 192 / 119; 400 rows, 8 of 4096 x 12288 125 / 113; 1000 rows, 32 of 8192 x 1024 67 / 62; with rows of 2560, 5120, 6144, 7168 or 14336 bytes alike.  Rows of
+        // other lengths lie in all channels anyhow and lose 1 % by it.  One matrix for all rows gains up to 8 % (28672 x 8192, 20 rows) or loses 25 % (48 rows) and stays as it is.
+        turn = p.offsets && wbytes % 1024 == 0 ? (n0 / C::TO + 3 * t.group) % groups : 0;
         wbytes = p.K;
         xbytes = C::X8 ? p.K : p.K * 2;
         const size_t wfirst = (size_t)t.group * p.N + n0;
