@@ -73,7 +73,16 @@ __global__ __launch_bounds__(64 * F8S_W) __attribute__((amdgpu_waves_per_eu(4)))
             for (int c = 0; c < sq; ++c) to_lds4(row, U * 4, lds + (i * S + c * 64) * 4, (u0 + c * 64 + lane) * 4);
         }
     };
-    stage(0);
+    // Workgroups that all go through k alike meet in a few of the memory's channels where rows are a large power of two apart: each begins at a chunk and a round in it of its own and
+    // goes round (where the last one is whole).  us, all from 0 / each from its own, weights from memory: 1 x 14336 x 4096 11.8 / 10.6, 8 x 8192 x 8192 17.8 / 13.0, 16 x 4096 x 4096
+    // 7.4 / 6.8, 64 rows by group on 32 of 4096 x 8192 199 / 156; with rows of 2048, 7168 and 14336 bytes alike
+    const int own = U % (D << wk) == 0 ? (int)blockIdx.y + 3 * t.group : 0;
+    int len = rounds < chunk ? rounds : chunk;  // the chunk's rounds
+    const int start = GROUPED && len < rounds && rounds % len == 0 ? own / len * len % rounds : 0;
+    int base = start;  // the first of them
+    stage(base);
+    const int first = own % len;
+    int at = first;  // the round in it
 
     // ---- weights: the lane's row and piece of a unit
     const int wr = l16 >> 1, wb = X8 ? kg * 2 + (l16 & 1) : (l16 & 1) * 4 + kg, pieces = K >> 4;
@@ -95,14 +104,8 @@ __global__ __launch_bounds__(64 * F8S_W) __attribute__((amdgpu_waves_per_eu(4)))
     };
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    // Workgroups that all go through k alike meet in a few of the memory's channels where rows are a large power of two apart: each begins a chunk at a round of its own and
-    // goes round (where the last round is a whole one).  us, all from 0 / each from its own, weights from memory: 1 x 14336 x 4096 11.8 / 10.6, 8 x 8192 x 8192 17.8 / 13.0, 16 x 4096 x 4096
-    // 7.4 / 6.8, 64 rows by group with 8-bit x on 32 of 4096 x 8192 199 / 156; with rows of 2048, 7168 and 14336 bytes alike
-    int base = 0, len = rounds < chunk ? rounds : chunk, at = 0;  // the chunk's first round, its rounds, the round in it
-    const int first = U % (D << wk) == 0 ? (int)((blockIdx.y + 3 * t.group) % len) : 0;
-    at = first;
 #pragma unroll
-    for (int d = 0; d < D; ++d) load_w(at, d);
+    for (int d = 0; d < D; ++d) load_w(base + at, d);
     __builtin_amdgcn_sched_barrier(0);
 
     // the sums of lane (kg, m < 8): weight rows 2 kg and 2 kg + 1, activation row m
@@ -179,8 +182,8 @@ __global__ __launch_bounds__(64 * F8S_W) __attribute__((amdgpu_waves_per_eu(4)))
             turn(base + next, true);
             at = next;
         }
-        const int begin = base + len;
-        if (begin == rounds) break;
+        const int begin = base + len == rounds ? 0 : base + len;
+        if (begin == start) break;
         const int size = rounds - begin < chunk ? rounds - begin : chunk, next = first < size ? first : 0;
         turn(begin + next, true);
         base = begin;
