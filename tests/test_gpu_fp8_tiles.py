@@ -102,6 +102,41 @@ def test_layer_of_many_pairs(ops, tokens, experts, top_k, most, x8):
 
 
 @KINDS
+@pytest.mark.parametrize("k", [1024, 2048, 4096, 8192, 11264])
+def test_rows_a_power_of_two_apart(ops, k, x8):
+    """Where workgroups begin at a k of their own: groups and single matrices, streamed and in tiles, long rows in chunks; on every tile that the rule takes for such rows."""
+    r = np.random.Generator(np.random.PCG64(k))
+    for m in (1, 7, 16):
+        w, x = weights(r, 1290, k, values=narrow), activations(r, m, k, x8, values=narrow)
+        check(ops.qlinear(x, w), x64(x), w64(w))
+    seen = {"streamed": (9, 40, 1290), "uneven": (9, 71, 130)}
+    for e in (2, 9, 33):
+        for m in (17, 64, 300, 700, 1501, 4100, 8200):
+            for n in (64, 272, 1040, 2064, 8200):
+                if m > 8 * e and e * n * k <= 1 << 28 and m * n * k <= 1 << 34:
+                    seen.setdefault(pick(m, n, k, e, x8)[0], (e, m, n))
+    assert len(seen) >= 7 or k > 4096
+    for name, (e, m, n) in seen.items():
+        print(name, e, m, n, flush=True)
+        w, x = weights(r, n, k, e, values=narrow), activations(r, m, k, x8, values=narrow)
+        bounds = [0, *np.sort(r.integers(0, m + 1, e - 1)).tolist(), m]
+        check_groups(ops.qgemm_grouped(x, w, torch.tensor(bounds, dtype=torch.int32, device=DEV)), x, w, bounds, cut=False)
+
+
+@KINDS
+@pytest.mark.parametrize("pairs,h,f,e", [(60, 64, 8192, 2), (700, 272, 8192, 2), (2050, 512, 8192, 2), (300, 2048, 4096, 5), (700, 4096, 1024, 9), (66, 1024, 2048, 9)])
+def test_layer_of_rows_a_power_of_two_apart(ops, pairs, h, f, e, x8):
+    """Down products of that kind in parts of K among them.  Bounds as above."""
+    r = np.random.Generator(np.random.PCG64(pairs + h))
+    triple = (*(weights(r, f, h, e, values=narrow) for _ in range(2)), weights(r, h, f, e))
+    x = activations(r, pairs // 2, h, x8, values=narrow)
+    logits = torch.from_numpy(r.standard_normal((pairs // 2, e)).astype(np.float32)).to(DEV)
+    want, s = layer_in_64(ops, x, triple, *ops.moe_route(logits, top_k=2))
+    off = (ops.moe_ffn(x, logits, triple, top_k=2).double() - want).norm()
+    assert off <= (2 * 2.0 ** -8 + 2.0 ** -18) * want.norm() + (7 * 2.0 ** -13 * s.norm() if x8 else 0)
+
+
+@KINDS
 @pytest.mark.parametrize("n", [136, 75])
 def test_results_at_any_address(ops, n, x8):
     """Results that begin at any element, from either kernel; what lies around them stays."""
