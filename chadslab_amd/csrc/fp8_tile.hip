@@ -66,15 +66,15 @@ template <typename C>
 struct Source {
     const Fp8Product &p;
     uint8_t *const lds;
-    int tid, lane, wave, s0, kend, steps, nrows;  // s0: first step of the workgroup's part of K; nrows: result columns that there are
-    int groups, turn;  // of two steps; which of them is the first
+    int tid = 0, lane = 0, wave = 0, s0 = 0, kend = 0, steps = 0, nrows = 0;  // s0: first step of the workgroup's part of K; nrows: result columns that there are
+    int groups = 1, turn = 0;  // of two steps; which of them is the first
     __amdgpu_buffer_rsrc_t wrsrc, w2rsrc, xrsrc;
     // of the lane's piece in a part of a row (the rows of a wave's requests of a kind are a multiple of 16 apart), and in a request's rows
-    int wplace, xplace;
-    uint32_t wlane, xlane[C::GATED ? C::XI : 1];  // (GATED: rows through an index, each from x's first)
-    int wbytes, xbytes;  // of a row
-    const __attribute__((address_space(1))) float *srow;
-    int whole;
+    int wplace = 0, xplace = 0;
+    uint32_t wlane = 0, xlane[C::GATED ? C::XI : 1];  // (GATED: rows through an index, each from x's first)
+    int wbytes = 0, xbytes = 0;  // of a row
+    const __attribute__((address_space(1))) float *srow = nullptr;
+    int whole = 0;
     float sv[C::GE], tail[C::GE];
     static constexpr uint32_t kOut = 0x80000000u;
 
@@ -88,10 +88,11 @@ struct Source {
         nrows = p.N - n0 < C::TO ? p.N - n0 : C::TO;
         groups = (steps + 1) / 2;
         // Groups' weights come from memory once, and rows a large power of two apart (or a multiple of it) share its channels: workgroups that all go through k alike meet in a
-        // few of them.  So by group each begins at a k of its own and goes round.  us, all from 0 / each from its own: 1000 rows, 32 of 4096 x 4096 8-bit 130 / 97, bf16 131 / 105; 600
-        // rows, 8 of 8192 x 8192 192 / 119; 400 rows, 8 of 4096 x 12288 125 / 113; 1000 rows, 32 of 8192 x 1024 67 / 62; with rows of 2560, 5120, 6144, 7168 or 14336 bytes alike.  Rows of
-        // other lengths lie in all channels anyhow and lose 1 % by it.  One matrix for all rows gains up to 8 % (28672 x 8192, 20 rows) or loses 25 % (48 rows) and stays as it is.
-        turn = p.offsets && wbytes % 1024 == 0 ? (n0 / C::TO + 3 * t.group) % groups : 0;
+        // few of them.  So by group each begins at a k of its own and goes round.  us, all from 0 / each from its own, 24 rows a group: 32 of 4096 x 4096 8-bit 130 / 94, bf16 138 / 99; 8 of
+        // 8192 x 8192 116 / 102 and 127 / 97; 94 rows on average, 32 of 4096 x 4096 149 / 129 and 203 / 199.  Rows of 1408, 1536 and 2560 bytes, which lie in all channels anyhow: 8-bit alike
+        // within 2 %, bf16 2 to 3 % behind a form that knows no turn, and as much if these alone began at 0: it is the arithmetic, not the order, so there is no rule by length.  One
+        // matrix for all rows gains up to 8 % (28672 x 8192, 20 rows) or loses 25 % (48 rows) and stays as it is.
+        turn = p.offsets ? (n0 / C::TO + 3 * t.group) % groups : 0;
         wbytes = p.K;
         xbytes = C::X8 ? p.K : p.K * 2;
         const size_t wfirst = (size_t)t.group * p.N + n0;
