@@ -2,7 +2,9 @@
 //   score s = softmax(z) or 1 / (1 + exp(-z));  an expert is chosen by c = s + bias, or by z where there is neither a bias nor a sum over a group
 //   a group's value is the sum of its group_sum largest c; the experts of the top_groups largest groups are open
 //   the top_k open experts with the largest c, ties to the lowest index;  weights s, divided by their sum if asked (0 where that is 0), times scale
-// An expert whose logit is -infinity or NaN comes behind all others that are open and has the score 0.
+// An expert whose logit is -infinity or NaN (a masked one) comes behind all others that are open, also behind those that a bias of -infinity switches off, and has
+// the score 0; a group with fewer than group_sum unmasked experts comes behind those that have them.  So choices are compared by keys, where a masked expert has one
+// below that of -infinity.  A c that is NaN (a NaN in bias) counts as -infinity, a group's +infinity + -infinity as +infinity.
 //
 // c and the sums of groups are formed in 64 bits: in 32 two experts whose scores differ by less than a rounding change places, which happens to a few of some
 // thousand tokens, and then another expert's output is added.  By z alone, 32 bits are exact.
@@ -23,6 +25,8 @@ __device__ __forceinline__ uint64_t route_key(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);
     return b ^ ((b >> 63) ? ~0ull : 1ull << 63);
 }
+__device__ __forceinline__ double route_value(uint64_t key) { return __builtin_bit_cast(double, key ^ ((key >> 63) ? 1ull << 63 : ~0ull)); }
+constexpr uint32_t kKeyClosed = 0, kKeyMasked = 1;  // (-infinity's, the least of a number, is larger)
 
 // f(v, the value of the lane that differs in one bit of its number) for a value that is the same in all lanes with the same number without the lower bits
 template <int S, typename T, typename F>
@@ -98,7 +102,7 @@ struct Two {
     }
 };
 
-// All lanes of the wave; the token's choices come back in its lanes 0 .. top_k - 1.  lds: [tokens of the workgroup][L * PER] choice values (groups > 1)
+// All lanes of the wave; the token's choices come back in its lanes 0 .. top_k - 1.  lds: [tokens of the workgroup][L * PER] keys (groups > 1)
 template <int L, int PER, bool WIDE>
 __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, int E, const Routing &r, void *lds, int &chosen, float &weight) {
     typedef std::conditional_t<WIDE, double, float> V;
@@ -151,7 +155,10 @@ __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, i
             for (int i = 0; i < PER; ++i) c[i] /= total;
         }
 #pragma unroll
-        for (int i = 0; i < PER; ++i) c[i] = masked[i] ? -1e300 : c[i] + (double)bias[i];
+        for (int i = 0; i < PER; ++i) {
+            c[i] += (double)bias[i];
+            c[i] = c[i] == c[i] ? c[i] : -INFINITY;
+        }
     } else {
         if (!r.sigmoid && !r.renorm) {
 #pragma unroll
@@ -162,24 +169,27 @@ __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, i
             total = over_lanes<L>(total, [](float a, float b) { return a + b; });
         }
 #pragma unroll
-        for (int i = 0; i < PER; ++i) c[i] = masked[i] ? -INFINITY : zr[i];
+        for (int i = 0; i < PER; ++i) c[i] = zr[i];
     }
+    K key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = masked[i] ? kKeyMasked : route_key(c[i]);
     uint32_t open = 0;  // bit i: expert i of the lane may still be chosen
 #pragma unroll
     for (int i = 0; i < PER; ++i) open |= (ls * PER + i < E ? 1u : 0u) << i;
     if (r.groups > 1) {
         const int G = r.groups, per = E / G;
         int q;  // lanes that share a group: a power of two
-        Two<V> two = {-INFINITY, -INFINITY};
+        Two<K> two = {kKeyClosed, kKeyClosed};
         if (E == L * PER && per % PER == 0 && ((per / PER) & (per / PER - 1)) == 0) {  // whole lanes to a group: as they are
             q = per / PER;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) two.take(c[i]);
+            for (int i = 0; i < PER; ++i) two.take(key[i]);
         } else {  // through LDS, each of a group's lanes every q-th
             for (q = L; q * G > L;) q >>= 1;
-            V *const mine = reinterpret_cast<V *>(lds) + (threadIdx.x / L) * (L * PER);
+            K *const mine = reinterpret_cast<K *>(lds) + (threadIdx.x / L) * (L * PER);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) mine[ls * PER + i] = c[i];
+            for (int i = 0; i < PER; ++i) mine[ls * PER + i] = key[i];
             __builtin_amdgcn_wave_barrier();
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's own: its LDS accesses keep their order
             if (ls / q < G)
@@ -192,20 +202,25 @@ __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, i
         if (q > 16) two.template join<16>();
         const int g = ls / q;
         // (a sum of two, one of them masked: behind all sums without, by the other one)
-        const bool cut = WIDE && r.group_sum == 2 && two.a > V(-1e299) && two.b < V(-1e299);
-        const V value = cut ? two.a : r.group_sum == 2 ? two.a + two.b : two.a;
+        const bool cut = WIDE && r.group_sum == 2 && two.a > kKeyMasked && two.b <= kKeyMasked;
+        K value = two.a;
+        if constexpr (WIDE)
+            if (r.group_sum == 2 && two.b > kKeyMasked) {
+                const double sum = route_value(two.a) + route_value(two.b);
+                value = sum == sum ? route_key(sum) : two.a;
+            }
         const unsigned long long cuts = __ballot(cut);
         int rank = 0;
         if (!cuts) {  // (one answer for the wave)
             for (int h = 0; h < G; ++h) {
-                const V o = from_lane<L>(value, seg + h * q);
+                const K o = from_lane<L>(value, seg + h * q);
                 rank += o > value || (o == value && h < g);
             }
         } else {
             for (int h = 0; h < G; ++h) {
                 const int from = seg + h * q;
-                const V o = from_lane<L>(value, from);
-                const bool ocut = cuts >> from & 1, one = ocut != cut && o > V(-1e299) && value > V(-1e299);  // (what is all masked is behind both)
+                const K o = from_lane<L>(value, from);
+                const bool ocut = cuts >> from & 1, one = ocut != cut && o > kKeyMasked && value > kKeyMasked;  // (what is all masked is behind both)
                 rank += one ? cut : o > value || (o == value && h < g);
             }
         }
@@ -216,9 +231,8 @@ __device__ __forceinline__ void route_token_lanes(const float *__restrict__ z, i
             if (e < E && !(kept >> (e / per * q) & 1)) open &= ~(1u << i);
         }
     }
-    K key[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) key[i] = open >> i & 1 ? route_key(c[i]) : 0;
+    for (int i = 0; i < PER; ++i) key[i] = open >> i & 1 ? key[i] : kKeyClosed;
     K best;
     int at;
     auto own = [&] {

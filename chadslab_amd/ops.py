@@ -520,8 +520,8 @@ def moe_route(logits: torch.Tensor, top_k: int = 2, renorm: bool = True, *, scor
 
     score "sigmoid": 1 / (1 + exp(-logit)) instead.  bias fp32 [E]: the experts are chosen by score + bias, in 64 bits; w has no bias in it.  groups: E / groups
     consecutive experts form a group, whose value is the sum of the group_sum (1 or 2) largest of what its experts are chosen by, and only the experts of the
-    top_groups largest groups may be chosen.  scale: a factor of w.  An expert whose logit is -infinity or NaN comes behind all others that may be chosen and has
-    the score 0.  E up to 512, top_k up to 32.
+    top_groups largest groups may be chosen.  scale: a factor of w.  An expert whose logit is -infinity or NaN comes behind all others that may be chosen, also behind
+    those that a bias of -infinity switches off, and has the score 0.  A NaN in bias counts as -infinity.  E up to 512, top_k up to 32.
 
     With none of these, E up to 16 and top_k up to 8 the arithmetic is chadq_moe_route's, in 32 bits, which takes a row as it is: a NaN in it, or nothing but -infinity, makes
     its weights NaN."""

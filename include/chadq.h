@@ -497,7 +497,9 @@ int chadq_product_fp8_grouped(const void *x, const float *x_scale, const uint8_t
  * NULL: 0), in 64 bits; by its logit where bias is NULL and group_sum is 1.  The experts form `groups` groups of consecutive ones; a group's value is the sum of its
  * group_sum (1 or 2) largest c, and the experts of the top_groups groups of the largest value may be chosen: the top_k of the largest c among them, in that order.
  * Ties go to the lowest index.  weight = s, divided by the sum of the chosen ones if renorm (0 where that is 0), times scale.  An expert whose logit is -infinity
- * or NaN comes behind all others that may be chosen and has the score 0; a group with fewer than group_sum others comes behind those that have them.
+ * or NaN comes behind all others that may be chosen, also behind those whose bias is -infinity, and has the score 0; a group with fewer than group_sum others comes
+ * behind those that have them.  A c that is NaN (from a NaN in bias, or softmax's scores beside a logit of +infinity) counts as -infinity, +infinity + -infinity in the sum
+ * of a group as +infinity.
  * E <= 512, groups <= 64 and a divisor of E, group_sum <= E / groups, top_groups <= groups, top_k <= min(32, top_groups * E / groups).
  */
 typedef struct chadq_routing {

@@ -359,11 +359,12 @@ def moe_route_experts(logits, top_k, renorm=True, score="softmax", bias=None, gr
                 s = s / s[~masked].sum() if not masked.all() else s
         s = np.where(masked, 0.0, s)
         c = z if bias is None and group_sum == 1 else s + (0 if bias is None else np.asarray(bias, np.float64))
+        c = np.where(np.isnan(c), -np.inf, c)
         per = e // groups
         # (masked first, so that a plain sort puts them behind everything)
         order = lambda members: sorted(members, key=lambda j: (masked[j], -c[j] if not masked[j] else 0.0, j))
         value = [tuple((not masked[j], c[j] if not masked[j] else 0.0) for j in order(range(g * per, (g + 1) * per))[:group_sum]) for g in range(groups)]
-        size = lambda v: (sum(a for a, _ in v), sum(b for _, b in v))
+        size = lambda v: (sum(a for a, _ in v), np.inf if any(b == np.inf for _, b in v) else sum(b for _, b in v))
         kept = sorted(range(groups), key=lambda g: (tuple(-x for x in size(value[g])), g))[:top_groups]
         taken = order(j for g in kept for j in range(g * per, (g + 1) * per))[:top_k]
         idx[i], w[i] = taken, s[taken]

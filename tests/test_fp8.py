@@ -121,3 +121,14 @@ def test_what_the_operators_refuse_without_a_gpu():
     with pytest.raises(TypeError, match="FP8 activations"):
         from chadslab_amd import QWeightInt8
         ops.qlinear(QRowsFP8(torch.zeros(3, 32).to(FP8), torch.zeros(3, 1)), QWeightInt8(torch.zeros(8, 32, dtype=torch.int8), torch.zeros(8)))
+
+
+def test_routing_bias_that_is_not_finite():
+    """Switched off: behind all others, in front of masked ones.  NaN as -infinity; a group's +infinity + -infinity as +infinity."""
+    z = np.array([[0, -np.inf, 1, -np.inf]])
+    inf = np.inf
+    assert O.moe_route_experts(z, 2, score="sigmoid", bias=np.array([-inf, 0, 0, 0]))[0].tolist() == [[2, 0]]
+    assert O.moe_route_experts(z, 3, score="sigmoid", bias=np.array([np.nan, 0, 0, 0]))[0].tolist() == [[2, 0, 1]]
+    z = np.array([[0.0, 1, 2, 3, 4, 5]])
+    assert O.moe_route_experts(z, 2, groups=3, group_sum=2, bias=np.array([inf, -inf, -inf, 0, -inf, -inf]))[0].tolist() == [[0, 1]]
+    assert O.moe_route_experts(z, 2, groups=3, group_sum=2, bias=np.array([-inf, -inf, -inf, 0, -inf, -inf]))[0].tolist() == [[0, 1]]  # (all sums alike)

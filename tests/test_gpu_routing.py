@@ -164,3 +164,48 @@ def test_refusals(ops):
                         (lambda: ops.moe_route(z, 2, bias=z[0].cpu()), "GPU tensor"), (lambda: ops.moe_route(z, 2, bias=z[0].half()), "float32")):
         with pytest.raises(ValueError, match=match):
             call()
+
+
+def test_switched_off_experts_come_before_masked_ones(ops):
+    z = np.array([[0, -np.inf, 1, -np.inf]], np.float32)
+    bias = np.array([-np.inf, 0, 0, 0], np.float32)
+    idx, _ = ops.moe_route(torch.from_numpy(z).to(DEV), 2, score="sigmoid", bias=torch.from_numpy(bias).to(DEV))
+    assert idx.tolist() == [[2, 0]]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups", [(8, 1), (8, 2), (12, 3), (16, 4), (40, 5), (64, 1), (64, 8), (64, 32), (160, 20), (256, 8), (300, 6), (512, 64)])
+def test_bias_that_is_not_finite(ops, experts, groups, score):
+    """Experts switched off (-infinity, NaN) and always taken (+infinity), beside masked ones, in groups that have none, one or more of each; as many chosen as there may be."""
+    r = np.random.Generator(np.random.PCG64(experts + groups))
+    per = experts // groups
+    for kind in (0.3, 0.9, 1.0):
+        bias = (r.standard_normal(experts) * 0.1).astype(np.float32)
+        bias[r.random(experts) < kind] = -np.inf
+        bias[r.random(experts) < 0.1] = np.nan
+        if kind < 1:
+            bias[r.random(experts) < 0.1] = np.inf
+        z = (r.standard_normal((70, experts)) * 2).astype(np.float32)
+        z[::2][r.random(z[::2].shape) < 0.5] = -np.inf
+        z[::5][r.random(z[::5].shape) < 0.1] = np.nan
+        z[0], z[1] = -np.inf, 0.5
+        for top_groups in {1, (groups + 1) // 2, groups}:
+            for group_sum in (1, 2)[:per]:
+                check(ops, z, bias, top_k=min(32, top_groups * per), score=score, groups=groups, top_groups=top_groups, group_sum=group_sum, renorm=False)
+
+
+@pytest.mark.parametrize("tokens", [3, 70, 3000])
+def test_layer_with_experts_switched_off(ops, tokens):
+    """-infinity is the least of all biases: the layer is the one with a very low finite one, bit for bit, also where no more experts are left but masked ones."""
+    r = np.random.Generator(np.random.PCG64(tokens))
+    triple = [ops.quantize_fp8(torch.from_numpy(r.standard_normal(shape).astype(np.float32)).to(DEV), rows=False) for shape in ((8, 48, 64), (8, 48, 64), (8, 64, 48))]
+    x = torch.from_numpy(r.standard_normal((tokens, 64)).astype(np.float32)).to(DEV).bfloat16()
+    z = torch.from_numpy(r.standard_normal((tokens, 8)).astype(np.float32)).to(DEV)
+    z[:, 5:] = -np.inf
+    bias = torch.zeros(8, device=DEV)
+    for off in ([0, 1], [0, 1, 2, 3], list(range(8))):
+        for how in (dict(score="sigmoid"), dict(groups=4, top_groups=3, group_sum=2)):
+            bias[off] = -1e30
+            want = ops.moe_ffn(x, z, triple, top_k=4, bias=bias, **how)
+            bias[off] = -np.inf
+            assert torch.equal(ops.moe_ffn(x, z, triple, top_k=4, bias=bias, **how), want)
