@@ -77,3 +77,18 @@ def test_measured_choices():
     assert pick(17, 4096, 4096, x8=True, most_parts=8)[0] == "64x32"
     assert pick(8192, 8192, 8192, x8=True, most_parts=8) == ("256x256", 0)
     assert pick(1000, 4096, 14336, most_parts=8) == ("128x128", 0)
+
+
+class CombineShape(ctypes.Structure):
+    _fields_ = [("flat", I), ("threads", I), ("items", ctypes.c_int64)]
+
+
+def test_weighted_sum_leaves_few_threads_idle():
+    """The last step of a layer of experts: whatever the width, every column has a thread, and more than half of the threads have columns."""
+    fn = _lib.load()["_ZN5chadq17moe_combine_shapeEii"]
+    fn.restype, fn.argtypes = CombineShape, [I, I]
+    for h in [*range(16, 4400, 16), 7168, 8192, 1 << 20]:
+        s = fn(4000, h)
+        quads = 4000 * (h // 4)
+        assert s.threads % 64 == 0 and s.threads <= 256 and s.items * s.threads >= quads and (s.flat or s.threads * (s.items // 4000) >= h // 4), h
+        assert quads > s.items * s.threads // 2, h

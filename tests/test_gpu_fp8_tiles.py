@@ -280,3 +280,27 @@ def test_two_threads(ops):
     [t.join() for t in threads]
     assert all(len(g) == 10 for g in got)
     assert all(torch.equal(a, b) for i in range(2) for turn in got[i] for a, b in zip(turn, want[i]))
+
+
+@pytest.mark.parametrize("h", [16, 48, 240, 256, 272, 1008, 1024, 1040, 1104, 2064, 3088])
+@pytest.mark.parametrize("tokens,top_k", [(1, 1), (3, 2), (301, 3)])
+def test_weighted_sum_of_every_width(ops, tokens, top_k, h):
+    """The layer's last step deals columns to threads by their number: widths at its borders.  Bounds as above."""
+    r = np.random.Generator(np.random.PCG64(h + tokens))
+    triple = (*(weights(r, 32, h, 4, values=narrow) for _ in range(2)), weights(r, h, 32, 4))
+    x = activations(r, tokens, h, False, values=narrow)
+    logits = torch.from_numpy(r.standard_normal((tokens, 4)).astype(np.float32)).to(DEV)
+    want, _ = layer_in_64(ops, x, triple, *ops.moe_route(logits, top_k=top_k, score="sigmoid"))
+    off = (ops.moe_ffn(x, logits, triple, top_k=top_k, score="sigmoid").double() - want).norm()
+    assert off <= (2 * 2.0 ** -8 + 2.0 ** -18) * want.norm()
+
+
+def test_weighted_sum_of_very_many_tokens(ops):
+    """More tokens than a grid has workgroups for: they repeat, and so does the result."""
+    r = np.random.Generator(np.random.PCG64(9))
+    for h in (16, 256):
+        triple = (*(weights(r, 16, h, 2) for _ in range(2)), weights(r, h, 16, 2))
+        x = activations(r, 4096, h, False).repeat(257, 1)
+        logits = torch.from_numpy(r.standard_normal((4096, 2)).astype(np.float32)).to(DEV).repeat(257, 1)
+        y = ops.moe_ffn(x, logits, triple, top_k=1)
+        assert bool(y.any()) and torch.equal(y, y[:4096].repeat(257, 1))
