@@ -443,9 +443,15 @@ int route_experts_launch(const float *logits, int32_t *idx, float *w, int T, int
     return with_shape(E, r.bias || r.group_sum == 2, [&](auto l, auto per, auto wide) {
         constexpr int L = decltype(l)::value, PER = decltype(per)::value;
         constexpr bool WIDE = decltype(wide)::value;
-        const int tokens = 256 / L, lds = r.groups > 1 ? 256 * PER * (WIDE ? 8 : 4) : 0;
-        hipLaunchKernelGGL((route_experts_kernel<L, PER, WIDE>), dim3((int)(((int64_t)T + tokens - 1) / tokens)), dim3(256), lds, st, logits, idx, w, T, E, r);
-        return hip_check(hipGetLastError(), "moe route launch");
+        constexpr int tokens = 256 / L, most = tokens << 22;  // a launch has fewer than 2^32 threads
+        const int lds = r.groups > 1 ? 256 * PER * (WIDE ? 8 : 4) : 0;
+        for (int64_t t = 0; t < T; t += most) {
+            const int n = (int)(T - t < most ? T - t : most);
+            hipLaunchKernelGGL((route_experts_kernel<L, PER, WIDE>), dim3((n + tokens - 1) / tokens), dim3(256), lds, st, logits + t * E, idx + t * r.top_k, w + t * r.top_k, n, E, r);
+            const int rc = hip_check(hipGetLastError(), "moe route launch");
+            if (rc) return rc;
+        }
+        return 0;
     });
 }
 

@@ -209,3 +209,20 @@ def test_layer_with_experts_switched_off(ops, tokens):
             want = ops.moe_ffn(x, z, triple, top_k=4, bias=bias, **how)
             bias[off] = -np.inf
             assert torch.equal(ops.moe_ffn(x, z, triple, top_k=4, bias=bias, **how), want)
+
+
+@pytest.mark.parametrize("experts,tokens", [(33, 2 ** 26 + 5), (2, 2 ** 29 + 70)])
+def test_more_tokens_than_a_launch_has_threads_for(ops, experts, tokens):
+    """2^32 lanes and more: every token is somebody's, and the ones at the borders are right."""
+    r = np.random.Generator(np.random.PCG64(experts))
+    z = torch.from_numpy(r.standard_normal((7, experts)).astype(np.float32)).to(DEV)
+    at = torch.tensor([0, 2 ** 24 - 1, 2 ** 24, 2 ** 26 - 1, 2 ** 26, tokens // 2, tokens - 1], device=DEV)
+    logits = torch.zeros(tokens, experts, device=DEV)
+    logits[at] = z
+    bias = torch.zeros(experts, device=DEV)
+    bias[1] = 0.25  # (so that no token's answer is what fresh memory may hold)
+    idx, w = ops.moe_route(logits, 1, score="sigmoid", bias=bias, renorm=False)
+    want = ops.moe_route(z, 1, score="sigmoid", bias=bias, renorm=False)
+    assert torch.equal(idx[at], want[0]) and torch.equal(w[at], want[1])
+    idx[at], w[at] = 1, 0.5
+    assert bool((idx == 1).all()) and bool((w == 0.5).all())
