@@ -23,12 +23,12 @@ __global__ __launch_bounds__(256) void quantize_fp8_rows_kernel(const T *__restr
     }
 }
 
-// Weights: a workgroup to a block of 128 x 128, 64 values to a thread: row tid / 16 + 16 i.
+// Weights: a workgroup to a block of 128 x 128, 64 values to a thread: row tid / 16 + 16 i.  first: the launch's first block
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_fp8_blocks_kernel(const T *__restrict__ x, uint8_t *__restrict__ q, float *__restrict__ scale, int N, int K, int GN,
-                                                                  int G) {
+                                                                  int G, int64_t first) {
     __shared__ uint32_t s_max[4];
-    const int64_t b = blockIdx.x;
+    const int64_t b = first + blockIdx.x;
     const int g = (int)(b % G);
     const int64_t rest = b / G;
     const int n0 = (int)(rest % GN) * 128, k = g * 128 + (threadIdx.x & 15) * 8;
@@ -81,12 +81,14 @@ __global__ __launch_bounds__(256) void dequant_fp8_kernel(const uint32_t *__rest
 int quantize_fp8_launch(const void *x, int dtype, uint8_t *q, float *scale, int64_t matrices, int N, int K, bool rows, hipStream_t st) {
     const int G = fp8_blocks(K), GN = fp8_blocks(N);
     const int64_t blocks = rows ? (matrices * N * G + 15) / 16 : matrices * GN * G;
-    if (!rows && blocks > INT32_MAX) return fail(CHADQ_ERR_SHAPE, "quantize_fp8: %lld blocks are too many", (long long)blocks);
-    const int grid = (int)(rows && blocks > 256 * 32 ? 256 * 32 : blocks);
     auto go = [&](auto t) {
         typedef decltype(t) T;
-        if (rows) hipLaunchKernelGGL(quantize_fp8_rows_kernel<T>, dim3(grid), dim3(256), 0, st, reinterpret_cast<const T *>(x), q, scale, matrices * N, K, G);
-        else hipLaunchKernelGGL(quantize_fp8_blocks_kernel<T>, dim3(grid), dim3(256), 0, st, reinterpret_cast<const T *>(x), q, scale, N, K, GN, G);
+        const T *const from = reinterpret_cast<const T *>(x);
+        constexpr int64_t most = 1 << 22;  // workgroups: a launch has fewer than 2^32 threads
+        if (rows) hipLaunchKernelGGL(quantize_fp8_rows_kernel<T>, dim3((int)(blocks > 256 * 32 ? 256 * 32 : blocks)), dim3(256), 0, st, from, q, scale, matrices * N, K, G);
+        else
+            for (int64_t b = 0; b < blocks; b += most)
+                hipLaunchKernelGGL(quantize_fp8_blocks_kernel<T>, dim3((int)(blocks - b < most ? blocks - b : most)), dim3(256), 0, st, from, q, scale, N, K, GN, G, b);
     };
     if (dtype == CHADQ_F32) go(float());
     else if (dtype == CHADQ_BF16) go(__bf16());

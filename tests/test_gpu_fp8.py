@@ -643,3 +643,18 @@ def test_library_refuses(ops):
         assert lib.chadq_moe_route_experts(a, byref(_lib.Routing(**dict(good, **change))), a, a, 1, 64, None) == -2, change
     assert lib.chadq_moe_route_experts(None, byref(_lib.Routing(**good)), a, a, 1, 64, None) == -1 and lib.chadq_moe_route_experts(a, None, a, a, 1, 64, None) == -1
     assert lib.chadq_moe_route_experts(a + 2, byref(_lib.Routing(**good)), a, a, 1, 64, None) == -3 and lib.chadq_moe_route_experts(a, byref(_lib.Routing(**good)), a, a, 1, 513, None) == -2
+
+
+def test_more_blocks_than_a_launch_has_threads_for(ops):
+    """2^24 small matrices and more, a workgroup to each: all are done, and the ones at the borders are right."""
+    e = 2 ** 24 + 3
+    at = torch.tensor([0, 2 ** 22 - 1, 2 ** 22, 2 ** 24 - 1, 2 ** 24, e - 1], device=DEV)
+    some = dev(np.random.Generator(np.random.PCG64(8)).standard_normal((6, 1, 16)).astype(np.float32)).to(torch.bfloat16)
+    x = torch.full((e, 1, 16), 3.5, dtype=torch.bfloat16, device=DEV)
+    x[at] = some
+    q, want = ops.quantize_fp8(x, rows=False), ops.quantize_fp8(some, rows=False)
+    values = q.w.view(torch.uint8)
+    assert torch.equal(values[at], want.w.view(torch.uint8)) and torch.equal(q.scale[at], want.scale)
+    values[at], q.scale[at] = 0x7E, 2.0 ** -7  # 448 and 3.5 / 448, as of all others
+    assert bool((values == 0x7E).all()) and bool((q.scale == 2.0 ** -7).all())
+    assert torch.equal(ops.dequantize(q)[at], torch.full((6, 1, 16), 3.5, device=DEV))
