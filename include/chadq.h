@@ -512,7 +512,8 @@ int chadq_moe_route_experts(const float *logits, const chadq_routing *routing, i
 /*
  * Mixture-of-experts FFN on FP8 experts: routing as above, y[t] = bf16( sum_j w[t,j] down_e( h ) ), h = silu(gate_e x_t) * (up_e x_t).  gate, up [E,F,H], down
  * [E,H,F], values and scales of the E matrices one behind the other.  x_scale NULL: x bf16 [T,H] and h rounded to bf16; else x holds values [T,H] and h becomes
- * 8-bit as chadq_quantize_fp8 by_row does it.  H, F multiples of 16.  workspace: chadq_moe_ffn_fp8_workspace_bytes bytes (0: sizes that are not served).
+ * 8-bit as chadq_quantize_fp8 by_row does it.  H, F multiples of 16.  Tokens of more than 2^20 pairs, or of 2^31 bytes of x and more, go through the layer in equal ranges, one
+ * behind the other in the same workspace.  workspace: chadq_moe_ffn_fp8_workspace_bytes bytes (0: sizes that are not served).
  */
 typedef struct chadq_moe_fp8 {
     const uint8_t *gate, *up, *down;

@@ -92,3 +92,15 @@ def test_weighted_sum_leaves_few_threads_idle():
         quads = 4000 * (h // 4)
         assert s.threads % 64 == 0 and s.threads <= 256 and s.items * s.threads >= quads and (s.flat or s.threads * (s.items // 4000) >= h // 4), h
         assert quads > s.items * s.threads // 2, h
+
+
+@pytest.mark.parametrize("x8", [0, 1])
+def test_layers_of_very_many_tokens_go_in_ranges(x8):
+    """Activations of 2 GB and more, and more than 2^20 pairs: equal ranges, whose workspace is the call's."""
+    need = _lib.load().chadq_moe_ffn_fp8_workspace_bytes
+    for h, f, e, top_k in ((4096, 64, 4, 1), (7168, 2048, 8, 2), (16, 16, 2, 1), (256, 128, 256, 8)):
+        most = min((2 ** 31 - 2) // (h * (1 if x8 else 2)), 2 ** 20 // top_k)
+        assert need(most, h, f, e, top_k, x8) >= most * top_k * h * 4
+        for t in (most + 1, 2 * most, 2 * most + 1, 5 * most + 3):
+            ranges = -(-t // most)
+            assert need(t, h, f, e, top_k, x8) == need(-(-t // ranges), h, f, e, top_k, x8), (t, h)

@@ -304,3 +304,20 @@ def test_weighted_sum_of_very_many_tokens(ops):
         logits = torch.from_numpy(r.standard_normal((4096, 2)).astype(np.float32)).to(DEV).repeat(257, 1)
         y = ops.moe_ffn(x, logits, triple, top_k=1)
         assert bool(y.any()) and torch.equal(y, y[:4096].repeat(257, 1))
+
+
+@KINDS
+@pytest.mark.parametrize("more", ["bytes", "pairs"])
+def test_layer_of_more_tokens_than_go_together(ops, more, x8):
+    """Just past 2^31 bytes of activations, or 2^20 pairs: the layer is its two halves', bit for bit, and those are tested above."""
+    r = np.random.Generator(np.random.PCG64(12))
+    h, f, e, top_k, tokens = (4096, 32, 4, 1, 2 ** 31 // (4096 if x8 else 8192) + 5) if more == "bytes" else (64, 48, 12, 8, 2 ** 17 + 5)
+    triple = (*(weights(r, f, h, e) for _ in range(2)), weights(r, h, f, e))
+    some = activations(r, 4099, h, x8)
+    x = rows_of(some, torch.arange(tokens, device=DEV) % 4099)
+    logits = torch.from_numpy(r.standard_normal((tokens, e)).astype(np.float32)).to(DEV)
+    half = (tokens + 1) // 2
+    y = ops.moe_ffn(x, logits, triple, top_k=top_k, score="sigmoid")
+    for part in (slice(0, half), slice(half, tokens)):
+        assert torch.equal(y[part], ops.moe_ffn(rows_of(x, part), logits[part], triple, top_k=top_k, score="sigmoid"))
+    assert bool(y.any(1).all())
