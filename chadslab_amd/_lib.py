@@ -157,7 +157,7 @@ _NATIVE_ENTRIES = ("chadq_gemv_i4g32", "chadq_gemv_i4g32_bf16", "chadq_gemm_i4g3
 _NATIVE_MX_ENTRIES = ("chadq_quantize_mxfp4", "chadq_dequant_mxfp4", "chadq_product_mxfp4_workspace_bytes", "chadq_product_mxfp4", "chadq_product_mxfp4_grouped",
                       "chadq_moe_ffn_mxfp4_workspace_bytes", "chadq_moe_ffn_mxfp4")
 _NATIVE_FP8_ENTRIES = ("chadq_quantize_fp8", "chadq_dequant_fp8", "chadq_product_fp8_workspace_bytes", "chadq_product_fp8", "chadq_product_fp8_grouped",
-                       "chadq_moe_route_experts", "chadq_moe_ffn_fp8_workspace_bytes", "chadq_moe_ffn_fp8")
+                       "chadq_moe_route_experts", "chadq_moe_ffn_fp8_workspace_bytes", "chadq_moe_ffn_fp8", "chadq_moe_route")
 
 
 HOST_PATH = Path(__file__).resolve().parent / "_host_call.so"

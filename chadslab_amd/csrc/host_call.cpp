@@ -36,9 +36,9 @@ enum MxEntry { MX_QUANTIZE, MX_DEQUANT, MX_BYTES, MX_PRODUCT, MX_GROUPED, MX_MOE
 const char *const kMxNames[MX_ENTRIES] = {"chadq_quantize_mxfp4", "chadq_dequant_mxfp4", "chadq_product_mxfp4_workspace_bytes", "chadq_product_mxfp4", "chadq_product_mxfp4_grouped",
                                           "chadq_moe_ffn_mxfp4_workspace_bytes", "chadq_moe_ffn_mxfp4"};
 void *g_mx_entry[MX_ENTRIES];                          // (bind_mx)
-enum Fp8Entry { FP8_QUANTIZE, FP8_DEQUANT, FP8_BYTES, FP8_PRODUCT, FP8_GROUPED, FP8_ROUTE, FP8_MOE_BYTES, FP8_MOE, FP8_ENTRIES };
+enum Fp8Entry { FP8_QUANTIZE, FP8_DEQUANT, FP8_BYTES, FP8_PRODUCT, FP8_GROUPED, FP8_ROUTE, FP8_MOE_BYTES, FP8_MOE, FP8_ROUTE_PLAIN, FP8_ENTRIES };
 const char *const kFp8Names[FP8_ENTRIES] = {"chadq_quantize_fp8", "chadq_dequant_fp8", "chadq_product_fp8_workspace_bytes", "chadq_product_fp8", "chadq_product_fp8_grouped",
-                                            "chadq_moe_route_experts", "chadq_moe_ffn_fp8_workspace_bytes", "chadq_moe_ffn_fp8"};
+                                            "chadq_moe_route_experts", "chadq_moe_ffn_fp8_workspace_bytes", "chadq_moe_ffn_fp8", "chadq_moe_route"};
 void *g_fp8_entry[FP8_ENTRIES];                        // (bind_fp8)
 PyObject *g_fp8 = nullptr, *g_fp8_experts = nullptr, *g_fp8_rows = nullptr;
 PyObject *g_int4 = nullptr, *g_int8 = nullptr, *g_tiles = nullptr, *g_mx = nullptr, *g_mx_experts = nullptr;  // the weight containers
@@ -488,7 +488,7 @@ struct Route {
     }
 };
 
-// route(logits, *Route) -> (idx, w), or None
+// route(logits, *Route) -> (idx, w), or None.  What chadq_moe_route serves, softmax over at most 16 experts and top_k, goes there
 PyObject *route(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
     const int dev = n_args == 9 && THPVariable_CheckExact(args[0]) ? device_of(args[0]) : -1;
@@ -497,6 +497,7 @@ PyObject *route(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     Route how;
     if (!zt || zt->size(0) < 1 || zt->size(0) > INT_MAX || zt->size(1) < 1 || zt->size(1) > kRouteExperts || !how.of(args + 1, zt->size(1), dev)) Py_RETURN_NONE;
     const at::Tensor z = *zt;
+    const bool few = how.r.top_k <= 8 && z.size(1) <= 16 && !how.r.bias && !how.r.sigmoid && how.r.groups == 1 && how.r.top_groups == 1 && how.r.group_sum == 1 && how.r.scale == 1.f;
     at::Tensor idx, w;
     int rc;
     {
@@ -504,10 +505,12 @@ PyObject *route(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
         idx = at::empty({z.size(0), how.r.top_k}, z.options().dtype(at::kInt).requires_grad(false));
         w = at::empty({z.size(0), how.r.top_k}, z.options().requires_grad(false));
         if (!held(idx) || !held(w)) rc = CHADQ_ERR_NULL;
+        else if (few) rc = fp8_entry(FP8_ROUTE_PLAIN, &chadq_moe_route)(z.const_data_ptr<float>(), idx.mutable_data_ptr<int32_t>(), w.mutable_data_ptr<float>(), (int)z.size(0),
+                                                                      (int)z.size(1), how.r.top_k, how.r.renorm, stream_of(dev));
         else rc = fp8_entry(FP8_ROUTE, &chadq_moe_route_experts)(z.const_data_ptr<float>(), &how.r, idx.mutable_data_ptr<int32_t>(), w.mutable_data_ptr<float>(),
                                                                   (int)z.size(0), (int)z.size(1), stream_of(dev));
     }
-    if (rc != 0) return failed(rc, kFp8Names[FP8_ROUTE]);
+    if (rc != 0) return failed(rc, kFp8Names[few ? FP8_ROUTE_PLAIN : FP8_ROUTE]);
     const Ref io(THPVariable_Wrap(std::move(idx))), wo(THPVariable_Wrap(std::move(w)));
     if (!io.p || !wo.p) return PyErr_NoMemory();
     return PyTuple_Pack(2, io.p, wo.p);

@@ -525,19 +525,18 @@ def moe_route(logits: torch.Tensor, top_k: int = 2, renorm: bool = True, *, scor
 
     With none of these, E up to 16 and top_k up to 8 the arithmetic is chadq_moe_route's, in 32 bits, which takes a row as it is: a NaN in it, or nothing but -infinity, makes
     its weights NaN."""
+    how = _routing(top_k, renorm, score, bias, groups, top_groups, group_sum, scale)
+    got = _lib.native().route(logits, bias, *how)
+    if got is not None:
+        return got
     if score == "softmax" and bias is None and groups == 1 and scale == 1.0 and logits.dim() == 2 and logits.size(1) <= 16 and top_k <= 8 and group_sum == 1 \
             and top_groups in (None, 1):
         z = _dev(logits, "logits", torch.float32)
         t, e = z.shape
         idx = torch.empty(t, top_k, dtype=torch.int32, device=z.device)
         w = torch.empty(t, top_k, dtype=torch.float32, device=z.device)
-        _lib.check(_lib.load().chadq_moe_route(z.data_ptr(), idx.data_ptr(), w.data_ptr(), t, e, top_k, int(renorm), _stream()),
-                   "chadq_moe_route")
+        _launch(z.device, "chadq_moe_route", z.data_ptr(), idx.data_ptr(), w.data_ptr(), t, e, top_k, int(renorm))
         return idx, w
-    how = _routing(top_k, renorm, score, bias, groups, top_groups, group_sum, scale)
-    got = _lib.native().route(logits, bias, *how)
-    if got is not None:
-        return got
     z = _dev(logits, "logits", torch.float32)
     if z.dim() != 2:
         raise ValueError("logits must be [T,E], got %s" % (tuple(z.shape),))

@@ -226,3 +226,18 @@ def test_more_tokens_than_a_launch_has_threads_for(ops, experts, tokens):
     assert torch.equal(idx[at], want[0]) and torch.equal(w[at], want[1])
     idx[at], w[at] = 1, 0.5
     assert bool((idx == 1).all()) and bool((w == 0.5).all())
+
+
+@pytest.mark.parametrize("experts,top_k", [(1, 1), (3, 2), (8, 2), (8, 8), (16, 1), (16, 8)])
+def test_plain_routing_goes_the_short_way(ops, experts, top_k):
+    """Softmax over at most 16: chadq_moe_route's bits from the native call, NaN and rows of nothing but -infinity as they are there."""
+    from chadslab_amd import _lib
+
+    r = np.random.Generator(np.random.PCG64(experts + top_k))
+    z = torch.from_numpy(r.standard_normal((33, experts)).astype(np.float32)).to(DEV)
+    z[3], z[5, 0], z[7] = -np.inf, np.nan, 0.25
+    for renorm in (True, False):
+        idx, w = torch.empty(33, top_k, dtype=torch.int32, device=DEV), torch.empty(33, top_k, device=DEV)
+        _lib.check(_lib.load().chadq_moe_route(z.data_ptr(), idx.data_ptr(), w.data_ptr(), 33, experts, top_k, int(renorm), torch.cuda.current_stream().cuda_stream), "chadq_moe_route")
+        for got in (_lib.native().route(z, None, False, renorm, 1, 1, 1, top_k, 1.0), ops.moe_route(z, top_k, renorm), ops.moe_route(z, top_k, np.bool_(renorm))):
+            assert torch.equal(got[0], idx) and torch.equal(got[1].view(torch.int32), w.view(torch.int32))
