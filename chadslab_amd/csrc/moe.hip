@@ -348,8 +348,8 @@ __global__ __launch_bounds__(256) void moe_act_kernel(const float *__restrict__ 
 template <bool FLAT>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const float *__restrict__ yp, const int32_t *__restrict__ pos,
                                                           const float *__restrict__ w, uint16_t *__restrict__ y, int T,
-                                                          int H, int top_k, int nsplit, size_t split_stride) {
-    const int q = H / 4, width = (int)blockDim.x, chunks = FLAT ? 1 : (q + width - 1) / width;
+                                                          int H, int top_k, int nsplit, size_t split_stride, int chunks, int width) {
+    const int q = H / 4;  // (chunks of width threads to a token: arguments, which arrive in registers, where the launch's own shape is read from memory)
     const int64_t items = FLAT ? ((int64_t)T * q + 255) / 256 : (int64_t)T * chunks;
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
         int t, c;
@@ -387,7 +387,7 @@ CombineShape moe_combine_shape(int T, int H) {
 static int moe_combine_launch(const float *yp, const int32_t *pos, const float *w, uint16_t *y, int T, int H, int top_k, int nsplit, hipStream_t st) {
     const CombineShape s = moe_combine_shape(T, H);
     hipLaunchKernelGGL(s.flat ? moe_combine_kernel<true> : moe_combine_kernel<false>, dim3((int)(s.items < (1 << 20) ? s.items : 1 << 20)), dim3(s.threads), 0, st, yp, pos, w, y, T, H,
-                       top_k, nsplit, (size_t)T * top_k * H);
+                       top_k, nsplit, (size_t)T * top_k * H, (int)(s.items / T), s.threads);
     return hip_check(hipGetLastError(), "moe combine launch");
 }
 
