@@ -1,5 +1,5 @@
-// FP8: quantisation (of a block: fp8.h) and its inverse.  Bound by memory, each value read once and written once: 14336 x 4096 fp32 by 128 x 128 45 us, back 42 (294 MB
-// each, 6.5 and 6.9 TB/s of which the last-level cache serves a part), 4096 x 4096 bf16 by rows 10.3 (4.9 TB/s), 16 x 4096 2.2 (a launch).
+// FP8: quantisation (of a block: fp8.h) and its inverse.  Bound by memory, each value read once and written once: 14336 x 4096 fp32 by 128 x 128 46 us, back 42 (294 MB
+// each, 6.4 and 7.0 TB/s of which the last-level cache serves a part), 4096 x 4096 bf16 by rows 10.9 (4.7 TB/s), 16 x 4096 2.2 (a launch).
 #include "fp8.h"
 #include "load8.h"
 

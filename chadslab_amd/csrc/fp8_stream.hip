@@ -294,7 +294,11 @@ int fp8_stream_launch(const Fp8Product &p, hipStream_t st) {
     return p.xs ? launch_rows<true, false, false, 2>(p, st) : launch_rows<false, false, false, 2>(p, st);
 }
 
-// Up to 16 rows, or 8 of a group on average, stream the weights, more go through the tiles.
+// Up to 16 rows, or 8 of a group on average, stream the weights, more go through the tiles.  By group, us streamed / in tiles, bf16 x: 8 of 14336 x 4096, 4 rows to each 73 / 90, 8 to each
+// 75 / 92, 12 to each 141 / 92; 64 of 1408 x 2048, the same, 31 / 44, 33 / 44, 61 / 45.  The host does not know how the rows are spread: drawn groups of 8 on average, whose larger ones read
+// their weights twice, lose by it (114 / 89, 44 / 43), and so do 4 on average only at many small groups (256 of 1024 x 1024, 58 / 51); all rows in one group, 8 times as many as there
+// are groups, 75 / 41.  8-bit x: streamed the same, in tiles up to 12 % less than bf16 (one group
+// 40 %; 256 groups 9 % more).
 // Columns beyond what the streaming grid holds (4194240) go through the tiles whatever the rows.
 bool fp8_streams(const Fp8Product &p) { return (p.offsets ? p.M <= (int64_t)8 * p.E : p.M <= 16) && stream_shape(p).cols(p.N) <= kFp8StreamCols; }
 

@@ -3,16 +3,16 @@
 // A workgroup's WN x WM waves share a tile of TN weight rows x TM activation rows; a wave sums NB x MB blocks of 32 x 32.  The weights are the
 // matrix cores' first operand, so that a lane holds four consecutive n of one activation row.
 //   FP8 x   v_mfma_f32_16x16x128_f8f6f4 takes a whole scale block of k: its result, from 0, times the block's two scales is added to the sum by FMAs that
-//           follow some instructions behind.  The instruction adds eight products as multiples of 2^-13 of the largest: 2^-16 of a result on normal data, beside the
-//           2^-9 of its rounding to bf16.  (32x32x64, two to a block: 3.3 instead of 3.6 PFLOP/s with the FMAs, from registers)
+//           follow some instructions behind.  The instruction adds eight products as multiples of 2^-13 of the largest: 2^-16 of a result's norm on normal data, beside
+//           the up to 2^-8 of its rounding to bf16.  (32x32x64, two to a block: 3.3 instead of 3.6 PFLOP/s with the FMAs, from registers)
 //   bf16 x  the values become bf16, exactly, v_mfma_f32_32x32x16_bf16; the sums of a block begin from 0 and are added, times its scale, when the next begins
 // A step is SK of K.  Values and activations go global -> LDS by DMA, ST stages, requests dealt to the waves in equal numbers and placed between
 // the MFMAs; a piece past the end of a row or of the matrix is requested beyond the buffer's range and arrives as zeros, so nothing in the loop knows about
 // edges.  Scales: a thread loads two steps' of a row of x, or of a block of weight rows, two steps ahead, and puts them into LDS.  16-byte
 // pieces of a row are XOR-swizzled by the row so that the 16 rows that a read takes at a time cover all banks.  WK > 1: waves of a workgroup split the k of a
 // step and add their sums at the end, so that a small tile too has eight waves to hide its reads.
-// us, matrix cores' busy share: 4096 x 14336 x 4096 8-bit 236, 50 % (2.0 PFLOP/s; 256 x 256); 1000 x 4096 x 14336 bf16 130, 45 % (0.9 PFLOP/s; 128 x 128, one round); 2048 rows by group on
-// 16 of 4096 x 2048 8-bit 42, 23 %; gate and up of 6000 pairs, 64 experts of 1408 x 2048, 112, 19 % (400 MB, 3.6 TB/s).  Of 4096^3 with 256 x 256 tiles, 69 us, some 8 are outside
+// us, matrix cores' busy share: 4096 x 14336 x 4096 8-bit 234-241, 51 % (2.0 PFLOP/s; 256 x 256); 1000 x 4096 x 14336 bf16 124-130, 47 % (0.9 PFLOP/s; 128 x 128, one round); 2048 rows by group on
+// 16 of 4096 x 2048 8-bit 42-46, 22 %; gate and up of 6000 pairs, 64 experts of 1408 x 2048, 111, 19 % (407 MB, 3.7 TB/s).  Of 4096^3 with 256 x 256 tiles, 69 us, some 8 are outside
 // the loop, 13 are the requests and 9 the scales' FMAs; the MFMAs alone take 32.
 #include <cmath>
 #include <type_traits>
@@ -606,7 +606,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) __attribute__((amdgpu_waves_per_
         t = {0, tm * TM, p.M - tm * TM < TM ? p.M - tm * TM : TM, 0, 0};
     }
     t = {uniform(t.group), uniform(t.row0), uniform(t.rows), 0, 0};
-    // A cut tile takes as many blocks of 32 rows as it has
+    // A cut tile whose waves all share its rows takes as many blocks of 32 of them as it has; where two or four waves split them (WM) it works on all, on zeros behind the last
     if constexpr (WM == 1 && MB > 1) {
         if (t.rows <= 32) return tile_body<Cfg<X8, GATED, WN, WM, WK, NB, 1, SK, ST>>(p, t, n0, lds);
         if constexpr (MB > 2)

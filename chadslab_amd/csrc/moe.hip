@@ -602,8 +602,8 @@ int moe_ffn_mxfp4_launch(const uint16_t *x, const float *logits, const chadq_moe
 
 // ---- the same on FP8 experts, routed as route.hip does it: gate and up with the SiLU gate in one product by group, down to fp32, combine.  With 8-bit
 // activations h becomes 8-bit too, from its fp32 values.
-// us, 1000 tokens to 6 of 64 experts of 1408 x 2048, 8-bit: routing 5, sort 5, gate and up with h 112, down 67, sum 9 (554 MB of weights alone: 108); 4 tokens to 2 of 8
-// experts of 14336 x 4096: 5, none, 124, 62, 5.
+// us, 1000 tokens to 6 of 64 experts of 1408 x 2048, 8-bit: routing 5, sort 6, gate and up with h 111, down 66, sum 9 (554 MB of weights alone: 108); 4 tokens to 2 of 8
+// experts of 14336 x 4096: 5, none, 127, 63, 5.
 struct MoeFp8Ws {
     int32_t *idx, *pos, *tok, *offsets, *hist;
     float *w;

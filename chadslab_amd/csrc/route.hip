@@ -12,7 +12,7 @@
 // A token takes L lanes of a wave (8 to 64), each with PER consecutive experts: a lane's best is found among its own, the token's by a reduction over the lanes,
 // and the lowest lane that holds it wins, so that equal ones go to the lowest index with no index in the keys.
 // Bound by the chain of a token's rounds (a reduction over 64 lanes each, in registers) and, with many tokens, by the 64-bit exponentials and comparisons: 8 of 256
-// experts in 8 groups, sigmoid and bias, 16 tokens 5.9 us, 8192 tokens 19 (8.4 MB: 1.6 from memory).  16 lanes of 16 experts to a token took 18.7, a choice in 32 bits first, with
+// experts in 8 groups, sigmoid and bias, 16 tokens 6.0 us, 8192 tokens 19.4 (8.4 MB: 1.6 from memory).  16 lanes of 16 experts to a token took 18.7, a choice in 32 bits first, with
 // 64 where it is near, 25.
 #include <type_traits>
 

@@ -477,7 +477,8 @@ int chadq_dequant_fp8(const uint8_t *values, const float *scale, float *w, int64
  * y[m,n] = sum over blocks b of x_scale[m,b] w_scale[n/128,b] sum_{k in b} x[m,k] w[n,k]: a block's sum in fp32 of exact products, its scales multiplied with each
  * other in fp32, one FMA to the result; y fp32 or (y_bf16) the same rounded once.  x_scale NULL: x is bf16 [M,K], multiplied as it is, with no scale; else x holds
  * values [M,K]; of more than 16 rows (by group: of more than 8 E) those meet the 8-bit matrix instruction, which adds the products of eight k as multiples of 2^-13
- * of the power of two that their largest exponent sum makes, cut: off by less than 7 * 2^-13 sum |x w|, some 2^-15 of the norm of a result.  M, N >= 0; K a positive multiple of 16 up to 2^26; x and w 16-byte aligned.  NaN and infinities act as IEEE has them.  workspace:
+ * of the power of two that their largest exponent sum makes, cut: off by less than 7 * 2^-13 sum |x w|, 2^-16 of a result's norm on normal data (rows of
+ * 2^23 values and more, and their groups, always take bf16 ones, and more than 4194240 columns the 8-bit one whatever the rows).  M, N >= 0; K a positive multiple of 16 up to 2^26; x and w 16-byte aligned.  NaN and infinities act as IEEE has them.  workspace:
  * chadq_product_fp8_workspace_bytes bytes (16-byte aligned; 0: none needed), for the sums of parts of K where that is the quicker form; without it (NULL or
  * fewer bytes) the product is one part.
  */
