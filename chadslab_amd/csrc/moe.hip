@@ -604,6 +604,8 @@ int moe_ffn_mxfp4_launch(const uint16_t *x, const float *logits, const chadq_moe
 // activations h becomes 8-bit too, from its fp32 values.
 // us, 1000 tokens to 6 of 64 experts of 1408 x 2048, 8-bit: routing 5, sort 6, gate and up with h 111, down 66, sum 9 (554 MB of weights alone: 108); 4 tokens to 2 of 8
 // experts of 14336 x 4096: 5, none, 127, 63, 5.
+// With bf16 activations h goes to bf16, the type that the down product takes: half the bytes of fp32 and no second product for its lower part.  It costs up to 2^-8 of each h: the layer
+// of 4 tokens is off by 0.0023 of its norm from 64 bits, where the rounding of the result alone takes 0.0017.
 struct MoeFp8Ws {
     int32_t *idx, *pos, *tok, *offsets, *hist;
     float *w;
